@@ -271,7 +271,8 @@ def _plain_verify(d):
         less = torch.where(less.sum(-1, keepdim=True) > 0, less, row)
         row = torch.where(refused, less, row)
     cum = row.cumsum(-1)
-    token = (cum <= u.gather(1, acc[:, None]) * cum[:, -1:]).sum(-1)
+    # by a random number of its own, the last: the one that refused a draft is not free any more
+    token = (cum <= u[:, n:] * cum[:, -1:]).sum(-1)
     steps = torch.arange(n + 1, device=w.device)
     tokens = torch.cat([drafts, torch.full((b, 1), -1, device=w.device)], 1)
     tokens = torch.where(steps < acc[:, None], tokens, torch.where(steps == acc[:, None], token[:, None], -1))
@@ -412,7 +413,7 @@ def _exact_verify(c, seed):
         part = torch.cumsum(want, 0)
         acc[s] = a
         tokens[s, :a] = torch.tensor(drafted[s][:a], dtype=torch.int32)
-        tokens[s, a] = int(torch.searchsorted(part, rnd[s][a] * part[-1], right=True))
+        tokens[s, a] = int(torch.searchsorted(part, rnd[s][n] * part[-1], right=True))
     return dict(accepted=acc, tokens=tokens, p=p)
 
 
