@@ -227,6 +227,70 @@ int mk_kv_config(void * h, const char * key, long long value);
  * out[0..4): attend calls, then total milliseconds of attention, combine, append.  Returns the count written. */
 int mk_kv_profile(void * h, int enable, double * out, int cap);
 
+/*
+ * ---- The operators of a decode step around the store: what a decoder runs between its attention layers' calls, on the
+ * activation units that mk_kv_attend_gated / mk_kv_attend_prep leave.  No handle, no memory of their own; asynchronous on
+ * `stream`; every buffer is memory of the current device (checked).  dtype: 0 fp32, 1 fp16, 2 bf16.  Strides count
+ * elements between rows.  Calls on different streams are independent of each other as long as their outputs and workspaces are.
+ * The same call gives the same bits on every run.
+ */
+
+/*
+ * Residual addition and root-mean-square norm of rows [rows][dim], dim 1..32768 (the norm before a projection; the
+ * reference's resid / norm phases around attn_proj, qwen38_mk.cu:2587-2621):
+ *   h = x + res (fp32, rounded to dtype; res NULL: h = x), y = h / sqrt(mean(h^2) + eps) * w
+ * with the mean in 64 bits.  x, res, sum, y: dtype; w: fp32 [dim].  Outputs, each optional, one at least: sum = h (may be
+ * res itself: the residual stream updated in place), y (may be x itself), and the units of y (dim a multiple of 64; a set):
+ * q32a / q32b [rows][dim / 32][16] and q32meta [rows][dim / 32][4] in the layout of mk_kv_attend_gated.  A block's codes are
+ * round(t 127 / max |t|), ties to even, of t = h w, its scale max |t| / (sqrt(mean(h^2) + eps) 127) as fp16: codes do not depend on the order
+ * of the row's sum.  A row with an infinity or a NaN gives NaN scales, or codes of zero, as its y.
+ * q32a / q32b are aligned to 16 bytes, q32meta to 8.  Other overlaps of outputs and inputs are not allowed.
+ */
+int mk_norm_q32(const void * x, long long x_stride, const void * res, long long res_stride, const float * w, int rows, int dim, float eps, int dtype,
+                void * sum, long long sum_stride, void * y, long long y_stride, void * q32a, void * q32b, unsigned short * q32meta, void * stream);
+
+/*
+ * Products with 4-bit weights: y[m][j] = sum_k W[j][k] x[m][k] for `rows` rows of x and n weight rows of k values
+ * (the projections around the store; the reference's dp4a products over q32 activations), y fp32 [rows][y_stride].
+ *   codes   [n][k / 2]: code c = 0..15 of value 8 w + i of a row in word w (4 bytes): i < 4 in the low nibble of byte i, else in
+ *           the high nibble of byte i - 4 (the order of the store's 4-bit rows); aligned to 16 bytes
+ *   scales  fp16 [n][ceil(k / group)], group 32, 64 or 128; mins fp16 of the same shape, or NULL
+ *   W = scales (c - 8) + mins
+ * mk_w4_units takes x as the int8 units of mk_kv_attend_gated or mk_norm_q32 ([rows][k / 32][16 | 4]; k a multiple of 64),
+ * mk_w4_rows as plain rows [rows][x_stride] of dtype (k a multiple of 32).  Products and sums are exact or in fp32: the units'
+ * integer sums are exact per 32 values, fp16 and bf16 rows enter as they are and fp32 rows to 2^-24 of each value.
+ * Meant for the tokens of a decode or verify step: 1 to 64 rows, more are allowed.
+ */
+int mk_w4_units(int rows, int n, int k, int group, const void * codes, const void * scales, const void * mins, const void * q32a, const void * q32b,
+                const unsigned short * q32meta, float * y, long long y_stride, void * stream);
+int mk_w4_rows(int rows, int n, int k, int group, const void * codes, const void * scales, const void * mins, const void * x, long long x_stride,
+               int dtype, float * y, long long y_stride, void * stream);
+
+/*
+ * Verification of drafted tokens against the target's distribution, from given random numbers (what follows a verify attention and the
+ * output head; the accepted length is what mk_kv_rewind keeps).  For each of n_seq sequences, with n = n_draft (0..64) drafts:
+ *   target      [n_seq][n + 1][row_stride] logits of dtype (probs 0), or fp32 probabilities (probs 1); vocab 1..2^24 entries a row.  Row
+ *               i is the distribution after draft i - 1
+ *   temperature fp32 [n_seq] or NULL (1): p = softmax(logits / temperature); 0: all on the largest logit, the lowest
+ *               index of equal ones.  -infinity masks an entry
+ *   draft_probs fp32 [n_seq][n][vocab], the distributions q the drafts were drawn from, or NULL: q is 1 at the draft (a greedy drafter)
+ *   drafts      int [n_seq][n]; one outside the vocabulary is refused.  n_drafts int [n_seq] or NULL: sequences with fewer drafts
+ *               (clamped to 0 .. n); rows behind them are not read
+ *   u           fp32 [n_seq][n + 1], uniform in [0, 1): draft i is accepted while u[i] q_i(draft) < p_i(draft); the next token
+ *               comes by u[n] from max(p - q, 0) at the first refused draft (from p where that is nothing), else from the row behind
+ *               the last draft: the first index at which the sum of the weights up to it exceeds u[n] times their total
+ *   accepted    int [n_seq]: drafts accepted; tokens int [n_seq][n + 1]: these, the next token, then -1.  A row with a NaN, a
+ *               +infinity or no weight at all refuses its draft and gives no token (-1)
+ *   draft_p     fp32 [n_seq][n] or NULL: p_i(draft i), 0 behind a sequence's last draft
+ * Weights, sums and comparisons are in 64 bits.  ws: device memory of at least mk_verify_ws(n_seq, n_draft, vocab) bytes (16 for every
+ * 4,096 entries of a row, and 8 for every 4,096 of a sequence's vocabulary), aligned to 16, that no other call uses until this
+ * one has finished; nothing in it needs clearing.  mk_verify_ws returns -1 for a shape the call refuses.
+ */
+long long mk_verify_ws(int n_seq, int n_draft, int vocab);
+int mk_verify_drafts(int n_seq, int n_draft, int vocab, const void * target, long long row_stride, int dtype, int probs, const float * temperature,
+                     const float * draft_probs, const int * drafts, const int * n_drafts, const float * u, int * accepted, int * tokens, float * draft_p,
+                     void * ws, long long ws_bytes, void * stream);
+
 /* Host-only geometry and grammar helpers (no GPU needed). */
 int mk_kv_window_start(int L, int win);  /* kv_ws, qwen38_mk.cu:2118-2126 */
 int mk_kv_ring_rows(int win);            /* kvrc, loader.cu:1479-1486 */

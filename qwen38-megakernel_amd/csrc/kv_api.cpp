@@ -413,6 +413,11 @@ static void * noalloc_scratch(int dev) {
     return addr[dev];
 }
 
+// the message of a call outside this file (step_api.cpp)
+namespace qkv {
+void set_error(const char * msg) { g_err = msg; }
+} // namespace qkv
+
 extern "C" {
 
 const char * mk_last_error(void) { return g_err.c_str(); }

@@ -1,0 +1,89 @@
+// Device-side building blocks of the step operators (step_*.hip): rows of fp32 / fp16 / bf16 values at any alignment, and
+// reductions over a wave.
+#pragma once
+#include "kv_dev.h"
+#include "step_launch.h"
+
+namespace qkv {
+
+// 8 consecutive values as loads of 16 bytes that need no more than the type's own alignment (the rows of a strided or
+// odd-sized tensor; the hardware splits a load that crosses a cache line)
+typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x8_u __attribute__((ext_vector_type(8), aligned(2)));
+typedef _Float16 f16x8_u __attribute__((ext_vector_type(8), aligned(2)));
+typedef __bf16 bf16x8_u __attribute__((ext_vector_type(8), aligned(2)));
+
+template <int DT> struct Elem;
+template <> struct Elem<DT_F32> {
+    typedef float T;
+    static __device__ __forceinline__ float up(T v) { return v; }
+    static __device__ __forceinline__ T down(float v) { return v; }
+    static __device__ __forceinline__ void load8(const T * p, float (&v)[8]) {
+        const f32x4_u a = *reinterpret_cast<const f32x4_u *>(p), b = *reinterpret_cast<const f32x4_u *>(p + 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+    }
+    static __device__ __forceinline__ void store8(T * p, const float (&v)[8]) {
+        *reinterpret_cast<f32x4_u *>(p) = f32x4_u{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4_u *>(p + 4) = f32x4_u{v[4], v[5], v[6], v[7]};
+    }
+};
+template <> struct Elem<DT_F16> {
+    typedef _Float16 T;
+    static __device__ __forceinline__ float up(T v) { return (float) v; }
+    static __device__ __forceinline__ T down(float v) { return (T) v; }
+    static __device__ __forceinline__ void load8(const T * p, float (&v)[8]) {
+        const f16x8_u a = *reinterpret_cast<const f16x8_u *>(p);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = (float) a[i];
+    }
+    static __device__ __forceinline__ void store8(T * p, const float (&v)[8]) {
+        f16x8_u a;
+#pragma unroll
+        for (int i = 0; i < 8; i++) a[i] = (T) v[i];
+        *reinterpret_cast<f16x8_u *>(p) = a;
+    }
+};
+template <> struct Elem<DT_BF16> {
+    typedef __bf16 T;
+    static __device__ __forceinline__ float up(T v) { return __builtin_bit_cast(float, (unsigned) __builtin_bit_cast(uint16_t, v) << 16); }
+    static __device__ __forceinline__ T down(float v) { return (T) v; }
+    static __device__ __forceinline__ void load8(const T * p, float (&v)[8]) {
+        const u16x8_u a = *reinterpret_cast<const u16x8_u *>(p);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = __builtin_bit_cast(float, (unsigned) a[i] << 16);
+    }
+    static __device__ __forceinline__ void store8(T * p, const float (&v)[8]) {
+        bf16x8_u a;
+#pragma unroll
+        for (int i = 0; i < 8; i++) a[i] = (T) v[i];
+        *reinterpret_cast<bf16x8_u *>(p) = a;
+    }
+};
+
+// the first n (1..8) of 8 values, the rest zero
+template <int DT> __device__ __forceinline__ void load_n(const typename Elem<DT>::T * p, int n, float (&v)[8]) {
+    if (n >= 8) return Elem<DT>::load8(p, v);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = i < n ? Elem<DT>::up(p[i]) : 0.f;
+}
+template <int DT> __device__ __forceinline__ void store_n(typename Elem<DT>::T * p, int n, const float (&v)[8]) {
+    if (n >= 8) return Elem<DT>::store8(p, v);
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (i < n) p[i] = Elem<DT>::down(v[i]);
+}
+
+__device__ __forceinline__ double shfl_xor_d(double v, int m) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const unsigned lo = shfl_xor_u((unsigned) b, m), hi = shfl_xor_u((unsigned) (b >> 32), m);
+    return __builtin_bit_cast(double, (uint64_t) hi << 32 | lo);
+}
+// sum over the wave, the same bits in every lane
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) v += shfl_xor_d(v, m);
+    return v;
+}
+
+} // namespace qkv

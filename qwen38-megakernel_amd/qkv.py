@@ -51,6 +51,13 @@ SIGNATURES = {
     "mk_kv_ring_restore": (_c_int, [_c_vp, _c_int, _c_int, _c_vp, _c_ll]),
     "mk_kv_config": (_c_int, [_c_vp, _c_cp, _c_ll]),
     "mk_kv_profile": (_c_int, [_c_vp, _c_int, ctypes.POINTER(ctypes.c_double), _c_int]),
+    "mk_norm_q32": (_c_int, [_c_vp, _c_ll, _c_vp, _c_ll, _c_vp, _c_int, _c_int, ctypes.c_float, _c_int, _c_vp, _c_ll, _c_vp, _c_ll, _c_vp, _c_vp,
+                             _c_vp, _c_vp]),
+    "mk_w4_units": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_ll, _c_vp]),
+    "mk_w4_rows": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_ll, _c_int, _c_vp, _c_ll, _c_vp]),
+    "mk_verify_ws": (_c_ll, [_c_int, _c_int, _c_int]),
+    "mk_verify_drafts": (_c_int, [_c_int, _c_int, _c_int, _c_vp, _c_ll, _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp,
+                                  _c_ll, _c_vp]),
     "mk_kv_window_start": (_c_int, [_c_int, _c_int]),
     "mk_kv_ring_rows": (_c_int, [_c_int]),
     "mk_kv_cap_T": (_c_int, [_c_int, _c_int]),
@@ -114,6 +121,34 @@ def parse_spec(spec, n_layers):
     _check(lib().mk_kv_parse_spec(spec.encode() if spec is not None else None, n_layers, out))
     v = list(out)
     return v[:n_layers], v[n_layers:2 * n_layers], v[2 * n_layers:3 * n_layers], v[3 * n_layers:]
+
+
+# ---- the operators of a decode step around the store (device addresses and strides in elements; dtype 0 fp32, 1 fp16, 2 bf16)
+def norm_q32(x, x_stride, res, res_stride, w, rows, dim, eps, dtype, sum_ptr=0, sum_stride=0, y=0, y_stride=0, q32a=0, q32b=0, q32meta=0, stream=0):
+    """sum = x + res (res 0: x), y = RMSNorm(sum) * w, and y as int8 units; each output optional (mk_norm_q32)."""
+    _check(lib().mk_norm_q32(x, x_stride, res, res_stride, w, rows, dim, eps, dtype, sum_ptr, sum_stride, y, y_stride, q32a, q32b, q32meta, stream))
+
+
+def w4_units(rows, n, k, group, codes, scales, mins, q32a, q32b, q32meta, y, y_stride, stream=0):
+    """y [rows][n] = x W^T, x as int8 units, W 4-bit codes with fp16 scales (and mins, or 0) per group (mk_w4_units)."""
+    _check(lib().mk_w4_units(rows, n, k, group, codes, scales, mins, q32a, q32b, q32meta, y, y_stride, stream))
+
+
+def w4_rows(rows, n, k, group, codes, scales, mins, x, x_stride, dtype, y, y_stride, stream=0):
+    """w4_units on plain rows x [rows][x_stride] of dtype (mk_w4_rows)."""
+    _check(lib().mk_w4_rows(rows, n, k, group, codes, scales, mins, x, x_stride, dtype, y, y_stride, stream))
+
+
+def verify_ws(n_seq, n_draft, vocab):
+    """Bytes of workspace that verify_drafts needs."""
+    return _check(lib().mk_verify_ws(n_seq, n_draft, vocab))
+
+
+def verify_drafts(n_seq, n_draft, vocab, target, row_stride, dtype, probs, temperature, draft_probs, drafts, n_drafts, u, accepted, tokens, draft_p,
+                  ws, ws_bytes, stream=0):
+    """Accept drafts against the target's logits (probs 0) or probabilities (1) and draw the next token (mk_verify_drafts)."""
+    _check(lib().mk_verify_drafts(n_seq, n_draft, vocab, target, row_stride, dtype, probs, temperature, draft_probs, drafts, n_drafts, u, accepted,
+                                  tokens, draft_p, ws, ws_bytes, stream))
 
 
 class KVStore:

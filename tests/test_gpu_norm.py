@@ -1,0 +1,150 @@
+"""Residual norm and its int8 units (mk_norm_q32) against the definition in 64 bits.
+
+The stored sum and the units are compared bit for bit: the sum is one fp32 addition and one rounding, the codes and scales follow
+from single float32 operations and a factor whose sum is in 64 bits.  y carries three float32 roundings (the factor, two
+products) and the output's."""
+import numpy as np
+import pytest
+
+from stepcase import CODE, EPS_HALF, dtype_of, norm_ref, norm_units_ref, ptr, unpack_units
+
+pytestmark = pytest.mark.gpu
+
+
+def run(torch, qkv, rows, dim, dt, res=True, out="both", pad=0, off=0, inplace=False, eps=1e-6, edit=None, seed=0, stream=None):
+    g = torch.Generator().manual_seed(seed)
+    T = dtype_of(torch, dt)
+
+    def rowsof(scale):
+        buf = torch.zeros(rows * (dim + pad) + off + 64, dtype=T)
+        v = buf[off:off + rows * (dim + pad)].view(rows, dim + pad)
+        v[:, :dim] = (torch.randn(rows, dim, generator=g) * scale).to(T)
+        return buf, v
+    xb, x = rowsof(1.0)
+    rb, r = rowsof(3.0)
+    if edit:
+        edit(x, r)
+    w = 1 + 0.2 * torch.randn(dim, generator=g)
+    want_h = ((x[:, :dim].float() + r[:, :dim].float()).to(T) if res else x[:, :dim].clone())
+    xd, rd, wd = xb.cuda(), rb.cuda(), w.cuda()
+    guard = 7.0
+    sb = rd if inplace else torch.full_like(rb, guard, device="cuda")
+    yb = torch.full_like(xb, guard, device="cuda")
+    units = out != "rows"
+    nu = dim // 32
+    a = torch.full((rows + 1, nu, 16), 99, dtype=torch.int8, device="cuda") if units else None
+    b = torch.full((rows + 1, nu, 16), 99, dtype=torch.int8, device="cuda") if units else None
+    m = torch.full((rows + 1, nu, 4), 999, dtype=torch.int16, device="cuda") if units else None
+    es = xd.element_size()
+    st, ld = off * es, dim + pad
+    s = stream or torch.cuda.current_stream()
+    qkv.norm_q32(xd.data_ptr() + st, ld, rd.data_ptr() + st if res else 0, ld, wd.data_ptr(), rows, dim, eps, CODE[dt],
+                 sb.data_ptr() + st if res else 0, ld, yb.data_ptr() + st if out != "units" else 0, ld, ptr(a), ptr(b), ptr(m), s.cuda_stream)
+    torch.cuda.synchronize()
+    h = want_h.float().numpy()
+    y64, rs = norm_ref(h, w.numpy(), eps)
+
+    def inner(buf):
+        return buf.cpu()[off:off + rows * ld].view(rows, ld)
+    if res:
+        got = inner(sb)
+        # the same bits (a NaN's payload is the hardware's own)
+        ints, nan = torch.int16 if es == 2 else torch.int32, torch.isnan(want_h)
+        assert torch.equal(torch.isnan(got[:, :dim]), nan)
+        assert torch.equal(got[:, :dim].contiguous().view(ints)[~nan], want_h.contiguous().view(ints)[~nan])
+        if pad and not inplace:
+            assert (got[:, dim:] == guard).all(), "columns behind the row were written"
+    if out != "units":
+        got = inner(yb)[:, :dim].float().numpy().astype(np.float64)
+        ok = np.isfinite(y64)
+        assert np.array_equal(np.isfinite(got), ok)
+        tol = np.abs(y64[ok]) * (3.01 * 2.0 ** -24 + EPS_HALF[dt]) + {"fp32": 1e-44, "bf16": 1e-40, "fp16": 2.0 ** -25}[dt]
+        assert (np.abs(got[ok] - y64[ok]) <= tol).all()
+        if pad:
+            assert (inner(yb)[:, dim:] == guard).all()
+    if units:
+        q, sc, sums = unpack_units(a[:rows].cpu().numpy(), b[:rows].cpu().numpy(), m[:rows].cpu().numpy().view(np.uint16))
+        eq, es_ = norm_units_ref(h, w.numpy(), rs)
+        fine = np.isfinite(h).all(1)
+        assert np.array_equal(q[fine], eq[fine])
+        assert np.array_equal(sc.view(np.uint16)[fine], es_.view(np.uint16)[fine])
+        assert np.array_equal(sums, q.reshape(rows, nu, 2, 16).astype(np.int16).sum(-1, dtype=np.int16))
+        # the values stand within half a code and the scale's half step of y
+        val = q.astype(np.float64) * sc.astype(np.float64)[..., None]
+        yb_ = y64.reshape(rows, nu, 32)
+        step = np.abs(yb_).max(-1, keepdims=True) / 127
+        assert (np.abs(val - yb_)[fine] <= (step * (0.5 + 127 * 2.0 ** -11 + 1e-3) + 127 * 2.0 ** -25)[fine]).all()
+        for t, v in ((a, 99), (b, 99), (m, 999)):
+            assert (t[rows] == v).all(), "written behind the last row"
+        return q, sc
+    return None
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("rows,dim", [(1, 64), (3, 128), (2, 1984), (5, 2048), (1, 2112), (4, 5120), (2, 8192), (3, 8256), (2, 16448), (2, 32768)])
+def test_units_and_rows(qkv, torch_gpu, rows, dim, dt):
+    run(torch_gpu, qkv, rows, dim, dt)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("rows,dim,pad,off", [(1, 1, 0, 0), (3, 7, 0, 0), (2, 8, 3, 1), (9, 1001, 0, 3), (17, 6143, 41, 0), (2, 20001, 5, 1), (1, 32767, 0, 0)])
+def test_odd_rows(qkv, torch_gpu, rows, dim, pad, off, dt):
+    run(torch_gpu, qkv, rows, dim, dt, out="rows", pad=pad, off=off)
+    run(torch_gpu, qkv, rows, dim, dt, out="rows", res=False, pad=pad, off=off)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+def test_unaligned_rows_with_units(qkv, torch_gpu, dt):
+    run(torch_gpu, qkv, 6, 5120, dt, pad=13, off=1)
+    run(torch_gpu, qkv, 6, 1024, dt, out="units", pad=1, off=5)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16", "bf16"])
+def test_in_place_and_many_rows(qkv, torch_gpu, dt):
+    run(torch_gpu, qkv, 2500, 512, dt, inplace=True)
+    run(torch_gpu, qkv, 1300, 5120, dt, inplace=True, out="units")
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+def test_zero_tiny_and_wild_rows(qkv, torch_gpu, dt):
+    def edit(x, r):
+        x[0] = 0
+        r[0] = 0              # a row of zeros
+        x[1] = 0
+        r[1] = 0
+        x[1, :32] = 1e-38     # a block without a finite 127 / max
+        r[2, 5] = float("inf")
+        x[3, 100] = float("nan")
+        x[4] *= 1e-20
+        r[4] = 0
+    run(torch_gpu, qkv, 6, 256, dt, edit=edit)
+
+
+def test_wild_rows_units_propagate(qkv, torch_gpu):
+    """A NaN in a row makes every scale of the row NaN; an infinity the scale of its block, the others zero."""
+    def edit(x, r):
+        x[0, 100] = float("nan")
+        x[1, 40] = float("inf")
+    q, sc = run(torch_gpu, qkv, 3, 256, "fp32", edit=edit)
+    assert np.isnan(sc[0]).all() and np.isnan(sc[1, 1]) and (sc[1, [0, 2, 3, 4, 5, 6, 7]] == 0).all() and np.isfinite(sc[2]).all()
+
+
+def test_no_rows(qkv, torch_gpu):
+    torch = torch_gpu
+    x = torch.ones(64, device="cuda")
+    y = torch.full((64,), 5.0, device="cuda")
+    qkv.norm_q32(x.data_ptr(), 64, 0, 0, x.data_ptr(), 0, 64, 1e-6, 0, 0, 0, y.data_ptr(), 64)
+    torch.cuda.synchronize()
+    assert (y == 5).all()
+
+
+def test_host_memory_refused(qkv, torch_gpu):
+    torch = torch_gpu
+    x = torch.ones(64, device="cuda")
+    for h in (torch.ones(64), torch.ones(64).pin_memory()):
+        with pytest.raises(qkv.KVError, match="not device memory"):
+            qkv.norm_q32(x.data_ptr(), 64, 0, 0, h.data_ptr(), 1, 64, 1e-6, 0, 0, 0, x.data_ptr(), 64)
+        with pytest.raises(qkv.KVError, match="not device memory"):
+            qkv.norm_q32(x.data_ptr(), 64, 0, 0, x.data_ptr(), 1, 64, 1e-6, 0, 0, 0, h.data_ptr(), 64)
+    torch.zeros(1, device="cuda")  # (no error left behind)
+    torch.cuda.synchronize()

@@ -1,0 +1,149 @@
+"""Products with 4-bit weights (mk_w4_units, mk_w4_rows) against the products in 64 bits, within the roundings that
+stepcase.w4_bound counts."""
+import numpy as np
+import pytest
+
+from stepcase import CODE, dtype_of, pack_codes, ptr, units_of, unpack_units, w4_bound, w4_ref
+
+pytestmark = pytest.mark.gpu
+
+
+def weights(rng, n, k, group, mins):
+    c = rng.integers(0, 16, (n, k))
+    gs = -(-k // group)
+    s = (rng.uniform(0.2, 1.5, (n, gs)) * 0.01).astype(np.float16)
+    m = (rng.standard_normal((n, gs)) * 0.02).astype(np.float16) if mins else None
+    return c, s, m
+
+
+def run(torch, qkv, rows, n, k, group, mins, x, seed=0, y_pad=0, x_pad=0, x_off=0, edit=None, scale=1.0):
+    rng = np.random.default_rng(seed + 1000 * rows + n + k)
+    c, s, m = weights(rng, n, k, group, mins)
+    v = (rng.standard_normal((rows, k)) * scale).astype(np.float32)
+    if edit:
+        edit(v, s)
+    codes = torch.from_numpy(pack_codes(c)).cuda()
+    sd = torch.from_numpy(s).cuda()
+    md = torch.from_numpy(m).cuda() if mins else None
+    y = torch.full((rows + 1, n + y_pad), 77.0, device="cuda")
+    if x == "units":
+        a, b, meta = units_of(v)
+        q, sc, _ = unpack_units(a, b, meta)
+        v = (q.astype(np.float64) * sc.astype(np.float64)[..., None]).reshape(rows, k)
+        ad, bd, xm = torch.from_numpy(a).cuda(), torch.from_numpy(b).cuda(), torch.from_numpy(meta.view(np.int16)).cuda()
+        qkv.w4_units(rows, n, k, group, codes.data_ptr(), sd.data_ptr(), ptr(md), ad.data_ptr(), bd.data_ptr(), xm.data_ptr(), y.data_ptr(), n + y_pad,
+                     torch.cuda.current_stream().cuda_stream)
+    else:
+        t = torch.from_numpy(v).to(dtype_of(torch, x))
+        v = t.double().numpy()
+        buf = torch.full((rows * (k + x_pad) + x_off,), 3.0, dtype=t.dtype)
+        buf[x_off:].view(rows, k + x_pad)[:, :k] = t
+        xd = buf.cuda()
+        qkv.w4_rows(rows, n, k, group, codes.data_ptr(), sd.data_ptr(), ptr(md), xd.data_ptr() + x_off * xd.element_size(), k + x_pad, CODE[x],
+                    y.data_ptr(), n + y_pad, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    got = y.cpu().numpy()
+    assert (got[rows] == 77).all() and (got[:, n:] == 77).all(), "written outside the result"
+    with np.errstate(all="ignore"):
+        ref, mag = w4_ref(c, s, m, group, v)
+    return got[:rows, :n].astype(np.float64), ref, mag
+
+
+def check(torch, qkv, rows, n, k, group, mins, x, **kw):
+    got, ref, mag = run(torch, qkv, rows, n, k, group, mins, x, **kw)
+    err = np.abs(got - ref)
+    bad = err > w4_bound(k, mag, x != "units")
+    assert not bad.any(), (np.argwhere(bad)[:4], err.max(), mag.max())
+
+
+@pytest.mark.parametrize("x", ["units", "fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 8, 9, 16, 17, 33, 64])
+def test_rows(qkv, torch_gpu, rows, x):
+    check(torch_gpu, qkv, rows, 100, 1024, 32, False, x)
+    check(torch_gpu, qkv, rows, 48, 704, 64, True, x)
+
+
+@pytest.mark.parametrize("x", ["units", "bf16"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("mins", [False, True])
+def test_groups(qkv, torch_gpu, group, mins, x):
+    for rows in (1, 3, 8, 20):
+        check(torch_gpu, qkv, rows, 33, 1088, group, mins, x)  # (1,088: the last group of 128 is half as long)
+
+
+@pytest.mark.parametrize("n", [1, 15, 16, 17, 127, 129, 1000])
+@pytest.mark.parametrize("k", [64, 128, 192, 2240])
+def test_shapes(qkv, torch_gpu, n, k):
+    check(torch_gpu, qkv, 1, n, k, 32, False, "units")
+    check(torch_gpu, qkv, 6, n, k, 64, True, "units")
+    check(torch_gpu, qkv, 2, n, k, 128, False, "fp16")
+
+
+@pytest.mark.parametrize("k", [32, 96, 160, 1056])
+def test_plain_rows_of_odd_blocks(qkv, torch_gpu, k):
+    for x in ("fp16", "bf16", "fp32"):
+        for rows in (1, 7, 24):
+            check(torch_gpu, qkv, rows, 40, k, 32, True, x, x_pad=5, x_off=3, y_pad=2)
+
+
+@pytest.mark.parametrize("x,rows", [("units", 1), ("units", 8), ("units", 64), ("bf16", 1), ("fp32", 4), ("fp32", 64)])
+def test_long_rows(qkv, torch_gpu, x, rows):
+    """Rows of x that do not fit a workgroup's LDS at once."""
+    check(torch_gpu, qkv, rows, 50, 25600, 128, True, x)
+
+
+@pytest.mark.parametrize("x", ["units", "fp16"])
+def test_many_weight_rows(qkv, torch_gpu, x):
+    """More 16-row tiles than the launch has waves: every number of waves per tile, workgroups with several tiles."""
+    for n in (3000, 9001, 20011, 70003):
+        check(torch_gpu, qkv, 1, n, 256, 32, False, x)
+        check(torch_gpu, qkv, 5, n, 128, 128, True, x)
+        check(torch_gpu, qkv, 40, n, 128, 64, False, x)
+
+
+@pytest.mark.parametrize("x", ["fp16", "bf16", "fp32"])
+def test_value_ranges(qkv, torch_gpu, x):
+    """Blocks of very different sizes, zeros, and the types' smallest values."""
+    def edit(v, s):
+        v[0, :32] *= 1e4
+        v[0, 32:64] = 0
+        v[0, 64:96] *= 2e-7
+        v[1] *= 1e-6 if x == "fp16" else 1e-30
+        v[2, ::2] *= 1e-5
+    check(torch_gpu, qkv, 3, 64, 256, 32, True, x, edit=edit)
+    if x != "fp16":
+        check(torch_gpu, qkv, 2, 64, 256, 32, False, x, scale=1e30)
+
+
+@pytest.mark.parametrize("x", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("rows", [4, 20])
+def test_wild_values(qkv, torch_gpu, x, rows):
+    """An infinity or a NaN in a row of x reaches that row alone; a weight row's infinite scale that column alone."""
+    def edit(v, s):
+        v[1, 40] = np.inf
+        v[2, 50] = np.nan
+        s[5, 1] = np.inf
+    got, ref, mag = run(torch_gpu, qkv, rows, 37, 256, 64, False, x, edit=edit)
+    ok = np.ones(rows, bool)
+    ok[[1, 2]] = False
+    cols = np.arange(37) != 5
+    g, r = got[ok][:, cols], ref[ok][:, cols]
+    assert np.isfinite(g).all() and (np.abs(g - r) <= w4_bound(256, mag[ok][:, cols], True)).all()
+    assert np.isnan(got[2]).all()
+    assert np.array_equal(np.isnan(got[1, cols]), np.isnan(ref[1, cols])) and np.array_equal(np.sign(got[1, cols]), np.sign(ref[1, cols]), equal_nan=True)
+    assert not np.isfinite(got[ok][:, 5]).any()
+
+
+def test_no_rows_and_refusals(qkv, torch_gpu):
+    torch = torch_gpu
+    t = torch.zeros(4096, dtype=torch.uint8, device="cuda")
+    y = torch.full((64,), 5.0, device="cuda")
+    p = t.data_ptr()
+    qkv.w4_rows(0, 64, 64, 32, p, p, 0, p, 64, 1, y.data_ptr(), 64)
+    qkv.w4_units(0, 64, 64, 32, p, p, 0, p, p, p, y.data_ptr(), 64)
+    torch.cuda.synchronize()
+    assert (y == 5).all()
+    h = torch.zeros(4096, dtype=torch.uint8)
+    with pytest.raises(qkv.KVError, match="codes is not device memory"):
+        qkv.w4_rows(1, 16, 64, 32, (h.data_ptr() + 15) // 16 * 16, p, 0, p, 64, 1, y.data_ptr(), 64)
+    torch.cuda.synchronize()
