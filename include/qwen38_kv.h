@@ -275,7 +275,7 @@ int mk_w4_rows(int rows, int n, int k, int group, const void * codes, const void
  *               index of equal ones.  -infinity masks an entry
  *   draft_probs fp32 [n_seq][n][vocab], the distributions q the drafts were drawn from, or NULL: q is 1 at the draft (a greedy drafter)
  *   drafts      int [n_seq][n]; one outside the vocabulary is refused.  n_drafts int [n_seq] or NULL: sequences with fewer drafts
- *               (clamped to 0 .. n); rows behind them are not read
+ *               (clamped to 0 .. n); what the rows behind them hold is not used
  *   u           fp32 [n_seq][n + 1], uniform in [0, 1): draft i is accepted while u[i] q_i(draft) < p_i(draft); the next token
  *               comes by u[n] from max(p - q, 0) at the first refused draft (from p where that is nothing), else from the row behind
  *               the last draft: the first index at which the sum of the weights up to it exceeds u[n] times their total
@@ -283,7 +283,7 @@ int mk_w4_rows(int rows, int n, int k, int group, const void * codes, const void
  *               +infinity or no weight at all refuses its draft and gives no token (-1)
  *   draft_p     fp32 [n_seq][n] or NULL: p_i(draft i), 0 behind a sequence's last draft
  * Weights, sums and comparisons are in 64 bits.  ws: device memory of at least mk_verify_ws(n_seq, n_draft, vocab) bytes (16 for every
- * 4,096 entries of a row, and 8 for every 4,096 of a sequence's vocabulary), aligned to 16, that no other call uses until this
+ * 4,096 entries of a row, and per sequence 8 for every row or every 4,096 entries, whichever are more), aligned to 16, that no other call uses until this
  * one has finished; nothing in it needs clearing.  mk_verify_ws returns -1 for a shape the call refuses.
  */
 long long mk_verify_ws(int n_seq, int n_draft, int vocab);

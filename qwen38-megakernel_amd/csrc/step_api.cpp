@@ -5,6 +5,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <stdexcept>
 #include <string>
@@ -103,7 +104,7 @@ void verify_shape(int n_seq, int n_draft, int vocab) {
 long long verify_ws(int n_seq, int n_draft, int vocab) {
     verify_shape(n_seq, n_draft, vocab);
     const long long nsl = slices(vocab);
-    return n_seq * nsl * ((n_draft + 1) * (long long) sizeof(VerifyPart) + (long long) sizeof(double));
+    return n_seq * (nsl * (n_draft + 1) * (long long) sizeof(VerifyPart) + std::max<long long>(nsl, n_draft + 1) * (long long) sizeof(double));
 }
 
 } // namespace

@@ -9,7 +9,9 @@ namespace qkv {
 // 8 consecutive values as loads of 16 bytes that need no more than the type's own alignment (the rows of a strided or
 // odd-sized tensor; the hardware splits a load that crosses a cache line)
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x4_u __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint16_t u16x8_u __attribute__((ext_vector_type(8), aligned(2)));
+typedef _Float16 f16x4_u __attribute__((ext_vector_type(4), aligned(2)));
 typedef _Float16 f16x8_u __attribute__((ext_vector_type(8), aligned(2)));
 typedef __bf16 bf16x8_u __attribute__((ext_vector_type(8), aligned(2)));
 
@@ -22,6 +24,11 @@ template <> struct Elem<DT_F32> {
         const f32x4_u a = *reinterpret_cast<const f32x4_u *>(p), b = *reinterpret_cast<const f32x4_u *>(p + 4);
 #pragma unroll
         for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+    }
+    static __device__ __forceinline__ void load4(const T * p, float (&v)[4]) {
+        const f32x4_u a = *reinterpret_cast<const f32x4_u *>(p);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = a[i];
     }
     static __device__ __forceinline__ void store8(T * p, const float (&v)[8]) {
         *reinterpret_cast<f32x4_u *>(p) = f32x4_u{v[0], v[1], v[2], v[3]};
@@ -36,6 +43,11 @@ template <> struct Elem<DT_F16> {
         const f16x8_u a = *reinterpret_cast<const f16x8_u *>(p);
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = (float) a[i];
+    }
+    static __device__ __forceinline__ void load4(const T * p, float (&v)[4]) {
+        const f16x4_u a = *reinterpret_cast<const f16x4_u *>(p);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = (float) a[i];
     }
     static __device__ __forceinline__ void store8(T * p, const float (&v)[8]) {
         f16x8_u a;
@@ -52,6 +64,11 @@ template <> struct Elem<DT_BF16> {
         const u16x8_u a = *reinterpret_cast<const u16x8_u *>(p);
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = __builtin_bit_cast(float, (unsigned) a[i] << 16);
+    }
+    static __device__ __forceinline__ void load4(const T * p, float (&v)[4]) {
+        const u16x4_u a = *reinterpret_cast<const u16x4_u *>(p);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = __builtin_bit_cast(float, (unsigned) a[i] << 16);
     }
     static __device__ __forceinline__ void store8(T * p, const float (&v)[8]) {
         bf16x8_u a;

@@ -61,7 +61,9 @@ struct VerifyArgs {
     int * tokens;         // [n_seq][n + 1]
     float * p;            // optional [n_seq][n]
     VerifyPart * part;    // [n_seq (n + 1)][nsl]
-    double * rest;        // [n_seq][nsl] (with q): sums of max(p - q, 0) of the refused row
+    // with q: [n_seq][nsl] sums of max(p - q, 0) of the refused row; without: [n_seq (n + 1)] per row the sum of its draft's
+    // slice without the draft
+    double * rest;
     long long row_stride;
     int n_seq, n, vocab, nsl;
 };

@@ -9,7 +9,8 @@
 // sums and the comparison are in 64 bits: two orders of summation then differ by 1e-16 of the total, and a token changes
 // with a probability of 1e-11.
 //
-// k_verify_rows: every row once, in slices of 4,096 entries (the slice's largest logit and its sum relative to that).
+// k_verify_rows: every row once, in slices of 4,096 entries (the slice's largest logit and its sum relative to that; for the
+// slice of a row's draft also the sum without it).
 // k_verify_residual (with q): the slices' sums of max(p - q, 0) of the one row that was refused, if any.
 // k_verify_pick: one workgroup per sequence: the decision, the slice of the next token by the slices' sums, and the token
 // inside the slice.
@@ -56,29 +57,36 @@ template <bool PROBS> __device__ __forceinline__ double weight(float v, float to
     else return exp2_neg(((double) v - (double) top) * beta);
 }
 
-// 16 consecutive entries of a row from j on; those past the end are -infinity / 0
-template <int DT> __device__ __forceinline__ void load16(const typename Elem<DT>::T * p, int j, int vocab, float none, float (&v)[VE]) {
+// E consecutive entries of a row from j on (one load of at most 16 bytes where all of them exist); those past the end are
+// `none`
+template <int DT, int E> __device__ __forceinline__ void load_run(const typename Elem<DT>::T * p, int j, int vocab, float none, float (&v)[E]) {
+    if (j + E <= vocab) {
+        if constexpr (E == 8) Elem<DT>::load8(p + j, v);
+        else Elem<DT>::load4(p + j, v);
+    } else {
 #pragma unroll
-    for (int c = 0; c < VE; c += 8) {
-        float t[8];
-        const int n = vocab - (j + c);
-        if (n > 0) load_n<DT>(p + j + c, n, t);
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[c + i] = i < n ? t[i] : none;
+        for (int k = 0; k < E; k++) v[k] = j + k < vocab ? Elem<DT>::up(p[j + k]) : none;
     }
 }
+// entries of a thread's piece of a slice that lie together: 16 bytes of them
+constexpr int run_of(int dt) { return dt == DT_F32 ? 4 : 8; }
 
 template <int DT, bool PROBS>
 __global__ __launch_bounds__(VT) void k_verify_rows(VerifyArgs a) {
     __shared__ float top[VT / 64];
-    __shared__ double sums[VT / 64];
+    __shared__ double sums[VT / 64], rests[VT / 64];
     __shared__ int args[VT / 64], bad[VT / 64];
     const int row = blockIdx.x / a.nsl, sl = blockIdx.x - row * a.nsl, b = row / (a.n + 1), i = row - b * (a.n + 1);
     if (i > count_of(a, b)) return; // (a row behind the sequence's last draft)
     const Temp t = temp_of(a, b);
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, j0 = sl * VERIFY_SLICE + threadIdx.x * VE;
+    constexpr int E = run_of(DT);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, j0 = sl * VERIFY_SLICE + threadIdx.x * E;
+    const auto at = [&](int k) { return j0 + k / E * (VT * E) + k % E; };
     float v[VE];
-    load16<DT>(static_cast<const typename Elem<DT>::T *>(a.target) + (long long) row * a.row_stride, j0, a.vocab, PROBS ? 0.f : -__builtin_inff(), v);
+#pragma unroll
+    for (int c = 0; c < VE / E; c++)
+        load_run<DT, E>(static_cast<const typename Elem<DT>::T *>(a.target) + (long long) row * a.row_stride, at(c * E), a.vocab,
+                        PROBS ? 0.f : -__builtin_inff(), *reinterpret_cast<float (*)[E]>(v + c * E));
     float m = -__builtin_inff();
     bool wild = false;
 #pragma unroll
@@ -103,7 +111,7 @@ __global__ __launch_bounds__(VT) void k_verify_rows(VerifyArgs a) {
     else if (!PROBS && t.greedy) {
         int arg = 0x7fffffff;
 #pragma unroll
-        for (int k = VE - 1; k >= 0; k--) arg = v[k] == m && j0 + k < a.vocab ? j0 + k : arg;
+        for (int k = VE - 1; k >= 0; k--) arg = v[k] == m && at(k) < a.vocab ? at(k) : arg;
 #pragma unroll
         for (int x = 1; x < 64; x <<= 1) arg = min(arg, (int) shfl_xor_u((unsigned) arg, x));
         if (lane == 0) args[wave] = arg;
@@ -118,34 +126,83 @@ __global__ __launch_bounds__(VT) void k_verify_rows(VerifyArgs a) {
 #pragma unroll
             for (int k = 0; k < VE; k++) s += weight<PROBS>(v[k], m, t.beta);
         }
+        // the slice of a draft that may be refused: also its sum without the draft, what is left over without q
+        const int d = !a.q && i < a.n ? a.drafts[b * a.n + i] : -1;
+        const bool holds = d >= 0 && d / VERIFY_SLICE == sl && d < a.vocab;
+        double rest = 0;
+        if (holds) {
+#pragma unroll
+            for (int k = 0; k < VE; k++)
+                if (at(k) != d) rest += weight<PROBS>(v[k], m, t.beta);
+            rest = wave_sum(rest);
+            if (lane == 0) rests[wave] = rest;
+        }
         s = wave_sum(s);
         if (lane == 0) sums[wave] = s;
         __syncthreads();
         p.sum = sums[0];
 #pragma unroll
         for (int k = 1; k < VT / 64; k++) p.sum += sums[k];
+        if (holds && threadIdx.x == 0) {
+            rest = rests[0];
+            for (int k = 1; k < VT / 64; k++) rest += rests[k];
+            a.rest[row] = rest;
+        }
     }
     if (threadIdx.x == 0) a.part[(size_t) row * a.nsl + sl] = p;
 }
 
 // what every workgroup of a sequence finds from the slices' sums
 struct Verdict {
-    float top[VERIFY_MAX_DRAFTS + 1];  // per row: the largest logit
-    double z[VERIFY_MAX_DRAFTS + 1];   // the sum of the weights relative to it (probabilities: their sum); not > 0: no row
+    float top[VERIFY_MAX_DRAFTS + 1]; // per row: the largest logit
+    double z[VERIFY_MAX_DRAFTS + 1];  // the sum of the weights relative to it (probabilities: their sum); 0: not a row to draw from
     int arg[VERIFY_MAX_DRAFTS + 1];
-    int acc;
+    float p[VERIFY_MAX_DRAFTS];       // the drafts' probabilities
+    int ok[VERIFY_MAX_DRAFTS];        // accepted on its own
+    int draft[VERIFY_MAX_DRAFTS];     // -1: outside the vocabulary
 };
 
-// all VT threads; draws the accepted count and, when p is given, stores the drafts' probabilities
-template <int DT, bool PROBS>
-__device__ __forceinline__ void decide(const VerifyArgs & a, int b, int count, const Temp t, Verdict & V, float * p) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+// what a wave reads of one row: its first 64 slices, one a lane, and what belongs to its draft
+struct RowIn {
+    VerifyPart part;
+    int d; // the draft, -1 outside the vocabulary
+    float v, u, q;
+};
+template <int DT> __device__ __forceinline__ RowIn load_row(const VerifyArgs & a, int b, int i) {
+    const long long row = (long long) b * (a.n + 1) + i;
+    const int lane = threadIdx.x & 63;
+    RowIn in{{0.0, -__builtin_inff(), 0x7fffffff}, -1, 0.f, 0.f, 1.f};
+    if (lane < a.nsl) in.part = a.part[row * a.nsl + lane];
+    if (i < a.n) {
+        const int d = a.drafts[b * a.n + i];
+        in.u = a.u[row];
+        if (d >= 0 && d < a.vocab) {
+            in.d = d;
+            in.v = Elem<DT>::up(static_cast<const typename Elem<DT>::T *>(a.target)[row * a.row_stride + d]);
+            if (a.q) in.q = a.q[((size_t) b * a.n + i) * a.vocab + d];
+        }
+    }
+    return in;
+}
+
+// a wave per row, all NT threads; count and t: the sequence's drafts and temperature; kept (optional): [row][64] the weights
+// of the rows' first 64 slices; returns the accepted count in every thread
+template <int DT, bool PROBS, int NT>
+__device__ __forceinline__ int decide(const VerifyArgs & a, int b, int & count, Temp & t, Verdict & V, double * kept) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const float ninf = -__builtin_inff();
-    for (int i = wave; i <= count; i += VT / 64) {
-        const VerifyPart * pp = a.part + (size_t) (b * (a.n + 1) + i) * a.nsl;
-        float m = ninf;
-        bool wild = false;
-        for (int s = lane; s < a.nsl; s += 64) {
+    // (ahead of the sequence's own values: one wait for all of them.  A row behind the last draft is memory of the workspace
+    // all the same, and what it holds is not used)
+    RowIn in;
+    if (wave <= a.n) in = load_row<DT>(a, b, wave);
+    count = count_of(a, b);
+    t = temp_of(a, b);
+    for (int i = wave; i <= count; i += NT / 64) {
+        if (i != wave) in = load_row<DT>(a, b, i);
+        const VerifyPart * pp = a.part + ((long long) b * (a.n + 1) + i) * a.nsl;
+        float m = in.part.top;
+        bool wild = m != m;
+        for (int s = lane + 64; s < a.nsl; s += 64) {
             const float x = pp[s].top;
             wild |= x != x;
             m = fmaxf(m, x);
@@ -155,49 +212,45 @@ __device__ __forceinline__ void decide(const VerifyArgs & a, int b, int count, c
         wild = __ballot(wild) != 0;
         double z = 0;
         int arg = 0x7fffffff;
-        for (int s = lane; s < a.nsl; s += 64) {
-            const VerifyPart x = pp[s];
+        const auto add = [&](const VerifyPart & x) {
             if (!PROBS && t.greedy) {
                 if (x.top == m) arg = min(arg, x.arg);
             } else if (x.sum > 0) z += PROBS ? x.sum : x.sum * exp2_neg(((double) x.top - (double) m) * t.beta);
-        }
+        };
+        add(in.part);
+        if (kept) kept[i * 64 + lane] = z;
+        for (int s = lane + 64; s < a.nsl; s += 64) add(pp[s]);
         if (!PROBS && t.greedy) {
 #pragma unroll
             for (int x = 1; x < 64; x <<= 1) arg = min(arg, (int) shfl_xor_u((unsigned) arg, x));
             z = m > ninf ? 1.0 : 0.0;
         } else z = wave_sum(z);
-        if (lane == 0) {
-            V.top[i] = m;
-            V.z[i] = wild || !(z < (double) __builtin_inff()) ? 0.0 : z;
-            V.arg[i] = arg;
-        }
-    }
-    __syncthreads();
-    if (wave == 0) { // a draft per lane
+        if (wild || !(z < (double) __builtin_inff())) z = 0;
         double pd = 0;
-        bool ok = false;
-        if (lane < count) {
-            const int d = a.drafts[b * a.n + lane];
-            const double z = V.z[lane];
-            if (d >= 0 && d < a.vocab && z > 0) {
-                if (!PROBS && t.greedy) pd = d == V.arg[lane] ? 1.0 : 0.0;
-                else {
-                    const float v = Elem<DT>::up(static_cast<const typename Elem<DT>::T *>(a.target)[(long long) (b * (a.n + 1) + lane) * a.row_stride + d]);
-                    pd = weight<PROBS>(v, V.top[lane], t.beta);
-                    if (!PROBS) pd /= z;
-                }
-                const double qd = a.q ? (double) a.q[((size_t) b * a.n + lane) * a.vocab + d] : 1.0;
-                ok = (double) a.u[b * (a.n + 1) + lane] * qd < pd;
+        if (i < count && in.d >= 0 && z > 0) {
+            if (!PROBS && t.greedy) pd = in.d == arg ? 1.0 : 0.0;
+            else {
+                pd = weight<PROBS>(in.v, m, t.beta);
+                if (!PROBS) pd /= z;
             }
         }
-        const uint64_t no = ~__ballot(ok);
-        if (lane == 0) V.acc = min(count, no ? (int) __builtin_ctzll(no) : 64);
-        if (p && lane < a.n) p[b * a.n + lane] = (float) pd;
+        if (lane == 0) {
+            V.top[i] = m;
+            V.z[i] = z;
+            V.arg[i] = arg;
+            if (i < count) {
+                V.draft[i] = in.d;
+                V.p[i] = (float) pd;
+                V.ok[i] = (double) in.u * (double) in.q < pd;
+            }
+        }
     }
     __syncthreads();
+    const uint64_t no = ~__ballot(lane < count && V.ok[lane < count ? lane : 0]);
+    return min(count, no ? (int) __builtin_ctzll(no) : 64);
 }
 
-// the weights of 16 entries of the row the next token is drawn from
+// the weights of E entries of the row the next token is drawn from
 struct Source {
     long long row;   // of the target
     const float * q; // subtracted, or null
@@ -205,17 +258,16 @@ struct Source {
     double beta, zinv;
     int skip;        // an entry that counts as zero (-1: none)
 };
-template <int DT, bool PROBS>
-__device__ __forceinline__ void weights16(const VerifyArgs & a, const Source & S, int j, double (&w)[VE]) {
-    float v[VE];
-    load16<DT>(static_cast<const typename Elem<DT>::T *>(a.target) + S.row * a.row_stride, j, a.vocab, PROBS ? 0.f : -__builtin_inff(), v);
+template <int DT, bool PROBS, int E>
+__device__ __forceinline__ void weights(const VerifyArgs & a, const Source & S, int j, double (&w)[E]) {
+    float v[E], q[E];
+    load_run<DT, E>(static_cast<const typename Elem<DT>::T *>(a.target) + S.row * a.row_stride, j, a.vocab, PROBS ? 0.f : -__builtin_inff(), v);
+    if (S.q) load_run<DT_F32, E>(S.q, j, a.vocab, 0.f, q);
 #pragma unroll
-    for (int k = 0; k < VE; k++) w[k] = j + k == S.skip ? 0.0 : weight<PROBS>(v[k], S.top, S.beta);
+    for (int k = 0; k < E; k++) w[k] = j + k == S.skip ? 0.0 : weight<PROBS>(v[k], S.top, S.beta);
     if (S.q) {
-        float q[VE];
-        load16<DT_F32>(S.q, j, a.vocab, 0.f, q);
 #pragma unroll
-        for (int k = 0; k < VE; k++) {
+        for (int k = 0; k < E; k++) {
             const double r = (PROBS ? w[k] : w[k] * S.zinv) - (double) q[k];
             w[k] = r > 0 ? r : 0.0;
         }
@@ -226,17 +278,21 @@ template <int DT, bool PROBS>
 __global__ __launch_bounds__(VT) void k_verify_residual(VerifyArgs a) {
     __shared__ Verdict V;
     __shared__ double sums[VT / 64];
-    const int b = blockIdx.x / a.nsl, sl = blockIdx.x - b * a.nsl, count = count_of(a, b);
-    const Temp t = temp_of(a, b);
-    if (!PROBS && t.greedy) return;
-    decide<DT, PROBS>(a, b, count, t, V, nullptr);
-    const int r = V.acc;
-    if (r == count || !(V.z[r] > 0)) return;
+    const int b = blockIdx.x / a.nsl, sl = blockIdx.x - b * a.nsl;
+    int count;
+    Temp t;
+    const int r = decide<DT, PROBS, VT>(a, b, count, t, V, nullptr);
+    if ((!PROBS && t.greedy) || r == count || !(V.z[r] > 0)) return;
     const Source S{(long long) b * (a.n + 1) + r, a.q + ((size_t) b * a.n + r) * a.vocab, V.top[r], t.beta, 1.0 / V.z[r], -1};
-    double w[VE], s = 0;
-    weights16<DT, PROBS>(a, S, sl * VERIFY_SLICE + threadIdx.x * VE, w);
+    constexpr int E = run_of(DT);
+    double s = 0;
 #pragma unroll
-    for (int k = 0; k < VE; k++) s += w[k];
+    for (int c = 0; c < VE / E; c++) {
+        double w[E];
+        weights<DT, PROBS, E>(a, S, sl * VERIFY_SLICE + (c * VT + threadIdx.x) * E, w);
+#pragma unroll
+        for (int k = 0; k < E; k++) s += w[k];
+    }
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -247,114 +303,116 @@ __global__ __launch_bounds__(VT) void k_verify_residual(VerifyArgs a) {
     }
 }
 
-// exclusive sum over the VT threads' values, and the total: thread k + 1's sum is thread k's sum plus its value
-__device__ __forceinline__ double block_scan(double v, double * tmp, double & total) {
-    tmp[threadIdx.x] = v;
-    __syncthreads();
-    double ex = 0, all = 0;
-    for (int k = 0; k < VT; k++) {
-        if (k == (int) threadIdx.x) ex = all;
-        all += tmp[k];
+// inclusive sum over the lanes
+__device__ __forceinline__ double wave_scan(double v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const double o = __shfl_up(v, m, 64);
+        if (lane >= m) v += o;
     }
-    total = all;
-    __syncthreads();
-    return ex;
+    return v;
 }
 
+constexpr int PT = 1024; // threads of the pick: a wave per row, four entries of the slice per thread
+constexpr int PE = VERIFY_SLICE / PT;
+
 template <int DT, bool PROBS>
-__global__ __launch_bounds__(VT) void k_verify_pick(VerifyArgs a) {
+__global__ __launch_bounds__(PT) void k_verify_pick(VerifyArgs a) {
     __shared__ Verdict V;
-    __shared__ double tmp[VT], s_base;
+    __shared__ double sums[PT / 64];
+    __shared__ double kept[(VERIFY_MAX_DRAFTS + 1) * 64];
     __shared__ int s_at, s_last;
-    const int b = blockIdx.x, count = count_of(a, b), tid = threadIdx.x;
-    const Temp t = temp_of(a, b);
-    decide<DT, PROBS>(a, b, count, t, V, a.p);
-    const int r = V.acc;
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float u32 = a.u[(long long) b * (a.n + 1) + a.n];
+    if (tid == 0) s_at = s_last = -1;
+    int count;
+    Temp t;
+    const int r = decide<DT, PROBS, PT>(a, b, count, t, V, kept);
     int token = -1;
     if (V.z[r] > 0) {
         if (!PROBS && t.greedy) token = V.arg[r];
         else {
             const long long row = (long long) b * (a.n + 1) + r;
             const VerifyPart * pp = a.part + row * a.nsl;
-            const bool refused = r < count;
             Source S{row, nullptr, V.top[r], t.beta, 1.0 / V.z[r], -1};
-            if (refused) {
+            double less = 0; // the refused draft's slice without it
+            if (r < count) {
                 if (a.q) S.q = a.q + ((size_t) b * a.n + r) * a.vocab;
-                else {
-                    const int d = a.drafts[b * a.n + r];
-                    if (d >= 0 && d < a.vocab) S.skip = d;
+                else if ((S.skip = V.draft[r]) >= 0) {
+                    less = a.rest[row];
+                    if (!PROBS) {
+                        const float top = pp[S.skip / VERIFY_SLICE].top; // (-infinity: a slice of masked entries, less is 0)
+                        less = less > 0 ? less * exp2_neg(((double) top - (double) S.top) * S.beta) : 0.0;
+                    }
                 }
             }
-            const int per = (a.nsl + VT - 1) / VT; // slices per thread
-            const double u = (double) a.u[b * (a.n + 1) + a.n];
+            // every wave finds the slice by itself: lane l holds `per` slices from l per on
+            const int per = (a.nsl + 63) / 64;
             for (int pass = 0; pass < 2; pass++) { // (again without q and skip where they leave nothing)
-                // the sum of the skipped entry's slice, without it
-                double less = 0;
-                if (S.skip >= 0) {
-                    double w[VE], s = 0;
-                    weights16<DT, PROBS>(a, S, S.skip / VERIFY_SLICE * VERIFY_SLICE + tid * VE, w);
-#pragma unroll
-                    for (int k = 0; k < VE; k++) s += w[k];
-                    (void) block_scan(s, tmp, less);
-                }
                 const auto slice = [&](int s) -> double {
                     if (s >= a.nsl) return 0.0;
                     if (S.q) return a.rest[(size_t) b * a.nsl + s];
                     if (S.skip >= 0 && s == S.skip / VERIFY_SLICE) return less;
+                    if (per == 1) return kept[r * 64 + s];
                     const double x = pp[s].sum;
                     return PROBS ? x : x > 0 ? x * exp2_neg(((double) pp[s].top - (double) S.top) * S.beta) : 0.0;
                 };
-                double mine = 0, total;
-                for (int k = 0; k < per; k++) mine += slice(tid * per + k);
-                const double ex = block_scan(mine, tmp, total);
+                double mine = 0;
+                for (int k = 0; k < per; k++) mine += slice(lane * per + k);
+                const double incl = wave_scan(mine), total = __shfl(incl, 63, 64);
                 if (!(total > 0)) {
                     S.q = nullptr;
                     S.skip = -1;
                     continue;
                 }
-                if (tid == 0) s_at = s_last = -1;
-                __syncthreads();
-                const double want = u * total;
-                if (mine > 0) {
-                    const bool here = ex <= want && want < ex + mine;
-                    double run = ex;
-                    int last = -1;
-                    for (int k = 0; k < per; k++) {
-                        const double x = slice(tid * per + k);
-                        if (!(x > 0)) continue;
-                        last = tid * per + k;
-                        if (here) {
-                            s_at = last;
-                            s_base = run;
-                            run += x;
-                            if (want < run) break;
-                        }
-                    }
-                    atomicMax(&s_last, last);
+                double ex = __shfl_up(incl, 1, 64); // (a lane's sum begins exactly where the one before it ends)
+                if (lane == 0) ex = 0;
+                const double want = (double) u32 * total;
+                const uint64_t in = __ballot(mine > 0 && ex <= want && want < incl), any = __ballot(mine > 0);
+                // (none, for a random number of 1 or more: the last slice with a weight, and its last entry)
+                const int l = in ? (int) __builtin_ctzll(in) : 63 - (int) __builtin_clzll(any);
+                int sl = -1;
+                double run = ex;
+                for (int k = 0; k < per; k++) {
+                    const double x = slice(lane * per + k);
+                    if (!(x > 0)) continue;
+                    if (sl >= 0 && in && want < run) break;
+                    if (sl >= 0) ex = run;
+                    sl = lane * per + k;
+                    run += x;
                 }
-                __syncthreads();
-                // (want at or past the total, for a random number of 1 or more: the last slice with a weight, its last entry)
-                const bool past = s_at < 0;
-                const int sl = past ? s_last : s_at;
-                const double left = past ? __builtin_inf() : want - s_base;
-                __syncthreads();
-                if (tid == 0) s_at = s_last = -1;
-                double w[VE], s = 0, all;
-                weights16<DT, PROBS>(a, S, sl * VERIFY_SLICE + tid * VE, w);
+                sl = __shfl(sl, l, 64);
+                const double left = in ? want - __shfl(ex, l, 64) : __builtin_inf();
+                double w[PE], s = 0;
+                weights<DT, PROBS, PE>(a, S, sl * VERIFY_SLICE + tid * PE, w);
 #pragma unroll
-                for (int k = 0; k < VE; k++) s += w[k];
-                const double e0 = block_scan(s, tmp, all);
+                for (int k = 0; k < PE; k++) s += w[k];
+                const double part = wave_scan(s);
+                if (lane == 63) sums[wave] = part;
+                __syncthreads();
+                double base = 0;
+                for (int k = 0; k < wave; k++) base += sums[k];
+                const double end = base + part;
+                double begin = __shfl_up(end, 1, 64);
+                if (lane == 0) begin = base;
                 if (s > 0) {
-                    const bool here = e0 <= left && left < e0 + s;
-                    double run = e0;
-                    int last = -1, at = -1;
-                    for (int k = 0; k < VE; k++) {
+                    double at = begin;
+                    int last = -1, found = -1;
+#pragma unroll
+                    for (int k = 0; k < PE; k++) {
                         if (!(w[k] > 0)) continue;
-                        last = sl * VERIFY_SLICE + tid * VE + k;
-                        run += w[k];
-                        if (at < 0 && left < run) at = last;
+                        last = sl * VERIFY_SLICE + tid * PE + k;
+                        at += w[k];
+                        if (found < 0 && left < at) found = last;
                     }
-                    if (here) s_at = at < 0 ? last : at;
+                    if (begin <= left && left < end) s_at = found < 0 ? last : found;
+                }
+                const uint64_t some = __ballot(s > 0);
+                if (some && lane == 63 - (int) __builtin_clzll(some)) {
+                    int last = -1;
+#pragma unroll
+                    for (int k = 0; k < PE; k++) last = w[k] > 0 ? sl * VERIFY_SLICE + tid * PE + k : last;
                     atomicMax(&s_last, last);
                 }
                 __syncthreads();
@@ -364,14 +422,15 @@ __global__ __launch_bounds__(VT) void k_verify_pick(VerifyArgs a) {
         }
     }
     if (tid == 0) a.accepted[b] = r;
-    for (int k = tid; k <= a.n; k += VT) a.tokens[b * (a.n + 1) + k] = k < r ? a.drafts[b * a.n + k] : k == r ? token : -1;
+    if (tid <= a.n) a.tokens[(long long) b * (a.n + 1) + tid] = tid < r ? a.drafts[b * a.n + tid] : tid == r ? token : -1;
+    if (a.p && tid < a.n) a.p[(long long) b * a.n + tid] = tid < count ? V.p[tid] : 0.f;
 }
 
 template <int DT, bool PROBS>
 static hipError_t launch_v(const VerifyArgs & a, hipStream_t st) {
     hipLaunchKernelGGL((k_verify_rows<DT, PROBS>), dim3((unsigned) a.n_seq * (a.n + 1) * a.nsl), dim3(VT), 0, st, a);
     if (a.q && a.n) hipLaunchKernelGGL((k_verify_residual<DT, PROBS>), dim3((unsigned) a.n_seq * a.nsl), dim3(VT), 0, st, a);
-    hipLaunchKernelGGL((k_verify_pick<DT, PROBS>), dim3(a.n_seq), dim3(VT), 0, st, a);
+    hipLaunchKernelGGL((k_verify_pick<DT, PROBS>), dim3(a.n_seq), dim3(PT), 0, st, a);
     return hipGetLastError();
 }
 

@@ -68,7 +68,7 @@ def test_verify_refusals(qkv, kw, msg):
 
 def test_workspace_size(qkv):
     assert qkv.verify_ws(0, 3, 1000) == 0
-    assert qkv.verify_ws(2, 3, 4096) == 2 * (4 * 16 + 8) and qkv.verify_ws(1, 0, 4097) == 2 * (16 + 8)
+    assert qkv.verify_ws(2, 3, 4096) == 2 * (4 * 16 + 4 * 8) and qkv.verify_ws(1, 0, 4097) == 2 * (16 + 8)
     for bad in ((-1, 0, 1), (1, 65, 10), (1, 1, 0)):
         with pytest.raises(qkv.KVError):
             qkv.verify_ws(*bad)
