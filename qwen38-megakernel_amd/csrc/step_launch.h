@@ -39,7 +39,7 @@ struct W4Args {
     int rows, n, k;
     int gsh, gs;             // a scale serves 32 << gsh values; gs = ceil(k / that) scales per row
     int wk_log;              // (set by the launcher) waves of a workgroup that share a tile: 1 << wk_log
-    int kcb;                 // (set by the launcher) 32-value blocks of x held in LDS at a time, a multiple of 4
+    int kcb;                 // (set by the launcher) 32-value blocks of x held in LDS at a time; more than 8 rows: tiles of a workgroup
 };
 enum { W4_UNITS = 3 };       // launch_w4: x as int8 units, else a Dtype
 hipError_t launch_w4(const W4Args & a, int xform, hipStream_t st);

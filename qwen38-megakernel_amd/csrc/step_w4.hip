@@ -15,9 +15,10 @@
 namespace qkv {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int W4_WAVES = 8;
+
 enum { XM_UNITS = 0, XM_HALF = 1, XM_SPLIT = 2 }; // x as int8 units, as one fp16 part, as two
 
 // 16-byte planes per block of 32 values in LDS
@@ -27,37 +28,46 @@ constexpr int planes(int mode) { return mode == XM_UNITS ? 2 : mode == XM_HALF ?
 // blocks' sums and [kcb][MR] float factors of m
 template <int MODE, int MR> __device__ __forceinline__ constexpr int blk_bytes() { return planes(MODE) * MR * 16; }
 
-template <int MODE, int DT, int MR>
+// 16 bytes per lane from its own address to LDS at lds + 16 lane, without a register (waited for with vm_drain)
+__device__ __forceinline__ void dma16(const void * g, unsigned lds) {
+    lds = (unsigned) __builtin_amdgcn_readfirstlane(lds);
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
+}
+__device__ __forceinline__ void vm_drain() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// x of blocks b0 .. b0 + nblk - 1 (nblk a multiple of 4) into LDS; blocks past the last one get factors of zero
+template <int MODE, int DT, int MR, int W>
 __device__ __forceinline__ void w4_stage(const W4Args & a, uint8_t * lds, int row0, int b0, int nblk) {
     constexpr int BB = blk_bytes<MODE, MR>();
     const int nb = a.k >> 5, tid = threadIdx.x;
     float * dx = reinterpret_cast<float *>(lds + (size_t) (a.kcb + 1) * BB), * ds = dx + a.kcb * MR;
-    for (int i = tid; i < BB / 16; i += W4_WAVES * 64) reinterpret_cast<uint4 *>(lds + (size_t) a.kcb * BB)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < BB / 16; i += W * 64) reinterpret_cast<uint4 *>(lds + (size_t) a.kcb * BB)[i] = make_uint4(0, 0, 0, 0);
     if constexpr (MODE == XM_UNITS) {
-        // (block, half, row) pieces of 16 bytes; the lane of half 0 brings the block's scale and sum
-        for (int i = tid; i < nblk * 2 * MR; i += W4_WAVES * 64) {
-            const int m = i % MR, half = (i / MR) & 1, bl = i / (2 * MR), blk = b0 + bl, row = row0 + m;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            float d = 0.f, s = 0.f;
-            if (row < a.rows && blk < nb) {
-                const int part = blk & 1;
-                const size_t gi = (size_t) row * nb + (blk & ~1) + half;
-                v = *reinterpret_cast<const uint4 *>((part ? a.xb : a.xa) + gi * 16);
-                if (!half) {
-                    d = h2f_bits(a.xmeta[gi * 4 + part]);
-                    s = d * (float) ((int) (int16_t) a.xmeta[gi * 4 + 2 + part] + (int) (int16_t) a.xmeta[gi * 4 + 6 + part]);
-                }
-            }
-            *reinterpret_cast<uint4 *>(lds + (size_t) bl * BB + (half * MR + m) * 16) = v;
-            if (!half) {
-                dx[bl * MR + m] = d * 0.0625f; // (the codes go in 16 times as large)
-                ds[bl * MR + m] = s;
-            }
+        // (block, half, row) pieces of 16 bytes, 64 a copy; rows past the last one repeat it (their sums are dropped)
+        const unsigned base = (unsigned) __builtin_amdgcn_readfirstlane((unsigned) (size_t) (__attribute__((address_space(3))) uint8_t *) lds);
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, pieces = nblk * 2 * MR;
+        for (int i0 = wave * 64; i0 < pieces; i0 += W * 64) {
+            const int i = i0 + lane;
+            const int m = i % MR, half = (i / MR) & 1, blk = min(b0 + i / (2 * MR), nb - 1), row = min(row0 + m, a.rows - 1);
+            if (i < pieces) dma16(((blk & 1) ? a.xb : a.xa) + ((size_t) row * nb + (blk & ~1) + half) * 16, base + i0 * 16);
         }
+        // a pair of blocks' scales and sums per lane: two units of {scale a, scale b, sum a, sum b}
+        for (int i = tid; i < (nblk >> 1) * MR; i += W * 64) {
+            const int m = i % MR, bl = i / MR * 2, row = min(row0 + m, a.rows - 1);
+            const bool in = b0 + bl < nb; // (nb is even)
+            const uint2 * mp = reinterpret_cast<const uint2 *>(a.xmeta) + (size_t) row * nb + (in ? b0 + bl : 0);
+            const uint2 u0 = mp[0], u1 = mp[1];
+            const float da = in ? h2f_bits((uint16_t) u0.x) : 0.f, db = in ? h2f_bits((uint16_t) (u0.x >> 16)) : 0.f;
+            dx[bl * MR + m] = da * 0.0625f; // (the codes go in 16 times as large)
+            dx[(bl + 1) * MR + m] = db * 0.0625f;
+            ds[bl * MR + m] = in ? da * (float) ((int) (int16_t) u0.y + (int) (int16_t) u1.y) : 0.f;
+            ds[(bl + 1) * MR + m] = in ? db * (float) (((int) u0.y >> 16) + ((int) u1.y >> 16)) : 0.f;
+        }
+        vm_drain();
     } else {
         // a quarter of a block (8 values) per lane
         const typename Elem<DT>::T * x = static_cast<const typename Elem<DT>::T *>(a.x);
-        for (int i = tid; i < nblk * 4 * MR; i += W4_WAVES * 64) { // (a multiple of 4 lanes: whole blocks)
+        for (int i = tid; i < nblk * 4 * MR; i += W * 64) { // (a multiple of 4 lanes: whole blocks)
             const int q = i & 3, m = (i >> 2) % MR, bl = (i >> 2) / MR, blk = b0 + bl, row = row0 + m;
             float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
             if (row < a.rows && blk < nb) Elem<DT>::load8(x + (long long) row * a.x_stride + 32 * blk + 8 * q, v);
@@ -106,144 +116,555 @@ __device__ __forceinline__ void w4_bytes(unsigned w, int & lo, int & hi) {
     lo = (int) ((w << 4) & 0xf0f0f0f0u);
     hi = (int) (w & 0xf0f0f0f0u);
 }
-// ... as fp16 pairs (0, 2) (1, 3) (4, 6) (5, 7): 0x6400 | n is 1024 + n exactly
+// ... as fp16 pairs (0, 2) (1, 3) (4, 6) (5, 7): 0x6400 | n is 1024 + n and 0x5400 | 16 n is 64 + n, both exact
 __device__ __forceinline__ half8 w4_halves(unsigned w) {
-    const half2v b = {(_Float16) -1032.f, (_Float16) -1032.f};
-    const half2v p0 = as_h2((w & 0x000f000fu) | 0x64006400u) + b, p1 = as_h2(((w >> 8) & 0x000f000fu) | 0x64006400u) + b,
-                 p2 = as_h2(((w >> 4) & 0x000f000fu) | 0x64006400u) + b, p3 = as_h2(((w >> 12) & 0x000f000fu) | 0x64006400u) + b;
+    const half2v b0 = {(_Float16) -1032.f, (_Float16) -1032.f}, b1 = {(_Float16) -72.f, (_Float16) -72.f};
+    const unsigned v = w >> 8;
+    const half2v p0 = as_h2((w & 0x000f000fu) | 0x64006400u) + b0, p1 = as_h2((v & 0x000f000fu) | 0x64006400u) + b0,
+                 p2 = as_h2((w & 0x00f000f0u) | 0x54005400u) + b1, p3 = as_h2((v & 0x00f000f0u) | 0x54005400u) + b1;
     return half8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
 }
 
-// NR activation rows per group of four operand rows (4, or 1 / 2 with one group), RG groups: MR = NR RG rows a pass
-template <int MODE, int DT, int NR, int RG>
-__global__ __launch_bounds__(W4_WAVES * 64) void k_w4(W4Args a) {
-    constexpr int MR = NR * RG, BB = blk_bytes<MODE, MR>();
+typedef unsigned u32x4_u2 __attribute__((ext_vector_type(4), aligned(2)));
+// scales grp .. grp + 7 of a weight row of gs (p: its first), zeros past the row's end: the last eight of the row, moved down
+__device__ __forceinline__ u32x4 w4_scales(const uint16_t * p, int gs, int grp) {
+    if (__builtin_expect(gs < 8, 0)) {
+        unsigned v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = grp + k < gs ? p[grp + k] : 0;
+        return u32x4{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+    }
+    const int at = min(grp, gs - 8), off = grp - at;
+    u32x4 e = *reinterpret_cast<const u32x4_u2 *>(p + at);
+    if (__builtin_expect(off != 0, 0)) {
+        if (off & 4) e = u32x4{e[2], e[3], 0, 0};
+        if (off & 2) e = u32x4{e[1], e[2], e[3], 0};
+        if (off & 1) e = u32x4{e[0] >> 16 | e[1] << 16, e[1] >> 16 | e[2] << 16, e[2] >> 16 | e[3] << 16, e[3] >> 16};
+        if (off >= 8) e = u32x4{0, 0, 0, 0};
+    }
+    return e;
+}
+
+constexpr int W4_RUN = 2;   // steps a wave takes together: the 128 bytes of a cache line of every row
+constexpr int W4_WIN = 32;  // scales of a weight row that a wave holds in LDS at a time
+
+// NR activation rows per group of four operand rows, RG groups: MR = NR RG rows a pass.
+// P parts: a tile is 16 / P weight rows, and lanes n = 16 / P h + j hold row j of part h, a P-th of its blocks.  A group's
+// operand row NR h + m is then x[m] of part h's block (P NR <= 4), and a lane takes its own part's sums: with few
+// rows of x the tiles get smaller, and a short projection has enough of them for every CU.
+// W waves: 1 << wk_log of them share a tile, each a run of its steps, the others have tiles of their own.
+// The codes of the next run are loaded while a run is worked on, over the tiles' borders too.  The scales come
+// 32 a row at a time (64 contiguous bytes; a lane's own two bytes of each step would fetch every cache line many times),
+// through 1 KiB of LDS of the wave's own, in which every lane then finds its block's.
+template <int MODE, int DT, int NR, int RG, int P, int W, bool MINS>
+__global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
+    static_assert(P * NR <= 4, "parts share a group's four operand rows");
+    constexpr int MR = NR * RG, BB = blk_bytes<MODE, MR>(), TR = 16 / P, U = W4_RUN;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const float * dx = reinterpret_cast<const float *>(lds + (size_t) (a.kcb + 1) * BB), * ds = dx + a.kcb * MR;
-    float * red = const_cast<float *>(ds) + a.kcb * MR; // [2][waves][MR][16]
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int WK = 1 << a.wk_log, wk = wave & (WK - 1), wn = wave >> a.wk_log, WN = W4_WAVES >> a.wk_log;
-    const int nb = a.k >> 5, tiles = (a.n + 15) >> 4, sets = (tiles + WN - 1) / WN;
-    const int row0 = blockIdx.y * MR;
-    // the lane's piece of the diagonal operand: row n = 4 b + m, lane group b
-    const int m = n & 3;
-    const bool active = (n >> 2) == g && m < NR;
-    const int abase = active ? g * BB + m * 16 : a.kcb * BB, astep = active ? 4 * BB : 0;
-    const size_t rowb = (size_t) a.k >> 1;
-    int par = 0;
+    const int WK = 1 << a.wk_log, wk = wave & (WK - 1), wn = wave >> a.wk_log, WN = W >> a.wk_log;
+    const int nb = a.k >> 5, tiles = (a.n + TR - 1) / TR, sets = (tiles + WN - 1) / WN;
+    const int nbp = (nb + 4 * U * P - 1) / (4 * U * P) * (4 * U * P), pb = nbp / P; // blocks with padding, blocks of a part
+    const int row0 = blockIdx.y * MR, j = n % TR, h = n / TR;
+    uint16_t * win = reinterpret_cast<uint16_t *>(const_cast<float *>(ds) + a.kcb * MR) + wave * (MINS ? 2 : 1) * 16 * W4_WIN; // [16][32] scales, then m
+    float * red = reinterpret_cast<float *>(reinterpret_cast<uint16_t *>(const_cast<float *>(ds) + a.kcb * MR) + W * (MINS ? 2 : 1) * 16 * W4_WIN); // [2][waves][MR][TR]
+    // the lane's piece of the diagonal operand: row n = 4 b + NR part + m, lane group b
+    const int m = n % NR, a_part = (n & 3) / NR;
+    const bool active = (n >> 2) == g && a_part < P;
+    const int abase = active ? (a_part * pb + g) * BB + m * 16 : a.kcb * BB, astep = active ? 4 * BB : 0;
+    const int hb = P == 1 ? 0 : h * pb, myb = hb + g; // the first block of the lane's part, the lane's block of step 0
+    // runs of the chunk of x that begins at block b0 (parts: all of x at once), and the wave's steps of them
+    const auto runs = [&](int b0) { return (P == 1 ? min(a.kcb, nbp - b0) : pb) / (4 * U); };
+    const auto begin = [&](int b0) { return U * ((runs(b0) * wk) >> a.wk_log); };
+    const auto end = [&](int b0) { return U * ((runs(b0) * (wk + 1)) >> a.wk_log); };
+    // what the wave loads next: a tile's first row in scalars, the lane's row and block in 32 bits
+    struct Next {
+        int set, b0, s, sw; // sw: the step at which the window of scales begins
+        const uint8_t * cp;
+        const uint16_t * sp, * mp;
+        unsigned vc, vs;
+    } nx;
+    const int G = gridDim.x, wsteps = (W4_WIN / 4) << a.gsh;
+    bool fresh = false; // nx begins a window: its scales (and m) are in the registers below
+    u32x4 ws, wm;
+    const auto window = [&] {
+        nx.sw = nx.s;
+        fresh = true;
+        const int first = (hb + nx.b0 + 4 * nx.s) >> a.gsh; // (exact: runs and parts are whole groups)
+        // (only what the wave's steps of this window need: 8 g groups in)
+        if (8 * g < (4 * (end(nx.b0) - nx.s) + 3) >> a.gsh) {
+            ws = w4_scales(nx.sp + nx.vs, a.gs, first + 8 * g);
+            if constexpr (MINS) wm = w4_scales(nx.mp + nx.vs, a.gs, first + 8 * g);
+        }
+    };
+    const auto enter = [&](int set) {
+        const int first = min((set * WN + wn) * TR, a.n - 1), nr = min(j, a.n - 1 - first);
+        nx.set = set;
+        nx.b0 = 0;
+        nx.s = begin(0);
+        nx.cp = a.codes + (size_t) first * (a.k >> 1);
+        nx.sp = a.scales + (size_t) first * a.gs;
+        nx.mp = a.mins + (size_t) first * a.gs;
+        nx.vc = (unsigned) (nr * (a.k >> 1));
+        nx.vs = (unsigned) (nr * a.gs);
+    };
+    const auto load = [&](int u) {
+        const unsigned blk = (unsigned) min(nx.b0 + 4 * (nx.s + u) + myb, nb - 1); // (past the last block the factors of x are zero)
+        return *reinterpret_cast<const u32x4 *>(nx.cp + (nx.vc + blk * 16));
+    };
+    const auto advance = [&] { // (past the launch's last run: that run once more, unused)
+        fresh = false;
+        nx.s += U;
+        if (nx.s < end(nx.b0)) {
+            if (nx.s - nx.sw >= wsteps) window();
+            return;
+        }
+        int b0 = nx.b0, s;
+        do {
+            b0 += P == 1 ? a.kcb : nbp;
+            s = begin(b0);
+        } while (b0 < nbp && s >= end(b0)); // (a last chunk without a run of this wave's)
+        if (b0 < nbp) {
+            nx.b0 = b0;
+            nx.s = s;
+            window();
+        } else if (nx.set + G < sets) {
+            enter(nx.set + G);
+            window();
+        } else nx.s -= U;
+    };
+    enter(blockIdx.x);
+    window();
+    u32x4 in[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        in[u] = load(u);
+        __builtin_amdgcn_sched_barrier(0); // (in the loop's order: its waits count the younger loads)
+    }
+    float acc[RG][NR];
+    int par = 0, sw = 0;
     bool staged = false;
-    for (int set = blockIdx.x; set < sets; set += gridDim.x, par ^= 1) {
-        const int tile = set * WN + wn, row = min(tile * 16 + n, a.n - 1);
-        const uint8_t * cp = a.codes + (size_t) row * rowb;
-        const size_t sp = (size_t) row * a.gs;
-        float acc[RG][NR];
+    for (int set = blockIdx.x; set < sets; set += G, par ^= 1) {
 #pragma unroll
         for (int i = 0; i < RG; i++)
 #pragma unroll
             for (int r = 0; r < NR; r++) acc[i][r] = 0.f;
-        for (int b0 = 0; b0 < nb; b0 += a.kcb) {
-            const int nblk = min(a.kcb, (nb - b0 + 3) & ~3);
+        for (int b0 = 0; b0 < nbp; b0 += P == 1 ? a.kcb : nbp) {
             if (!staged) {
                 __syncthreads();
-                w4_stage<MODE, DT, MR>(a, lds, row0, b0, nblk);
+                w4_stage<MODE, DT, MR, W>(a, lds, row0, b0, P == 1 ? min(a.kcb, nbp - b0) : nbp);
                 __syncthreads();
-                staged = nb <= a.kcb;
+                staged = nbp <= a.kcb;
             }
-            for (int s = wk; s < nblk >> 2; s += WK) {
-                const int blk = min(b0 + 4 * s + g, nb - 1); // (past the last block x is zero)
-                const u32x4 w = *reinterpret_cast<const u32x4 *>(cp + (size_t) blk * 16);
-                const float sc = h2f_bits(a.scales[sp + (blk >> a.gsh)]);
-                const uint8_t * ap = lds + abase + s * astep;
-                const float * dxp = dx + (4 * s + g) * MR, * dsp = ds + (4 * s + g) * MR;
-                const float mn = a.mins ? h2f_bits(a.mins[sp + (blk >> a.gsh)]) : 0.f;
-                if constexpr (MODE == XM_UNITS) {
-                    i32x4 h0, h1;
-                    int t0, t1;
-                    w4_bytes(w[0], t0, t1), h0[0] = t0, h0[1] = t1;
-                    w4_bytes(w[1], t0, t1), h0[2] = t0, h0[3] = t1;
-                    w4_bytes(w[2], t0, t1), h1[0] = t0, h1[1] = t1;
-                    w4_bytes(w[3], t0, t1), h1[2] = t0, h1[3] = t1;
-#pragma unroll
-                    for (int i = 0; i < RG; i++) {
-                        const i32x4 a0 = *reinterpret_cast<const i32x4 *>(ap + i * 64), a1 = *reinterpret_cast<const i32x4 *>(ap + MR * 16 + i * 64);
-                        i32x4 c = {0, 0, 0, 0};
-                        c = __builtin_amdgcn_mfma_i32_16x16x64_i8(a0, h0, c, 0, 0, 0);
-                        c = __builtin_amdgcn_mfma_i32_16x16x64_i8(a1, h1, c, 0, 0, 0);
-#pragma unroll
-                        for (int r = 0; r < NR; r++) acc[i][r] = __builtin_fmaf((float) c[r], sc * dxp[4 * i + r], acc[i][r]);
-                    }
-                } else {
-                    half8 hw[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) hw[k] = w4_halves(w[k]);
-#pragma unroll
-                    for (int i = 0; i < RG; i++) {
-                        f32x4 c = {0, 0, 0, 0};
-#pragma unroll
-                        for (int k = planes(MODE) - 1; k >= 0; k--)
-                            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const half8 *>(ap + k * MR * 16 + i * 64), hw[k & 3], c, 0, 0, 0);
-#pragma unroll
-                        for (int r = 0; r < NR; r++) acc[i][r] = __builtin_fmaf(c[r], sc * dxp[4 * i + r], acc[i][r]);
-                    }
+            const int s1 = end(b0);
+#pragma unroll 1
+            for (int s = begin(b0); s < s1; s += U) {
+                if (fresh) { // (the run's window: nx stands on this run)
+                    *reinterpret_cast<u32x4 *>(win + n * W4_WIN + 8 * g) = ws;
+                    if constexpr (MINS) *reinterpret_cast<u32x4 *>(win + 16 * W4_WIN + n * W4_WIN + 8 * g) = wm;
+                    sw = s;
                 }
-                if (a.mins) {
+                advance();
+                const uint16_t * wp = win + n * W4_WIN;
 #pragma unroll
-                    for (int i = 0; i < RG; i++)
+                for (int u = 0; u < U; u++) {
+                    // the codes leave their registers, then the next run's take them
+                    const int at = (4 * (s + u - sw) + g) >> a.gsh;
+                    const float sc = h2f_bits(wp[at]), mn = MINS ? h2f_bits(wp[16 * W4_WIN + at]) : 0.f;
+                    i32x4 hbv[2];
+                    half8 hw[4];
+                    if constexpr (MODE == XM_UNITS) {
 #pragma unroll
-                        for (int r = 0; r < NR; r++) acc[i][r] = __builtin_fmaf(mn, dsp[4 * i + r], acc[i][r]);
+                        for (int k = 0; k < 4; k++) {
+                            int t0, t1;
+                            w4_bytes(in[u][k], t0, t1);
+                            hbv[k >> 1][2 * (k & 1)] = t0;
+                            hbv[k >> 1][2 * (k & 1) + 1] = t1;
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) hw[k] = w4_halves(in[u][k]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    in[u] = load(u);
+                    __builtin_amdgcn_sched_barrier(0);
+                    const uint8_t * ap = lds + abase + (s + u) * astep;
+                    const float * dxp = dx + (4 * (s + u) + myb) * MR, * dsp = ds + (4 * (s + u) + myb) * MR;
+                    // the sums of the lane's own part
+                    const auto mine = [&](const auto & c, int r) {
+                        if constexpr (P == 1) return c[r];
+                        else if constexpr (P == 2) return h ? c[NR + r] : c[r];
+                        else return h & 2 ? (h & 1 ? c[3] : c[2]) : (h & 1 ? c[1] : c[0]);
+                    };
+#pragma unroll
+                    for (int i = 0; i < RG; i++) {
+                        if constexpr (MODE == XM_UNITS) {
+                            const i32x4 a0 = *reinterpret_cast<const i32x4 *>(ap + i * NR * 16), a1 = *reinterpret_cast<const i32x4 *>(ap + (MR + i * NR) * 16);
+                            i32x4 c = {0, 0, 0, 0};
+                            c = __builtin_amdgcn_mfma_i32_16x16x64_i8(a0, hbv[0], c, 0, 0, 0);
+                            c = __builtin_amdgcn_mfma_i32_16x16x64_i8(a1, hbv[1], c, 0, 0, 0);
+#pragma unroll
+                            for (int r = 0; r < NR; r++) acc[i][r] = __builtin_fmaf((float) mine(c, r), sc * dxp[NR * i + r], acc[i][r]);
+                        } else {
+                            f32x4 c = {0, 0, 0, 0};
+#pragma unroll
+                            for (int k = planes(MODE) - 1; k >= 0; k--)
+                                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const half8 *>(ap + (k * MR + i * NR) * 16), hw[k & 3], c, 0, 0, 0);
+#pragma unroll
+                            for (int r = 0; r < NR; r++) acc[i][r] = __builtin_fmaf(mine(c, r), sc * dxp[NR * i + r], acc[i][r]);
+                        }
+                        if constexpr (MINS) {
+#pragma unroll
+                            for (int r = 0; r < NR; r++) acc[i][r] = __builtin_fmaf(mn, dsp[NR * i + r], acc[i][r]);
+                        }
+                    }
                 }
             }
         }
-        // the four lane groups' blocks, then the waves of the tile in order
+        const int tile = set * WN + wn;
+        // the four lane groups' blocks, the parts, then the waves of the tile in order
 #pragma unroll
         for (int i = 0; i < RG; i++)
 #pragma unroll
-            for (int r = 0; r < NR; r++) acc[i][r] = quad_sum(acc[i][r]);
+            for (int r = 0; r < NR; r++) {
+                acc[i][r] = quad_sum(acc[i][r]);
+                if constexpr (P >= 2) acc[i][r] += shfl_xor(acc[i][r], 8);
+                if constexpr (P >= 4) acc[i][r] += shfl_xor(acc[i][r], 4);
+            }
         if (WK == 1) {
-            if (g == 0 && tile * 16 + n < a.n) {
+            if (lane < TR && tile * TR + lane < a.n) {
 #pragma unroll
                 for (int i = 0; i < MR; i++)
-                    if (row0 + i < a.rows) a.y[(long long) (row0 + i) * a.y_stride + tile * 16 + n] = acc[i / NR][i % NR];
+                    if (row0 + i < a.rows) a.y[(long long) (row0 + i) * a.y_stride + tile * TR + lane] = acc[i / NR][i % NR];
             }
             continue;
         }
-        float * rp = red + par * (W4_WAVES * MR * 16);
-        if (g == 0) {
+        float * rp = red + par * (W * MR * TR);
+        if (lane < TR) {
 #pragma unroll
-            for (int i = 0; i < MR; i++) rp[(wave * MR + i) * 16 + n] = acc[i / NR][i % NR];
+            for (int i = 0; i < MR; i++) rp[(wave * MR + i) * TR + lane] = acc[i / NR][i % NR];
         }
         __syncthreads(); // (the other parity's sums are not written again before every wave has passed this barrier)
-        for (int i = threadIdx.x; i < WN * MR * 16; i += W4_WAVES * 64) {
-            const int j = i & 15, mm = (i >> 4) % MR, t = (i >> 4) / MR, col = (set * WN + t) * 16 + j;
-            float v = rp[((t << a.wk_log) * MR + mm) * 16 + j];
-            for (int k = 1; k < WK; k++) v += rp[(((t << a.wk_log) + k) * MR + mm) * 16 + j];
+        for (int i = threadIdx.x; i < WN * MR * TR; i += W * 64) {
+            const int c = i % TR, mm = i / TR % MR, t = i / TR / MR, col = (set * WN + t) * TR + c;
+            float v = rp[((t << a.wk_log) * MR + mm) * TR + c];
+            for (int k = 1; k < WK; k++) v += rp[(((t << a.wk_log) + k) * MR + mm) * TR + c];
             if (col < a.n && row0 + mm < a.rows) a.y[(long long) (row0 + mm) * a.y_stride + col] = v;
         }
     }
 }
 
-constexpr int W4_LDS = 64 * 1024;
+// ------------------------------------------------------------------------------------------------ more than 8 rows
+// With more rows of x the diagonal operand's zeros cost: three of four lanes' LDS reads and matrix multiplications.  Here the
+// four dwords of a block's codes go to the four lane groups instead (a 4 x 4 exchange of registers and lane groups), so
+// that one instruction takes 16 rows of x against one block of 16 weight rows, without zeros, and every lane has its weight
+// row's scale of each block.  A workgroup takes up to 2 NTW tiles: 4 waves along the blocks of a chunk (U steps each) times 2
+// along the tiles; a piece of x read from LDS serves the wave's NTW tiles.  What bounds it is the fold of the blocks'
+// integer sums into fp32: three instructions per (row, block, weight row).
+constexpr int WIDE_W = 8; // waves
 
-template <int MODE, int DT, int NR, int RG>
+__device__ __forceinline__ void w4_exchange(const u32x4 & d, unsigned (&t)[4]) { // t[b] in lane group q: dword q of lane group b's d
+    const auto x = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false), y = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
+    const auto v = __builtin_amdgcn_permlane16_swap(x[0], y[0], false, false), w = __builtin_amdgcn_permlane16_swap(x[1], y[1], false, false);
+    t[0] = v[0], t[1] = v[1], t[2] = w[0], t[3] = w[1];
+}
+
+// LDS of a chunk of x, CB blocks of TM rows.  Units: a row's CB units of the even blocks, then CB of the odd ones (one 1 KiB
+// copy brings 64 of them from two contiguous pieces of memory), 16 bytes of padding behind each copy (16 rows' pieces
+// then lie in different banks), and the factors [CB][TM + 4].  Plain rows: w4_stage's layout.
+template <int MODE, int MT, int CB, bool MINS> constexpr int wide_buf() {
+    constexpr int TM = 16 * MT;
+    return MODE == XM_UNITS ? CB * 2 * TM / 64 * 1040 + (MINS ? 2 : 1) * CB * (TM + 4) * 4 : (CB + 1) * planes(MODE) * TM * 16 + 2 * CB * TM * 4;
+}
+
+// WK waves along the blocks of a chunk, U steps each, the others along the tiles
+template <int MODE, int DT, int MT, int NTW, int WK, int U, bool MINS>
+__global__ __launch_bounds__(WIDE_W * 64, 2) void k_w4_wide(W4Args a) {
+    constexpr int TM = 16 * MT, WN = WIDE_W / WK, CB = 4 * WK * U, BB = planes(MODE) * TM * 16, BUF = wide_buf<MODE, MT, CB, MINS>();
+    constexpr bool ASYNC = MODE == XM_UNITS; // x copied into the other buffer while a chunk is worked on
+    constexpr int RPC = 32 / CB; // rows of a copy
+    constexpr int DX = ASYNC ? TM / RPC * 1040 : (CB + 1) * BB, DS = ASYNC ? TM + 4 : TM; // the factors of x behind the blocks, their stride
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const int wk = wave % WK, wn = wave / WK;
+    const int nb = a.k >> 5, tiles = (a.n + 15) >> 4, row0 = blockIdx.y * TM;
+    const int t0 = blockIdx.x * a.kcb, t1 = min(tiles, t0 + a.kcb); // (kcb: tiles of a workgroup)
+    const int chunks = (nb + CB - 1) / CB;
+
+    // ---- x
+    const unsigned base = (unsigned) __builtin_amdgcn_readfirstlane((unsigned) (size_t) (__attribute__((address_space(3))) uint8_t *) lds);
+    constexpr int PAIRS = CB / 2 * TM, META = (PAIRS + WIDE_W * 64 - 1) / (WIDE_W * 64); // pairs of blocks whose scales a thread brings
+    uint4 meta[META];
+    const auto issue = [&](int c, int buf) { // units of chunk c on their way to LDS, their scales and sums to registers
+        const int b0 = c * CB, part = lane / CB & 1, unit = min(b0 + lane % CB, nb - 1);
+        const int8_t * src = part ? a.xb : a.xa;
+#pragma unroll 1
+        for (int k = wave; k < TM / RPC; k += WIDE_W) {
+            const int row = min(row0 + k * RPC + lane / (2 * CB), a.rows - 1);
+            dma16(src + ((size_t) row * nb + unit) * 16, base + buf * BUF + k * 1040);
+        }
+#pragma unroll
+        for (int k = 0; k < META; k++) {
+            const int i = min(tid + k * WIDE_W * 64, PAIRS - 1), m = i / (CB / 2), blk = min(b0 + i % (CB / 2) * 2, nb - 2), row = min(row0 + m, a.rows - 1);
+            const uint2 * mp = reinterpret_cast<const uint2 *>(a.xmeta) + (size_t) row * nb + blk;
+            const uint2 u0 = mp[0], u1 = mp[1];
+            meta[k] = make_uint4(u0.x, u0.y, u1.x, u1.y);
+        }
+    };
+    const auto commit = [&](int c, int buf) { // the factors of chunk c, zeros past the last block
+        float * dx = reinterpret_cast<float *>(lds + buf * BUF + DX), * ds = dx + CB * DS;
+#pragma unroll
+        for (int k = 0; k < META; k++) {
+            const int i = tid + k * WIDE_W * 64, m = i / (CB / 2), bl = i % (CB / 2) * 2;
+            if (i >= PAIRS) continue;
+            const uint4 v = meta[k];
+            const bool in = c * CB + bl < nb;
+            const float da = in ? h2f_bits((uint16_t) v.x) : 0.f, db = in ? h2f_bits((uint16_t) (v.x >> 16)) : 0.f;
+            dx[bl * DS + m] = da * 0.0625f;
+            dx[(bl + 1) * DS + m] = db * 0.0625f;
+            if constexpr (MINS) {
+                ds[bl * DS + m] = in ? da * (float) ((int) (int16_t) v.y + (int) (int16_t) v.w) : 0.f;
+                ds[(bl + 1) * DS + m] = in ? db * (float) (((int) v.y >> 16) + ((int) v.w >> 16)) : 0.f;
+            }
+        }
+    };
+
+    // ---- weights: per tile the codes of the wave's U steps of a chunk, and its scales
+    const uint8_t * cp[NTW];
+    const uint16_t * sp[NTW], * mp[NTW];
+#pragma unroll
+    for (int t = 0; t < NTW; t++) {
+        const int tile = t0 + wn + WN * t, row = min((tile < t1 ? tile : t0) * 16 + n, a.n - 1);
+        cp[t] = a.codes + (size_t) row * (a.k >> 1);
+        sp[t] = a.scales + (size_t) row * a.gs;
+        mp[t] = MINS ? a.mins + (size_t) row * a.gs : nullptr;
+    }
+    u32x4 in[NTW][U];
+    u32x4 is[NTW], im[NTW];
+    const auto load = [&](int c, int t, int u) {
+        in[t][u] = *reinterpret_cast<const u32x4 *>(cp[t] + 16 * min(c * CB + 4 * (wk * U + u) + g, nb - 1));
+    };
+    const auto load_s = [&](int c, int t) {
+        const int grp = (c * CB + 4 * wk * U) >> a.gsh;
+        is[t] = w4_scales(sp[t], a.gs, grp);
+        if constexpr (MINS) im[t] = w4_scales(mp[t], a.gs, grp);
+    };
+
+    // the scale of each block of the wave's steps from the groups'
+    const auto blocks_of = [&](u32x4 e, float (&f)[4 * U]) {
+        const auto lo = [](unsigned x) { return (x & 0xffffu) | x << 16; };
+        const auto hi = [](unsigned x) { return (x & 0xffff0000u) | x >> 16; };
+        if (a.gsh == 1) e = u32x4{lo(e[0]), hi(e[0]), lo(e[1]), hi(e[1])};
+        else if (a.gsh == 2) e = u32x4{lo(e[0]), lo(e[0]), hi(e[0]), hi(e[0])};
+#pragma unroll
+        for (int k = 0; k < 4 * U; k++) f[k] = (float) as_h2(e[k >> 1])[k & 1];
+    };
+    float acc[NTW][MT][4];
+#pragma unroll
+    for (int t = 0; t < NTW; t++)
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) acc[t][i][r] = 0.f;
+    if constexpr (ASYNC) issue(0, 0);
+#pragma unroll
+    for (int t = 0; t < NTW; t++) {
+#pragma unroll
+        for (int u = 0; u < U; u++) load(0, t, u);
+        load_s(0, t);
+    }
+    if constexpr (ASYNC) {
+        commit(0, 0);
+        vm_drain();
+        __syncthreads();
+    }
+#pragma unroll 1
+    for (int c = 0; c < chunks; c++) {
+        const int buf = ASYNC ? c & 1 : 0, cn = min(c + 1, chunks - 1);
+        if constexpr (ASYNC) issue(cn, buf ^ 1); // (past the last chunk: that one once more, unused)
+        else {
+            __syncthreads();
+            W4Args b = a;
+            b.kcb = CB;
+            w4_stage<MODE, DT, TM, WIDE_W>(b, lds, row0, c * CB, CB);
+            __syncthreads();
+        }
+        // the codes to their lane groups, the scales of each block to floats; the next chunk's take their registers
+        unsigned bt[NTW][U][4];
+        float sc[NTW][4 * U], mn[NTW][4 * U];
+#pragma unroll
+        for (int t = 0; t < NTW; t++) {
+#pragma unroll
+            for (int u = 0; u < U; u++) w4_exchange(in[t][u], bt[t][u]);
+            blocks_of(is[t], sc[t]);
+            if constexpr (MINS) blocks_of(im[t], mn[t]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < NTW; t++) {
+            load_s(cn, t);
+        }
+#pragma unroll
+        for (int t = 0; t < NTW; t++)
+#pragma unroll
+            for (int u = 0; u < U; u++) load(cn, t, u);
+        __builtin_amdgcn_sched_barrier(0);
+        const uint8_t * xp = lds + buf * BUF;
+        const float * dx = reinterpret_cast<const float *>(xp + DX), * ds = dx + CB * DS;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int bl = 4 * (wk * U + u) + q;
+                i32x2 bi[NTW];
+                half8 bh[NTW];
+#pragma unroll
+                for (int t = 0; t < NTW; t++) {
+                    if constexpr (MODE == XM_UNITS) {
+                        int lo, hi;
+                        w4_bytes(bt[t][u][q], lo, hi);
+                        bi[t] = i32x2{lo, hi};
+                    } else bh[t] = w4_halves(bt[t][u][q]);
+                }
+#pragma unroll
+                for (int i = 0; i < MT; i++) {
+                    const f32x4 d = *reinterpret_cast<const f32x4 *>(dx + bl * DS + 16 * i + 4 * g);
+                    f32x4 e;
+                    if constexpr (MINS) e = *reinterpret_cast<const f32x4 *>(ds + bl * DS + 16 * i + 4 * g);
+#pragma unroll
+                    for (int t = 0; t < NTW; t++) {
+                        f32x4 f;
+                        if constexpr (MODE == XM_UNITS) {
+                            const i32x2 x = *reinterpret_cast<const i32x2 *>(xp + (16 * i + n) / RPC * 1040 + (16 * i + n) % RPC * 512 + (bl & 1) * CB * 16 +
+                                                                              (bl & ~1) * 16 + 8 * g);
+                            i32x4 v = {0, 0, 0, 0};
+                            v = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, x), __builtin_bit_cast(long, bi[t]), v, 0, 0, 0);
+#pragma unroll
+                            for (int r = 0; r < 4; r++) f[r] = (float) v[r];
+                        } else {
+                            f = f32x4{0, 0, 0, 0};
+#pragma unroll
+                            for (int k = planes(MODE) - 4; k >= 0; k -= 4)
+                                f = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const half8 *>(xp + bl * BB + ((k + g) * TM + 16 * i + n) * 16),
+                                                                           bh[t], f, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            acc[t][i][r] = __builtin_fmaf(f[r], sc[t][4 * u + q] * d[r], acc[t][i][r]);
+                            if constexpr (MINS) acc[t][i][r] = __builtin_fmaf(mn[t][4 * u + q], e[r], acc[t][i][r]);
+                        }
+                    }
+                }
+                // (a block at a time: the compiler would fold the chunk's sums at its end, and they do not fit the registers)
+#pragma unroll
+                for (int t = 0; t < NTW; t++)
+#pragma unroll
+                    for (int i = 0; i < MT; i++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) asm volatile("" : "+v"(acc[t][i][r]));
+            }
+        if constexpr (ASYNC) {
+            commit(cn, buf ^ 1);
+            // the copies of x have landed: the U codes of NTW tiles behind them may still be on their way
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NTW * U) : "memory");
+            __syncthreads();
+        }
+    }
+    // the waves along the blocks, a tile of every wave at a time
+    if constexpr (!ASYNC) __syncthreads();
+    float * red = reinterpret_cast<float *>(lds); // [waves][TM][16]
+#pragma unroll
+    for (int t = 0; t < NTW; t++) {
+        if (t) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) red[(wave * TM + 16 * i + 4 * g + r) * 16 + n] = acc[t][i][r];
+        __syncthreads();
+        for (int i = tid; i < WN * TM * 16; i += WIDE_W * 64) {
+            const int c = i & 15, m = (i >> 4) % TM, w = (i >> 4) / TM, tile = t0 + w + WN * t, col = tile * 16 + c;
+            const float * rp = red + (w * WK * TM + m) * 16 + c;
+            float v = rp[0];
+#pragma unroll
+            for (int k = 1; k < WK; k++) v += rp[k * TM * 16];
+            if (tile < t1 && col < a.n && row0 + m < a.rows) a.y[(long long) (row0 + m) * a.y_stride + col] = v;
+        }
+    }
+}
+
+constexpr int W4_LDS = 64 * 1024;
+constexpr int W4_WAVES = 4096; // of a launch: 16 for each of 256 CUs, a quarter of what they hold
+
+template <int MODE, int DT, int NR, int RG, int P, int W>
 static hipError_t launch_k(W4Args a, hipStream_t st) {
-    constexpr int MR = NR * RG, per = planes(MODE) * MR * 16 + 2 * MR * 4;
-    const int nb4 = (a.k / 32 + 3) & ~3, tiles = (a.n + 15) / 16;
-    const int red = 2 * W4_WAVES * MR * 16 * 4, zero = planes(MODE) * MR * 16;
-    a.kcb = std::min(nb4, ((W4_LDS - red - zero) / per) & ~3);
-    while (a.wk_log < 3 && (tiles << a.wk_log) < 2048) a.wk_log++;
-    const int wn = W4_WAVES >> a.wk_log, sets = (tiles + wn - 1) / wn;
+    constexpr int MR = NR * RG, per = planes(MODE) * MR * 16 + 2 * MR * 4, TR = 16 / P;
+    constexpr int PAD = 4 * W4_RUN;
+    const int nb4 = (a.k / 32 + PAD * P - 1) / (PAD * P) * (PAD * P), tiles = (a.n + TR - 1) / TR;
+    const int red = 2 * W * MR * TR * 4 + W * (a.mins ? 2 : 1) * 16 * W4_WIN * 2, zero = planes(MODE) * MR * 16; // (with the windows of scales)
+    a.kcb = std::min(nb4, (W4_LDS - red - zero) / per / PAD * PAD);
+    if constexpr (P > 1) {
+        if (a.kcb < nb4) return launch_k<MODE, DT, 4, (MR + 3) / 4, 1, 8>(a, st); // (x in pieces)
+    }
+    // (every wave has a run of the first chunk)
+    while ((1 << a.wk_log) < W && (tiles << a.wk_log) < W4_WAVES / 2 && a.kcb / P / PAD >= 2 << a.wk_log) a.wk_log++;
+    const int wn = W >> a.wk_log, sets = (tiles + wn - 1) / wn;
     const size_t lds = (size_t) a.kcb * per + zero + red;
-    hipLaunchKernelGGL((k_w4<MODE, DT, NR, RG>), dim3(std::min(sets, 512), (a.rows + MR - 1) / MR), dim3(W4_WAVES * 64), lds, st, a);
+    const dim3 grid(std::min(sets, W4_WAVES / W), (a.rows + MR - 1) / MR), block(W * 64);
+    if (a.mins) hipLaunchKernelGGL((k_w4<MODE, DT, NR, RG, P, W, true>), grid, block, lds, st, a);
+    else hipLaunchKernelGGL((k_w4<MODE, DT, NR, RG, P, W, false>), grid, block, lds, st, a);
     return hipGetLastError();
+}
+
+template <int MODE, int DT, int MT, int NTW, int WK, int U, bool MINS>
+static hipError_t launch_wide_k(const W4Args & a, dim3 grid, hipStream_t st) {
+    constexpr int lds = std::max((MODE == XM_UNITS ? 2 : 1) * wide_buf<MODE, MT, 4 * WK * U, MINS>(), WIDE_W * 16 * MT * 16 * 4);
+    static_assert(lds <= 160 * 1024, "a workgroup's LDS");
+    const auto k = k_w4_wide<MODE, DT, MT, NTW, WK, U, MINS>;
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(k, grid, dim3(WIDE_W * 64), lds, st, a);
+    return hipGetLastError();
+}
+template <int MODE, int DT, int MT, int U, bool MINS>
+static hipError_t launch_wide_m(W4Args a, hipStream_t st) {
+    // a workgroup per CU: as few rounds of at most 2 * 3 tiles each as there are, of the same number of tiles
+    constexpr int CUS = 256, MOST = 6;
+    const int tiles = (a.n + 15) / 16, rounds = (tiles + CUS * MOST - 1) / (CUS * MOST);
+    a.kcb = (tiles + CUS * rounds - 1) / (CUS * rounds);
+    const dim3 grid((tiles + a.kcb - 1) / a.kcb, (a.rows + 16 * MT - 1) / (16 * MT));
+    if constexpr (U == 2) {
+        if (a.kcb == 1) return launch_wide_k<MODE, DT, MT, 1, 8, 1, MINS>(a, grid, st);
+    }
+    if (a.kcb <= 2) return launch_wide_k<MODE, DT, MT, 1, 4, U, MINS>(a, grid, st);
+    if (a.kcb <= 4) return launch_wide_k<MODE, DT, MT, 2, 4, U, MINS>(a, grid, st);
+    return launch_wide_k<MODE, DT, MT, 3, 4, U, MINS>(a, grid, st);
+}
+template <int MODE, int DT>
+static hipError_t launch_wide(const W4Args & a, hipStream_t st) {
+    if constexpr (MODE == XM_UNITS) {
+        if (a.rows <= 16) return a.mins ? launch_wide_m<MODE, DT, 1, 2, true>(a, st) : launch_wide_m<MODE, DT, 1, 2, false>(a, st);
+        if (a.rows <= 32) return a.mins ? launch_wide_m<MODE, DT, 2, 2, true>(a, st) : launch_wide_m<MODE, DT, 2, 2, false>(a, st);
+        return a.mins ? launch_wide_m<MODE, DT, 4, 1, true>(a, st) : launch_wide_m<MODE, DT, 4, 2, false>(a, st);
+    } else {
+        if (a.rows <= 16) return a.mins ? launch_wide_m<MODE, DT, 1, 1, true>(a, st) : launch_wide_m<MODE, DT, 1, 1, false>(a, st);
+        return a.mins ? launch_wide_m<MODE, DT, 2, 1, true>(a, st) : launch_wide_m<MODE, DT, 2, 1, false>(a, st);
+    }
 }
 
 template <int MODE, int DT>
 static hipError_t launch_mode(const W4Args & a, hipStream_t st) {
-    if (a.rows == 1) return launch_k<MODE, DT, 1, 1>(a, st);
-    if (a.rows == 2) return launch_k<MODE, DT, 2, 1>(a, st);
-    if (a.rows <= 4) return launch_k<MODE, DT, 4, 1>(a, st);
-    if (a.rows <= 8) return launch_k<MODE, DT, 4, 2>(a, st);
-    return launch_k<MODE, DT, 4, 4>(a, st);
+    if (a.rows == 1) return launch_k<MODE, DT, 1, 1, 4, 4>(a, st);
+    if (a.rows == 2) return launch_k<MODE, DT, 2, 1, 2, 4>(a, st);
+    if (a.rows <= 4) return launch_k<MODE, DT, 4, 1, 1, 8>(a, st);
+    if (a.rows <= 8) return launch_k<MODE, DT, 4, 2, 1, 8>(a, st);
+#ifdef W4_NOWIDE
+    return launch_k<MODE, DT, 4, 4, 1, 8>(a, st);
+#else
+    return launch_wide<MODE, DT>(a, st);
+#endif
 }
 
 hipError_t launch_w4(const W4Args & a, int xform, hipStream_t st) {
