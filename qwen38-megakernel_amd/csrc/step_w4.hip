@@ -362,8 +362,6 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
 // row's scale of each block.  A workgroup takes up to 2 NTW tiles: 4 waves along the blocks of a chunk (U steps each) times 2
 // along the tiles; a piece of x read from LDS serves the wave's NTW tiles.  What bounds it is the fold of the blocks'
 // integer sums into fp32: three instructions per (row, block, weight row).
-constexpr int WIDE_W = 8; // waves
-
 __device__ __forceinline__ void w4_exchange(const u32x4 & d, unsigned (&t)[4]) { // t[b] in lane group q: dword q of lane group b's d
     const auto x = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false), y = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
     const auto v = __builtin_amdgcn_permlane16_swap(x[0], y[0], false, false), w = __builtin_amdgcn_permlane16_swap(x[1], y[1], false, false);
@@ -378,10 +376,12 @@ template <int MODE, int MT, int CB, bool MINS> constexpr int wide_buf() {
     return MODE == XM_UNITS ? CB * 2 * TM / 64 * 1040 + (MINS ? 2 : 1) * CB * (TM + 4) * 4 : (CB + 1) * planes(MODE) * TM * 16 + 2 * CB * TM * 4;
 }
 
-// WK waves along the blocks of a chunk, U steps each, the others along the tiles
-template <int MODE, int DT, int MT, int NTW, int WK, int U, bool MINS>
-__global__ __launch_bounds__(WIDE_W * 64, 2) void k_w4_wide(W4Args a) {
-    constexpr int TM = 16 * MT, WN = WIDE_W / WK, CB = 4 * WK * U, BB = planes(MODE) * TM * 16, BUF = wide_buf<MODE, MT, CB, MINS>();
+// WK waves along the blocks of a chunk, U steps each, times WN along the tiles.  ODD: a workgroup of an odd number of tiles,
+// whose second half of the waves has one less (an even number needs no branch: 64 rows of 14,336 x 5,120, 30.7 us, with it
+// 32.7; 17,408, five tiles a workgroup: 41.3 without and 37.9 with)
+template <int MODE, int DT, int MT, int NTW, int WK, int WN, int U, bool ODD, bool MINS>
+__global__ __launch_bounds__(WK * WN * 64, WK * WN / 4) void k_w4_wide(W4Args a) {
+    constexpr int WIDE_W = WK * WN, TM = 16 * MT, CB = 4 * WK * U, BB = planes(MODE) * TM * 16, BUF = wide_buf<MODE, MT, CB, MINS>();
     constexpr bool ASYNC = MODE == XM_UNITS; // x copied into the other buffer while a chunk is worked on
     constexpr int RPC = 32 / CB; // rows of a copy
     constexpr int DX = ASYNC ? TM / RPC * 1040 : (CB + 1) * BB, DS = ASYNC ? TM + 4 : TM; // the factors of x behind the blocks, their stride
@@ -440,6 +440,7 @@ __global__ __launch_bounds__(WIDE_W * 64, 2) void k_w4_wide(W4Args a) {
         sp[t] = a.scales + (size_t) row * a.gs;
         mp[t] = MINS ? a.mins + (size_t) row * a.gs : nullptr;
     }
+    const bool last = t0 + wn + WN * (NTW - 1) < t1;
     u32x4 in[NTW][U];
     u32x4 is[NTW], im[NTW];
     const auto load = [&](int c, int t, int u) {
@@ -529,17 +530,20 @@ __global__ __launch_bounds__(WIDE_W * 64, 2) void k_w4_wide(W4Args a) {
                 }
 #pragma unroll
                 for (int i = 0; i < MT; i++) {
-                    const f32x4 d = *reinterpret_cast<const f32x4 *>(dx + bl * DS + 16 * i + 4 * g);
-                    f32x4 e;
+                    // 16 rows of x and their factors, for every tile of the wave
+                    f32x4 d = *reinterpret_cast<const f32x4 *>(dx + bl * DS + 16 * i + 4 * g), e;
                     if constexpr (MINS) e = *reinterpret_cast<const f32x4 *>(ds + bl * DS + 16 * i + 4 * g);
+                    i32x2 xi;
+                    if constexpr (MODE == XM_UNITS)
+                        xi = *reinterpret_cast<const i32x2 *>(xp + (16 * i + n) / RPC * 1040 + (16 * i + n) % RPC * 512 + (bl & 1) * CB * 16 +
+                                                              (bl & ~1) * 16 + 8 * g);
 #pragma unroll
                     for (int t = 0; t < NTW; t++) {
+                        if (ODD && t == NTW - 1 && !last) break; // (this wave has a tile less)
                         f32x4 f;
                         if constexpr (MODE == XM_UNITS) {
-                            const i32x2 x = *reinterpret_cast<const i32x2 *>(xp + (16 * i + n) / RPC * 1040 + (16 * i + n) % RPC * 512 + (bl & 1) * CB * 16 +
-                                                                              (bl & ~1) * 16 + 8 * g);
                             i32x4 v = {0, 0, 0, 0};
-                            v = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, x), __builtin_bit_cast(long, bi[t]), v, 0, 0, 0);
+                            v = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, xi), __builtin_bit_cast(long, bi[t]), v, 0, 0, 0);
 #pragma unroll
                             for (int r = 0; r < 4; r++) f[r] = (float) v[r];
                         } else {
@@ -616,11 +620,12 @@ static hipError_t launch_k(W4Args a, hipStream_t st) {
     return hipGetLastError();
 }
 
-template <int MODE, int DT, int MT, int NTW, int WK, int U, bool MINS>
+template <int MODE, int DT, int MT, int NTW, int WK, int WN, int U, bool ODD, bool MINS>
 static hipError_t launch_wide_k(const W4Args & a, dim3 grid, hipStream_t st) {
+    constexpr int WIDE_W = WK * WN;
     constexpr int lds = std::max((MODE == XM_UNITS ? 2 : 1) * wide_buf<MODE, MT, 4 * WK * U, MINS>(), WIDE_W * 16 * MT * 16 * 4);
     static_assert(lds <= 160 * 1024, "a workgroup's LDS");
-    const auto k = k_w4_wide<MODE, DT, MT, NTW, WK, U, MINS>;
+    const auto k = k_w4_wide<MODE, DT, MT, NTW, WK, WN, U, ODD, MINS>;
     if (lds > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
@@ -636,11 +641,16 @@ static hipError_t launch_wide_m(W4Args a, hipStream_t st) {
     a.kcb = (tiles + CUS * rounds - 1) / (CUS * rounds);
     const dim3 grid((tiles + a.kcb - 1) / a.kcb, (a.rows + 16 * MT - 1) / (16 * MT));
     if constexpr (U == 2) {
-        if (a.kcb == 1) return launch_wide_k<MODE, DT, MT, 1, 8, 1, MINS>(a, grid, st);
+        if (a.kcb == 1) return launch_wide_k<MODE, DT, MT, 1, 8, 1, 1, false, MINS>(a, grid, st);
     }
-    if (a.kcb <= 2) return launch_wide_k<MODE, DT, MT, 1, 4, U, MINS>(a, grid, st);
-    if (a.kcb <= 4) return launch_wide_k<MODE, DT, MT, 2, 4, U, MINS>(a, grid, st);
-    return launch_wide_k<MODE, DT, MT, 3, 4, U, MINS>(a, grid, st);
+    switch (a.kcb) {
+    case 1:
+    case 2: return launch_wide_k<MODE, DT, MT, 1, 4, 2, U, false, MINS>(a, grid, st);
+    case 3: return launch_wide_k<MODE, DT, MT, 2, 4, 2, U, true, MINS>(a, grid, st);
+    case 4: return launch_wide_k<MODE, DT, MT, 2, 4, 2, U, false, MINS>(a, grid, st);
+    case 5: return launch_wide_k<MODE, DT, MT, 3, 4, 2, U, true, MINS>(a, grid, st);
+    default: return launch_wide_k<MODE, DT, MT, 3, 4, 2, U, false, MINS>(a, grid, st);
+    }
 }
 template <int MODE, int DT>
 static hipError_t launch_wide(const W4Args & a, hipStream_t st) {
