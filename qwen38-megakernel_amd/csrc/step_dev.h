@@ -91,6 +91,9 @@ template <int DT> __device__ __forceinline__ void store_n(typename Elem<DT>::T *
         if (i < n) p[i] = Elem<DT>::down(v[i]);
 }
 
+// a workgroup barrier for LDS data only: __syncthreads() also waits for the wave's loads and stores in flight
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 __device__ __forceinline__ double shfl_xor_d(double v, int m) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
     const unsigned lo = shfl_xor_u((unsigned) b, m), hi = shfl_xor_u((unsigned) (b >> 32), m);

@@ -14,102 +14,106 @@ namespace qkv {
 // a block whose largest value is below this has no finite 127 / a: its codes and scale are zero
 constexpr float NORM_TINY = 4e-37f;
 
-// One workgroup of NT threads per row; thread t holds the chunks t, t + NT, .. (C of them) of 8 values, so a block of 32
-// is four neighbouring lanes.
-template <int DT, int NT, int C>
-__global__ __launch_bounds__(NT) void k_norm(NormArgs a) {
+// A workgroup per row; thread t holds the chunks t, t + NT, .. (C of them) of 8 values, so a block of 32 is four
+// neighbouring lanes.
+template <int DT, int C>
+__global__ __launch_bounds__(1024) void k_norm(NormArgs a) {
     using E = Elem<DT>;
     using T = typename E::T;
-    __shared__ double red[2][NT / 64];
-    const int tid = threadIdx.x, wave = tid >> 6;
+    __shared__ double red[16];
+    const int tid = threadIdx.x, wave = tid >> 6, NT = blockDim.x;
     const int nu = a.dim >> 5;
-    int par = 0;
-    for (int row = blockIdx.x; row < a.rows; row += gridDim.x, par ^= 1) {
-        const T * x = static_cast<const T *>(a.x) + (long long) row * a.x_stride;
-        const T * r = a.res ? static_cast<const T *>(a.res) + (long long) row * a.res_stride : nullptr;
-        float h[C][8];
-        double s = 0;
+    int j[C], n[C]; // the chunks' first values and how many of the 8 exist
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-            const int j = 8 * (tid + NT * c), n = min(8, a.dim - j);
+    for (int c = 0; c < C; c++) {
+        j[c] = 8 * (tid + NT * c);
+        n[c] = max(0, min(8, a.dim - j[c]));
+    }
+    const int row = blockIdx.x;
+    const T * xp = static_cast<const T *>(a.x) + (long long) row * a.x_stride;
+    const T * rp = static_cast<const T *>(a.res) + (long long) row * a.res_stride;
+    float h[C][8], r[C][8], w[C][8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) h[c][i] = 0.f;
-            if (n <= 0) continue;
-            load_n<DT>(x + j, n, h[c]);
-            if (r) {
-                float q[8];
-                load_n<DT>(r + j, n, q);
+    for (int c = 0; c < C; c++) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) h[c][i] = E::up(E::down(h[c][i] + q[i]));
-            }
+        for (int i = 0; i < 8; i++) h[c][i] = 0.f;
+        if (n[c] <= 0) continue;
+        load_n<DT>(xp + j[c], n[c], h[c]);
+        if (a.res) load_n<DT>(rp + j[c], n[c], r[c]);
+        load_n<DT_F32>(a.w + j[c], n[c], w[c]);
+    }
+    double s = 0;
+    if (a.res) {
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) h[c][i] = n[c] > 0 ? E::up(E::down(h[c][i] + r[c][i])) : 0.f;
+    }
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        if (a.sum && n[c] > 0) store_n<DT>(static_cast<T *>(a.sum) + (long long) row * a.sum_stride + j[c], n[c], h[c]);
+#pragma unroll
+        for (int i = 0; i < 8; i++) s = __builtin_fma((double) h[c][i], (double) h[c][i], s);
+    }
+    s = wave_sum(s);
+    if ((tid & 63) == 0) red[wave] = s;
+    lds_barrier();
+    s = red[0];
+    for (int i = 1; i < NT / 64; i++) s += red[i];
+    const float rs = (float) (1.0 / __builtin_sqrt(s / a.dim + (double) a.eps));
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        const int ch = tid + NT * c;
+        if (n[c] <= 0) continue; // (units: dim is a multiple of 64, so whole blocks of four lanes leave)
+        if (a.y) {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] = (h[c][i] * rs) * w[c][i];
+            store_n<DT>(static_cast<T *>(a.y) + (long long) row * a.y_stride + j[c], n[c], y);
         }
+        if (a.a) {
+            float t[8], am = 0.f;
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-            const int j = 8 * (tid + NT * c), n = min(8, a.dim - j);
-            if (a.sum && n > 0) store_n<DT>(static_cast<T *>(a.sum) + (long long) row * a.sum_stride + j, n, h[c]);
-#pragma unroll
-            for (int i = 0; i < 8; i++) s = __builtin_fma((double) h[c][i], (double) h[c][i], s);
-        }
-        s = wave_sum(s);
-        if ((tid & 63) == 0) red[par][wave] = s;
-        __syncthreads(); // (the other parity's slots are not written again before every wave has passed this barrier)
-        s = red[par][0];
-#pragma unroll
-        for (int i = 1; i < NT / 64; i++) s += red[par][i];
-        const float rs = (float) (1.0 / __builtin_sqrt(s / a.dim + (double) a.eps));
-#pragma unroll
-        for (int c = 0; c < C; c++) {
-            const int ch = tid + NT * c, j = 8 * ch, n = min(8, a.dim - j);
-            if (n <= 0) continue; // (units: dim is a multiple of 64, so whole blocks of four lanes leave)
-            float w[8];
-            load_n<DT_F32>(a.w + j, n, w);
-            if (a.y) {
-                float y[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) y[i] = (h[c][i] * rs) * w[i];
-                store_n<DT>(static_cast<T *>(a.y) + (long long) row * a.y_stride + j, n, y);
+            for (int i = 0; i < 8; i++) {
+                t[i] = h[c][i] * w[c][i];
+                am = fmaxf(am, fabsf(t[i]));
             }
-            if (a.a) {
-                float t[8], am = 0.f;
+            am = fmaxf(am, shfl_xor(am, 1));
+            am = fmaxf(am, shfl_xor(am, 2));
+            const float id = am < NORM_TINY ? 0.f : 127.0f / am;
+            int sum = 0;
+            unsigned q[2] = {0, 0};
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    t[i] = h[c][i] * w[i];
-                    am = fmaxf(am, fabsf(t[i]));
-                }
-                am = fmaxf(am, shfl_xor(am, 1));
-                am = fmaxf(am, shfl_xor(am, 2));
-                const float id = am < NORM_TINY ? 0.f : 127.0f / am;
-                int sum = 0;
-                unsigned q[2] = {0, 0};
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int v = f2i_rn(t[i] * id);
-                    sum += v;
-                    q[i >> 2] |= ((unsigned) v & 0xffu) << (8 * (i & 3));
-                }
-                sum += (int) shfl_xor_u((unsigned) sum, 1); // the half of 16 values
-                const unsigned sc = f2h_bits(am < NORM_TINY ? am * 0.f * rs : am * (rs / 127.0f));
-                const int blk = ch >> 2, part = blk & 1, gi = 2 * (blk >> 1) + ((ch >> 1) & 1);
-                const long long u = (long long) row * nu + gi;
-                *reinterpret_cast<uint2 *>((part ? a.b : a.a) + u * 16 + 8 * (ch & 1)) = make_uint2(q[0], q[1]);
-                // meta: scale of the even / odd block, sum of the even / odd half (the odd block is four lanes away)
-                const unsigned mine = sc | (unsigned) sum << 16, other = shfl_xor_u(mine, 4);
-                if (!(ch & 5))
-                    *reinterpret_cast<uint2 *>(a.meta + u * 4) = make_uint2((mine & 0xffffu) | other << 16, mine >> 16 | (other & 0xffff0000u));
+            for (int i = 0; i < 8; i++) {
+                const int v = f2i_rn(t[i] * id);
+                sum += v;
+                q[i >> 2] |= ((unsigned) v & 0xffu) << (8 * (i & 3));
             }
+            sum += (int) shfl_xor_u((unsigned) sum, 1); // the half of 16 values
+            const unsigned sc = f2h_bits(am < NORM_TINY ? am * 0.f * rs : am * (rs / 127.0f));
+            const int blk = ch >> 2, part = blk & 1, gi = 2 * (blk >> 1) + ((ch >> 1) & 1);
+            const long long u = (long long) row * nu + gi;
+            *reinterpret_cast<uint2 *>((part ? a.b : a.a) + u * 16 + 8 * (ch & 1)) = make_uint2(q[0], q[1]);
+            // meta: scale of the even / odd block, sum of the even / odd half (the odd block is four lanes away)
+            const unsigned mine = sc | (unsigned) sum << 16, other = shfl_xor_u(mine, 4);
+            if (!(ch & 5))
+                *reinterpret_cast<uint2 *>(a.meta + u * 4) = make_uint2((mine & 0xffffu) | other << 16, mine >> 16 | (other & 0xffff0000u));
         }
     }
 }
 
+// Chunks per thread: one for few rows, whose time is the row's chain of load, sum and store (1 row of 5,120: 3.1 us, with
+// four 5.2; 32 rows 4.7 and 7.0), two for many, which leave room for more rows per CU (4,096 rows of bf16, residual and units:
+// 37 us or 4.0 TB/s of what has to move, with one 40, with four 44; persistent workgroups that read the next row ahead 47 to
+// 62: their registers leave half the waves), four only where two are not enough for 1,024 threads.
+constexpr int NORM_FEW = 512;
 template <int DT>
 static hipError_t launch_dt(const NormArgs & a, hipStream_t st) {
     const int chunks = (a.dim + 7) / 8;
-    const dim3 grid(a.rows);
-    if (chunks <= 256) hipLaunchKernelGGL((k_norm<DT, 256, 1>), grid, dim3(256), 0, st, a);
-    else if (chunks <= 512) hipLaunchKernelGGL((k_norm<DT, 256, 2>), grid, dim3(256), 0, st, a);
-    else if (chunks <= 1024) hipLaunchKernelGGL((k_norm<DT, 256, 4>), grid, dim3(256), 0, st, a);
-    else if (chunks <= 2048) hipLaunchKernelGGL((k_norm<DT, 1024, 2>), grid, dim3(1024), 0, st, a);
-    else hipLaunchKernelGGL((k_norm<DT, 1024, 4>), grid, dim3(1024), 0, st, a);
+    const auto nt = [&](int c) { return dim3((chunks + 64 * c - 1) / (64 * c) * 64); };
+    if (chunks <= 1024 && a.rows <= NORM_FEW) hipLaunchKernelGGL((k_norm<DT, 1>), dim3(a.rows), nt(1), 0, st, a);
+    else if (chunks <= 2048) hipLaunchKernelGGL((k_norm<DT, 2>), dim3(a.rows), nt(2), 0, st, a);
+    else hipLaunchKernelGGL((k_norm<DT, 4>), dim3(a.rows), nt(4), 0, st, a);
     return hipGetLastError();
 }
 
