@@ -263,6 +263,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
                 if (fresh) { // (the run's window: nx stands on this run)
                     *reinterpret_cast<u32x4 *>(win + n * W4_WIN + 8 * g) = ws;
                     if constexpr (MINS) *reinterpret_cast<u32x4 *>(win + 16 * W4_WIN + n * W4_WIN + 8 * g) = wm;
+                    asm volatile("" ::: "memory"); // (read below by other lanes and as another type)
                     sw = s;
                 }
                 advance();
