@@ -84,11 +84,11 @@ __global__ __launch_bounds__(VT) void k_verify_rows(VerifyArgs a) {
     // the slice of a draft that may be refused: also its sum without the draft, what is left over without q
     const int d = !a.q && i < a.n ? a.drafts[b * a.n + i] : -1;
     float m = -__builtin_inff();
-    bool wild = false;
+    bool wild = false; // a NaN (a maximum leaves it out)
 #pragma unroll
-    for (int k = 0; k < VE; k++) {
-        wild |= !(v[k] < __builtin_inff()); // +infinity or NaN
-        m = fmaxf(m, v[k]);
+    for (int k = 0; k < VE; k += 2) {
+        wild |= __builtin_isunordered(v[k], v[k + 1]);
+        m = fmaxf(fmaxf(m, v[k]), v[k + 1]);
     }
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, shfl_xor(m, x));
@@ -102,6 +102,7 @@ __global__ __launch_bounds__(VT) void k_verify_rows(VerifyArgs a) {
         m = fmaxf(m, top[k]);
         wild |= bad[k] != 0;
     }
+    wild |= m == __builtin_inff();
     VerifyPart p{0.0, PROBS ? 0.f : m, 0};
     if (wild) p.top = __builtin_nanf("");
     else if (!PROBS && t.greedy) {
@@ -118,18 +119,22 @@ __global__ __launch_bounds__(VT) void k_verify_rows(VerifyArgs a) {
         p.sum = m > -__builtin_inff() ? 1.0 : 0.0;
     } else {
         const bool holds = d >= 0 && d / VERIFY_SLICE == sl && d < a.vocab;
-        double s = 0, rest = 0;
-        if (PROBS || m > -__builtin_inff()) {
+        double s = 0;
+        if (holds) { // (on its own: the selects cost every slice a quarter more)
+            double rest = 0;
+            if (PROBS || m > -__builtin_inff()) {
 #pragma unroll
-            for (int k = 0; k < VE; k++) {
-                const double w = weight<PROBS>(v[k], m, t.beta);
-                s += w;
-                if (holds && at(k) != d) rest += w;
+                for (int k = 0; k < VE; k++) {
+                    const double w = weight<PROBS>(v[k], m, t.beta);
+                    s += w;
+                    rest += at(k) != d ? w : 0.0;
+                }
             }
-        }
-        if (holds) {
             rest = wave_sum(rest);
             if (lane == 0) rests[wave] = rest;
+        } else if (PROBS || m > -__builtin_inff()) {
+#pragma unroll
+            for (int k = 0; k < VE; k++) s += weight<PROBS>(v[k], m, t.beta);
         }
         s = wave_sum(s);
         if (lane == 0) sums[wave] = s;
@@ -138,7 +143,7 @@ __global__ __launch_bounds__(VT) void k_verify_rows(VerifyArgs a) {
 #pragma unroll
         for (int k = 1; k < VT / 64; k++) p.sum += sums[k];
         if (holds && threadIdx.x == 0) {
-            rest = rests[0];
+            double rest = rests[0];
             for (int k = 1; k < VT / 64; k++) rest += rests[k];
             a.rest[row] = rest;
         }
