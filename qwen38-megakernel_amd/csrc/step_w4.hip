@@ -11,12 +11,15 @@
 #include "step_dev.h"
 
 #include <algorithm>
+#include <atomic>
 
 namespace qkv {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4_u8 __attribute__((ext_vector_type(4), aligned(8)));
+typedef unsigned u32x4_u2 __attribute__((ext_vector_type(4), aligned(2)));
 
 
 enum { XM_UNITS = 0, XM_HALF = 1, XM_SPLIT = 2 }; // x as int8 units, as one fp16 part, as two
@@ -24,9 +27,22 @@ enum { XM_UNITS = 0, XM_HALF = 1, XM_SPLIT = 2 }; // x as int8 units, as one fp1
 // 16-byte planes per block of 32 values in LDS
 constexpr int planes(int mode) { return mode == XM_UNITS ? 2 : mode == XM_HALF ? 4 : 8; }
 
-// LDS: [kcb blocks][planes][MR rows][16 bytes], a zero region of one block's size, then [kcb][MR] float factors of the
-// blocks' sums and [kcb][MR] float factors of m
-template <int MODE, int MR> __device__ __forceinline__ constexpr int blk_bytes() { return planes(MODE) * MR * 16; }
+// x in LDS, kcb blocks at a time.  Units, as they come: per row the even blocks' kcb units, then the odd ones', padded so that the
+// 16 pieces an instruction takes (4 blocks of 4 rows) lie in different banks.  Plain rows, as fp16:
+// [kcb blocks][planes][MR rows][16 bytes].  Then zeros for the operand's other lanes, [kcb][MR] float factors of the blocks'
+// sums and (with m) [kcb][MR] float factors of m.
+struct W4Lds {
+    int half, row, zero, dx, end; // units: bytes of a row's even blocks, of a row; offsets of the zeros, the factors, what follows
+};
+template <int MODE, int MR, bool MINS> __host__ __device__ __forceinline__ constexpr W4Lds w4_lds(int kcb) {
+    W4Lds l{};
+    l.half = ((kcb * 16 + 255) & ~255) + 16;
+    l.row = 2 * l.half + 32;
+    l.zero = MODE == XM_UNITS ? MR * l.row : kcb * planes(MODE) * MR * 16;
+    l.dx = l.zero + (MODE == XM_UNITS ? 32 : planes(MODE) * MR * 16);
+    l.end = (l.dx + (MINS ? 2 : 1) * kcb * MR * 4 + 15) & ~15;
+    return l;
+}
 
 // 16 bytes per lane from its own address to LDS at lds + 16 lane, without a register (waited for with vm_drain)
 __device__ __forceinline__ void dma16(const void * g, unsigned lds) {
@@ -36,33 +52,50 @@ __device__ __forceinline__ void dma16(const void * g, unsigned lds) {
 __device__ __forceinline__ void vm_drain() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // x of blocks b0 .. b0 + nblk - 1 (nblk a multiple of 4) into LDS; blocks past the last one get factors of zero
-template <int MODE, int DT, int MR, int W>
+template <int MODE, int DT, int MR, int W, bool MINS>
 __device__ __forceinline__ void w4_stage(const W4Args & a, uint8_t * lds, int row0, int b0, int nblk) {
-    constexpr int BB = blk_bytes<MODE, MR>();
+    constexpr int BB = planes(MODE) * MR * 16;
+    const W4Lds L = w4_lds<MODE, MR, MINS>(a.kcb);
     const int nb = a.k >> 5, tid = threadIdx.x;
-    float * dx = reinterpret_cast<float *>(lds + (size_t) (a.kcb + 1) * BB), * ds = dx + a.kcb * MR;
-    for (int i = tid; i < BB / 16; i += W * 64) reinterpret_cast<uint4 *>(lds + (size_t) a.kcb * BB)[i] = make_uint4(0, 0, 0, 0);
+    float * dx = reinterpret_cast<float *>(lds + L.dx), * ds = dx + a.kcb * MR;
+    for (int i = tid; i < (L.dx - L.zero) / 16; i += W * 64) reinterpret_cast<uint4 *>(lds + L.zero)[i] = make_uint4(0, 0, 0, 0);
     if constexpr (MODE == XM_UNITS) {
-        // (block, half, row) pieces of 16 bytes, 64 a copy; rows past the last one repeat it (their sums are dropped)
         const unsigned base = (unsigned) __builtin_amdgcn_readfirstlane((unsigned) (size_t) (__attribute__((address_space(3))) uint8_t *) lds);
-        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, pieces = nblk * 2 * MR;
-        for (int i0 = wave * 64; i0 < pieces; i0 += W * 64) {
-            const int i = i0 + lane;
-            const int m = i % MR, half = (i / MR) & 1, blk = min(b0 + i / (2 * MR), nb - 1), row = min(row0 + m, a.rows - 1);
-            if (i < pieces) dma16(((blk & 1) ? a.xb : a.xa) + ((size_t) row * nb + (blk & ~1) + half) * 16, base + i0 * 16);
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, np = nblk >> 1;
+        // a pair of blocks' scales and sums per lane, two units of {scale a, scale b, sum a, sum b}: a wave has one row's; all
+        // loads ahead of the copies, and one wait for both
+        static_assert(W % MR == 0, "waves per row");
+        constexpr int STEP = 64 * (W / MR), NI = 2;
+        const int m = wave % MR, mrow = min(row0 + m, a.rows - 1), p0 = lane + 64 * (wave / MR);
+        u32x4 mt[NI];
+        const auto load = [&](int p) {
+            return *reinterpret_cast<const u32x4_u8 *>(a.xmeta + ((size_t) mrow * nb + min(b0 + 2 * p, nb - 2)) * 4); // (nb is even)
+        };
+        const auto store = [&](int p, u32x4 v) {
+            const bool in = b0 + 2 * p < nb;
+            const float da = in ? h2f_bits((uint16_t) v[0]) : 0.f, db = in ? h2f_bits((uint16_t) (v[0] >> 16)) : 0.f;
+            dx[2 * p * MR + m] = da * 0.0625f; // (the codes go in 16 times as large)
+            dx[(2 * p + 1) * MR + m] = db * 0.0625f;
+            if (MINS) {
+                ds[2 * p * MR + m] = da * (float) ((int) (int16_t) v[1] + (int) (int16_t) v[3]);
+                ds[(2 * p + 1) * MR + m] = db * (float) (((int) v[1] >> 16) + ((int) v[3] >> 16));
+            }
+        };
+#pragma unroll
+        for (int u = 0; u < NI; u++) mt[u] = load(min(p0 + u * STEP, np - 1));
+        // 64 units of a row's even or odd blocks a copy; rows past the last one repeat it (their sums are dropped)
+        const int per = (nblk + 63) >> 6; // copies of a half
+#pragma unroll 1
+        for (int c = wave; c < MR * 2 * per; c += W) {
+            const int h = c / per, u0 = (c - h * per) * 64, row = min(row0 + (h >> 1), a.rows - 1);
+            if (u0 + lane < nblk)
+                dma16(((h & 1) ? a.xb : a.xa) + ((size_t) row * nb + min(b0 + u0 + lane, nb - 1)) * 16,
+                      base + (h >> 1) * L.row + (h & 1) * L.half + u0 * 16);
         }
-        // a pair of blocks' scales and sums per lane: two units of {scale a, scale b, sum a, sum b}
-        for (int i = tid; i < (nblk >> 1) * MR; i += W * 64) {
-            const int m = i % MR, bl = i / MR * 2, row = min(row0 + m, a.rows - 1);
-            const bool in = b0 + bl < nb; // (nb is even)
-            const uint2 * mp = reinterpret_cast<const uint2 *>(a.xmeta) + (size_t) row * nb + (in ? b0 + bl : 0);
-            const uint2 u0 = mp[0], u1 = mp[1];
-            const float da = in ? h2f_bits((uint16_t) u0.x) : 0.f, db = in ? h2f_bits((uint16_t) (u0.x >> 16)) : 0.f;
-            dx[bl * MR + m] = da * 0.0625f; // (the codes go in 16 times as large)
-            dx[(bl + 1) * MR + m] = db * 0.0625f;
-            ds[bl * MR + m] = in ? da * (float) ((int) (int16_t) u0.y + (int) (int16_t) u1.y) : 0.f;
-            ds[(bl + 1) * MR + m] = in ? db * (float) (((int) u0.y >> 16) + ((int) u1.y >> 16)) : 0.f;
-        }
+#pragma unroll
+        for (int u = 0; u < NI; u++)
+            if (p0 + u * STEP < np) store(p0 + u * STEP, mt[u]);
+        for (int p = p0 + NI * STEP; p < np; p += STEP) store(p, load(p));
         vm_drain();
     } else {
         // a quarter of a block (8 values) per lane
@@ -71,16 +104,13 @@ __device__ __forceinline__ void w4_stage(const W4Args & a, uint8_t * lds, int ro
             const int q = i & 3, m = (i >> 2) % MR, bl = (i >> 2) / MR, blk = b0 + bl, row = row0 + m;
             float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
             if (row < a.rows && blk < nb) Elem<DT>::load8(x + (long long) row * a.x_stride + 32 * blk + 8 * q, v);
-            float am = 0.f, s = 0.f;
+            float s = 0.f;
             unsigned top = 0;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                am = fmaxf(am, fabsf(v[k]));
                 top = max(top, __builtin_bit_cast(unsigned, v[k]) & 0x7fffffffu);
                 s += v[k];
             }
-            am = fmaxf(am, shfl_xor(am, 1));
-            am = fmaxf(am, shfl_xor(am, 2));
             s += shfl_xor(s, 1);
             s += shfl_xor(s, 2);
             top = max(top, shfl_xor_u(top, 1));
@@ -104,7 +134,7 @@ __device__ __forceinline__ void w4_stage(const W4Args & a, uint8_t * lds, int ro
             if constexpr (MODE == XM_SPLIT) *reinterpret_cast<half8 *>(lds + (size_t) bl * BB + ((4 + q) * MR + m) * 16) = lo;
             if (q == 0) {
                 dx[bl * MR + m] = wild ? 1.f : __builtin_bit_cast(float, (unsigned) (E - 14) << 23);
-                ds[bl * MR + m] = s;
+                if (MINS) ds[bl * MR + m] = s;
             }
         }
     }
@@ -125,7 +155,6 @@ __device__ __forceinline__ half8 w4_halves(unsigned w) {
     return half8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
 }
 
-typedef unsigned u32x4_u2 __attribute__((ext_vector_type(4), aligned(2)));
 // scales grp .. grp + 7 of a weight row of gs (p: its first), zeros past the row's end: the last eight of the row, moved down
 __device__ __forceinline__ u32x4 w4_scales(const uint16_t * p, int gs, int grp) {
     if (__builtin_expect(gs < 8, 0)) {
@@ -159,20 +188,23 @@ constexpr int W4_WIN = 32;  // scales of a weight row that a wave holds in LDS a
 template <int MODE, int DT, int NR, int RG, int P, int W, bool MINS>
 __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
     static_assert(P * NR <= 4, "parts share a group's four operand rows");
-    constexpr int MR = NR * RG, BB = blk_bytes<MODE, MR>(), TR = 16 / P, U = W4_RUN;
+    constexpr int MR = NR * RG, BB = planes(MODE) * MR * 16, TR = 16 / P, U = W4_RUN;
+    const W4Lds L = w4_lds<MODE, MR, MINS>(a.kcb);
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    const float * dx = reinterpret_cast<const float *>(lds + (size_t) (a.kcb + 1) * BB), * ds = dx + a.kcb * MR;
+    const float * dx = reinterpret_cast<const float *>(lds + L.dx), * ds = dx + a.kcb * MR;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int WK = 1 << a.wk_log, wk = wave & (WK - 1), wn = wave >> a.wk_log, WN = W >> a.wk_log;
     const int nb = a.k >> 5, tiles = (a.n + TR - 1) / TR, sets = (tiles + WN - 1) / WN;
     const int nbp = (nb + 4 * U * P - 1) / (4 * U * P) * (4 * U * P), pb = nbp / P; // blocks with padding, blocks of a part
     const int row0 = blockIdx.y * MR, j = n % TR, h = n / TR;
-    uint16_t * win = reinterpret_cast<uint16_t *>(const_cast<float *>(ds) + a.kcb * MR) + wave * (MINS ? 2 : 1) * 16 * W4_WIN; // [16][32] scales, then m
-    float * red = reinterpret_cast<float *>(reinterpret_cast<uint16_t *>(const_cast<float *>(ds) + a.kcb * MR) + W * (MINS ? 2 : 1) * 16 * W4_WIN); // [2][waves][MR][TR]
+    uint16_t * win = reinterpret_cast<uint16_t *>(lds + L.end) + wave * (MINS ? 2 : 1) * 16 * W4_WIN; // [16][32] scales, then m
+    float * red = reinterpret_cast<float *>(lds + L.end + W * (MINS ? 2 : 1) * 16 * W4_WIN * 2);       // [2][waves][MR][TR]
     // the lane's piece of the diagonal operand: row n = 4 b + NR part + m, lane group b
     const int m = n % NR, a_part = (n & 3) / NR;
     const bool active = (n >> 2) == g && a_part < P;
-    const int abase = active ? (a_part * pb + g) * BB + m * 16 : a.kcb * BB, astep = active ? 4 * BB : 0;
+    constexpr bool ROWS = MODE == XM_UNITS; // x by rows: a block's two units in its row's even or odd part
+    const int abase = !active ? L.zero : ROWS ? m * L.row + (g & 1) * L.half + (a_part * pb + (g & 2)) * 16 : (a_part * pb + g) * BB + m * 16;
+    const int astep = !active ? 0 : ROWS ? 64 : 4 * BB, agroup = !active ? 0 : ROWS ? NR * L.row : NR * 16;
     const int hb = P == 1 ? 0 : h * pb, myb = hb + g; // the first block of the lane's part, the lane's block of step 0
     // runs of the chunk of x that begins at block b0 (parts: all of x at once), and the wave's steps of them
     const auto runs = [&](int b0) { return (P == 1 ? min(a.kcb, nbp - b0) : pb) / (4 * U); };
@@ -253,7 +285,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
         for (int b0 = 0; b0 < nbp; b0 += P == 1 ? a.kcb : nbp) {
             if (!staged) {
                 __syncthreads();
-                w4_stage<MODE, DT, MR, W>(a, lds, row0, b0, P == 1 ? min(a.kcb, nbp - b0) : nbp);
+                w4_stage<MODE, DT, MR, W, MINS>(a, lds, row0, b0, P == 1 ? min(a.kcb, nbp - b0) : nbp);
                 __syncthreads();
                 staged = nbp <= a.kcb;
             }
@@ -301,7 +333,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
 #pragma unroll
                     for (int i = 0; i < RG; i++) {
                         if constexpr (MODE == XM_UNITS) {
-                            const i32x4 a0 = *reinterpret_cast<const i32x4 *>(ap + i * NR * 16), a1 = *reinterpret_cast<const i32x4 *>(ap + (MR + i * NR) * 16);
+                            const i32x4 a0 = *reinterpret_cast<const i32x4 *>(ap + i * agroup), a1 = *reinterpret_cast<const i32x4 *>(ap + i * agroup + 16);
                             i32x4 c = {0, 0, 0, 0};
                             c = __builtin_amdgcn_mfma_i32_16x16x64_i8(a0, hbv[0], c, 0, 0, 0);
                             c = __builtin_amdgcn_mfma_i32_16x16x64_i8(a1, hbv[1], c, 0, 0, 0);
@@ -374,7 +406,7 @@ __device__ __forceinline__ void w4_exchange(const u32x4 & d, unsigned (&t)[4]) {
 // then lie in different banks), and the factors [CB][TM + 4].  Plain rows: w4_stage's layout.
 template <int MODE, int MT, int CB, bool MINS> constexpr int wide_buf() {
     constexpr int TM = 16 * MT;
-    return MODE == XM_UNITS ? CB * 2 * TM / 64 * 1040 + (MINS ? 2 : 1) * CB * (TM + 4) * 4 : (CB + 1) * planes(MODE) * TM * 16 + 2 * CB * TM * 4;
+    return MODE == XM_UNITS ? CB * 2 * TM / 64 * 1040 + (MINS ? 2 : 1) * CB * (TM + 4) * 4 : w4_lds<MODE, TM, MINS>(CB).end;
 }
 
 // WK waves along the blocks of a chunk, U steps each, times WN along the tiles.  ODD: a workgroup of an odd number of tiles,
@@ -385,7 +417,7 @@ __global__ __launch_bounds__(WK * WN * 64, WK * WN / 4) void k_w4_wide(W4Args a)
     constexpr int WIDE_W = WK * WN, TM = 16 * MT, CB = 4 * WK * U, BB = planes(MODE) * TM * 16, BUF = wide_buf<MODE, MT, CB, MINS>();
     constexpr bool ASYNC = MODE == XM_UNITS; // x copied into the other buffer while a chunk is worked on
     constexpr int RPC = 32 / CB; // rows of a copy
-    constexpr int DX = ASYNC ? TM / RPC * 1040 : (CB + 1) * BB, DS = ASYNC ? TM + 4 : TM; // the factors of x behind the blocks, their stride
+    constexpr int DX = ASYNC ? TM / RPC * 1040 : w4_lds<MODE, TM, MINS>(CB).dx, DS = ASYNC ? TM + 4 : TM; // the factors of x behind the blocks, their stride
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
     const int wk = wave % WK, wn = wave / WK;
@@ -401,7 +433,8 @@ __global__ __launch_bounds__(WK * WN * 64, WK * WN / 4) void k_w4_wide(W4Args a)
         const int b0 = c * CB, part = lane / CB & 1, unit = min(b0 + lane % CB, nb - 1);
         const int8_t * src = part ? a.xb : a.xa;
 #pragma unroll 1
-        for (int k = wave; k < TM / RPC; k += WIDE_W) {
+        for (int k0 = wave; k0 < TM / RPC; k0 += WIDE_W) {
+            const int k = (k0 + blockIdx.x) % (TM / RPC); // (every workgroup reads the same rows: each begins with others)
             const int row = min(row0 + k * RPC + lane / (2 * CB), a.rows - 1);
             dma16(src + ((size_t) row * nb + unit) * 16, base + buf * BUF + k * 1040);
         }
@@ -489,7 +522,7 @@ __global__ __launch_bounds__(WK * WN * 64, WK * WN / 4) void k_w4_wide(W4Args a)
             __syncthreads();
             W4Args b = a;
             b.kcb = CB;
-            w4_stage<MODE, DT, TM, WIDE_W>(b, lds, row0, c * CB, CB);
+            w4_stage<MODE, DT, TM, WIDE_W, MINS>(b, lds, row0, c * CB, CB);
             __syncthreads();
         }
         // the codes to their lane groups, the scales of each block to floats; the next chunk's take their registers
@@ -598,26 +631,42 @@ __global__ __launch_bounds__(WK * WN * 64, WK * WN / 4) void k_w4_wide(W4Args a)
     }
 }
 
-constexpr int W4_LDS = 64 * 1024;
+constexpr int W4_LDS = 80 * 1024; // two workgroups per CU
+// lets a kernel have more than 64 KiB of LDS: once per kernel and device (the flag is the kernel's own)
+template <class K> static hipError_t allow_lds(K k, size_t lds, std::atomic<uint64_t> & done) {
+    if (lds <= 64 * 1024) return hipSuccess;
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return hipSuccess;
+    e = hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (e == hipSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 constexpr int W4_WAVES = 4096; // of a launch: 16 for each of 256 CUs, a quarter of what they hold
 
 template <int MODE, int DT, int NR, int RG, int P, int W>
 static hipError_t launch_k(W4Args a, hipStream_t st) {
-    constexpr int MR = NR * RG, per = planes(MODE) * MR * 16 + 2 * MR * 4, TR = 16 / P;
-    constexpr int PAD = 4 * W4_RUN;
+    constexpr int MR = NR * RG, TR = 16 / P, PAD = 4 * W4_RUN;
     const int nb4 = (a.k / 32 + PAD * P - 1) / (PAD * P) * (PAD * P), tiles = (a.n + TR - 1) / TR;
-    const int red = 2 * W * MR * TR * 4 + W * (a.mins ? 2 : 1) * 16 * W4_WIN * 2, zero = planes(MODE) * MR * 16; // (with the windows of scales)
-    a.kcb = std::min(nb4, (W4_LDS - red - zero) / per / PAD * PAD);
+    const int more = 2 * W * MR * TR * 4 + W * (a.mins ? 2 : 1) * 16 * W4_WIN * 2; // the waves' sums, the windows of scales
+    const auto size = [&](int kcb) { return (a.mins ? w4_lds<MODE, MR, true>(kcb) : w4_lds<MODE, MR, false>(kcb)).end + more; };
+    a.kcb = std::min(nb4, W4_LDS / (planes(MODE) * MR * 16 + MR * 4) / PAD * PAD);
+    while (size(a.kcb) > W4_LDS) a.kcb -= PAD;
     if constexpr (P > 1) {
         if (a.kcb < nb4) return launch_k<MODE, DT, 4, (MR + 3) / 4, 1, 8>(a, st); // (x in pieces)
     }
     // (every wave has a run of the first chunk)
     while ((1 << a.wk_log) < W && (tiles << a.wk_log) < W4_WAVES / 2 && a.kcb / P / PAD >= 2 << a.wk_log) a.wk_log++;
     const int wn = W >> a.wk_log, sets = (tiles + wn - 1) / wn;
-    const size_t lds = (size_t) a.kcb * per + zero + red;
+    const size_t lds = size(a.kcb);
     const dim3 grid(std::min(sets, W4_WAVES / W), (a.rows + MR - 1) / MR), block(W * 64);
-    if (a.mins) hipLaunchKernelGGL((k_w4<MODE, DT, NR, RG, P, W, true>), grid, block, lds, st, a);
-    else hipLaunchKernelGGL((k_w4<MODE, DT, NR, RG, P, W, false>), grid, block, lds, st, a);
+    static std::atomic<uint64_t> done[2];
+    const auto k = a.mins ? k_w4<MODE, DT, NR, RG, P, W, true> : k_w4<MODE, DT, NR, RG, P, W, false>;
+    const hipError_t e = allow_lds(k, lds, done[a.mins != nullptr]);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(k, grid, block, lds, st, a);
     return hipGetLastError();
 }
 
@@ -627,10 +676,9 @@ static hipError_t launch_wide_k(const W4Args & a, dim3 grid, hipStream_t st) {
     constexpr int lds = std::max((MODE == XM_UNITS ? 2 : 1) * wide_buf<MODE, MT, 4 * WK * U, MINS>(), WIDE_W * 16 * MT * 16 * 4);
     static_assert(lds <= 160 * 1024, "a workgroup's LDS");
     const auto k = k_w4_wide<MODE, DT, MT, NTW, WK, WN, U, ODD, MINS>;
-    if (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        if (e != hipSuccess) return e;
-    }
+    static std::atomic<uint64_t> done;
+    const hipError_t e = allow_lds(k, lds, done);
+    if (e != hipSuccess) return e;
     hipLaunchKernelGGL(k, grid, dim3(WIDE_W * 64), lds, st, a);
     return hipGetLastError();
 }
