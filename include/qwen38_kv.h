@@ -258,7 +258,8 @@ int mk_norm_q32(const void * x, long long x_stride, const void * res, long long 
  *   W = scales (c - 8) + mins
  * mk_w4_units takes x as the int8 units of mk_kv_attend_gated or mk_norm_q32 ([rows][k / 32][16 | 4]; k a multiple of 64),
  * mk_w4_rows as plain rows [rows][x_stride] of dtype (k a multiple of 32).  Products and sums are exact or in fp32: the units'
- * integer sums are exact per 32 values, fp16 and bf16 rows enter as they are and fp32 rows to 2^-24 of each value.
+ * integer sums are exact per 32 values, fp16 and bf16 rows enter as they are and fp32 rows to 2^-23 of each value, all of them to
+ * 2^-39 of the largest of a block's 32.
  * Meant for the tokens of a decode or verify step: 1 to 64 rows, more are allowed.
  */
 int mk_w4_units(int rows, int n, int k, int group, const void * codes, const void * scales, const void * mins, const void * q32a, const void * q32b,

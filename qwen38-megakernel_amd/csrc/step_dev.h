@@ -15,15 +15,43 @@ typedef _Float16 f16x4_u __attribute__((ext_vector_type(4), aligned(2)));
 typedef _Float16 f16x8_u __attribute__((ext_vector_type(8), aligned(2)));
 typedef __bf16 bf16x8_u __attribute__((ext_vector_type(8), aligned(2)));
 
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+
+// the largest of 8 16-bit floats by their bits without the sign
+__device__ __forceinline__ uint16_t top16(u16x8 v) {
+    typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    v &= (uint16_t) 0x7fff;
+    const u16x4 a = __builtin_elementwise_max(v.lo, v.hi);
+    const u16x2 b = __builtin_elementwise_max(a.lo, a.hi);
+    return b[0] > b[1] ? b[0] : b[1];
+}
+
+// Raw8: 8 values as they are in memory; open8: as floats; top8: the bits of the largest one's absolute value as fp32 (an
+// infinity or a NaN where there is one)
 template <int DT> struct Elem;
 template <> struct Elem<DT_F32> {
     typedef float T;
     static __device__ __forceinline__ float up(T v) { return v; }
     static __device__ __forceinline__ T down(float v) { return v; }
-    static __device__ __forceinline__ void load8(const T * p, float (&v)[8]) {
-        const f32x4_u a = *reinterpret_cast<const f32x4_u *>(p), b = *reinterpret_cast<const f32x4_u *>(p + 4);
+    struct Raw8 {
+        f32x4 a, b;
+    };
+    static __device__ __forceinline__ Raw8 raw8(const T * p) {
+        return Raw8{*reinterpret_cast<const f32x4_u *>(p), *reinterpret_cast<const f32x4_u *>(p + 4)};
+    }
+    static __device__ __forceinline__ void open8(const Raw8 & r, float (&v)[8]) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+        for (int i = 0; i < 4; i++) v[i] = r.a[i], v[4 + i] = r.b[i];
+    }
+    static __device__ __forceinline__ unsigned top8(const Raw8 & r) {
+        unsigned t = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float x = r.a[i], y = r.b[i]; // (a bit cast of a vector's element itself takes the first one)
+            t = max(max(t, __builtin_bit_cast(unsigned, x) & 0x7fffffffu), __builtin_bit_cast(unsigned, y) & 0x7fffffffu);
+        }
+        return t;
     }
     static __device__ __forceinline__ void load4(const T * p, float (&v)[4]) {
         const f32x4_u a = *reinterpret_cast<const f32x4_u *>(p);
@@ -39,10 +67,14 @@ template <> struct Elem<DT_F16> {
     typedef _Float16 T;
     static __device__ __forceinline__ float up(T v) { return (float) v; }
     static __device__ __forceinline__ T down(float v) { return (T) v; }
-    static __device__ __forceinline__ void load8(const T * p, float (&v)[8]) {
-        const f16x8_u a = *reinterpret_cast<const f16x8_u *>(p);
+    typedef half8 Raw8;
+    static __device__ __forceinline__ Raw8 raw8(const T * p) { return *reinterpret_cast<const f16x8_u *>(p); }
+    static __device__ __forceinline__ void open8(const Raw8 & r, float (&v)[8]) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = (float) a[i];
+        for (int i = 0; i < 8; i++) v[i] = (float) r[i];
+    }
+    static __device__ __forceinline__ unsigned top8(const Raw8 & r) {
+        return __builtin_bit_cast(unsigned, (float) __builtin_bit_cast(_Float16, top16(__builtin_bit_cast(u16x8, r))));
     }
     static __device__ __forceinline__ void load4(const T * p, float (&v)[4]) {
         const f16x4_u a = *reinterpret_cast<const f16x4_u *>(p);
@@ -60,11 +92,13 @@ template <> struct Elem<DT_BF16> {
     typedef __bf16 T;
     static __device__ __forceinline__ float up(T v) { return __builtin_bit_cast(float, (unsigned) __builtin_bit_cast(uint16_t, v) << 16); }
     static __device__ __forceinline__ T down(float v) { return (T) v; }
-    static __device__ __forceinline__ void load8(const T * p, float (&v)[8]) {
-        const u16x8_u a = *reinterpret_cast<const u16x8_u *>(p);
+    typedef u16x8 Raw8;
+    static __device__ __forceinline__ Raw8 raw8(const T * p) { return *reinterpret_cast<const u16x8_u *>(p); }
+    static __device__ __forceinline__ void open8(const Raw8 & r, float (&v)[8]) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = __builtin_bit_cast(float, (unsigned) a[i] << 16);
+        for (int i = 0; i < 8; i++) v[i] = __builtin_bit_cast(float, (unsigned) r[i] << 16);
     }
+    static __device__ __forceinline__ unsigned top8(const Raw8 & r) { return (unsigned) top16(r) << 16; }
     static __device__ __forceinline__ void load4(const T * p, float (&v)[4]) {
         const u16x4_u a = *reinterpret_cast<const u16x4_u *>(p);
 #pragma unroll
@@ -78,9 +112,11 @@ template <> struct Elem<DT_BF16> {
     }
 };
 
+template <int DT> __device__ __forceinline__ void load8(const typename Elem<DT>::T * p, float (&v)[8]) { Elem<DT>::open8(Elem<DT>::raw8(p), v); }
+
 // the first n (1..8) of 8 values, the rest zero
 template <int DT> __device__ __forceinline__ void load_n(const typename Elem<DT>::T * p, int n, float (&v)[8]) {
-    if (n >= 8) return Elem<DT>::load8(p, v);
+    if (n >= 8) return load8<DT>(p, v);
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = i < n ? Elem<DT>::up(p[i]) : 0.f;
 }

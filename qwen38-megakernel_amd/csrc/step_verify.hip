@@ -55,7 +55,7 @@ template <bool PROBS> __device__ __forceinline__ double weight(float v, float to
 // `none`
 template <int DT, int E> __device__ __forceinline__ void load_run(const typename Elem<DT>::T * p, int j, int vocab, float none, float (&v)[E]) {
     if (j + E <= vocab) {
-        if constexpr (E == 8) Elem<DT>::load8(p + j, v);
+        if constexpr (E == 8) load8<DT>(p + j, v);
         else Elem<DT>::load4(p + j, v);
     } else {
 #pragma unroll

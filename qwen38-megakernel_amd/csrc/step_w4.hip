@@ -32,7 +32,7 @@ constexpr int planes(int mode) { return mode == XM_UNITS ? 2 : mode == XM_HALF ?
 // [kcb blocks][planes][MR rows][16 bytes].  Then zeros for the operand's other lanes, [kcb][MR] float factors of the blocks'
 // sums and (with m) [kcb][MR] float factors of m.
 struct W4Lds {
-    int half, row, zero, dx, end; // units: bytes of a row's even blocks, of a row; offsets of the zeros, the factors, what follows
+    int half, row, zero, dx, ds, end; // units: bytes of a row's even blocks, of a row; offsets of the zeros, the factors, what follows
 };
 template <int MODE, int MR, bool MINS> __host__ __device__ __forceinline__ constexpr W4Lds w4_lds(int kcb) {
     W4Lds l{};
@@ -40,7 +40,8 @@ template <int MODE, int MR, bool MINS> __host__ __device__ __forceinline__ const
     l.row = 2 * l.half + 32;
     l.zero = MODE == XM_UNITS ? MR * l.row : kcb * planes(MODE) * MR * 16;
     l.dx = l.zero + (MODE == XM_UNITS ? 32 : planes(MODE) * MR * 16);
-    l.end = (l.dx + (MINS ? 2 : 1) * kcb * MR * 4 + 15) & ~15;
+    l.ds = l.dx + kcb * MR * 4;
+    l.end = ((MINS ? l.ds + kcb * MR * 4 : l.ds) + 15) & ~15;
     return l;
 }
 
@@ -51,22 +52,77 @@ __device__ __forceinline__ void dma16(const void * g, unsigned lds) {
 }
 __device__ __forceinline__ void vm_drain() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// a quarter of a block of plain x (8 values) on its way to LDS as fp16: piece i = 4 (MR block + row) + quarter of the blocks from
+// b0 and the rows from row0 on; zeros for rows past the last one and blocks past the row's end
+template <int DT> struct W4Eighth {
+    typename Elem<DT>::Raw8 raw;
+    __device__ __forceinline__ void load(const W4Args & a, int i, int mr, int row0, int b0) {
+        const int blk = min(b0 + (i >> 2) / mr, (a.k >> 5) - 1), row = min(row0 + (i >> 2) % mr, a.rows - 1);
+        raw = Elem<DT>::raw8(static_cast<const typename Elem<DT>::T *>(a.x) + (long long) row * a.x_stride + 32 * blk + 8 * (i & 3));
+    }
+    // (whole blocks: the lanes of all four quarters)
+    template <int MODE, int MR, bool MINS>
+    __device__ __forceinline__ void store(const W4Args & a, uint8_t * lds, const W4Lds & L, int i, int row0, int b0) const {
+        const int q = i & 3, m = (i >> 2) % MR, bl = (i >> 2) / MR;
+        float * dx = reinterpret_cast<float *>(lds + L.dx), * ds = dx + (L.ds - L.dx) / 4;
+        const bool in = row0 + m < a.rows && b0 + bl < a.k >> 5;
+        float v[8], s = 0.f;
+        const typename Elem<DT>::Raw8 r = in ? raw : typename Elem<DT>::Raw8{};
+        unsigned top = Elem<DT>::top8(r);
+        top = max(top, shfl_xor_u(top, 1));
+        top = max(top, shfl_xor_u(top, 2));
+        Elem<DT>::open8(r, v);
+        if (MINS) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) s += v[k];
+            s += shfl_xor(s, 1);
+            s += shfl_xor(s, 2);
+        }
+        // times 2^e, which brings the block's largest value to [2^14, 2^15), without rounding
+        const bool wild = top >= 0x7f800000u;
+        const int E = max((int) (top >> 23), 15);
+        const float up = __builtin_bit_cast(float, (unsigned) (268 - E) << 23);
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] *= up;
+        if (__builtin_expect(wild, 0)) { // an infinity or a NaN in the block: these as they are, its finite values as zeros (they cannot change the result)
+            Elem<DT>::open8(r, v);
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = __builtin_fabsf(v[k]) < __builtin_inff() ? 0.f : v[k];
+        }
+        // element order of the codes' fp16 pairs: (0, 2) (1, 3) (4, 6) (5, 7)
+        half8 hi, lo;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int e = (k & 4) + 2 * (k & 1) + ((k >> 1) & 1);
+            hi[e] = (_Float16) v[k];
+            lo[e] = (_Float16) (v[k] - (float) hi[e]);
+        }
+        if (MODE == XM_SPLIT && __builtin_expect(wild, 0)) lo = half8{};
+        uint8_t * to = lds + (size_t) bl * (planes(MODE) * MR * 16) + (q * MR + m) * 16;
+        *reinterpret_cast<half8 *>(to) = hi;
+        if constexpr (MODE == XM_SPLIT) *reinterpret_cast<half8 *>(to + 4 * MR * 16) = lo;
+        if (q == 0) {
+            dx[bl * MR + m] = wild ? 1.f : __builtin_bit_cast(float, (unsigned) (E - 14) << 23);
+            if (MINS) ds[bl * MR + m] = s;
+        }
+    }
+};
+
 // x of blocks b0 .. b0 + nblk - 1 (nblk a multiple of 4) into LDS; blocks past the last one get factors of zero
 template <int MODE, int DT, int MR, int W, bool MINS>
-__device__ __forceinline__ void w4_stage(const W4Args & a, uint8_t * lds, int row0, int b0, int nblk) {
-    constexpr int BB = planes(MODE) * MR * 16;
+__device__ __forceinline__ void w4_stage(const W4Args & a, uint8_t * lds, int b0, int nblk) {
     const W4Lds L = w4_lds<MODE, MR, MINS>(a.kcb);
-    const int nb = a.k >> 5, tid = threadIdx.x;
-    float * dx = reinterpret_cast<float *>(lds + L.dx), * ds = dx + a.kcb * MR;
+    const int tid = threadIdx.x;
     for (int i = tid; i < (L.dx - L.zero) / 16; i += W * 64) reinterpret_cast<uint4 *>(lds + L.zero)[i] = make_uint4(0, 0, 0, 0);
     if constexpr (MODE == XM_UNITS) {
         const unsigned base = (unsigned) __builtin_amdgcn_readfirstlane((unsigned) (size_t) (__attribute__((address_space(3))) uint8_t *) lds);
-        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, np = nblk >> 1;
+        const int nb = a.k >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, np = nblk >> 1;
+        float * dx = reinterpret_cast<float *>(lds + L.dx), * ds = dx + a.kcb * MR;
         // a pair of blocks' scales and sums per lane, two units of {scale a, scale b, sum a, sum b}: a wave has one row's; all
         // loads ahead of the copies, and one wait for both
         static_assert(W % MR == 0, "waves per row");
         constexpr int STEP = 64 * (W / MR), NI = 2;
-        const int m = wave % MR, mrow = min(row0 + m, a.rows - 1), p0 = lane + 64 * (wave / MR);
+        const int m = wave % MR, mrow = min(m, a.rows - 1), p0 = lane + 64 * (wave / MR);
         u32x4 mt[NI];
         const auto load = [&](int p) {
             return *reinterpret_cast<const u32x4_u8 *>(a.xmeta + ((size_t) mrow * nb + min(b0 + 2 * p, nb - 2)) * 4); // (nb is even)
@@ -87,7 +143,7 @@ __device__ __forceinline__ void w4_stage(const W4Args & a, uint8_t * lds, int ro
         const int per = (nblk + 63) >> 6; // copies of a half
 #pragma unroll 1
         for (int c = wave; c < MR * 2 * per; c += W) {
-            const int h = c / per, u0 = (c - h * per) * 64, row = min(row0 + (h >> 1), a.rows - 1);
+            const int h = c / per, u0 = (c - h * per) * 64, row = min(h >> 1, a.rows - 1);
             if (u0 + lane < nblk)
                 dma16(((h & 1) ? a.xb : a.xa) + ((size_t) row * nb + min(b0 + u0 + lane, nb - 1)) * 16,
                       base + (h >> 1) * L.row + (h & 1) * L.half + u0 * 16);
@@ -98,44 +154,13 @@ __device__ __forceinline__ void w4_stage(const W4Args & a, uint8_t * lds, int ro
         for (int p = p0 + NI * STEP; p < np; p += STEP) store(p, load(p));
         vm_drain();
     } else {
-        // a quarter of a block (8 values) per lane
-        const typename Elem<DT>::T * x = static_cast<const typename Elem<DT>::T *>(a.x);
-        for (int i = tid; i < nblk * 4 * MR; i += W * 64) { // (a multiple of 4 lanes: whole blocks)
-            const int q = i & 3, m = (i >> 2) % MR, bl = (i >> 2) / MR, blk = b0 + bl, row = row0 + m;
-            float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (row < a.rows && blk < nb) Elem<DT>::load8(x + (long long) row * a.x_stride + 32 * blk + 8 * q, v);
-            float s = 0.f;
-            unsigned top = 0;
+        for (int i = tid; i < nblk * 4 * MR; i += 4 * W * 64) { // (four loads, then their values)
+            W4Eighth<DT> e[4];
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                top = max(top, __builtin_bit_cast(unsigned, v[k]) & 0x7fffffffu);
-                s += v[k];
-            }
-            s += shfl_xor(s, 1);
-            s += shfl_xor(s, 2);
-            top = max(top, shfl_xor_u(top, 1));
-            top = max(top, shfl_xor_u(top, 2));
-            // 2^e with the block's largest value in [2^14, 2^15); a block with an infinity or a NaN goes in as it is, its
-            // finite values as zeros (they cannot change the result)
-            const bool wild = top >= 0x7f800000u;
-            const int E = max((int) (top >> 23), 15);
-            const float up = wild ? 1.f : __builtin_bit_cast(float, (unsigned) (268 - E) << 23);
-            half8 hi, lo;
+            for (int u = 0; u < 4; u++) e[u].load(a, min(i + u * W * 64, nblk * 4 * MR - 1), MR, 0, b0);
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const float t = wild && __builtin_fabsf(v[k]) < __builtin_inff() ? 0.f : v[k] * up;
-                const _Float16 h = (_Float16) t;
-                // element order of the codes' fp16 pairs: (0, 2) (1, 3) (4, 6) (5, 7)
-                const int e = (k & 4) + 2 * (k & 1) + ((k >> 1) & 1);
-                hi[e] = h;
-                lo[e] = wild ? (_Float16) 0.f : (_Float16) (t - (float) h);
-            }
-            *reinterpret_cast<half8 *>(lds + (size_t) bl * BB + (q * MR + m) * 16) = hi;
-            if constexpr (MODE == XM_SPLIT) *reinterpret_cast<half8 *>(lds + (size_t) bl * BB + ((4 + q) * MR + m) * 16) = lo;
-            if (q == 0) {
-                dx[bl * MR + m] = wild ? 1.f : __builtin_bit_cast(float, (unsigned) (E - 14) << 23);
-                if (MINS) ds[bl * MR + m] = s;
-            }
+            for (int u = 0; u < 4; u++)
+                if (i + u * W * 64 < nblk * 4 * MR) e[u].template store<MODE, MR, MINS>(a, lds, L, i + u * W * 64, 0, b0);
         }
     }
 }
@@ -196,7 +221,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
     const int WK = 1 << a.wk_log, wk = wave & (WK - 1), wn = wave >> a.wk_log, WN = W >> a.wk_log;
     const int nb = a.k >> 5, tiles = (a.n + TR - 1) / TR, sets = (tiles + WN - 1) / WN;
     const int nbp = (nb + 4 * U * P - 1) / (4 * U * P) * (4 * U * P), pb = nbp / P; // blocks with padding, blocks of a part
-    const int row0 = blockIdx.y * MR, j = n % TR, h = n / TR;
+    const int j = n % TR, h = n / TR;
     uint16_t * win = reinterpret_cast<uint16_t *>(lds + L.end) + wave * (MINS ? 2 : 1) * 16 * W4_WIN; // [16][32] scales, then m
     float * red = reinterpret_cast<float *>(lds + L.end + W * (MINS ? 2 : 1) * 16 * W4_WIN * 2);       // [2][waves][MR][TR]
     // the lane's piece of the diagonal operand: row n = 4 b + NR part + m, lane group b
@@ -285,7 +310,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
         for (int b0 = 0; b0 < nbp; b0 += P == 1 ? a.kcb : nbp) {
             if (!staged) {
                 __syncthreads();
-                w4_stage<MODE, DT, MR, W, MINS>(a, lds, row0, b0, P == 1 ? min(a.kcb, nbp - b0) : nbp);
+                w4_stage<MODE, DT, MR, W, MINS>(a, lds, b0, P == 1 ? min(a.kcb, nbp - b0) : nbp);
                 __syncthreads();
                 staged = nbp <= a.kcb;
             }
@@ -369,7 +394,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
             if (lane < TR && tile * TR + lane < a.n) {
 #pragma unroll
                 for (int i = 0; i < MR; i++)
-                    if (row0 + i < a.rows) a.y[(long long) (row0 + i) * a.y_stride + tile * TR + lane] = acc[i / NR][i % NR];
+                    if (i < a.rows) a.y[i * a.y_stride + tile * TR + lane] = acc[i / NR][i % NR];
             }
             continue;
         }
@@ -383,7 +408,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
             const int c = i % TR, mm = i / TR % MR, t = i / TR / MR, col = (set * WN + t) * TR + c;
             float v = rp[((t << a.wk_log) * MR + mm) * TR + c];
             for (int k = 1; k < WK; k++) v += rp[(((t << a.wk_log) + k) * MR + mm) * TR + c];
-            if (col < a.n && row0 + mm < a.rows) a.y[(long long) (row0 + mm) * a.y_stride + col] = v;
+            if (col < a.n && mm < a.rows) a.y[mm * a.y_stride + col] = v;
         }
     }
 }
@@ -519,10 +544,13 @@ __global__ __launch_bounds__(WK * WN * 64, WK * WN / 4) void k_w4_wide(W4Args a)
         const int buf = ASYNC ? c & 1 : 0, cn = min(c + 1, chunks - 1);
         if constexpr (ASYNC) issue(cn, buf ^ 1); // (past the last chunk: that one once more, unused)
         else {
+            constexpr int NX = CB * 4 * TM / (WIDE_W * 64);
+            W4Eighth<DT> xr[NX]; // (loaded a chunk ahead they would cost the second workgroup of a CU: 32 rows of 65,536 x 5,120 fp32, 115 us, then 165)
+#pragma unroll
+            for (int u = 0; u < NX; u++) xr[u].load(a, tid + u * WIDE_W * 64, TM, row0, c * CB);
             __syncthreads();
-            W4Args b = a;
-            b.kcb = CB;
-            w4_stage<MODE, DT, TM, WIDE_W, MINS>(b, lds, row0, c * CB, CB);
+#pragma unroll
+            for (int u = 0; u < NX; u++) xr[u].template store<MODE, TM, MINS>(a, lds, w4_lds<MODE, TM, MINS>(CB), tid + u * WIDE_W * 64, row0, c * CB);
             __syncthreads();
         }
         // the codes to their lane groups, the scales of each block to floats; the next chunk's take their registers
@@ -661,7 +689,7 @@ static hipError_t launch_k(W4Args a, hipStream_t st) {
     while ((1 << a.wk_log) < W && (tiles << a.wk_log) < W4_WAVES / 2 && a.kcb / P / PAD >= 2 << a.wk_log) a.wk_log++;
     const int wn = W >> a.wk_log, sets = (tiles + wn - 1) / wn;
     const size_t lds = size(a.kcb);
-    const dim3 grid(std::min(sets, W4_WAVES / W), (a.rows + MR - 1) / MR), block(W * 64);
+    const dim3 grid(std::min(sets, W4_WAVES / W)), block(W * 64);
     static std::atomic<uint64_t> done[2];
     const auto k = a.mins ? k_w4<MODE, DT, NR, RG, P, W, true> : k_w4<MODE, DT, NR, RG, P, W, false>;
     const hipError_t e = allow_lds(k, lds, done[a.mins != nullptr]);
@@ -684,11 +712,14 @@ static hipError_t launch_wide_k(const W4Args & a, dim3 grid, hipStream_t st) {
 }
 template <int MODE, int DT, int MT, int U, bool MINS>
 static hipError_t launch_wide_m(W4Args a, hipStream_t st) {
-    // a workgroup per CU: as few rounds of at most 2 * 3 tiles each as there are, of the same number of tiles
+    // a workgroup per CU with up to 2 * 3 tiles each where that is all of them, else two per CU with four tiles at a time,
+    // whose registers (and, of 64 rows, shorter chunks of x) leave room for both
     constexpr int CUS = 256, MOST = 6;
-    const int tiles = (a.n + 15) / 16, rounds = (tiles + CUS * MOST - 1) / (CUS * MOST);
-    a.kcb = (tiles + CUS * rounds - 1) / (CUS * rounds);
+    const int tiles = (a.n + 15) / 16;
+    const bool many = tiles > CUS * MOST;
+    a.kcb = many ? 4 : (tiles + CUS - 1) / CUS;
     const dim3 grid((tiles + a.kcb - 1) / a.kcb, (a.rows + 16 * MT - 1) / (16 * MT));
+    if (many) return launch_wide_k<MODE, DT, MT, 2, 4, 2, MT == 4 ? 1 : U, false, MINS>(a, grid, st);
     if constexpr (U == 2) {
         if (a.kcb == 1) return launch_wide_k<MODE, DT, MT, 1, 8, 1, 1, false, MINS>(a, grid, st);
     }
@@ -719,11 +750,7 @@ static hipError_t launch_mode(const W4Args & a, hipStream_t st) {
     if (a.rows == 2) return launch_k<MODE, DT, 2, 1, 2, 4>(a, st);
     if (a.rows <= 4) return launch_k<MODE, DT, 4, 1, 1, 8>(a, st);
     if (a.rows <= 8) return launch_k<MODE, DT, 4, 2, 1, 8>(a, st);
-#ifdef W4_NOWIDE
-    return launch_k<MODE, DT, 4, 4, 1, 8>(a, st);
-#else
     return launch_wide<MODE, DT>(a, st);
-#endif
 }
 
 hipError_t launch_w4(const W4Args & a, int xform, hipStream_t st) {

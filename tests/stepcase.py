@@ -91,8 +91,9 @@ def w4_ref(c, scales, mins, group, x):
 def w4_bound(k, mag, plain):
     """How far a row's fp32 result may be off: every block's term is added once (mins: twice) in fp32, half a step each, a wave's
     four blocks at a time, then over lanes and waves; plain rows: 32 values per block (64 for fp32's two parts) summed inside the
-    matrix instructions, a whole step each, x itself to half a step."""
-    ops = k / 32 / 2 + 16 + (2 * 64 + 33 if plain else 0)
+    matrix instructions, a whole step each, x itself to a step (fp32: the first part, rounded to 11 bits, leaves at most 2^-11 of the
+    value's power of two, in steps of 2^-23; the second has steps of 2^-22 there, and half of one is 2^-23)."""
+    ops = k / 32 / 2 + 16 + (2 * 64 + 34 if plain else 0)
     return ops * 2.0 ** -24 * mag + 1e-38
 
 

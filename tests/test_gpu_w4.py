@@ -134,6 +134,24 @@ def test_wild_values(qkv, torch_gpu, x, rows):
     assert not np.isfinite(got[ok][:, 5]).any()
 
 
+@pytest.mark.parametrize("x", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("rows", [1, 2, 8, 20])
+def test_lone_values(qkv, torch_gpu, x, rows):
+    """One value far above the rest of its block, at every place of it; an infinity in a last block that others pad."""
+    def edit(v, s):
+        for i in range(5 * 32):
+            v[i % rows, i] = 4096.0 * (1 + i / 256) * (-1) ** i
+    got, ref, mag = run(torch_gpu, qkv, rows, 37, 160, 32, rows == 2, x, edit=edit)
+    assert (np.abs(got - ref) <= w4_bound(160, mag, True)).all()
+
+    def last(v, s):
+        v[0, 150] = np.inf
+    got, ref, mag = run(torch_gpu, qkv, rows, 37, 160, 32, False, x, edit=last)
+    assert np.isinf(ref[0]).any() and np.array_equal(np.isnan(got[0]), np.isnan(ref[0]))
+    there = ~np.isnan(ref[0])
+    assert np.array_equal(got[0][there], ref[0][there])
+
+
 def test_no_rows_and_refusals(qkv, torch_gpu):
     torch = torch_gpu
     t = torch.zeros(4096, dtype=torch.uint8, device="cuda")
