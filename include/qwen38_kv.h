@@ -236,7 +236,7 @@ int mk_kv_profile(void * h, int enable, double * out, int cap);
  */
 
 /*
- * Residual addition and root-mean-square norm of rows [rows][dim], dim 1..32768 (the norm before a projection; the
+ * Residual addition and root-mean-square norm of rows [rows][dim], rows 0..2^21, dim 1..32768 (the norm before a projection; the
  * reference's resid / norm phases around attn_proj, qwen38_mk.cu:2587-2621):
  *   h = x + res (fp32, rounded to dtype; res NULL: h = x), y = h / sqrt(mean(h^2) + eps) * w
  * with the mean in 64 bits.  x, res, sum, y: dtype; w: fp32 [dim].  Outputs, each optional, one at least: sum = h (may be
@@ -285,7 +285,8 @@ int mk_w4_rows(int rows, int n, int k, int group, const void * codes, const void
  *   draft_p     fp32 [n_seq][n] or NULL: p_i(draft i), 0 behind a sequence's last draft
  * Weights, sums and comparisons are in 64 bits.  ws: device memory of at least mk_verify_ws(n_seq, n_draft, vocab) bytes (16 for every
  * 4,096 entries of a row, and per sequence 8 for every row or every 4,096 entries, whichever are more), aligned to 16, that no other call uses until this
- * one has finished; nothing in it needs clearing.  mk_verify_ws returns -1 for a shape the call refuses.
+ * one has finished; nothing in it needs clearing.  mk_verify_ws returns -1 for a shape the call refuses (more than 2^23 slices of 4,096
+ * entries among them).
  */
 long long mk_verify_ws(int n_seq, int n_draft, int vocab);
 int mk_verify_drafts(int n_seq, int n_draft, int vocab, const void * target, long long row_stride, int dtype, int probs, const float * temperature,

@@ -99,7 +99,8 @@ void verify_shape(int n_seq, int n_draft, int vocab) {
     if (n_seq < 0 || n_seq > 65535) bad("n_seq outside 0 .. 65535");
     if (n_draft < 0 || n_draft > VERIFY_MAX_DRAFTS) bad("n_draft outside 0 .. 64");
     if (vocab < 1 || vocab > VERIFY_MAX_VOCAB) bad("vocab outside 1 .. 2^24");
-    if ((long long) n_seq * (n_draft + 1) * slices(vocab) >= 1ll << 31) bad("too many rows of this vocabulary in one call");
+    // (a workgroup of 256 threads per slice, fewer than 2^32 threads in a launch)
+    if ((long long) n_seq * (n_draft + 1) * slices(vocab) > VERIFY_MAX_SLICES) bad("too many rows of this vocabulary in one call");
 }
 long long verify_ws(int n_seq, int n_draft, int vocab) {
     verify_shape(n_seq, n_draft, vocab);
@@ -115,7 +116,7 @@ int mk_norm_q32(const void * x, long long x_stride, const void * res, long long 
                 void * sum, long long sum_stride, void * y, long long y_stride, void * q32a, void * q32b, unsigned short * q32meta, void * stream) {
     return guarded<int>([&] {
         const unsigned sz = size_of(dtype);
-        if (rows < 0) bad("negative rows");
+        if (rows < 0 || rows > NORM_MAX_ROWS) bad("rows outside 0 .. 2^21");
         if (dim < 1 || dim > NORM_MAX_DIM) bad("dim outside 1 .. 32768");
         if (!(eps >= 0.f) || std::isinf(eps)) bad("eps must be finite and not negative");
         if ((q32a != nullptr) != (q32b != nullptr) || (q32a != nullptr) != (q32meta != nullptr)) bad("the q32 outputs come as a set: a, b and meta");

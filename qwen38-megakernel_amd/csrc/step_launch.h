@@ -22,7 +22,7 @@ struct NormArgs {
     int rows, dim;
     float eps;
 };
-constexpr int NORM_MAX_DIM = 32768;
+constexpr int NORM_MAX_DIM = 32768, NORM_MAX_ROWS = 1 << 21; // (up to 1,024 threads a row, fewer than 2^32 in a launch)
 hipError_t launch_norm(const NormArgs & a, int dtype, hipStream_t st);
 
 // y[m][j] = sum_k W[j][k] x[m][k], W[j][k] = scales[j][k >> (5 + gsh)] (code - 8) + mins[..]
@@ -67,7 +67,7 @@ struct VerifyArgs {
     long long row_stride;
     int n_seq, n, vocab, nsl;
 };
-constexpr int VERIFY_SLICE = 4096, VERIFY_MAX_DRAFTS = 64, VERIFY_MAX_VOCAB = 1 << 24;
+constexpr int VERIFY_SLICE = 4096, VERIFY_MAX_DRAFTS = 64, VERIFY_MAX_VOCAB = 1 << 24, VERIFY_MAX_SLICES = 1 << 23;
 hipError_t launch_verify(const VerifyArgs & a, int dtype, bool probs, hipStream_t st);
 
 } // namespace qkv

@@ -344,6 +344,8 @@ __global__ __launch_bounds__(PT) void k_verify_pick(VerifyArgs a) {
                         const float top = pp[S.skip / VERIFY_SLICE].top; // (-infinity: a slice of masked entries, less is 0)
                         less = less > 0 ? less * exp2_neg(((double) top - (double) S.top) * S.beta) : 0.0;
                     }
+                    // (below it, the slice's sum could have a weight where each entry's alone is zero)
+                    if (!(less > 1e-290)) less = 0;
                 }
             }
             // every wave finds the slice by itself: lane l holds `per` slices from l per on

@@ -165,6 +165,15 @@ def test_strides_and_alignment(qkv, torch_gpu, dt):
     run(torch_gpu, qkv, *make(rng, 3, 2, 5003, True), dt=dt, pad=7, off=3)
 
 
+def test_weights_below_the_smallest(qkv, torch_gpu):
+    """A refused draft whose slice holds entries of e^-748 beside it: each is nothing in 64 bits, their sum would not be."""
+    logits = np.full((1, 2, 8192), -np.inf)
+    logits[0, 0, :4096], logits[0, 0, 5], logits[0, 0, 5000] = -374.0, 0.0, 374.0
+    logits[0, 1, 7] = 1.0
+    got = run(torch_gpu, qkv, logits, None, None, np.array([[5]], np.int32), np.array([[0.5, 0.0]], np.float32))
+    assert got[1].tolist() == [[5000, -1]]
+
+
 def test_random_numbers_outside(qkv, torch_gpu):
     """u[n] of 1 or more: the last entry with a weight; nothing is read or written outside."""
     v = 9000

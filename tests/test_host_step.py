@@ -13,7 +13,7 @@ def norm(qkv, **kw):
 
 
 @pytest.mark.parametrize("kw,msg", [
-    (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(rows=-1), "rows"), (dict(dim=0), "dim"), (dict(dim=32769, xs=40000), "dim"),
+    (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(rows=-1), "rows"), (dict(rows=(1 << 21) + 1), "rows"), (dict(dim=0), "dim"), (dict(dim=32769, xs=40000), "dim"),
     (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(eps=float("inf")), "eps"), (dict(a=0), "set"), (dict(m=0), "set"),
     (dict(dim=96, xs=96, rs=96, ss=96, ys=96), "multiple of 64"), (dict(sum=0, y=0, a=0, b=0, m=0), "no output"), (dict(x=0), "null x"), (dict(w=0), "null w"),
     (dict(xs=63), "x_stride"), (dict(rs=1), "res_stride"), (dict(ss=0), "sum_stride"), (dict(ys=63), "y_stride"), (dict(ss=65), "stride"),
@@ -56,7 +56,7 @@ def verify(qkv, **kw):
 
 @pytest.mark.parametrize("kw,msg", [
     (dict(b=-1), "n_seq"), (dict(b=65536), "n_seq"), (dict(n=-1), "n_draft"), (dict(n=65), "n_draft"), (dict(v=0), "vocab"), (dict(v=(1 << 24) + 1), "vocab"),
-    (dict(b=60000, n=64, v=1 << 22, rs=1 << 22), "too many"), (dict(dtype=3), "dtype"), (dict(probs=2), "probs"), (dict(probs=1, dtype=1), "fp32"),
+    (dict(b=60000, n=64, v=1 << 22, rs=1 << 22), "too many"), (dict(b=1 << 15, n=63, v=4 * 4096 + 1, rs=1 << 20), "too many"), (dict(dtype=3), "dtype"), (dict(probs=2), "probs"), (dict(probs=1, dtype=1), "fp32"),
     (dict(probs=1, temp=A), "temperature"), (dict(rs=99), "row_stride"), (dict(t=0), "target"), (dict(u=0), "null u"), (dict(acc=0), "accepted"),
     (dict(tok=0), "tokens"), (dict(d=0), "drafts"), (dict(t=A + 2), "target is not"), (dict(dtype=2, t=A + 1), "target is not"), (dict(u=A + 2), "aligned"),
     (dict(q=A + 1), "aligned"), (dict(ws=0), "workspace"), (dict(size=10), "workspace"), (dict(ws=A + 8), "ws is not"),
