@@ -12,6 +12,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 namespace qkv {
 
@@ -20,7 +21,6 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4_u8 __attribute__((ext_vector_type(4), aligned(8)));
 typedef unsigned u32x4_u2 __attribute__((ext_vector_type(4), aligned(2)));
-
 
 enum { XM_UNITS = 0, XM_HALF = 1, XM_SPLIT = 2 }; // x as int8 units, as one fp16 part, as two
 
@@ -199,10 +199,12 @@ __device__ __forceinline__ u32x4 w4_scales(const uint16_t * p, int gs, int grp) 
     return e;
 }
 
-constexpr int W4_RUN = 2;   // steps a wave takes together: the 128 bytes of a cache line of every row
+constexpr int W4_RUN = 2;   // steps a wave takes together: the 128 bytes of a cache line of every row (4 and 8: within 1% of it, with more code)
 constexpr int W4_WIN = 32;  // scales of a weight row that a wave holds in LDS at a time
 
 // NR activation rows per group of four operand rows, RG groups: MR = NR RG rows a pass.
+// What bounds it: the codes' way from HBM where there are many (150,001 x 5,120 on one row, 393 MB: 82 us, 5.2 TB/s with x and
+// y, of 6.0 that a plain read reaches), else the chain of launch, x and first loads (1,024 x 5,120: 4.6 us).
 // P parts: a tile is 16 / P weight rows, and lanes n = 16 / P h + j hold row j of part h, a P-th of its blocks.  A group's
 // operand row NR h + m is then x[m] of part h's block (P NR <= 4), and a lane takes its own part's sums: with few
 // rows of x the tiles get smaller, and a short projection has enough of them for every CU.
@@ -419,7 +421,8 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
 // that one instruction takes 16 rows of x against one block of 16 weight rows, without zeros, and every lane has its weight
 // row's scale of each block.  A workgroup takes up to 2 NTW tiles: 4 waves along the blocks of a chunk (U steps each) times 2
 // along the tiles; a piece of x read from LDS serves the wave's NTW tiles.  What bounds it is the fold of the blocks'
-// integer sums into fp32: three instructions per (row, block, weight row).
+// integer sums into fp32, three instructions per (row, block, weight row) in three of four vector instructions (64 rows of
+// 17,408 x 5,120: 35.6 us, the vector units busy for 71% of them, the matrix units for 16%).
 __device__ __forceinline__ void w4_exchange(const u32x4 & d, unsigned (&t)[4]) { // t[b] in lane group q: dword q of lane group b's d
     const auto x = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false), y = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
     const auto v = __builtin_amdgcn_permlane16_swap(x[0], y[0], false, false), w = __builtin_amdgcn_permlane16_swap(x[1], y[1], false, false);
@@ -435,8 +438,8 @@ template <int MODE, int MT, int CB, bool MINS> constexpr int wide_buf() {
 }
 
 // WK waves along the blocks of a chunk, U steps each, times WN along the tiles.  ODD: a workgroup of an odd number of tiles,
-// whose second half of the waves has one less (an even number needs no branch: 64 rows of 14,336 x 5,120, 30.7 us, with it
-// 32.7; 17,408, five tiles a workgroup: 41.3 without and 37.9 with)
+// whose second half of the waves has one less, with a loop body of its own (64 rows of 17,408 x 5,120, five tiles a workgroup:
+// 35.6 us, with the sixth worked on and dropped 41.3)
 template <int MODE, int DT, int MT, int NTW, int WK, int WN, int U, bool ODD, bool MINS>
 __global__ __launch_bounds__(WK * WN * 64, WK * WN / 4) void k_w4_wide(W4Args a) {
     constexpr int WIDE_W = WK * WN, TM = 16 * MT, CB = 4 * WK * U, BB = planes(MODE) * TM * 16, BUF = wide_buf<MODE, MT, CB, MINS>();
@@ -575,61 +578,65 @@ __global__ __launch_bounds__(WK * WN * 64, WK * WN / 4) void k_w4_wide(W4Args a)
         __builtin_amdgcn_sched_barrier(0);
         const uint8_t * xp = lds + buf * BUF;
         const float * dx = reinterpret_cast<const float *>(xp + DX), * ds = dx + CB * DS;
+        const auto fold = [&](auto of) { // the wave's first `of` tiles
+            constexpr int NT = decltype(of)::value;
 #pragma unroll
-        for (int u = 0; u < U; u++)
+            for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const int bl = 4 * (wk * U + u) + q;
-                i32x2 bi[NTW];
-                half8 bh[NTW];
+                for (int q = 0; q < 4; q++) {
+                    const int bl = 4 * (wk * U + u) + q;
+                    i32x2 bi[NT];
+                    half8 bh[NT];
 #pragma unroll
-                for (int t = 0; t < NTW; t++) {
-                    if constexpr (MODE == XM_UNITS) {
-                        int lo, hi;
-                        w4_bytes(bt[t][u][q], lo, hi);
-                        bi[t] = i32x2{lo, hi};
-                    } else bh[t] = w4_halves(bt[t][u][q]);
-                }
-#pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    // 16 rows of x and their factors, for every tile of the wave
-                    f32x4 d = *reinterpret_cast<const f32x4 *>(dx + bl * DS + 16 * i + 4 * g), e;
-                    if constexpr (MINS) e = *reinterpret_cast<const f32x4 *>(ds + bl * DS + 16 * i + 4 * g);
-                    i32x2 xi;
-                    if constexpr (MODE == XM_UNITS)
-                        xi = *reinterpret_cast<const i32x2 *>(xp + (16 * i + n) / RPC * 1040 + (16 * i + n) % RPC * 512 + (bl & 1) * CB * 16 +
-                                                              (bl & ~1) * 16 + 8 * g);
-#pragma unroll
-                    for (int t = 0; t < NTW; t++) {
-                        if (ODD && t == NTW - 1 && !last) break; // (this wave has a tile less)
-                        f32x4 f;
+                    for (int t = 0; t < NT; t++) {
                         if constexpr (MODE == XM_UNITS) {
-                            i32x4 v = {0, 0, 0, 0};
-                            v = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, xi), __builtin_bit_cast(long, bi[t]), v, 0, 0, 0);
+                            int lo, hi;
+                            w4_bytes(bt[t][u][q], lo, hi);
+                            bi[t] = i32x2{lo, hi};
+                        } else bh[t] = w4_halves(bt[t][u][q]);
+                    }
 #pragma unroll
-                            for (int r = 0; r < 4; r++) f[r] = (float) v[r];
-                        } else {
-                            f = f32x4{0, 0, 0, 0};
+                    for (int i = 0; i < MT; i++) {
+                        // 16 rows of x and their factors, for every tile of the wave
+                        f32x4 d = *reinterpret_cast<const f32x4 *>(dx + bl * DS + 16 * i + 4 * g), e;
+                        if constexpr (MINS) e = *reinterpret_cast<const f32x4 *>(ds + bl * DS + 16 * i + 4 * g);
+                        i32x2 xi;
+                        if constexpr (MODE == XM_UNITS)
+                            xi = *reinterpret_cast<const i32x2 *>(xp + (16 * i + n) / RPC * 1040 + (16 * i + n) % RPC * 512 + (bl & 1) * CB * 16 +
+                                                                  (bl & ~1) * 16 + 8 * g);
 #pragma unroll
-                            for (int k = planes(MODE) - 4; k >= 0; k -= 4)
-                                f = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const half8 *>(xp + bl * BB + ((k + g) * TM + 16 * i + n) * 16),
-                                                                           bh[t], f, 0, 0, 0);
-                        }
+                        for (int t = 0; t < NT; t++) {
+                            f32x4 f;
+                            if constexpr (MODE == XM_UNITS) {
+                                i32x4 v = {0, 0, 0, 0};
+                                v = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, xi), __builtin_bit_cast(long, bi[t]), v, 0, 0, 0);
 #pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            acc[t][i][r] = __builtin_fmaf(f[r], sc[t][4 * u + q] * d[r], acc[t][i][r]);
-                            if constexpr (MINS) acc[t][i][r] = __builtin_fmaf(mn[t][4 * u + q], e[r], acc[t][i][r]);
+                                for (int r = 0; r < 4; r++) f[r] = (float) v[r];
+                            } else {
+                                f = f32x4{0, 0, 0, 0};
+#pragma unroll
+                                for (int k = planes(MODE) - 4; k >= 0; k -= 4)
+                                    f = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const half8 *>(xp + bl * BB + ((k + g) * TM + 16 * i + n) * 16),
+                                                                               bh[t], f, 0, 0, 0);
+                            }
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                acc[t][i][r] = __builtin_fmaf(f[r], sc[t][4 * u + q] * d[r], acc[t][i][r]);
+                                if constexpr (MINS) acc[t][i][r] = __builtin_fmaf(mn[t][4 * u + q], e[r], acc[t][i][r]);
+                            }
                         }
                     }
+                    // (a block at a time: the compiler would fold the chunk's sums at its end, and they do not fit the registers)
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int i = 0; i < MT; i++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++) asm volatile("" : "+v"(acc[t][i][r]));
                 }
-                // (a block at a time: the compiler would fold the chunk's sums at its end, and they do not fit the registers)
-#pragma unroll
-                for (int t = 0; t < NTW; t++)
-#pragma unroll
-                    for (int i = 0; i < MT; i++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++) asm volatile("" : "+v"(acc[t][i][r]));
-            }
+        };
+        if (!ODD || last) fold(std::integral_constant<int, NTW>{});
+        else if constexpr (ODD) fold(std::integral_constant<int, NTW - 1>{});
         if constexpr (ASYNC) {
             commit(cn, buf ^ 1);
             // the copies of x have landed: the U codes of NTW tiles behind them may still be on their way
@@ -659,7 +666,7 @@ __global__ __launch_bounds__(WK * WN * 64, WK * WN / 4) void k_w4_wide(W4Args a)
     }
 }
 
-constexpr int W4_LDS = 80 * 1024; // two workgroups per CU
+constexpr int W4_LDS = 80 * 1024; // of k_w4: two workgroups per CU
 // lets a kernel have more than 64 KiB of LDS: once per kernel and device (the flag is the kernel's own)
 template <class K> static hipError_t allow_lds(K k, size_t lds, std::atomic<uint64_t> & done) {
     if (lds <= 64 * 1024) return hipSuccess;
@@ -672,7 +679,7 @@ template <class K> static hipError_t allow_lds(K k, size_t lds, std::atomic<uint
     if (e == hipSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
     return e;
 }
-constexpr int W4_WAVES = 4096; // of a launch: 16 for each of 256 CUs, a quarter of what they hold
+constexpr int W4_WAVES = 4096; // of k_w4: 16 for each of 256 CUs
 
 template <int MODE, int DT, int NR, int RG, int P, int W>
 static hipError_t launch_k(W4Args a, hipStream_t st) {
@@ -712,15 +719,16 @@ static hipError_t launch_wide_k(const W4Args & a, dim3 grid, hipStream_t st) {
 }
 template <int MODE, int DT, int MT, int U, bool MINS>
 static hipError_t launch_wide_m(W4Args a, hipStream_t st) {
-    // a workgroup per CU with up to 2 * 3 tiles each where that is all of them, else two per CU with four tiles at a time,
-    // whose registers (and, of 64 rows, shorter chunks of x) leave room for both
+    // a workgroup per CU with up to 2 * 3 tiles each where that is all of them (16 rows of 17,408 x 5,120: 19 us, with two per
+    // CU of four tiles 21), else two per CU with four tiles at a time, whose registers (and, of 64 rows, shorter chunks of x)
+    // leave room for both (65,536: 16 rows 50 us, with rounds of 2 * 3 tiles 63; 64 rows 105 and 121)
     constexpr int CUS = 256, MOST = 6;
     const int tiles = (a.n + 15) / 16;
     const bool many = tiles > CUS * MOST;
     a.kcb = many ? 4 : (tiles + CUS - 1) / CUS;
     const dim3 grid((tiles + a.kcb - 1) / a.kcb, (a.rows + 16 * MT - 1) / (16 * MT));
     if (many) return launch_wide_k<MODE, DT, MT, 2, 4, 2, MT == 4 ? 1 : U, false, MINS>(a, grid, st);
-    if constexpr (U == 2) {
+    if constexpr (U == 2) { // one tile: all eight waves along the blocks
         if (a.kcb == 1) return launch_wide_k<MODE, DT, MT, 1, 8, 1, 1, false, MINS>(a, grid, st);
     }
     switch (a.kcb) {
@@ -744,6 +752,12 @@ static hipError_t launch_wide(const W4Args & a, hipStream_t st) {
     }
 }
 
+// By the rows of x, in us for 1,024 / 17,408 / 150,001 weight rows of 5,120, units:
+//   1     four parts     4.6 / 13.2 / 82   whole tiles of 16 weight rows  6.4 / 15.9 / 92
+//   2     two parts      5.3 / 13.7 / 87   whole tiles                    6.6 / 15.8 / 92
+//   3, 4  one group      6.2 / 16.0 / 93   two groups                     7.4 / 17.4 / 95
+//   5..8  two groups     7.2 / 17.5 / 97   dense                          7.2 / 18.4 / 118
+//   16    dense          7.6 / 18.2 / 118  four groups                   19.7 / 25.5 / 137
 template <int MODE, int DT>
 static hipError_t launch_mode(const W4Args & a, hipStream_t st) {
     if (a.rows == 1) return launch_k<MODE, DT, 1, 1, 4, 4>(a, st);
