@@ -29,16 +29,18 @@ constexpr int planes(int mode) { return mode == XM_UNITS ? 2 : mode == XM_HALF ?
 
 // x in LDS, kcb blocks at a time.  Units, as they come: per row the even blocks' kcb units, then the odd ones', padded so that the
 // 16 pieces an instruction takes (4 blocks of 4 rows) lie in different banks.  Plain rows, as fp16:
-// [kcb blocks][planes][MR rows][16 bytes].  Then zeros for the operand's other lanes, [kcb][MR] float factors of the blocks'
+// [kcb blocks][planes][MR rows][16 bytes], with 16 bytes behind every 8 blocks where k is in parts (their pieces then lie in different
+// banks).  Then zeros for the operand's other lanes, [kcb][MR] float factors of the blocks'
 // sums and (with m) [kcb][MR] float factors of m.
 struct W4Lds {
     int half, row, zero, dx, ds, end; // units: bytes of a row's even blocks, of a row; offsets of the zeros, the factors, what follows
 };
+constexpr int run_pad(int mr) { return mr <= 2 ? 16 : 0; }
 template <int MODE, int MR, bool MINS> __host__ __device__ __forceinline__ constexpr W4Lds w4_lds(int kcb) {
     W4Lds l{};
     l.half = ((kcb * 16 + 255) & ~255) + 16;
     l.row = 2 * l.half + 32;
-    l.zero = MODE == XM_UNITS ? MR * l.row : kcb * planes(MODE) * MR * 16;
+    l.zero = MODE == XM_UNITS ? MR * l.row : kcb * planes(MODE) * MR * 16 + kcb / 8 * run_pad(MR);
     l.dx = l.zero + (MODE == XM_UNITS ? 32 : planes(MODE) * MR * 16);
     l.ds = l.dx + kcb * MR * 4;
     l.end = ((MINS ? l.ds + kcb * MR * 4 : l.ds) + 15) & ~15;
@@ -98,7 +100,7 @@ template <int DT> struct W4Eighth {
             lo[e] = (_Float16) (v[k] - (float) hi[e]);
         }
         if (MODE == XM_SPLIT && __builtin_expect(wild, 0)) lo = half8{};
-        uint8_t * to = lds + (size_t) bl * (planes(MODE) * MR * 16) + (q * MR + m) * 16;
+        uint8_t * to = lds + bl * (planes(MODE) * MR * 16) + (bl >> 3) * run_pad(MR) + (q * MR + m) * 16;
         *reinterpret_cast<half8 *>(to) = hi;
         if constexpr (MODE == XM_SPLIT) *reinterpret_cast<half8 *>(to + 4 * MR * 16) = lo;
         if (q == 0) {
@@ -201,6 +203,7 @@ __device__ __forceinline__ u32x4 w4_scales(const uint16_t * p, int gs, int grp) 
 
 constexpr int W4_RUN = 2;   // steps a wave takes together: the 128 bytes of a cache line of every row (4 and 8: within 1% of it, with more code)
 constexpr int W4_WIN = 32;  // scales of a weight row that a wave holds in LDS at a time
+constexpr int W4_WROW = W4_WIN + 8; // ... a row's place: 16 rows' 80 bytes begin in different banks
 
 // NR activation rows per group of four operand rows, RG groups: MR = NR RG rows a pass.
 // What bounds it: the codes' way from HBM where there are many (150,001 x 5,120 on one row, 393 MB: 82 us, 5.2 TB/s with x and
@@ -211,7 +214,7 @@ constexpr int W4_WIN = 32;  // scales of a weight row that a wave holds in LDS a
 // W waves: 1 << wk_log of them share a tile, each a run of its steps, the others have tiles of their own.
 // The codes of the next run are loaded while a run is worked on, over the tiles' borders too.  The scales come
 // 32 a row at a time (64 contiguous bytes; a lane's own two bytes of each step would fetch every cache line many times),
-// through 1 KiB of LDS of the wave's own, in which every lane then finds its block's.
+// through LDS of the wave's own, in which every lane then finds its block's.
 template <int MODE, int DT, int NR, int RG, int P, int W, bool MINS>
 __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
     static_assert(P * NR <= 4, "parts share a group's four operand rows");
@@ -224,14 +227,14 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
     const int nb = a.k >> 5, tiles = (a.n + TR - 1) / TR, sets = (tiles + WN - 1) / WN;
     const int nbp = (nb + 4 * U * P - 1) / (4 * U * P) * (4 * U * P), pb = nbp / P; // blocks with padding, blocks of a part
     const int j = n % TR, h = n / TR;
-    uint16_t * win = reinterpret_cast<uint16_t *>(lds + L.end) + wave * (MINS ? 2 : 1) * 16 * W4_WIN; // [16][32] scales, then m
-    float * red = reinterpret_cast<float *>(lds + L.end + W * (MINS ? 2 : 1) * 16 * W4_WIN * 2);       // [2][waves][MR][TR]
+    uint16_t * win = reinterpret_cast<uint16_t *>(lds + L.end) + wave * (MINS ? 2 : 1) * 16 * W4_WROW; // [16][40] scales, then m
+    float * red = reinterpret_cast<float *>(lds + L.end + W * (MINS ? 2 : 1) * 16 * W4_WROW * 2);       // [2][waves][MR][TR]
     // the lane's piece of the diagonal operand: row n = 4 b + NR part + m, lane group b
     const int m = n % NR, a_part = (n & 3) / NR;
     const bool active = (n >> 2) == g && a_part < P;
     constexpr bool ROWS = MODE == XM_UNITS; // x by rows: a block's two units in its row's even or odd part
-    const int abase = !active ? L.zero : ROWS ? m * L.row + (g & 1) * L.half + (a_part * pb + (g & 2)) * 16 : (a_part * pb + g) * BB + m * 16;
-    const int astep = !active ? 0 : ROWS ? 64 : 4 * BB, agroup = !active ? 0 : ROWS ? NR * L.row : NR * 16;
+    const int abase = !active ? L.zero : ROWS ? m * L.row + (g & 1) * L.half + (a_part * pb + (g & 2)) * 16 : (a_part * pb + g) * BB + a_part * (pb / 8) * run_pad(MR) + m * 16;
+    const int astep = !active ? 0 : ROWS ? 64 : 4 * BB, apad = !active || ROWS ? 0 : run_pad(MR), agroup = !active ? 0 : ROWS ? NR * L.row : NR * 16;
     const int hb = P == 1 ? 0 : h * pb, myb = hb + g; // the first block of the lane's part, the lane's block of step 0
     // runs of the chunk of x that begins at block b0 (parts: all of x at once), and the wave's steps of them
     const auto runs = [&](int b0) { return (P == 1 ? min(a.kcb, nbp - b0) : pb) / (4 * U); };
@@ -320,18 +323,18 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
 #pragma unroll 1
             for (int s = begin(b0); s < s1; s += U) {
                 if (fresh) { // (the run's window: nx stands on this run)
-                    *reinterpret_cast<u32x4 *>(win + n * W4_WIN + 8 * g) = ws;
-                    if constexpr (MINS) *reinterpret_cast<u32x4 *>(win + 16 * W4_WIN + n * W4_WIN + 8 * g) = wm;
+                    *reinterpret_cast<u32x4 *>(win + n * W4_WROW + 8 * g) = ws;
+                    if constexpr (MINS) *reinterpret_cast<u32x4 *>(win + (16 + n) * W4_WROW + 8 * g) = wm;
                     asm volatile("" ::: "memory"); // (read below by other lanes and as another type)
                     sw = s;
                 }
                 advance();
-                const uint16_t * wp = win + n * W4_WIN;
+                const uint16_t * wp = win + n * W4_WROW;
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     // the codes leave their registers, then the next run's take them
                     const int at = (4 * (s + u - sw) + g) >> a.gsh;
-                    const float sc = h2f_bits(wp[at]), mn = MINS ? h2f_bits(wp[16 * W4_WIN + at]) : 0.f;
+                    const float sc = h2f_bits(wp[at]), mn = MINS ? h2f_bits(wp[16 * W4_WROW + at]) : 0.f;
                     i32x4 hbv[2];
                     half8 hw[4];
                     if constexpr (MODE == XM_UNITS) {
@@ -349,7 +352,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
                     __builtin_amdgcn_sched_barrier(0);
                     in[u] = load(u);
                     __builtin_amdgcn_sched_barrier(0);
-                    const uint8_t * ap = lds + abase + (s + u) * astep;
+                    const uint8_t * ap = lds + abase + (s + u) * astep + s / 2 * apad;
                     const float * dxp = dx + (4 * (s + u) + myb) * MR, * dsp = ds + (4 * (s + u) + myb) * MR;
                     // the sums of the lane's own part
                     const auto mine = [&](const auto & c, int r) {
@@ -685,7 +688,7 @@ template <int MODE, int DT, int NR, int RG, int P, int W>
 static hipError_t launch_k(W4Args a, hipStream_t st) {
     constexpr int MR = NR * RG, TR = 16 / P, PAD = 4 * W4_RUN;
     const int nb4 = (a.k / 32 + PAD * P - 1) / (PAD * P) * (PAD * P), tiles = (a.n + TR - 1) / TR;
-    const int more = 2 * W * MR * TR * 4 + W * (a.mins ? 2 : 1) * 16 * W4_WIN * 2; // the waves' sums, the windows of scales
+    const int more = 2 * W * MR * TR * 4 + W * (a.mins ? 2 : 1) * 16 * W4_WROW * 2; // the waves' sums, the windows of scales
     const auto size = [&](int kcb) { return (a.mins ? w4_lds<MODE, MR, true>(kcb) : w4_lds<MODE, MR, false>(kcb)).end + more; };
     a.kcb = std::min(nb4, W4_LDS / (planes(MODE) * MR * 16 + MR * 4) / PAD * PAD);
     while (size(a.kcb) > W4_LDS) a.kcb -= PAD;
