@@ -66,8 +66,9 @@ template <int DT, int E> __device__ __forceinline__ void load_run(const typename
 constexpr int run_of(int dt) { return dt == DT_F32 ? 4 : 8; }
 
 // One row's slice: 16 entries a thread, all loads of them ahead of the first use.  What bounds it is the arithmetic in 64 bits, 17
-// instructions an entry (64 x 8 rows of 150,001 fp32 logits: 42.6 us, 4.1 TB/s, the vector units busy for 84% of it; workgroups
-// that loop over slices with the next one's loads ahead: 54 to 86 us, by their registers); of few rows the launch (8 of 32,768: 4.1).
+// instructions an entry (64 sequences of up to 7 drafts over 150,001 fp32 logits, 173 MB: 42.6 us, 4.1 TB/s, the vector units
+// busy for 84% of it; workgroups that loop over slices with the next one's loads ahead: 54 to 86 us, by their registers); of few
+// rows the launch (8 of 32,768: 4.1).
 template <int DT, bool PROBS>
 __global__ __launch_bounds__(VT) void k_verify_rows(VerifyArgs a) {
     __shared__ float top[VT / 64];
@@ -276,7 +277,7 @@ __device__ __forceinline__ void weights(const VerifyArgs & a, const Source & S, 
     }
 }
 
-// (4 sequences of 3 drafts over 151,552 bf16 logits: 5.3 us, most of them the slices' sums, the decision and the refused row one after
+// (4 sequences of 3 drafts over 150,001 bf16 logits: 5.3 us, most of them the slices' sums, the decision and the refused row one after
 // the other)
 template <int DT, bool PROBS>
 __global__ __launch_bounds__(VT) void k_verify_residual(VerifyArgs a) {
