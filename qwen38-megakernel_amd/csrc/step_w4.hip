@@ -234,7 +234,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
     const bool active = (n >> 2) == g && a_part < P;
     constexpr bool ROWS = MODE == XM_UNITS; // x by rows: a block's two units in its row's even or odd part
     const int abase = !active ? L.zero : ROWS ? m * L.row + (g & 1) * L.half + (a_part * pb + (g & 2)) * 16 : (a_part * pb + g) * BB + a_part * (pb / 8) * run_pad(MR) + m * 16;
-    const int astep = !active ? 0 : ROWS ? 64 : 4 * BB, apad = !active || ROWS ? 0 : run_pad(MR), agroup = !active ? 0 : ROWS ? NR * L.row : NR * 16;
+    const int astep = !active ? 0 : ROWS ? 64 : 4 * BB, arun = U * astep + (!active || ROWS ? 0 : run_pad(MR)), agroup = !active ? 0 : ROWS ? NR * L.row : NR * 16;
     const int hb = P == 1 ? 0 : h * pb, myb = hb + g; // the first block of the lane's part, the lane's block of step 0
     // runs of the chunk of x that begins at block b0 (parts: all of x at once), and the wave's steps of them
     const auto runs = [&](int b0) { return (P == 1 ? min(a.kcb, nbp - b0) : pb) / (4 * U); };
@@ -320,8 +320,9 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
                 staged = nbp <= a.kcb;
             }
             const int s1 = end(b0);
+            int ax = abase + begin(b0) / U * arun;
 #pragma unroll 1
-            for (int s = begin(b0); s < s1; s += U) {
+            for (int s = begin(b0); s < s1; s += U, ax += arun) {
                 if (fresh) { // (the run's window: nx stands on this run)
                     *reinterpret_cast<u32x4 *>(win + n * W4_WROW + 8 * g) = ws;
                     if constexpr (MINS) *reinterpret_cast<u32x4 *>(win + (16 + n) * W4_WROW + 8 * g) = wm;
@@ -352,7 +353,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
                     __builtin_amdgcn_sched_barrier(0);
                     in[u] = load(u);
                     __builtin_amdgcn_sched_barrier(0);
-                    const uint8_t * ap = lds + abase + (s + u) * astep + s / 2 * apad;
+                    const uint8_t * ap = lds + (ax + u * astep);
                     const float * dxp = dx + (4 * (s + u) + myb) * MR, * dsp = ds + (4 * (s + u) + myb) * MR;
                     // the sums of the lane's own part
                     const auto mine = [&](const auto & c, int r) {
