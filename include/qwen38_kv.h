@@ -232,7 +232,8 @@ int mk_kv_profile(void * h, int enable, double * out, int cap);
  * activation units that mk_kv_attend_gated / mk_kv_attend_prep leave.  No handle, no memory of their own; asynchronous on
  * `stream`; every buffer is memory of the current device (checked).  dtype: 0 fp32, 1 fp16, 2 bf16.  Strides count
  * elements between rows.  Calls on different streams are independent of each other as long as their outputs and workspaces are.
- * The same call gives the same bits on every run.
+ * The same call gives the same bits on every run.  Outputs overlap neither each other nor an input but where a call says so; no
+ * rows (or sequences) is a call that does nothing and looks at no pointer.
  */
 
 /*
@@ -244,7 +245,7 @@ int mk_kv_profile(void * h, int enable, double * out, int cap);
  * q32a / q32b [rows][dim / 32][16] and q32meta [rows][dim / 32][4] in the layout of mk_kv_attend_gated.  A block's codes are
  * round(t 127 / max |t|), ties to even, of t = h w, its scale max |t| / (sqrt(mean(h^2) + eps) 127) as fp16: codes do not depend on the order
  * of the row's sum.  A row with an infinity or a NaN gives NaN scales, or codes of zero, as its y.
- * q32a / q32b are aligned to 16 bytes, q32meta to 8.  Other overlaps of outputs and inputs are not allowed.
+ * q32a / q32b are aligned to 16 bytes, q32meta to 8.
  */
 int mk_norm_q32(const void * x, long long x_stride, const void * res, long long res_stride, const float * w, int rows, int dim, float eps, int dtype,
                 void * sum, long long sum_stride, void * y, long long y_stride, void * q32a, void * q32b, unsigned short * q32meta, void * stream);

@@ -63,8 +63,7 @@ unsigned size_of(int dtype) {
 
 constexpr int W4_MAX_ROWS = 1 << 19, W4_MAX_N = 1 << 28, W4_MAX_K = 1 << 20;
 
-int w4(const W4Args & in, int group, int xform, void * stream) {
-    W4Args a = in;
+int w4(W4Args a, int group, int xform, void * stream) {
     if (a.rows < 0 || a.rows > W4_MAX_ROWS) bad("rows outside 0 .. 524288");
     if (a.n < 1 || a.n > W4_MAX_N) bad("n outside 1 .. 2^28");
     const int unit = xform == W4_UNITS ? 64 : 32;
@@ -73,6 +72,18 @@ int w4(const W4Args & in, int group, int xform, void * stream) {
     if (a.y_stride < a.n) bad("y_stride is less than n");
     a.gsh = group == 32 ? 0 : group == 64 ? 1 : 2;
     a.gs = (a.k + group - 1) / group;
+    if (!a.rows) return 0; // (an empty tensor's pointers are null)
+    if (xform == W4_UNITS) {
+        need(a.xa, "q32a");
+        need(a.xb, "q32b");
+        need(a.xmeta, "q32meta");
+        aligned(a.xa, 16, "q32a");
+        aligned(a.xb, 16, "q32b");
+        aligned(a.xmeta, 8, "q32meta");
+    } else {
+        need(a.x, "x");
+        aligned(a.x, size_of(xform), "x");
+    }
     need(a.codes, "codes");
     need(a.scales, "scales");
     need(a.y, "y");
@@ -80,7 +91,6 @@ int w4(const W4Args & in, int group, int xform, void * stream) {
     aligned(a.scales, 2, "scales");
     aligned(a.mins, 2, "mins");
     aligned(a.y, 4, "y");
-    if (!a.rows) return 0;
     const Device d;
     d.holds(a.codes, "codes");
     d.holds(a.scales, "scales");
@@ -119,6 +129,7 @@ int mk_norm_q32(const void * x, long long x_stride, const void * res, long long 
         if (rows < 0 || rows > NORM_MAX_ROWS) bad("rows outside 0 .. 2^21");
         if (dim < 1 || dim > NORM_MAX_DIM) bad("dim outside 1 .. 32768");
         if (!(eps >= 0.f) || std::isinf(eps)) bad("eps must be finite and not negative");
+        if (!rows) return 0; // (an empty tensor's pointers are null)
         if ((q32a != nullptr) != (q32b != nullptr) || (q32a != nullptr) != (q32meta != nullptr)) bad("the q32 outputs come as a set: a, b and meta");
         if (q32a && dim % 64) bad("q32 units need a dim that is a multiple of 64");
         if (!sum && !y && !q32a) bad("no output given");
@@ -138,7 +149,6 @@ int mk_norm_q32(const void * x, long long x_stride, const void * res, long long 
         aligned(q32a, 16, "q32a");
         aligned(q32b, 16, "q32b");
         aligned(q32meta, 8, "q32meta");
-        if (!rows) return 0;
         const Device d;
         d.holds(x, "x");
         d.holds(res, "res");
@@ -158,12 +168,6 @@ int mk_norm_q32(const void * x, long long x_stride, const void * res, long long 
 int mk_w4_units(int rows, int n, int k, int group, const void * codes, const void * scales, const void * mins, const void * q32a, const void * q32b,
                 const unsigned short * q32meta, float * y, long long y_stride, void * stream) {
     return guarded<int>([&] {
-        need(q32a, "q32a");
-        need(q32b, "q32b");
-        need(q32meta, "q32meta");
-        aligned(q32a, 16, "q32a");
-        aligned(q32b, 16, "q32b");
-        aligned(q32meta, 8, "q32meta");
         W4Args a{};
         a.codes = static_cast<const uint8_t *>(codes);
         a.scales = static_cast<const uint16_t *>(scales);
@@ -183,8 +187,7 @@ int mk_w4_units(int rows, int n, int k, int group, const void * codes, const voi
 int mk_w4_rows(int rows, int n, int k, int group, const void * codes, const void * scales, const void * mins, const void * x, long long x_stride,
                int dtype, float * y, long long y_stride, void * stream) {
     return guarded<int>([&] {
-        need(x, "x");
-        aligned(x, size_of(dtype), "x");
+        (void) size_of(dtype);
         if (x_stride < k) bad("x_stride is less than k");
         W4Args a{};
         a.codes = static_cast<const uint8_t *>(codes);
@@ -215,6 +218,7 @@ int mk_verify_drafts(int n_seq, int n_draft, int vocab, const void * target, lon
         if (probs && dtype != DT_F32) bad("probabilities are fp32");
         if (probs && temperature) bad("a temperature applies to logits");
         if (row_stride < vocab) bad("row_stride is less than vocab");
+        if (!n_seq) return 0; // (an empty tensor's pointers are null)
         need(target, "target");
         need(u, "u");
         need(accepted, "accepted");
@@ -224,7 +228,6 @@ int mk_verify_drafts(int n_seq, int n_draft, int vocab, const void * target, lon
         for (const void * p : {(const void *) temperature, (const void *) draft_probs, (const void *) drafts, (const void *) n_drafts, (const void *) u,
                                (const void *) accepted, (const void *) tokens, (const void *) draft_p})
             aligned(p, 4, "an array of 4-byte values");
-        if (!n_seq) return 0;
         if (!ws || ws_bytes < want) bad("the call needs " + std::to_string(want) + " bytes of workspace (mk_verify_ws)");
         aligned(ws, 16, "ws");
         const Device d;

@@ -105,6 +105,23 @@ def test_in_place_and_many_rows(qkv, torch_gpu, dt):
     run(torch_gpu, qkv, 1300, 5120, dt, inplace=True, out="units")
 
 
+def test_offsets_past_32_bits(qkv, torch_gpu):
+    """Rows 2^24 + 1 elements apart, 17 GB of them: every row's norm and sum, and nothing between them."""
+    torch, rows, dim, ld = torch_gpu, 260, 100, (1 << 24) + 1
+    buf = torch.zeros(rows * ld, device="cuda")
+    x = torch.randn(rows, dim, device="cuda")
+    v = buf.view(rows, ld)
+    v[:, :dim] = x
+    w = torch.ones(dim, device="cuda")
+    y = torch.empty(rows, dim, device="cuda")
+    qkv.norm_q32(x.data_ptr(), dim, buf.data_ptr(), ld, w.data_ptr(), rows, dim, 1e-6, 0, buf.data_ptr(), ld, y.data_ptr(), dim, 0, 0, 0)
+    torch.cuda.synchronize()
+    h = (2 * x).double()
+    ref = h / torch.sqrt((h * h).mean(1, keepdim=True) + 1e-6)
+    assert torch.equal(v[:, :dim], 2 * x) and not v[:, dim:dim + 64].any() and not v[:, -64:].any()
+    assert ((y.double() - ref).abs() <= ref.abs() * 4.01 * 2.0 ** -24).all()
+
+
 @pytest.mark.parametrize("dt", ["fp32", "bf16"])
 def test_zero_tiny_and_wild_rows(qkv, torch_gpu, dt):
     def edit(x, r):

@@ -86,6 +86,27 @@ def test_large_vocabulary(qkv, torch_gpu, q):
     run(torch_gpu, qkv, *make(rng, 3, 2, 150001, q), dt="bf16" if q else "fp32")
 
 
+@pytest.mark.parametrize("q", [False, True])
+def test_largest_vocabulary_and_strides(qkv, torch_gpu, q):
+    """2^24 entries a row (64 slices a lane), then rows 2^25 elements apart, 8.6 GB of them."""
+    rng = np.random.default_rng(23 + q)
+    run(torch_gpu, qkv, *make(rng, 1, 1, 1 << 24, q, spread=4.0), dt="bf16")
+    torch, b, n, v, stride = torch_gpu, 2, 31, 5000, 1 << 25
+    logits, temp, dp, drafts, u = make(rng, b, n, v, q)
+    logits[:, np.arange(n), drafts[0]] += 4
+    t = torch.from_numpy(logits.astype(np.float32)).cuda()
+    wide = torch.empty(b * (n + 1) * stride, device="cuda")
+    wide.view(b, n + 1, stride)[..., :v] = t
+    td, qd, dd, ud = (None if z is None else torch.from_numpy(np.ascontiguousarray(z)).cuda() for z in (temp, dp, drafts, u))
+    acc, tok = torch.zeros(b, dtype=torch.int32, device="cuda"), torch.zeros(b, n + 1, dtype=torch.int32, device="cuda")
+    ws = torch.empty(qkv.verify_ws(b, n, v), dtype=torch.uint8, device="cuda")
+    qkv.verify_drafts(b, n, v, wide.data_ptr(), stride, 0, 0, ptr(td), ptr(qd), dd.data_ptr(), 0, ud.data_ptr(), acc.data_ptr(), tok.data_ptr(), 0,
+                      ws.data_ptr(), ws.numel())
+    torch.cuda.synchronize()
+    want = verify_ref(t.double().cpu().numpy(), temp, False, dp, drafts, None, u)
+    assert np.array_equal(acc.cpu().numpy(), want[0]) and np.array_equal(tok.cpu().numpy(), want[1])
+
+
 def test_flat_distribution(qkv, torch_gpu):
     """Equal logits: the token is the entry that the random number points at, in every slice."""
     v, b = 30011, 40

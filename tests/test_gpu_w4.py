@@ -101,6 +101,43 @@ def test_many_weight_rows(qkv, torch_gpu, x):
         check(torch_gpu, qkv, 40, n, 128, 64, False, x)
 
 
+@pytest.mark.parametrize("x", ["units", "bf16", "fp32"])
+@pytest.mark.parametrize("n", [4090, 8000, 12000, 16001, 20000, 24500, 24600])
+def test_tiles_per_workgroup(qkv, torch_gpu, n, x):
+    """The dense form's one to six tiles a workgroup and its two workgroups a CU, of 16, 32, 64 rows and of several times that."""
+    for rows, mins in ((9, False), (30, True), (64, False), (50, True), (130, False)):
+        check(torch_gpu, qkv, rows, n, 192, 32 if mins else 64, mins, x)
+
+
+@pytest.mark.parametrize("rows,x", [(1, "units"), (8, "bf16"), (20, "units"), (40, "bf16")])
+def test_offsets_past_32_bits(qkv, torch_gpu, rows, x):
+    """4.9 GB of codes, plain rows of x over 17 GB; the last weight rows and some on the way."""
+    torch, n, k = torch_gpu, 300001, 32768
+    rng = np.random.default_rng(rows)
+    codes = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda")
+    s = (torch.rand(n, k // 128, device="cuda") * 0.01 + 0.001).half()
+    v = rng.standard_normal((rows, k)).astype(np.float32)
+    y = torch.zeros(rows, n, device="cuda")
+    if x == "units":
+        a, b, meta = units_of(v)
+        q, sc, _ = unpack_units(a, b, meta)
+        v = (q.astype(np.float64) * sc.astype(np.float64)[..., None]).reshape(rows, k)
+        ad, bd, xm = torch.from_numpy(a).cuda(), torch.from_numpy(b).cuda(), torch.from_numpy(meta.view(np.int16)).cuda()
+        qkv.w4_units(rows, n, k, 128, codes.data_ptr(), s.data_ptr(), 0, ad.data_ptr(), bd.data_ptr(), xm.data_ptr(), y.data_ptr(), n)
+    else:
+        stride = (1 << 33) // 2 // rows * 2 + 8
+        buf = torch.empty(rows * stride, dtype=torch.bfloat16, device="cuda")
+        buf.view(rows, stride)[:, :k] = torch.from_numpy(v).cuda()
+        v = buf.view(rows, stride)[:, :k].double().cpu().numpy()
+        qkv.w4_rows(rows, n, k, 128, codes.data_ptr(), s.data_ptr(), 0, buf.data_ptr(), stride, 2, y.data_ptr(), n)
+    torch.cuda.synchronize()
+    pick = np.r_[0:3, 131070:131075, 262142:262147, n - 20:n]
+    words = codes[torch.from_numpy(pick).cuda()].cpu().numpy().reshape(len(pick), k // 8, 4)
+    c = np.concatenate([words & 15, words >> 4], -1).reshape(len(pick), k)
+    ref, mag = w4_ref(c, s[torch.from_numpy(pick).cuda()].cpu().numpy(), None, 128, v)
+    assert (np.abs(y.cpu().numpy()[:, pick] - ref) <= w4_bound(k, mag, x != "units")).all()
+
+
 @pytest.mark.parametrize("x", ["fp16", "bf16", "fp32"])
 def test_value_ranges(qkv, torch_gpu, x):
     """Blocks of very different sizes, zeros, and the types' smallest values."""

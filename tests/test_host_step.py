@@ -74,6 +74,17 @@ def test_workspace_size(qkv):
             qkv.verify_ws(*bad)
 
 
+def test_empty_tensors(qkv):
+    """No rows: the calls return without a look at their pointers (an empty tensor's are null), but not with wrong sizes."""
+    norm(qkv, rows=0, x=0, res=0, sum=0, y=0, a=0, b=0, m=0)
+    w4(qkv, True, rows=0, x=0, b=0, m=0, y=0)
+    w4(qkv, False, rows=0, x=0, y=0)
+    verify(qkv, b=0, t=0, d=0, u=0, acc=0, tok=0, ws=0, size=0)
+    for f, kw in ((norm, dict(rows=0, dim=0)), (lambda q, **k: w4(q, True, **k), dict(rows=0, k=96)), (verify, dict(b=0, v=0))):
+        with pytest.raises(qkv.KVError):
+            f(qkv, **kw)
+
+
 def test_no_device_memory(qkv):
     import torch
     if torch.cuda.is_available():
