@@ -48,7 +48,7 @@ hipError_t launch_w4(const W4Args & a, int xform, hipStream_t st);
 struct VerifyPart {
     double sum; // of the weights, relative to the slice's largest logit (probabilities: as they are)
     float top;  // the largest logit (probabilities: 0); NaN: the slice holds a NaN or a +infinity
-    int arg;    // the largest logit's index, the lowest of equal ones (temperature 0 only)
+    int arg;    // temperature 0: the largest logit's index, the lowest of equal ones; else, in a draft's slice, the bits of its value
 };
 struct VerifyArgs {
     const void * target;  // [n_seq][n + 1][row_stride]

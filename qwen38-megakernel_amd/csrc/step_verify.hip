@@ -85,8 +85,8 @@ __global__ __launch_bounds__(VT) void k_verify_rows(VerifyArgs a) {
     for (int c = 0; c < VE / E; c++)
         load_run<DT, E>(static_cast<const typename Elem<DT>::T *>(a.target) + (long long) row * a.row_stride, at(c * E), a.vocab,
                         PROBS ? 0.f : -__builtin_inff(), *reinterpret_cast<float (*)[E]>(v + c * E));
-    // the slice of a draft that may be refused: also its sum without the draft, what is left over without q
-    const int d = !a.q && i < a.n ? a.drafts[b * a.n + i] : -1;
+    // the slice of a draft also leaves the draft's own value and, without q, its sum without the draft, what a refusal leaves over
+    const int d = i < a.n ? a.drafts[b * a.n + i] : -1;
     float m = -__builtin_inff();
     bool wild = false; // a NaN (a maximum leaves it out)
 #pragma unroll
@@ -125,6 +125,7 @@ __global__ __launch_bounds__(VT) void k_verify_rows(VerifyArgs a) {
         const bool holds = d >= 0 && d / VERIFY_SLICE == sl && d < a.vocab;
         double s = 0;
         if (holds) { // (on its own: the selects cost every slice a quarter more)
+            p.arg = __builtin_bit_cast(int, Elem<DT>::up(static_cast<const typename Elem<DT>::T *>(a.target)[(long long) row * a.row_stride + d]));
             double rest = 0;
             if (PROBS || m > -__builtin_inff()) {
 #pragma unroll
@@ -149,7 +150,7 @@ __global__ __launch_bounds__(VT) void k_verify_rows(VerifyArgs a) {
         if (holds && threadIdx.x == 0) {
             double rest = rests[0];
             for (int k = 1; k < VT / 64; k++) rest += rests[k];
-            a.rest[row] = rest;
+            if (!a.q) a.rest[row] = rest;
         }
     }
     if (threadIdx.x == 0) a.part[(size_t) row * a.nsl + sl] = p;
@@ -163,25 +164,27 @@ struct Verdict {
     float p[VERIFY_MAX_DRAFTS];       // the drafts' probabilities
     int ok[VERIFY_MAX_DRAFTS];        // accepted on its own
     int draft[VERIFY_MAX_DRAFTS];     // -1: outside the vocabulary
+    double less[VERIFY_MAX_DRAFTS];   // without q: the draft's slice without it, relative to the row's largest logit
 };
 
 // what a wave reads of one row: its first 64 slices, one a lane, and what belongs to its draft
 struct RowIn {
     VerifyPart part;
     int d; // the draft, -1 outside the vocabulary
-    float v, u, q;
+    float u, q;
+    double rest;
 };
-template <int DT> __device__ __forceinline__ RowIn load_row(const VerifyArgs & a, int b, int i) {
+__device__ __forceinline__ RowIn load_row(const VerifyArgs & a, int b, int i) {
     const long long row = (long long) b * (a.n + 1) + i;
     const int lane = threadIdx.x & 63;
-    RowIn in{{0.0, -__builtin_inff(), 0x7fffffff}, -1, 0.f, 0.f, 1.f};
+    RowIn in{{0.0, -__builtin_inff(), 0x7fffffff}, -1, 0.f, 1.f, 0.0};
     if (lane < a.nsl) in.part = a.part[row * a.nsl + lane];
     if (i < a.n) {
         const int d = a.drafts[b * a.n + i];
         in.u = a.u[row];
+        if (!a.q) in.rest = a.rest[row];
         if (d >= 0 && d < a.vocab) {
             in.d = d;
-            in.v = Elem<DT>::up(static_cast<const typename Elem<DT>::T *>(a.target)[row * a.row_stride + d]);
             if (a.q) in.q = a.q[((size_t) b * a.n + i) * a.vocab + d];
         }
     }
@@ -190,18 +193,18 @@ template <int DT> __device__ __forceinline__ RowIn load_row(const VerifyArgs & a
 
 // a wave per row, all NT threads; count and t: the sequence's drafts and temperature; kept (optional): [row][64] the weights
 // of the rows' first 64 slices; returns the accepted count in every thread
-template <int DT, bool PROBS, int NT>
+template <bool PROBS, int NT>
 __device__ __forceinline__ int decide(const VerifyArgs & a, int b, int & count, Temp & t, Verdict & V, double * kept) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const float ninf = -__builtin_inff();
     // (ahead of the sequence's own values: one wait for all of them.  A row behind the last draft is memory of the workspace
     // all the same, and what it holds is not used)
     RowIn in;
-    if (wave <= a.n) in = load_row<DT>(a, b, wave);
+    if (wave <= a.n) in = load_row(a, b, wave);
     count = count_of(a, b);
     t = temp_of(a, b);
     for (int i = wave; i <= count; i += NT / 64) {
-        if (i != wave) in = load_row<DT>(a, b, i);
+        if (i != wave) in = load_row(a, b, i);
         const VerifyPart * pp = a.part + ((long long) b * (a.n + 1) + i) * a.nsl;
         float m = in.part.top;
         bool wild = m != m;
@@ -229,12 +232,18 @@ __device__ __forceinline__ int decide(const VerifyArgs & a, int b, int & count, 
             z = m > ninf ? 1.0 : 0.0;
         } else z = wave_sum(z);
         if (wild || !(z < (double) __builtin_inff())) z = 0;
-        double pd = 0;
+        double pd = 0, less = in.rest;
         if (i < count && in.d >= 0 && z > 0) {
             if (!PROBS && t.greedy) pd = in.d == arg ? 1.0 : 0.0;
             else {
-                pd = weight<PROBS>(in.v, m, t.beta);
-                if (!PROBS) pd /= z;
+                const int sl = __builtin_amdgcn_readfirstlane(in.d / VERIFY_SLICE);
+                const int own = sl < 64 ? __builtin_amdgcn_readlane(in.part.arg, sl) : pp[sl].arg;
+                pd = weight<PROBS>(__builtin_bit_cast(float, own), m, t.beta);
+                if (!PROBS) {
+                    pd /= z;
+                    const float top = sl < 64 ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, in.part.top), sl)) : pp[sl].top;
+                    less = less > 0 ? less * exp2_neg(((double) top - (double) m) * t.beta) : 0.0; // (-infinity: a slice of masked entries)
+                }
             }
         }
         if (lane == 0) {
@@ -245,6 +254,8 @@ __device__ __forceinline__ int decide(const VerifyArgs & a, int b, int & count, 
                 V.draft[i] = in.d;
                 V.p[i] = (float) pd;
                 V.ok[i] = (double) in.u * (double) in.q < pd;
+                // (below it, the slice's sum could have a weight where each entry's alone is zero)
+                V.less[i] = less > 1e-290 ? less : 0.0;
             }
         }
     }
@@ -277,8 +288,8 @@ __device__ __forceinline__ void weights(const VerifyArgs & a, const Source & S, 
     }
 }
 
-// (4 sequences of 3 drafts over 150,001 bf16 logits: 5.3 us, most of them the slices' sums, the decision and the refused row one after
-// the other)
+// (4 sequences of 3 drafts over 150,001 bf16 logits: 5.3 us, most of them the slices' sums, the decision and the refused row one
+// after the other)
 template <int DT, bool PROBS>
 __global__ __launch_bounds__(VT) void k_verify_residual(VerifyArgs a) {
     __shared__ Verdict V;
@@ -286,7 +297,7 @@ __global__ __launch_bounds__(VT) void k_verify_residual(VerifyArgs a) {
     const int b = blockIdx.x / a.nsl, sl = blockIdx.x - b * a.nsl;
     int count;
     Temp t;
-    const int r = decide<DT, PROBS, VT>(a, b, count, t, V, nullptr);
+    const int r = decide<PROBS, VT>(a, b, count, t, V, nullptr);
     if ((!PROBS && t.greedy) || r == count || !(V.z[r] > 0)) return;
     const Source S{(long long) b * (a.n + 1) + r, a.q + ((size_t) b * a.n + r) * a.vocab, V.top[r], t.beta, 1.0 / V.z[r], -1};
     constexpr int E = run_of(DT);
@@ -308,20 +319,26 @@ __global__ __launch_bounds__(VT) void k_verify_residual(VerifyArgs a) {
     }
 }
 
-// inclusive sum over the lanes
+// inclusive sum over the lanes: within rows of 16, then the rows' last values over the next row, the first half's over the second
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_d(double v) { // (0 where the lane has no source)
+    const uint64_t x = __builtin_bit_cast(uint64_t, v);
+    const unsigned lo = (unsigned) __builtin_amdgcn_update_dpp(0, (int) (unsigned) x, CTRL, ROWS, 0xf, false),
+                   hi = (unsigned) __builtin_amdgcn_update_dpp(0, (int) (unsigned) (x >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t) hi << 32 | lo);
+}
 __device__ __forceinline__ double wave_scan(double v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const double o = __shfl_up(v, m, 64);
-        if (lane >= m) v += o;
-    }
+    v += dpp_d<0x111, 0xf>(v); // row_shr 1, 2, 4, 8
+    v += dpp_d<0x112, 0xf>(v);
+    v += dpp_d<0x114, 0xf>(v);
+    v += dpp_d<0x118, 0xf>(v);
+    v += dpp_d<0x142, 0xa>(v); // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
+    v += dpp_d<0x143, 0xc>(v);
     return v;
 }
 
 // What bounds the pick is its chain: the slices' sums, the decision, one slice's entries, two scans (one sequence of 7 drafts over 32,768:
-// 6.7 us, 64 over 150,001: 7.9).
-constexpr int PT = 1024; // threads of the pick: a wave per row, four entries of the slice per thread
+// 5.9 us, 64 over 150,001: 7.0).
+constexpr int PT = 512; // threads of the pick: a wave per row, eight entries of the slice per thread (1,024: 0.4 us more, two waves more a SIMD)
 constexpr int PE = VERIFY_SLICE / PT;
 
 template <int DT, bool PROBS>
@@ -329,50 +346,46 @@ __global__ __launch_bounds__(PT) void k_verify_pick(VerifyArgs a) {
     __shared__ Verdict V;
     __shared__ double sums[PT / 64];
     __shared__ double kept[(VERIFY_MAX_DRAFTS + 1) * 64];
-    __shared__ int s_at, s_last;
+    __shared__ int s_at, s_last, s_slice, s_pass;
+    __shared__ double s_left;
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float u32 = a.u[(long long) b * (a.n + 1) + a.n];
-    if (tid == 0) s_at = s_last = -1;
+    if (tid == 0) s_at = s_last = s_slice = -1;
+    const double first = a.q && lane < a.nsl ? a.rest[(size_t) b * a.nsl + lane] : 0.0; // (of up to 64 slices)
     int count;
     Temp t;
-    const int r = decide<DT, PROBS, PT>(a, b, count, t, V, kept);
+    const int r = decide<PROBS, PT>(a, b, count, t, V, kept);
     int token = -1;
     if (V.z[r] > 0) {
         if (!PROBS && t.greedy) token = V.arg[r];
         else {
             const long long row = (long long) b * (a.n + 1) + r;
             const VerifyPart * pp = a.part + row * a.nsl;
-            Source S{row, nullptr, V.top[r], t.beta, 1.0 / V.z[r], -1};
+            Source S{row, nullptr, V.top[r], t.beta, a.q ? 1.0 / V.z[r] : 1.0, -1};
             double less = 0; // the refused draft's slice without it
             if (r < count) {
                 if (a.q) S.q = a.q + ((size_t) b * a.n + r) * a.vocab;
-                else if ((S.skip = V.draft[r]) >= 0) {
-                    less = a.rest[row];
-                    if (!PROBS) {
-                        const float top = pp[S.skip / VERIFY_SLICE].top; // (-infinity: a slice of masked entries, less is 0)
-                        less = less > 0 ? less * exp2_neg(((double) top - (double) S.top) * S.beta) : 0.0;
-                    }
-                    // (below it, the slice's sum could have a weight where each entry's alone is zero)
-                    if (!(less > 1e-290)) less = 0;
-                }
+                else if ((S.skip = V.draft[r]) >= 0) less = V.less[r];
             }
-            // every wave finds the slice by itself: lane l holds `per` slices from l per on
+            // the slice, by the first wave: lane l holds `per` slices from l per on
             const int per = (a.nsl + 63) / 64;
-            for (int pass = 0; pass < 2; pass++) { // (again without q and skip where they leave nothing)
+            Source R = S;
+            for (int pass = 0; wave == 0 && pass < 2; pass++) { // (again without q and skip where they leave nothing)
                 const auto slice = [&](int s) -> double {
                     if (s >= a.nsl) return 0.0;
-                    if (S.q) return a.rest[(size_t) b * a.nsl + s];
-                    if (S.skip >= 0 && s == S.skip / VERIFY_SLICE) return less;
+                    if (R.q) return per == 1 ? first : a.rest[(size_t) b * a.nsl + s];
+                    if (R.skip >= 0 && s == R.skip / VERIFY_SLICE) return less;
                     if (per == 1) return kept[r * 64 + s];
                     const double x = pp[s].sum;
                     return PROBS ? x : x > 0 ? x * exp2_neg(((double) pp[s].top - (double) S.top) * S.beta) : 0.0;
                 };
                 double mine = 0;
+#pragma unroll 1
                 for (int k = 0; k < per; k++) mine += slice(lane * per + k);
                 const double incl = wave_scan(mine), total = __shfl(incl, 63, 64);
                 if (!(total > 0)) {
-                    S.q = nullptr;
-                    S.skip = -1;
+                    R.q = nullptr;
+                    R.skip = -1;
                     continue;
                 }
                 double ex = __shfl_up(incl, 1, 64); // (a lane's sum begins exactly where the one before it ends)
@@ -381,18 +394,35 @@ __global__ __launch_bounds__(PT) void k_verify_pick(VerifyArgs a) {
                 const uint64_t in = __ballot(mine > 0 && ex <= want && want < incl), any = __ballot(mine > 0);
                 // (none, for a random number of 1 or more: the last slice with a weight, and its last entry)
                 const int l = in ? (int) __builtin_ctzll(in) : 63 - (int) __builtin_clzll(any);
-                int sl = -1;
-                double run = ex;
-                for (int k = 0; k < per; k++) {
-                    const double x = slice(lane * per + k);
-                    if (!(x > 0)) continue;
-                    if (sl >= 0 && in && want < run) break;
-                    if (sl >= 0) ex = run;
-                    sl = lane * per + k;
-                    run += x;
+                int sl = lane;
+                if (per > 1) {
+                    sl = -1;
+                    double run = ex;
+#pragma unroll 1
+                    for (int k = 0; k < per; k++) {
+                        const double x = slice(lane * per + k);
+                        if (!(x > 0)) continue;
+                        if (sl >= 0 && in && want < run) break;
+                        if (sl >= 0) ex = run;
+                        sl = lane * per + k;
+                        run += x;
+                    }
                 }
-                sl = __shfl(sl, l, 64);
-                const double left = in ? want - __shfl(ex, l, 64) : __builtin_inf();
+                if (lane == l) {
+                    s_slice = sl;
+                    s_pass = pass;
+                    s_left = in ? want - ex : __builtin_inf();
+                }
+                break;
+            }
+            __syncthreads();
+            const int sl = s_slice;
+            if (sl >= 0) {
+                const double left = s_left;
+                if (s_pass) {
+                    S.q = nullptr;
+                    S.skip = -1;
+                }
                 double w[PE], s = 0;
                 weights<DT, PROBS, PE>(a, S, sl * VERIFY_SLICE + tid * PE, w);
 #pragma unroll
@@ -401,11 +431,12 @@ __global__ __launch_bounds__(PT) void k_verify_pick(VerifyArgs a) {
                 if (lane == 63) sums[wave] = part;
                 __syncthreads();
                 double base = 0;
-                for (int k = 0; k < wave; k++) base += sums[k];
+#pragma unroll
+                for (int k = 0; k < PT / 64; k++) base += k < wave ? sums[k] : 0.0; // (one after the other, as every wave adds them)
                 const double end = base + part;
                 double begin = __shfl_up(end, 1, 64);
                 if (lane == 0) begin = base;
-                if (s > 0) {
+                if (s > 0 && begin <= left && left < end) { // one thread, if any
                     double at = begin;
                     int last = -1, found = -1;
 #pragma unroll
@@ -415,7 +446,7 @@ __global__ __launch_bounds__(PT) void k_verify_pick(VerifyArgs a) {
                         at += w[k];
                         if (found < 0 && left < at) found = last;
                     }
-                    if (begin <= left && left < end) s_at = found < 0 ? last : found;
+                    s_at = found < 0 ? last : found;
                 }
                 const uint64_t some = __ballot(s > 0);
                 if (some && lane == 63 - (int) __builtin_clzll(some)) {
@@ -426,7 +457,6 @@ __global__ __launch_bounds__(PT) void k_verify_pick(VerifyArgs a) {
                 }
                 __syncthreads();
                 token = s_at < 0 ? s_last : s_at;
-                break;
             }
         }
     }
