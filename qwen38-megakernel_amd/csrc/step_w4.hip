@@ -29,18 +29,19 @@ constexpr int planes(int mode) { return mode == XM_UNITS ? 2 : mode == XM_HALF ?
 
 // x in LDS, kcb blocks at a time.  Units, as they come: per row the even blocks' kcb units, then the odd ones', padded so that the
 // 16 pieces an instruction takes (4 blocks of 4 rows) lie in different banks.  Plain rows, as fp16:
-// [kcb blocks][planes][MR rows][16 bytes], with 16 bytes behind every 8 blocks where k is in parts (their pieces then lie in different
-// banks).  Then zeros for the operand's other lanes, [kcb][MR] float factors of the blocks'
+// [kcb blocks][planes][MR rows][16 bytes], fp32's two parts with 16 bytes behind every 8 blocks where k is in parts: their pieces then
+// lie in different banks (2 rows of fp32 x 17,408 x 5,120: 26 us without, 24 with; one row of bf16 x 150,001, half the planes: 82 and
+// 85).  Then zeros for the operand's other lanes, [kcb][MR] float factors of the blocks'
 // sums and (with m) [kcb][MR] float factors of m.
 struct W4Lds {
     int half, row, zero, dx, ds, end; // units: bytes of a row's even blocks, of a row; offsets of the zeros, the factors, what follows
 };
-constexpr int run_pad(int mr) { return mr <= 2 ? 16 : 0; }
+constexpr int run_pad(int mode, int mr) { return mode == XM_SPLIT && mr <= 2 ? 16 : 0; }
 template <int MODE, int MR, bool MINS> __host__ __device__ __forceinline__ constexpr W4Lds w4_lds(int kcb) {
     W4Lds l{};
     l.half = ((kcb * 16 + 255) & ~255) + 16;
     l.row = 2 * l.half + 32;
-    l.zero = MODE == XM_UNITS ? MR * l.row : kcb * planes(MODE) * MR * 16 + kcb / 8 * run_pad(MR);
+    l.zero = MODE == XM_UNITS ? MR * l.row : kcb * planes(MODE) * MR * 16 + kcb / 8 * run_pad(MODE, MR);
     l.dx = l.zero + (MODE == XM_UNITS ? 32 : planes(MODE) * MR * 16);
     l.ds = l.dx + kcb * MR * 4;
     l.end = ((MINS ? l.ds + kcb * MR * 4 : l.ds) + 15) & ~15;
@@ -100,7 +101,7 @@ template <int DT> struct W4Eighth {
             lo[e] = (_Float16) (v[k] - (float) hi[e]);
         }
         if (MODE == XM_SPLIT && __builtin_expect(wild, 0)) lo = half8{};
-        uint8_t * to = lds + bl * (planes(MODE) * MR * 16) + (bl >> 3) * run_pad(MR) + (q * MR + m) * 16;
+        uint8_t * to = lds + bl * (planes(MODE) * MR * 16) + (bl >> 3) * run_pad(MODE, MR) + (q * MR + m) * 16;
         *reinterpret_cast<half8 *>(to) = hi;
         if constexpr (MODE == XM_SPLIT) *reinterpret_cast<half8 *>(to + 4 * MR * 16) = lo;
         if (q == 0) {
@@ -233,8 +234,11 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
     const int m = n % NR, a_part = (n & 3) / NR;
     const bool active = (n >> 2) == g && a_part < P;
     constexpr bool ROWS = MODE == XM_UNITS; // x by rows: a block's two units in its row's even or odd part
-    const int abase = !active ? L.zero : ROWS ? m * L.row + (g & 1) * L.half + (a_part * pb + (g & 2)) * 16 : (a_part * pb + g) * BB + a_part * (pb / 8) * run_pad(MR) + m * 16;
-    const int astep = !active ? 0 : ROWS ? 64 : 4 * BB, arun = U * astep + (!active || ROWS ? 0 : run_pad(MR)), agroup = !active ? 0 : ROWS ? NR * L.row : NR * 16;
+    const int abase = !active ? L.zero
+                      : ROWS  ? m * L.row + (g & 1) * L.half + (a_part * pb + (g & 2)) * 16
+                              : (a_part * pb + g) * BB + a_part * (pb / 8) * run_pad(MODE, MR) + m * 16;
+    const int astep = !active ? 0 : ROWS ? 64 : 4 * BB, arun = U * astep + (!active || ROWS ? 0 : run_pad(MODE, MR)); // a step, a run
+    const int agroup = !active ? 0 : ROWS ? NR * L.row : NR * 16;
     const int hb = P == 1 ? 0 : h * pb, myb = hb + g; // the first block of the lane's part, the lane's block of step 0
     // runs of the chunk of x that begins at block b0 (parts: all of x at once), and the wave's steps of them
     const auto runs = [&](int b0) { return (P == 1 ? min(a.kcb, nbp - b0) : pb) / (4 * U); };
