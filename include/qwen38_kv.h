@@ -273,7 +273,7 @@ int mk_w4_rows(int rows, int n, int k, int group, const void * codes, const void
  * output head; the accepted length is what mk_kv_rewind keeps).  For each of n_seq sequences, with n = n_draft (0..64) drafts:
  *   target      [n_seq][n + 1][row_stride] logits of dtype (probs 0), or fp32 probabilities (probs 1); vocab 1..2^24 entries a row.  Row
  *               i is the distribution after draft i - 1
- *   temperature fp32 [n_seq] or NULL (1): p = softmax(logits / temperature); 0: all on the largest logit, the lowest
+ *   temperature fp32 [n_seq] or NULL (1): p = softmax(logits / temperature); 0 (less, or a NaN): all on the largest logit, the lowest
  *               index of equal ones.  -infinity masks an entry
  *   draft_probs fp32 [n_seq][n][vocab], the distributions q the drafts were drawn from, or NULL: q is 1 at the draft (a greedy drafter)
  *   drafts      int [n_seq][n]; one outside the vocabulary is refused.  n_drafts int [n_seq] or NULL: sequences with fewer drafts
