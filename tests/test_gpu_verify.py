@@ -186,6 +186,15 @@ def test_strides_and_alignment(qkv, torch_gpu, dt):
     run(torch_gpu, qkv, *make(rng, 3, 2, 5003, True), dt=dt, pad=7, off=3)
 
 
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+def test_temperatures(qkv, torch_gpu, dt):
+    """Greedy at zero, below it and for a NaN; the smallest and very large ones; all in one batch."""
+    rng = np.random.default_rng(41)
+    logits, _, _, drafts, u = make(rng, 8, 3, 5000, False)
+    temp = np.array([0.0, -1.0, np.nan, 1e-30, 1e-3, 0.05, 50.0, 1e30], np.float32)
+    run(torch_gpu, qkv, logits, temp, None, drafts, u, dt=dt)
+
+
 def test_weights_below_the_smallest(qkv, torch_gpu):
     """A refused draft whose slice holds entries of e^-748 beside it: each is nothing in 64 bits, their sum would not be."""
     logits = np.full((1, 2, 8192), -np.inf)
