@@ -200,7 +200,7 @@ __device__ __forceinline__ void vpairs(const VRaw<B> & v, int j, int w, unsigned
 // M0 + 16 lane), issued from inline assembly so that the waits are explicit: the compiler would otherwise wait for
 // every outstanding copy before the first LDS read.  Nothing else in the tile loop issues vector-memory loads, so
 // `s_waitcnt vmcnt(n)` with n = the copies of the younger tile in flight is exact.  M0 is not allocatable; only
-// these copies set it in this kernel.
+// these copies set it in this kernel (QKV_SET_M0, kv_dev.h).
 // Stage layout (STAGE_BYTES, one per wave and stage): K rows [32][32 KB], V rows [32][32 VB], K scales [32][8],
 // V scales [32][8] (fp16).  Rows past the end of the context are copies of the last row (finite, masked later).
 // The copies carry the non-temporal hint (nt): each tile is read once, so it is streamed through the L2 without
@@ -213,15 +213,15 @@ __device__ __forceinline__ void vpairs(const VRaw<B> & v, int j, int w, unsigned
 // the row batches of one decode segment)
 template <bool NT = true>
 __device__ __forceinline__ void dma16(const void * g, unsigned lds) {
-    if constexpr (NT) asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" QKV_DMA_CPOL ::"s"(lds), "v"(g) : "memory");
-    else asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
+    if constexpr (NT) asm volatile(QKV_SET_M0 "global_load_lds_dwordx4 %1, off" QKV_DMA_CPOL ::"s"(lds), "v"(g) : "memory");
+    else asm volatile(QKV_SET_M0 "global_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
 }
 // the same with a scalar base address and a 32-bit per-lane byte offset (no 64-bit vector address per copy)
 template <bool NT = true>
 __device__ __forceinline__ void dma16s(const void * base, unsigned voff, unsigned lds) {
     if constexpr (NT)
-        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" QKV_DMA_CPOL ::"s"(lds), "v"(voff), "s"(base) : "memory");
-    else asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(voff), "s"(base) : "memory");
+        asm volatile(QKV_SET_M0 "global_load_lds_dwordx4 %1, %2" QKV_DMA_CPOL ::"s"(lds), "v"(voff), "s"(base) : "memory");
+    else asm volatile(QKV_SET_M0 "global_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(voff), "s"(base) : "memory");
 }
 // N (1..4) consecutive 1 KiB pieces from one scalar base: M0 set once, the instruction offset (0, 1024, 2048, 3072)
 // added to both the global and the LDS address of each copy
@@ -230,22 +230,22 @@ template <int N, bool NT = true>
 __device__ __forceinline__ void dma16s_run(const void * base, unsigned voff, unsigned lds) {
     static_assert(N >= 1 && N <= 4, "one to four pieces");
     if constexpr (NT) {
-        if constexpr (N == 1) asm volatile("s_mov_b32 m0, %0\n\t" QKV_DMA_AT(0, QKV_DMA_CPOL) ::"s"(lds), "v"(voff), "s"(base) : "memory");
+        if constexpr (N == 1) asm volatile(QKV_SET_M0 QKV_DMA_AT(0, QKV_DMA_CPOL) ::"s"(lds), "v"(voff), "s"(base) : "memory");
         if constexpr (N == 2)
-            asm volatile("s_mov_b32 m0, %0\n\t" QKV_DMA_AT(0, QKV_DMA_CPOL) QKV_DMA_AT(1024, QKV_DMA_CPOL) ::"s"(lds), "v"(voff), "s"(base) : "memory");
+            asm volatile(QKV_SET_M0 QKV_DMA_AT(0, QKV_DMA_CPOL) QKV_DMA_AT(1024, QKV_DMA_CPOL) ::"s"(lds), "v"(voff), "s"(base) : "memory");
         if constexpr (N == 3)
-            asm volatile("s_mov_b32 m0, %0\n\t" QKV_DMA_AT(0, QKV_DMA_CPOL) QKV_DMA_AT(1024, QKV_DMA_CPOL) QKV_DMA_AT(2048, QKV_DMA_CPOL)
+            asm volatile(QKV_SET_M0 QKV_DMA_AT(0, QKV_DMA_CPOL) QKV_DMA_AT(1024, QKV_DMA_CPOL) QKV_DMA_AT(2048, QKV_DMA_CPOL)
                          ::"s"(lds), "v"(voff), "s"(base) : "memory");
         if constexpr (N == 4)
-            asm volatile("s_mov_b32 m0, %0\n\t" QKV_DMA_AT(0, QKV_DMA_CPOL) QKV_DMA_AT(1024, QKV_DMA_CPOL) QKV_DMA_AT(2048, QKV_DMA_CPOL)
+            asm volatile(QKV_SET_M0 QKV_DMA_AT(0, QKV_DMA_CPOL) QKV_DMA_AT(1024, QKV_DMA_CPOL) QKV_DMA_AT(2048, QKV_DMA_CPOL)
                              QKV_DMA_AT(3072, QKV_DMA_CPOL) ::"s"(lds), "v"(voff), "s"(base) : "memory");
     } else {
-        if constexpr (N == 1) asm volatile("s_mov_b32 m0, %0\n\t" QKV_DMA_AT(0, "") ::"s"(lds), "v"(voff), "s"(base) : "memory");
-        if constexpr (N == 2) asm volatile("s_mov_b32 m0, %0\n\t" QKV_DMA_AT(0, "") QKV_DMA_AT(1024, "") ::"s"(lds), "v"(voff), "s"(base) : "memory");
+        if constexpr (N == 1) asm volatile(QKV_SET_M0 QKV_DMA_AT(0, "") ::"s"(lds), "v"(voff), "s"(base) : "memory");
+        if constexpr (N == 2) asm volatile(QKV_SET_M0 QKV_DMA_AT(0, "") QKV_DMA_AT(1024, "") ::"s"(lds), "v"(voff), "s"(base) : "memory");
         if constexpr (N == 3)
-            asm volatile("s_mov_b32 m0, %0\n\t" QKV_DMA_AT(0, "") QKV_DMA_AT(1024, "") QKV_DMA_AT(2048, "") ::"s"(lds), "v"(voff), "s"(base) : "memory");
+            asm volatile(QKV_SET_M0 QKV_DMA_AT(0, "") QKV_DMA_AT(1024, "") QKV_DMA_AT(2048, "") ::"s"(lds), "v"(voff), "s"(base) : "memory");
         if constexpr (N == 4)
-            asm volatile("s_mov_b32 m0, %0\n\t" QKV_DMA_AT(0, "") QKV_DMA_AT(1024, "") QKV_DMA_AT(2048, "") QKV_DMA_AT(3072, "")
+            asm volatile(QKV_SET_M0 QKV_DMA_AT(0, "") QKV_DMA_AT(1024, "") QKV_DMA_AT(2048, "") QKV_DMA_AT(3072, "")
                          ::"s"(lds), "v"(voff), "s"(base) : "memory");
     }
 }

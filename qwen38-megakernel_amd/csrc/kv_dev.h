@@ -59,6 +59,12 @@ __device__ __forceinline__ unsigned shfl_xor_u(unsigned v, int m) {
 }
 __device__ __forceinline__ float shfl_xor(float v, int m) { return __builtin_bit_cast(float, shfl_xor_u(__builtin_bit_cast(unsigned, v), m)); }
 
+// The start of an inline-assembly copy from memory to LDS, %0 the LDS address: a scalar write of M0 needs one wait state before
+// the copy that reads it, and the compiler, which places it for its own copies, does not look into assembly (without it a copy can
+// land at the address of the one before).  M0 is not allocatable and no code here uses it for anything else, so it is not among
+// the clobbers (which would only warn that it is reserved).
+#define QKV_SET_M0 "s_mov_b32 m0, %0\n\ts_nop 0\n\t"
+
 // max / sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48 with v_permlane16_swap / v_permlane32_swap (VALU exchanges
 // between 16-lane rows, no LDS round trip).  Two copies of the value go in; afterwards one register holds rows
 // (0, 0, 2, 2) and the other rows (1, 1, 3, 3) (then halves (lo, lo) / (hi, hi)), so every lane gets

@@ -51,7 +51,7 @@ template <int MODE, int MR, bool MINS> __host__ __device__ __forceinline__ const
 // 16 bytes per lane from its own address to LDS at lds + 16 lane, without a register (waited for with vm_drain)
 __device__ __forceinline__ void dma16(const void * g, unsigned lds) {
     lds = (unsigned) __builtin_amdgcn_readfirstlane(lds);
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
+    asm volatile(QKV_SET_M0 "global_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
 }
 __device__ __forceinline__ void vm_drain() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
