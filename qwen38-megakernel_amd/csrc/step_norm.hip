@@ -7,11 +7,15 @@
 //   units, per block of 32: t_j = h_j w_j, a = max |t|, code = round_to_even(t_j (127 / a)), scale = fp16(a (rs / 127))
 // The codes are taken before the norm's factor, which cancels in t / a: they then depend on nothing that a sum's order
 // changes, and with the sum in 64 bits neither do rs and the scales.
+// In a row whose rs = m 2^e is far from one (values near fp32's ends that eps does not lift) rs itself, t or 127 / a would leave
+// fp32's range, or its normal numbers, where y does not: there h_j 2^e and m take the places of h_j and rs, with the same bits.
 #include "step_dev.h"
 
 namespace qkv {
 
-// a block whose largest value is below this has no finite 127 / a: its codes and scale are zero
+constexpr int NORM_FAR = 32; // the largest |e| of a row that is worked on as it is
+// a block whose largest value is below this has no finite 127 / a; with rs up to 2^32 its scale is far below 2^-25, zero in fp16,
+// and so are its codes
 constexpr float NORM_TINY = 4e-37f;
 
 // A workgroup per row; thread t holds the chunks t, t + NT, .. (C of them) of 8 values, so a block of 32 is four
@@ -60,7 +64,16 @@ __global__ __launch_bounds__(1024) void k_norm(NormArgs a) {
     lds_barrier();
     s = red[0];
     for (int i = 1; i < NT / 64; i++) s += red[i];
-    const float rs = (float) (1.0 / __builtin_sqrt(s / a.dim + (double) a.eps));
+    double rs64 = 1.0 / __builtin_sqrt(s / a.dim + (double) a.eps);
+    const int e = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_exp(rs64)); // (0 of zero, an infinity and a NaN)
+    if (__builtin_expect(e < -NORM_FAR || e > NORM_FAR, 0)) {
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) h[c][i] = __builtin_ldexpf(h[c][i], e);
+        rs64 = __builtin_ldexp(rs64, -e);
+    }
+    const float rs = (float) rs64;
 #pragma unroll
     for (int c = 0; c < C; c++) {
         const int ch = tid + NT * c;

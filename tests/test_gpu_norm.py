@@ -146,6 +146,46 @@ def test_wild_rows_units_propagate(qkv, torch_gpu):
     assert np.isnan(sc[0]).all() and np.isnan(sc[1, 1]) and (sc[1, [0, 2, 3, 4, 5, 6, 7]] == 0).all() and np.isfinite(sc[2]).all()
 
 
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("eps", [0.0, 1e-38])
+@pytest.mark.parametrize("dim", [256, 5120, 20032])
+def test_rows_near_the_ends_of_the_type(qkv, torch_gpu, dim, eps, dt):
+    """Rows whose factor 1 / sqrt(mean) is near fp32's largest or smallest number or past them: y and its units are ordinary.
+    y carries three roundings and its own; a code the rounding to an integer and four (t, 127 / max, their product, the largest
+    value's), a scale those and fp16's."""
+    torch, T = torch_gpu, dtype_of(torch_gpu, dt)
+    g = torch.Generator().manual_seed(dim)
+    sizes = [1e-42 if dt == "fp32" else 5e-40, 3e-39, 1e-38, 1e-36, 1e-20, 1e-6, 1.0, 1e6, 1e12, 1e20, 1e30, 5e36, 1.0, 1.0]
+    x = torch.randn(len(sizes), dim, generator=g).clamp(-4, 4).double() * torch.tensor(sizes, dtype=torch.float64)[:, None]
+    x[-2] = 3e38 * torch.sign(x[-2])                              # close to the largest number everywhere
+    x[-1, :32] *= 1e-38                                            # a block with next to nothing in an ordinary row
+    x = x.to(T)
+    w = 1 + 0.2 * torch.randn(dim, generator=g)
+    w[64:96] *= 1e4                                                # (a block's products beyond the row's own range)
+    rows, nu = len(sizes), dim // 32
+    xd, wd = x.cuda(), w.cuda()
+    y = torch.empty_like(xd)
+    a, b = (torch.empty(rows, nu, 16, dtype=torch.int8, device="cuda") for _ in range(2))
+    m = torch.empty(rows, nu, 4, dtype=torch.int16, device="cuda")
+    qkv.norm_q32(xd.data_ptr(), dim, 0, 0, wd.data_ptr(), rows, dim, eps, CODE[dt], 0, 0, y.data_ptr(), dim, a.data_ptr(), b.data_ptr(), m.data_ptr(),
+                 torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    h, wn = x.double().numpy(), w.double().numpy()
+    rs = 1 / np.sqrt((h * h).mean(1, keepdims=True) + np.float64(np.float32(eps)))
+    y64, got = h * rs * wn, y.double().cpu().numpy()
+    assert (np.abs(got - y64) <= np.abs(y64) * (3.01 * 2.0 ** -24 + EPS_HALF[dt]) + (1e-44 if dt == "fp32" else 1e-40)).all()
+    q, sc, sums = unpack_units(a.cpu().numpy(), b.cpu().numpy(), m.cpu().numpy().view(np.uint16))
+    assert np.array_equal(sums, q.reshape(rows, nu, 2, 16).astype(np.int16).sum(-1, dtype=np.int16))
+    t = (h * wn).reshape(rows, nu, 32)
+    top = np.abs(t).max(-1)
+    scale = top * rs / 127
+    assert (np.abs(sc.astype(np.float64) - scale) <= scale * (2.0 ** -11 + 4.01 * 2.0 ** -24) + 2.0 ** -25).all()
+    some = scale > 2.0 ** -25                                      # (a scale of zero leaves its codes without a meaning)
+    want = t[some] * 127 / top[some][:, None]
+    assert (np.abs(q[some] - want) <= 0.5 + 127 * 4.01 * 2.0 ** -24).all()
+    assert some[:-1].all() == (eps == 0)
+
+
 def test_no_rows(qkv, torch_gpu):
     torch = torch_gpu
     x = torch.ones(64, device="cuda")
