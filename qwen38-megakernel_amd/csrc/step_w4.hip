@@ -202,6 +202,107 @@ __device__ __forceinline__ u32x4 w4_scales(const uint16_t * p, int gs, int grp) 
     return e;
 }
 
+// Plain rows with minimums, results that are an infinity or a NaN: the folds add s (c - 8) x and m x apart, which of an infinite x
+// can leave NaN where (s (c - 8) + m) x is infinite, and the sum of 32 values close to fp32's largest can pass it.  Those are
+// summed again term by term in 64 bits, of a row with infinities these alone; beside a NaN everything is one already.
+// A wave for one row of x: what the row has in it ...
+enum { ROW_FINITE = 0, ROW_INF = 1, ROW_NAN = 2 };
+template <int DT> __device__ __forceinline__ int w4_kind(const W4Args & a, int row) {
+    const typename Elem<DT>::T * x = static_cast<const typename Elem<DT>::T *>(a.x) + row * a.x_stride;
+    bool inf = false, nan = false;
+    for (int j = 8 * (threadIdx.x & 63); j < a.k; j += 512) {
+        float t[8];
+        load8<DT>(x + j, t);
+#pragma unroll
+        for (int i = 0; i < 8; i++) inf |= __builtin_fabsf(t[i]) == __builtin_inff(), nan |= t[i] != t[i];
+    }
+    return __ballot(nan) ? ROW_NAN : __ballot(inf) ? ROW_INF : ROW_FINITE;
+}
+// ... and its results, a column a lane
+template <int DT> __device__ __forceinline__ float w4_terms(const W4Args & a, int row, int col, int kind) {
+    const typename Elem<DT>::T * x = static_cast<const typename Elem<DT>::T *>(a.x) + row * a.x_stride;
+    const uint8_t * cp = a.codes + (size_t) col * (a.k >> 1);
+    const size_t s0 = (size_t) col * a.gs;
+    double sum = 0;
+#pragma unroll 1
+    for (int j0 = 0; j0 < a.k; j0 += 512) {
+        const int mine = j0 + 8 * (threadIdx.x & 63);
+        bool look = mine < a.k;
+        float t[8];
+        if (look && kind == ROW_INF) {
+            load8<DT>(x + mine, t);
+            look = false;
+#pragma unroll
+            for (int i = 0; i < 8; i++) look |= __builtin_fabsf(t[i]) == __builtin_inff();
+        }
+#pragma unroll 1
+        for (uint64_t todo = __ballot(look); todo; todo &= todo - 1) {
+            const int j = j0 + 8 * (int) __builtin_ctzll(todo), g = j >> (5 + a.gsh);
+            load8<DT>(x + j, t);
+            const unsigned w = *reinterpret_cast<const unsigned *>(cp + (j >> 1));
+            const double sc = h2f_bits(a.scales[s0 + g]), mn = h2f_bits(a.mins[s0 + g]);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (kind == ROW_FINITE || __builtin_fabsf(t[i]) == __builtin_inff())
+                    sum += (sc * ((int) (w >> (8 * (i & 3) + (i & 4)) & 15u) - 8) + mn) * (double) t[i];
+        }
+        if (!__ballot(sum == sum)) break;
+    }
+    return (float) sum;
+}
+__device__ __forceinline__ bool wild(float v) { return !(__builtin_fabsf(v) < __builtin_inff()); }
+
+// Those of a wave's own results, read back once all are stored.  Functions of their own, called where something is not finite: in
+// line they changed the loops' schedules (64 rows of bf16 x 17,408 x 5,120: 92 -> 95 us, as calls 93).
+__device__ __forceinline__ const W4Args * kernel_args() { return (const W4Args *) __builtin_amdgcn_kernarg_segment_ptr(); }
+// k_w4: rows of x below MR, tiles of TR weight rows
+template <int DT, int MR, int TR, int W>
+__device__ __attribute__((noinline)) void w4_again(const W4Args * ap, int first, int step) {
+    const W4Args a = *ap;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const bool one = a.wk_log == 0; // a wave per tile: its first TR lanes a column each; else the set's results over all threads
+    const int wn = wave >> a.wk_log, WN = W >> a.wk_log, sets = ((a.n + TR - 1) / TR + WN - 1) / WN;
+    const int i0 = one ? wn * MR * TR : wave * 64, i1 = one ? i0 + MR * TR : WN * MR * TR;
+#pragma unroll 1
+    for (int row = 0; row < min(MR, a.rows); row++) {
+        int kind = -1;
+#pragma unroll 1
+        for (int set = first; set < sets && kind != ROW_NAN; set += step)
+#pragma unroll 1
+            for (int i = i0; i < i1; i += one ? TR : W * 64) {
+                const int at = i + lane, col = (set * WN + at / TR / MR) * TR + at % TR;
+                float * y = a.y + row * a.y_stride + col;
+                const bool mine = at < i1 && (!one || lane < TR) && at / TR % MR == row && col < a.n && wild(*y);
+                if (!__ballot(mine)) continue;
+                if (kind < 0) kind = w4_kind<DT>(a, row);
+                if (kind == ROW_NAN) break;
+                const float v = w4_terms<DT>(a, row, mine ? col : 0, kind);
+                if (mine) *y = v;
+            }
+    }
+}
+// k_w4_wide: 16 columns of four rows a wave
+template <int DT, int TM, int NTW, int WN, int W>
+__device__ __attribute__((noinline)) void w4_wide_again(const W4Args * ap, int t0, int t1, int row0) {
+    const W4Args a = *ap;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
+#pragma unroll 1
+    for (int t = 0; t < NTW; t++)
+#pragma unroll 1
+        for (int i = wave * 64; i < WN * TM * 16; i += W * 64)
+#pragma unroll 1
+            for (int q = 0; q < 4; q++) {
+                const int row = row0 + (i >> 4) % TM + q, tile = t0 + (i >> 4) / TM + WN * t, col = tile * 16 + n;
+                float * y = a.y + row * a.y_stride + col;
+                const bool mine = g == q && tile < t1 && col < a.n && row < a.rows && wild(*y);
+                if (!__ballot(mine)) continue;
+                const int kind = w4_kind<DT>(a, row);
+                if (kind == ROW_NAN) continue;
+                const float v = w4_terms<DT>(a, row, mine ? col : 0, kind);
+                if (mine) *y = v;
+            }
+}
+
 constexpr int W4_RUN = 2;   // steps a wave takes together: the 128 bytes of a cache line of every row (4 and 8: within 1% of it, with more code)
 constexpr int W4_WIN = 32;  // scales of a weight row that a wave holds in LDS at a time
 constexpr int W4_WROW = W4_WIN + 8; // ... a row's place: 16 rows' 80 bytes begin in different banks
@@ -300,6 +401,8 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
             window();
         } else nx.s -= U;
     };
+    constexpr bool TERMS = MINS && MODE != XM_UNITS; // results that are not finite are looked at again
+    bool again = false;
     enter(blockIdx.x);
     window();
     u32x4 in[U];
@@ -404,7 +507,10 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
             if (lane < TR && tile * TR + lane < a.n) {
 #pragma unroll
                 for (int i = 0; i < MR; i++)
-                    if (i < a.rows) a.y[i * a.y_stride + tile * TR + lane] = acc[i / NR][i % NR];
+                    if (i < a.rows) {
+                        a.y[i * a.y_stride + tile * TR + lane] = acc[i / NR][i % NR];
+                        if (TERMS) again |= wild(acc[i / NR][i % NR]);
+                    }
             }
             continue;
         }
@@ -418,8 +524,14 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
             const int c = i % TR, mm = i / TR % MR, t = i / TR / MR, col = (set * WN + t) * TR + c;
             float v = rp[((t << a.wk_log) * MR + mm) * TR + c];
             for (int k = 1; k < WK; k++) v += rp[(((t << a.wk_log) + k) * MR + mm) * TR + c];
-            if (col < a.n && mm < a.rows) a.y[mm * a.y_stride + col] = v;
+            if (col < a.n && mm < a.rows) {
+                a.y[mm * a.y_stride + col] = v;
+                if (TERMS) again |= wild(v);
+            }
         }
+    }
+    if constexpr (TERMS) {
+        if (__builtin_expect(__ballot(again) != 0, 0)) w4_again<DT, MR, TR, W>(kernel_args(), blockIdx.x, G);
     }
 }
 
@@ -652,6 +764,8 @@ __global__ __launch_bounds__(WK * WN * 64, WK * WN / 4) void k_w4_wide(W4Args a)
             __syncthreads();
         }
     }
+    constexpr bool TERMS = MINS && MODE != XM_UNITS;
+    bool again = false;
     // the waves along the blocks, a tile of every wave at a time
     if constexpr (!ASYNC) __syncthreads();
     float * red = reinterpret_cast<float *>(lds); // [waves][TM][16]
@@ -669,8 +783,14 @@ __global__ __launch_bounds__(WK * WN * 64, WK * WN / 4) void k_w4_wide(W4Args a)
             float v = rp[0];
 #pragma unroll
             for (int k = 1; k < WK; k++) v += rp[k * TM * 16];
-            if (tile < t1 && col < a.n && row0 + m < a.rows) a.y[(long long) (row0 + m) * a.y_stride + col] = v;
+            if (tile < t1 && col < a.n && row0 + m < a.rows) {
+                a.y[(long long) (row0 + m) * a.y_stride + col] = v;
+                if (TERMS) again |= wild(v);
+            }
         }
+    }
+    if constexpr (TERMS) {
+        if (__builtin_expect(__ballot(again) != 0, 0)) w4_wide_again<DT, TM, NTW, WN, WIDE_W>(kernel_args(), t0, t1, row0);
     }
 }
 

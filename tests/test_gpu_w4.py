@@ -189,6 +189,37 @@ def test_lone_values(qkv, torch_gpu, x, rows):
     assert np.array_equal(got[0][there], ref[0][there])
 
 
+@pytest.mark.parametrize("x", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("rows,k", [(1, 256), (1, 2240), (2, 256), (2, 2240), (4, 256), (4, 2240), (8, 256), (8, 2240), (20, 2240), (40, 256)])
+def test_infinities_with_minimums(qkv, torch_gpu, x, rows, k):
+    """W x of an infinite x is infinite where W = s (c - 8) + m is not zero, whatever the signs of its two parts and also for c = 8;
+    and finite values whose block's sum passes fp32's largest leave what their products sum to.  The same for the row beside it."""
+    for kind in ("one", "two", "last", "nan", "large"):
+        if kind == "large" and x == "fp16":
+            continue
+
+        def edit(v, s):
+            m = min(1, rows - 1)
+            if kind == "one":
+                v[m, 70] = np.inf
+            elif kind == "two":
+                v[m, 70], v[m, 200] = -np.inf, np.inf
+            elif kind == "last":
+                v[m, k - 1] = -np.inf
+            elif kind == "nan":
+                v[m, 70], v[m, 71] = np.inf, np.nan
+            else:
+                v[m, 64:72] = 1.5e38
+            s[3] = 0
+        got, ref, mag = run(torch_gpu, qkv, rows, 300, k, 64, True, x, edit=edit, seed=len(kind))
+        assert np.array_equal(np.isnan(got), np.isnan(ref)), kind
+        wild = np.isinf(ref)
+        assert np.array_equal(got[wild], ref[wild]) and (kind in ("nan", "large") or wild.any())
+        fine = np.isfinite(ref)
+        assert (np.abs(got - ref)[fine] <= w4_bound(k, mag, True)[fine]).all(), kind
+        assert kind != "large" or fine.all()
+
+
 def test_no_rows_and_refusals(qkv, torch_gpu):
     torch = torch_gpu
     t = torch.zeros(4096, dtype=torch.uint8, device="cuda")
