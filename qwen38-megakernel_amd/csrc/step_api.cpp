@@ -32,7 +32,9 @@ template <class R, class F> R guarded(F f) {
 [[noreturn]] void bad(const std::string & msg) { throw std::runtime_error(msg); }
 
 void ck(hipError_t e, const char * what) {
-    if (e != hipSuccess) bad(std::string(what) + ": " + hipGetErrorString(e));
+    if (e == hipSuccess) return;
+    (void) hipGetLastError(); // (reported here, not by a later call)
+    bad(std::string(what) + ": " + hipGetErrorString(e));
 }
 
 // every buffer is memory of the device that the call runs on (a host address or another device's would fault the GPU)

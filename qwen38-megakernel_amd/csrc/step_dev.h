@@ -114,6 +114,12 @@ template <> struct Elem<DT_BF16> {
 
 template <int DT> __device__ __forceinline__ void load8(const typename Elem<DT>::T * p, float (&v)[8]) { Elem<DT>::open8(Elem<DT>::raw8(p), v); }
 
+// a launch and its own status (hipGetLastError would also give what an earlier call of the thread left)
+template <class A> inline hipError_t launch(void (*k)(A), dim3 grid, dim3 block, size_t lds, hipStream_t st, A a) {
+    void * args[] = {&a};
+    return hipLaunchKernel(reinterpret_cast<const void *>(k), grid, block, args, lds, st);
+}
+
 // the first n (1..8) of 8 values, the rest zero
 template <int DT> __device__ __forceinline__ void load_n(const typename Elem<DT>::T * p, int n, float (&v)[8]) {
     if (n >= 8) return load8<DT>(p, v);

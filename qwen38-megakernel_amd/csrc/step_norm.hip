@@ -124,10 +124,9 @@ template <int DT>
 static hipError_t launch_dt(const NormArgs & a, hipStream_t st) {
     const int chunks = (a.dim + 7) / 8;
     const auto nt = [&](int c) { return dim3((chunks + 64 * c - 1) / (64 * c) * 64); };
-    if (chunks <= 1024 && a.rows <= NORM_FEW) hipLaunchKernelGGL((k_norm<DT, 1>), dim3(a.rows), nt(1), 0, st, a);
-    else if (chunks <= 2048) hipLaunchKernelGGL((k_norm<DT, 2>), dim3(a.rows), nt(2), 0, st, a);
-    else hipLaunchKernelGGL((k_norm<DT, 4>), dim3(a.rows), nt(4), 0, st, a);
-    return hipGetLastError();
+    if (chunks <= 1024 && a.rows <= NORM_FEW) return launch(k_norm<DT, 1>, dim3(a.rows), nt(1), 0, st, a);
+    if (chunks <= 2048) return launch(k_norm<DT, 2>, dim3(a.rows), nt(2), 0, st, a);
+    return launch(k_norm<DT, 4>, dim3(a.rows), nt(4), 0, st, a);
 }
 
 hipError_t launch_norm(const NormArgs & a, int dtype, hipStream_t st) {

@@ -467,10 +467,10 @@ __global__ __launch_bounds__(PT) void k_verify_pick(VerifyArgs a) {
 
 template <int DT, bool PROBS>
 static hipError_t launch_v(const VerifyArgs & a, hipStream_t st) {
-    hipLaunchKernelGGL((k_verify_rows<DT, PROBS>), dim3((unsigned) a.n_seq * (a.n + 1) * a.nsl), dim3(VT), 0, st, a);
-    if (a.q && a.n) hipLaunchKernelGGL((k_verify_residual<DT, PROBS>), dim3((unsigned) a.n_seq * a.nsl), dim3(VT), 0, st, a);
-    hipLaunchKernelGGL((k_verify_pick<DT, PROBS>), dim3(a.n_seq), dim3(PT), 0, st, a);
-    return hipGetLastError();
+    hipError_t e = launch(k_verify_rows<DT, PROBS>, dim3((unsigned) a.n_seq * (a.n + 1) * a.nsl), dim3(VT), 0, st, a);
+    if (e == hipSuccess && a.q && a.n) e = launch(k_verify_residual<DT, PROBS>, dim3((unsigned) a.n_seq * a.nsl), dim3(VT), 0, st, a);
+    if (e == hipSuccess) e = launch(k_verify_pick<DT, PROBS>, dim3(a.n_seq), dim3(PT), 0, st, a);
+    return e;
 }
 
 hipError_t launch_verify(const VerifyArgs & a, int dtype, bool probs, hipStream_t st) {

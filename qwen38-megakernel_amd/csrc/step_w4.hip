@@ -829,8 +829,7 @@ static hipError_t launch_k(W4Args a, hipStream_t st) {
     const auto k = a.mins ? k_w4<MODE, DT, NR, RG, P, W, true> : k_w4<MODE, DT, NR, RG, P, W, false>;
     const hipError_t e = allow_lds(k, lds, done[a.mins != nullptr]);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k, grid, block, lds, st, a);
-    return hipGetLastError();
+    return launch(k, grid, block, lds, st, a);
 }
 
 template <int MODE, int DT, int MT, int NTW, int WK, int WN, int U, bool ODD, bool MINS>
@@ -842,8 +841,7 @@ static hipError_t launch_wide_k(const W4Args & a, dim3 grid, hipStream_t st) {
     static std::atomic<uint64_t> done;
     const hipError_t e = allow_lds(k, lds, done);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k, grid, dim3(WIDE_W * 64), lds, st, a);
-    return hipGetLastError();
+    return launch(k, grid, dim3(WIDE_W * 64), lds, st, a);
 }
 template <int MODE, int DT, int MT, int U, bool MINS>
 static hipError_t launch_wide_m(W4Args a, hipStream_t st) {

@@ -249,3 +249,28 @@ def test_same_bits_every_run(qkv, torch_gpu):
             w(qkv, u, y, rows, 0)
         torch.cuda.synchronize()
         assert all(torch.equal(y, ys[0]) for y in ys)
+
+
+def test_an_earlier_error_is_not_this_calls(qkv, torch_gpu):
+    """A HIP call of the thread that failed before (here a device that does not exist) does not turn these calls into errors."""
+    torch, hip = torch_gpu, qkv.lib()  # (the library's own HIP runtime)
+    rng = np.random.default_rng(1)
+    w, u = W4(torch, rng, 100, 256, 32), units(torch, 2, 256)
+    x, y, one = torch.ones(2, 256, device="cuda"), torch.zeros(2, 100, device="cuda"), torch.ones(256, device="cuda")
+    drafts, rnd = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.zeros(1, 2, device="cuda")
+    acc, tok = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.full((1, 2), -7, dtype=torch.int32, device="cuda")
+    ws = torch.zeros(qkv.verify_ws(1, 1, 100), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    stream = torch.cuda.current_stream().cuda_stream
+    try:
+        for call in (lambda: qkv.norm_q32(x.data_ptr(), 256, 0, 0, one.data_ptr(), 2, 256, 1e-6, 0, 0, 0, 0, 0, *(t.data_ptr() for t in u), stream),
+                     lambda: w(qkv, u, y, 2, stream),
+                     lambda: qkv.w4_rows(2, 100, 256, 32, w.cd.data_ptr(), w.sd.data_ptr(), 0, x.data_ptr(), 256, 0, y.data_ptr(), 100, stream),
+                     lambda: qkv.verify_drafts(1, 1, 100, y.data_ptr(), 100, 0, 0, 0, 0, drafts.data_ptr(), 0, rnd.data_ptr(), acc.data_ptr(),
+                                               tok.data_ptr(), 0, ws.data_ptr(), ws.numel(), stream)):
+            assert hip.hipSetDevice(1 << 20) != 0
+            call()
+    finally:
+        hip.hipGetLastError()
+    torch.cuda.synchronize()
+    assert int(tok[0, 0]) >= 0 and bool(y.abs().sum() > 0)
