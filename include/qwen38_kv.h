@@ -230,7 +230,7 @@ int mk_kv_profile(void * h, int enable, double * out, int cap);
 /*
  * ---- The operators of a decode step around the store: what a decoder runs between its attention layers' calls, on the
  * activation units that mk_kv_attend_gated / mk_kv_attend_prep leave.  No handle, no memory of their own; asynchronous on
- * `stream`; every buffer is memory of the current device (checked).  dtype: 0 fp32, 1 fp16, 2 bf16.  Strides count
+ * `stream`, a stream of the current device; every buffer is memory of that device (both checked).  dtype: 0 fp32, 1 fp16, 2 bf16.  Strides count
  * elements between rows.  Calls on different streams are independent of each other as long as their outputs and workspaces are.
  * The same call gives the same bits on every run.  Outputs overlap neither each other nor an input but where a call says so; no
  * rows (or sequences) is a call that does nothing and looks at no pointer.

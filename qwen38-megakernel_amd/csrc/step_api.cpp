@@ -37,10 +37,16 @@ void ck(hipError_t e, const char * what) {
     bad(std::string(what) + ": " + hipGetErrorString(e));
 }
 
-// every buffer is memory of the device that the call runs on (a host address or another device's would fault the GPU)
+// the stream is of the current device, and every buffer is memory of it (a host address or another device's would fault the GPU)
 struct Device {
     int dev = -1;
-    Device() { ck(hipGetDevice(&dev), "hipGetDevice"); }
+    explicit Device(void * stream) {
+        ck(hipGetDevice(&dev), "hipGetDevice");
+        if (!stream || stream == hipStreamLegacy || stream == hipStreamPerThread) return; // (of the current device)
+        hipDevice_t of = -1;
+        ck(hipStreamGetDevice(static_cast<hipStream_t>(stream), &of), "stream");
+        if (of != dev) bad("stream is of device " + std::to_string(of) + ", the current device is " + std::to_string(dev));
+    }
     void holds(const void * p, const char * name) const {
         if (!p) return;
         hipPointerAttribute_t at{};
@@ -93,7 +99,7 @@ int w4(W4Args a, int group, int xform, void * stream) {
     aligned(a.scales, 2, "scales");
     aligned(a.mins, 2, "mins");
     aligned(a.y, 4, "y");
-    const Device d;
+    const Device d(stream);
     d.holds(a.codes, "codes");
     d.holds(a.scales, "scales");
     d.holds(a.mins, "mins");
@@ -151,7 +157,7 @@ int mk_norm_q32(const void * x, long long x_stride, const void * res, long long 
         aligned(q32a, 16, "q32a");
         aligned(q32b, 16, "q32b");
         aligned(q32meta, 8, "q32meta");
-        const Device d;
+        const Device d(stream);
         d.holds(x, "x");
         d.holds(res, "res");
         d.holds(w, "w");
@@ -232,7 +238,7 @@ int mk_verify_drafts(int n_seq, int n_draft, int vocab, const void * target, lon
             aligned(p, 4, "an array of 4-byte values");
         if (!ws || ws_bytes < want) bad("the call needs " + std::to_string(want) + " bytes of workspace (mk_verify_ws)");
         aligned(ws, 16, "ws");
-        const Device d;
+        const Device d(stream);
         d.holds(target, "target");
         d.holds(temperature, "temperature");
         d.holds(draft_probs, "draft_probs");

@@ -274,3 +274,16 @@ def test_an_earlier_error_is_not_this_calls(qkv, torch_gpu):
         hip.hipGetLastError()
     torch.cuda.synchronize()
     assert int(tok[0, 0]) >= 0 and bool(y.abs().sum() > 0)
+
+
+def test_kinds_of_streams(qkv, torch_gpu):
+    """The null stream, the thread's own (handle 2), a stream of torch's and the current one."""
+    torch = torch_gpu
+    x, w = torch.randn(3, 128, device="cuda"), torch.ones(128, device="cuda")
+    side = torch.cuda.Stream()
+    ys = [torch.zeros(3, 128, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    for y, s in zip(ys, (0, 2, side.cuda_stream, torch.cuda.current_stream().cuda_stream)):
+        qkv.norm_q32(x.data_ptr(), 128, 0, 0, w.data_ptr(), 3, 128, 1e-6, 0, 0, 0, y.data_ptr(), 128, 0, 0, 0, s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, ys[0]) for y in ys) and bool(ys[0].abs().sum() > 0)
