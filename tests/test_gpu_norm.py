@@ -186,6 +186,33 @@ def test_rows_near_the_ends_of_the_type(qkv, torch_gpu, dim, eps, dt):
     assert some[:-1].all() == (eps == 0)
 
 
+@pytest.mark.parametrize("dt", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("rows,dim,pad", [(1, 64, 0), (3, 5120, 0), (2, 777, 3), (600, 1024, 8), (2, 32768, 1)])
+def test_in_place_and_unstored(qkv, torch_gpu, rows, dim, pad, dt):
+    """y in the place of x, the sum in the place of the residual or not stored at all: the bits of the call with outputs of its own."""
+    torch, T, ld = torch_gpu, dtype_of(torch_gpu, dt), dim + pad
+    x, r = (torch.randn(rows, ld, device="cuda").to(T) for _ in range(2))
+    w = 1 + 0.2 * torch.randn(dim, device="cuda")
+    units = dim % 64 == 0
+
+    def call(x, r, sum, y):
+        u = [torch.zeros(rows, dim // 32, k, dtype=t, device="cuda") for k, t in ((16, torch.int8), (16, torch.int8), (4, torch.int16))] if units else [None] * 3
+        qkv.norm_q32(x.data_ptr(), ld, r.data_ptr(), ld, w.data_ptr(), rows, dim, 1e-6, CODE[dt], ptr(sum), ld, ptr(y), ld, *(ptr(t) for t in u),
+                     torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        return u
+    sums, y = torch.zeros_like(x), torch.zeros_like(x)
+    u0 = call(x, r, sums, y)
+    assert torch.equal(sums[:, :dim], (x.float() + r.float()).to(T)[:, :dim])
+    for inplace_x, inplace_r in ((True, False), (True, True), (False, False)):
+        x1, r1 = x.clone(), r.clone()
+        y1 = x1 if inplace_x else torch.zeros_like(x)
+        u1 = call(x1, r1, r1 if inplace_r else None, y1)
+        assert torch.equal(y1[:, :dim], y[:, :dim]) and torch.equal(y1[:, dim:], (x if inplace_x else torch.zeros_like(x))[:, dim:])
+        assert torch.equal(r1[:, :dim], (sums if inplace_r else r)[:, :dim]) and torch.equal(r1[:, dim:], r[:, dim:])
+        assert all(torch.equal(p, q) for p, q in zip(u0, u1)) if units else True
+
+
 def test_no_rows(qkv, torch_gpu):
     torch = torch_gpu
     x = torch.ones(64, device="cuda")
