@@ -230,8 +230,8 @@ int mk_kv_profile(void * h, int enable, double * out, int cap);
 /*
  * ---- The operators of a decode step around the store: what a decoder runs between its attention layers' calls, on the
  * activation units that mk_kv_attend_gated / mk_kv_attend_prep leave.  No handle, no memory of their own; asynchronous on
- * `stream`, a stream of the current device; every buffer is memory of that device (both checked).  dtype: 0 fp32, 1 fp16, 2 bf16.  Strides count
- * elements between rows.  Calls on different streams are independent of each other as long as their outputs and workspaces are.
+ * `stream`, a stream of the current device; every buffer is memory of that device (both checked).  dtype: 0 fp32, 1 fp16,
+ * 2 bf16.  Strides count elements between rows.  Calls on different streams are independent of each other as long as their outputs and workspaces are.
  * The same call gives the same bits on every run.  Outputs overlap neither each other nor an input but where a call says so; no
  * rows (or sequences) is a call that does nothing and looks at no pointer.
  */
@@ -244,7 +244,9 @@ int mk_kv_profile(void * h, int enable, double * out, int cap);
  * res itself: the residual stream updated in place), y (may be x itself), and the units of y (dim a multiple of 64; a set):
  * q32a / q32b [rows][dim / 32][16] and q32meta [rows][dim / 32][4] in the layout of mk_kv_attend_gated.  A block's codes are
  * round(t 127 / max |t|), ties to even, of t = h w, its scale max |t| / (sqrt(mean(h^2) + eps) 127) as fp16: codes do not depend on the order
- * of the row's sum.  A row with an infinity or a NaN gives NaN scales, or codes of zero, as its y.
+ * of the row's sum.  A scale past 65504 is infinite; where one is zero the codes may be zero too.  A NaN in a row makes its y and its
+ * scales NaN; an infinity its own y and its block's scale, the row's other values and scales are zero.  A row of zeros over an eps
+ * of 0 is NaN.
  * q32a / q32b are aligned to 16 bytes, q32meta to 8.
  */
 int mk_norm_q32(const void * x, long long x_stride, const void * res, long long res_stride, const float * w, int rows, int dim, float eps, int dtype,
@@ -261,7 +263,9 @@ int mk_norm_q32(const void * x, long long x_stride, const void * res, long long 
  * mk_w4_rows as plain rows [rows][x_stride] of dtype (k a multiple of 32).  Products and sums are exact or in fp32: the units'
  * integer sums are exact per 32 values, fp16 and bf16 rows enter as they are and fp32 rows to 2^-23 of each value, all of them to
  * 2^-39 of the largest of a block's 32.
- * Meant for the tokens of a decode or verify step: 1 to 64 rows, more are allowed.
+ * An infinity or a NaN of x reaches its row alone, as W x has it (of units: a scale that is not finite gives results that are not),
+ * one of a scale or a minimum its column alone.
+ * Meant for the tokens of a decode or verify step: 1 to 64 rows.  Allowed are rows 0..2^19, n 1..2^28 and k up to 2^20.
  */
 int mk_w4_units(int rows, int n, int k, int group, const void * codes, const void * scales, const void * mins, const void * q32a, const void * q32b,
                 const unsigned short * q32meta, float * y, long long y_stride, void * stream);
@@ -270,7 +274,7 @@ int mk_w4_rows(int rows, int n, int k, int group, const void * codes, const void
 
 /*
  * Verification of drafted tokens against the target's distribution, from given random numbers (what follows a verify attention and the
- * output head; the accepted length is what mk_kv_rewind keeps).  For each of n_seq sequences, with n = n_draft (0..64) drafts:
+ * output head; the accepted length is what mk_kv_rewind keeps).  For each of n_seq (0..65535) sequences, with n = n_draft (0..64) drafts:
  *   target      [n_seq][n + 1][row_stride] logits of dtype (probs 0), or fp32 probabilities (probs 1); vocab 1..2^24 entries a row.  Row
  *               i is the distribution after draft i - 1
  *   temperature fp32 [n_seq] or NULL (1): p = softmax(logits / temperature); 0 (less, or a NaN): all on the largest logit, the lowest

@@ -186,6 +186,24 @@ def test_rows_near_the_ends_of_the_type(qkv, torch_gpu, dim, eps, dt):
     assert some[:-1].all() == (eps == 0)
 
 
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+def test_rows_without_a_value(qkv, torch_gpu, dt):
+    """Zeros over an eps of 0: NaN.  An infinity: NaN in its own place and its block's scale, zeros elsewhere.  A NaN: all of its row."""
+    torch, T = torch_gpu, dtype_of(torch_gpu, dt)
+    x = torch.randn(4, 128).to(T)
+    x[0], x[1, 40], x[2, 3] = 0, -float("inf"), float("nan")
+    xd, w = x.cuda(), torch.ones(128, device="cuda")
+    y = torch.zeros_like(xd)
+    a, b = (torch.zeros(4, 4, 16, dtype=torch.int8, device="cuda") for _ in range(2))
+    m = torch.zeros(4, 4, 4, dtype=torch.int16, device="cuda")
+    qkv.norm_q32(xd.data_ptr(), 128, 0, 0, w.data_ptr(), 4, 128, 0.0, CODE[dt], 0, 0, y.data_ptr(), 128, a.data_ptr(), b.data_ptr(), m.data_ptr(),
+                 torch.cuda.current_stream().cuda_stream)
+    got = y.float().cpu().numpy()
+    _, sc, _ = unpack_units(a.cpu().numpy(), b.cpu().numpy(), m.cpu().numpy().view(np.uint16))
+    assert np.isnan(got[[0, 2]]).all() and np.isnan(sc[[0, 2]]).all() and np.isfinite(got[3]).all() and np.isfinite(sc[3]).all()
+    assert np.isnan(got[1, 40]) and (np.delete(got[1], 40) == 0).all() and np.isnan(sc[1, 1]) and (sc[1, [0, 2, 3]] == 0).all()
+
+
 @pytest.mark.parametrize("dt", ["fp32", "fp16", "bf16"])
 @pytest.mark.parametrize("rows,dim,pad", [(1, 64, 0), (3, 5120, 0), (2, 777, 3), (600, 1024, 8), (2, 32768, 1)])
 def test_in_place_and_unstored(qkv, torch_gpu, rows, dim, pad, dt):

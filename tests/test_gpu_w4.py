@@ -220,6 +220,40 @@ def test_infinities_with_minimums(qkv, torch_gpu, x, rows, k):
         assert kind != "large" or fine.all()
 
 
+@pytest.mark.parametrize("mins", [False, True])
+@pytest.mark.parametrize("rows", [1, 2, 4, 8, 20, 40])
+def test_scales_that_are_not_finite(qkv, torch_gpu, rows, mins):
+    """A unit's scale reaches its row alone, a weight's scale or minimum its column alone; both are then not finite."""
+    torch, n, k, group = torch_gpu, 90, 320, 64
+    rng = np.random.default_rng(rows)
+    c, s, m = weights(rng, n, k, group, mins)
+    c[c == 8] = 9
+    (m if mins else s)[7, 2] = np.inf
+    s[70, 1] = np.nan
+    a, b, meta = units_of(rng.standard_normal((rows, k)).astype(np.float32))
+    a[a == 0], b[b == 0] = 1, 1
+    q, sc, _ = unpack_units(a, b, meta)
+    sums = q.reshape(rows, k // 64, 2, 2, 16).astype(np.int16).sum(-1, dtype=np.int16)
+    meta = meta.reshape(rows, k // 64, 2, 4)
+    meta[..., 2:] = np.swapaxes(sums, 2, 3).view(np.uint16)
+    bad = {rows - 1: np.inf, rows // 2: np.nan} if rows > 2 else {}
+    for row, v in bad.items():
+        meta[row, 3, :, 1] = np.float16(v).view(np.uint16)
+    x = (q.astype(np.float64) * sc.astype(np.float64)[..., None]).reshape(rows, k)
+    y = torch.zeros(rows, n, device="cuda")
+    dev = [torch.from_numpy(np.ascontiguousarray(t)).cuda() for t in (pack_codes(c), s, a, b, meta.reshape(rows, k // 32, 4).view(np.int16))]
+    md = torch.from_numpy(m).cuda() if mins else None
+    qkv.w4_units(rows, n, k, group, dev[0].data_ptr(), dev[1].data_ptr(), ptr(md), dev[2].data_ptr(), dev[3].data_ptr(), dev[4].data_ptr(), y.data_ptr(), n,
+                 torch.cuda.current_stream().cuda_stream)
+    got = y.cpu().numpy().astype(np.float64)
+    fine_r, fine_c = ~np.isin(np.arange(rows), list(bad)), ~np.isin(np.arange(n), (7, 70))
+    with np.errstate(all="ignore"):
+        ref, mag = w4_ref(c, s, m, group, x)
+    at = np.ix_(fine_r, fine_c)
+    assert (np.abs(got[at] - ref[at]) <= w4_bound(k, mag[at], False)).all()
+    assert not np.isfinite(got[~fine_r]).any() and not np.isfinite(got[:, ~fine_c]).any()
+
+
 def test_no_rows_and_refusals(qkv, torch_gpu):
     torch = torch_gpu
     t = torch.zeros(4096, dtype=torch.uint8, device="cuda")

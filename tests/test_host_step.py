@@ -99,3 +99,19 @@ def test_nothing_to_do(qkv):
     w4(qkv, rows=0)
     w4(qkv, False, rows=0)
     verify(qkv, b=0, ws=0, size=0)
+
+
+def test_the_header_states_the_limits(qkv):
+    """One past each limit that include/qwen38_kv.h gives is refused; the limits themselves are not (they get as far as the addresses)."""
+    big = 1 << 40
+    for call, at, past in (
+            (lambda **k: norm(qkv, **{**dict(xs=big, rs=big, ss=big, ys=big), **k}), dict(rows=1 << 21, dim=32768), (dict(rows=(1 << 21) + 1), dict(dim=32769))),
+            (lambda **k: w4(qkv, True, **{**dict(ys=big), **k}), dict(rows=1 << 19, n=1 << 28, k=1 << 20), (dict(rows=(1 << 19) + 1), dict(n=(1 << 28) + 1), dict(k=(1 << 20) + 64))),
+            (lambda **k: w4(qkv, False, **{**dict(ys=big, xs=big), **k}), dict(rows=1 << 19, n=1 << 28, k=1 << 20), (dict(rows=(1 << 19) + 1), dict(n=(1 << 28) + 1), dict(k=(1 << 20) + 32))),
+            (lambda **k: verify(qkv, **{**dict(rs=big, size=1 << 40), **k}), dict(b=65535, n=64), (dict(b=65536), dict(n=65), dict(v=(1 << 24) + 1)))):
+        for kw in past:
+            with pytest.raises(qkv.KVError, match="outside|multiple"):
+                call(**kw)
+        with pytest.raises(qkv.KVError) as e:
+            call(**at)
+        assert "outside" not in str(e.value) and "multiple" not in str(e.value), e.value
