@@ -115,7 +115,7 @@ __global__ __launch_bounds__(1024) void k_norm(NormArgs a) {
     }
 }
 
-// Chunks per thread: one for few rows, whose time is the row's chain of load, sum and store (1 row of 5,120: 3.1 us, with
+// Chunks per thread: one for few rows, whose time is the row's chain of load, sum and store (1 row of 5,120: 3.5 us, with
 // four 5.2; 32 rows 4.7 and 7.0), two for many, which leave room for more rows per CU (4,096 rows of bf16, residual and units:
 // 37 us or 4.0 TB/s of what has to move, with one 40, with four 44; persistent workgroups that read the next row ahead 47 to
 // 62: their registers leave half the waves), four only where two are not enough for 1,024 threads.

@@ -65,10 +65,10 @@ template <int DT, int E> __device__ __forceinline__ void load_run(const typename
 // entries of a thread's piece of a slice that lie together: 16 bytes of them
 constexpr int run_of(int dt) { return dt == DT_F32 ? 4 : 8; }
 
-// One row's slice: 16 entries a thread, all loads of them ahead of the first use.  What bounds it is the arithmetic in 64 bits, 17
-// instructions an entry (64 sequences of up to 7 drafts over 150,001 fp32 logits, 173 MB: 42.6 us, 4.1 TB/s, the vector units
-// busy for 84% of it; workgroups that loop over slices with the next one's loads ahead: 54 to 86 us, by their registers); of few
-// rows the launch (8 of 32,768: 4.1).
+// One row's slice: 16 entries a thread, all loads of them ahead of the first use.  What bounds it is the arithmetic in 64 bits, 26
+// vector instructions an entry, 17 of them the exponential (64 sequences of up to 7 drafts over 150,001 fp32 logits, 173 MB: 43 us,
+// 4.0 TB/s, the vector units busy for 83 to 86% of it, 39 to 47 by the clock the card keeps; workgroups that loop over slices with the next one's loads ahead: 54 to 86 us, by their registers); of few
+// rows the launch (8 of 32,768: 4.2).
 template <int DT, bool PROBS>
 __global__ __launch_bounds__(VT) void k_verify_rows(VerifyArgs a) {
     __shared__ float top[VT / 64];
@@ -288,7 +288,7 @@ __device__ __forceinline__ void weights(const VerifyArgs & a, const Source & S, 
     }
 }
 
-// (4 sequences of 3 drafts over 150,001 bf16 logits: 5.3 us, most of them the slices' sums, the decision and the refused row one
+// (4 sequences of 3 drafts over 150,001 bf16 logits: 5.4 us, most of them the slices' sums, the decision and the refused row one
 // after the other)
 template <int DT, bool PROBS>
 __global__ __launch_bounds__(VT) void k_verify_residual(VerifyArgs a) {
@@ -337,7 +337,7 @@ __device__ __forceinline__ double wave_scan(double v) {
 }
 
 // What bounds the pick is its chain: the slices' sums, the decision, one slice's entries, two scans (one sequence of 7 drafts over 32,768:
-// 5.9 us, 64 over 150,001: 7.0).
+// 5.9 us, 64 over 150,001: 7.5).
 constexpr int PT = 512; // threads of the pick: a wave per row, eight entries of the slice per thread (1,024: 0.4 us more, two waves more a SIMD)
 constexpr int PE = VERIFY_SLICE / PT;
 

@@ -30,8 +30,7 @@ constexpr int planes(int mode) { return mode == XM_UNITS ? 2 : mode == XM_HALF ?
 // x in LDS, kcb blocks at a time.  Units, as they come: per row the even blocks' kcb units, then the odd ones', padded so that the
 // 16 pieces an instruction takes (4 blocks of 4 rows) lie in different banks.  Plain rows, as fp16:
 // [kcb blocks][planes][MR rows][16 bytes], fp32's two parts with 16 bytes behind every 8 blocks where k is in parts: their pieces then
-// lie in different banks (2 rows of fp32 x 17,408 x 5,120: 26 us without, 24 with; one row of bf16 x 150,001, half the planes: 82 and
-// 85).  Then zeros for the operand's other lanes, [kcb][MR] float factors of the blocks'
+// lie in different banks (2 rows of fp32 x 17,408 x 5,120: 8% less time; one row of bf16 x 150,001, half the planes: 4% more).  Then zeros for the operand's other lanes, [kcb][MR] float factors of the blocks'
 // sums and (with m) [kcb][MR] float factors of m.
 struct W4Lds {
     int half, row, zero, dx, ds, end; // units: bytes of a row's even blocks, of a row; offsets of the zeros, the factors, what follows
@@ -308,8 +307,11 @@ constexpr int W4_WIN = 32;  // scales of a weight row that a wave holds in LDS a
 constexpr int W4_WROW = W4_WIN + 8; // ... a row's place: 16 rows' 80 bytes begin in different banks
 
 // NR activation rows per group of four operand rows, RG groups: MR = NR RG rows a pass.
-// What bounds it: the codes' way from HBM where there are many (150,001 x 5,120 on one row, 393 MB: 82 us, 5.2 TB/s with x and
-// y, of 6.0 that a plain read reaches), else the chain of launch, x and first loads (1,024 x 5,120: 4.6 us).
+// What bounds it: the codes' way from HBM where there are many (150,001 x 5,120 on one row of units, group 32, 433 MB with x and y:
+// 83 us, 5.2 TB/s of 6.0 that a plain read reaches; plain rows the codes' way to fp16, 52 of a step's 75 vector instructions: 84 to
+// 87 us with group 128, 397 MB), else the chain of launch, x and first loads (1,024 x 5,120: 4.3 us).  Scalars do not all fit (23 to
+// 70 of them are kept in lanes of vector registers), nor do the vector registers of fp32 rows with minimums (24 to 72 bytes of
+// scratch a lane); neither is touched where the matrix instructions are.
 // P parts: a tile is 16 / P weight rows, and lanes n = 16 / P h + j hold row j of part h, a P-th of its blocks.  A group's
 // operand row NR h + m is then x[m] of part h's block (P NR <= 4), and a lane takes its own part's sums: with few
 // rows of x the tiles get smaller, and a short projection has enough of them for every CU.
@@ -542,7 +544,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_w4(W4Args a) {
 // row's scale of each block.  A workgroup takes up to 2 NTW tiles: 4 waves along the blocks of a chunk (U steps each) times 2
 // along the tiles; a piece of x read from LDS serves the wave's NTW tiles.  What bounds it is the fold of the blocks'
 // integer sums into fp32, three instructions per (row, block, weight row) in three of four vector instructions (64 rows of
-// 17,408 x 5,120: 35.6 us, the vector units busy for 71% of them, the matrix units for 16%).
+// 17,408 x 5,120: 35 us, the vector units busy for 74% of them, the matrix units for 16%).
 __device__ __forceinline__ void w4_exchange(const u32x4 & d, unsigned (&t)[4]) { // t[b] in lane group q: dword q of lane group b's d
     const auto x = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false), y = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
     const auto v = __builtin_amdgcn_permlane16_swap(x[0], y[0], false, false), w = __builtin_amdgcn_permlane16_swap(x[1], y[1], false, false);
@@ -559,11 +561,13 @@ template <int MODE, int MT, int CB, bool MINS> constexpr int wide_buf() {
 
 // WK waves along the blocks of a chunk, U steps each, times WN along the tiles.  ODD: a workgroup of an odd number of tiles,
 // whose second half of the waves has one less, with a loop body of its own (64 rows of 17,408 x 5,120, five tiles a workgroup:
-// 35.6 us, with the sixth worked on and dropped 41.3)
+// 35 us, with the sixth worked on and dropped 41)
 template <int MODE, int DT, int MT, int NTW, int WK, int WN, int U, bool ODD, bool MINS>
 __global__ __launch_bounds__(WK * WN * 64, WK * WN / 4) void k_w4_wide(W4Args a) {
     constexpr int WIDE_W = WK * WN, TM = 16 * MT, CB = 4 * WK * U, BB = planes(MODE) * TM * 16, BUF = wide_buf<MODE, MT, CB, MINS>();
-    constexpr bool ASYNC = MODE == XM_UNITS; // x copied into the other buffer while a chunk is worked on
+    // x copied into the other buffer while a chunk is worked on (its matrix instructions and folds: the compiler's waits for the chunk's
+    // codes do not know of the copies issued behind them, so the exchange of the codes begins when most copies have landed)
+    constexpr bool ASYNC = MODE == XM_UNITS;
     constexpr int RPC = 32 / CB; // rows of a copy
     constexpr int DX = ASYNC ? TM / RPC * 1040 : w4_lds<MODE, TM, MINS>(CB).dx, DS = ASYNC ? TM + 4 : TM; // the factors of x behind the blocks, their stride
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -878,7 +882,7 @@ static hipError_t launch_wide(const W4Args & a, hipStream_t st) {
     }
 }
 
-// By the rows of x, in us for 1,024 / 17,408 / 150,001 weight rows of 5,120, units:
+// By the rows of x, in us for 1,024 / 17,408 / 150,001 weight rows of 5,120, units, groups of 32:
 //   1     four parts     4.6 / 13.2 / 82   whole tiles of 16 weight rows  6.4 / 15.9 / 92
 //   2     two parts      5.3 / 13.7 / 87   whole tiles                    6.6 / 15.8 / 92
 //   3, 4  one group      6.2 / 16.0 / 93   two groups                     7.4 / 17.4 / 95
