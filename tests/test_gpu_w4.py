@@ -220,6 +220,48 @@ def test_infinities_with_minimums(qkv, torch_gpu, x, rows, k):
         assert kind != "large" or fine.all()
 
 
+@pytest.mark.parametrize("rows", [1, 2, 3, 8, 40, 130])
+@pytest.mark.parametrize("n,k", [(70003, 128), (9001, 640), (300001, 64)])
+def test_infinities_over_many_tiles(qkv, torch_gpu, rows, n, k):
+    """Workgroups of several tiles, the last of them short, rows of every kind beside each other, results with a stride; in a graph's
+    replay too (the same bits)."""
+    if rows * n > 8e6:
+        n = 70003 if rows == 40 else 20011
+    torch = torch_gpu
+    rng = np.random.default_rng(rows + n)
+    c, s, m = weights(rng, n, k, 32, True)
+    v = rng.standard_normal((rows, k)).astype(np.float16)
+    kinds = rng.permutation(rows)
+    v[kinds[0], k - 3] = np.inf
+    if rows > 2:
+        v[kinds[1], 5], v[kinds[2], 17], v[kinds[2], 40] = np.nan, -np.inf, -np.inf
+    dev = [torch.from_numpy(t).cuda() for t in (pack_codes(c), s, m, v)]
+    y, y2 = (torch.full((rows + 1, n + 3), 77.0, device="cuda") for _ in range(2))
+
+    def call(y, stream):
+        qkv.w4_rows(rows, n, k, 32, *(t.data_ptr() for t in dev), k, CODE["fp16"], y.data_ptr(), n + 3, stream)
+    call(y, torch.cuda.current_stream().cuda_stream)
+    g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(g, stream=side):
+            call(y2, side.cuda_stream)
+    for _ in range(3):
+        y2[:rows, :n] = 5
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y.view(torch.int32), y2.view(torch.int32))
+    got = y.cpu().numpy()
+    assert (got[rows] == 77).all() and (got[:, n:] == 77).all()
+    got = got[:rows, :n].astype(np.float64)
+    with np.errstate(all="ignore"):
+        ref, mag = w4_ref(c, s, m, 32, v)
+    fine = np.isfinite(ref)
+    assert np.array_equal(np.isnan(got), np.isnan(ref)) and np.array_equal(got[np.isinf(ref)], ref[np.isinf(ref)])
+    assert (np.abs(got[fine] - ref[fine]) <= w4_bound(k, mag, True)[fine]).all() and np.isinf(ref).any()
+
+
 @pytest.mark.parametrize("mins", [False, True])
 @pytest.mark.parametrize("rows", [1, 2, 4, 8, 20, 40])
 def test_scales_that_are_not_finite(qkv, torch_gpu, rows, mins):
