@@ -188,8 +188,11 @@ def prepare(case, seed):
         else:
             d["ids"], d["weights"] = chosen
         d["y"] = torch.empty(rows, c["dim"], device="cuda", dtype=torch.float32 if c["x"] == "units" else d["x"].dtype)
-        # kept between calls: the experts' inner values
-        d["ws"] = torch.empty(65536 + 8 * rows * c["top"] * (c["inner"] + 64), device="cuda", dtype=torch.uint8)
+    # kept between calls: partial sums of the logits, and the experts' values within and behind the layer
+    room = 65536 + 64 * min(rows, 256) * c["experts"]
+    if c["op"] == "moe":
+        room += rows * c["top"] * (8 * c["inner"] + 4 * c["dim"] + 1024)
+    d["ws"] = torch.empty(room, device="cuda", dtype=torch.uint8)
     if "w" in d:
         d["logits"] = torch.empty(rows, c["experts"], device="cuda")
         d["ids"] = torch.empty(rows, c["top"], device="cuda", dtype=torch.int32)
@@ -300,7 +303,7 @@ def run(d):
     if c["op"] == "route":
         qkv.moe_route(c["rows"], c["dim"], c["experts"], c["top"], x.data_ptr(), x.stride(0), _CODE[c["dtype"]], d["w"].data_ptr(), _CODE[c["wtype"]],
                       _ptr(d["bias"]), _FORM[c["form"]], SCALE if c["form"] == "sigmoid" else 1.0, d["logits"].data_ptr(), d["ids"].data_ptr(),
-                      d["weights"].data_ptr(), stream)
+                      d["weights"].data_ptr(), d["ws"].data_ptr(), d["ws"].numel(), stream)
         return dict(logits=d["logits"], ids=d["ids"], weights=d["weights"])
     head = (c["rows"], c["dim"], c["inner"], c["experts"], c["top"], c["group"], *map(_ptr, d["up"]), *map(_ptr, d["down"]))
     chosen = (d["ids"].data_ptr(), d["weights"].data_ptr())
