@@ -298,6 +298,68 @@ int mk_verify_drafts(int n_seq, int n_draft, int vocab, const void * target, lon
                      const float * draft_probs, const int * drafts, const int * n_drafts, const float * u, int * accepted, int * tokens, float * draft_p,
                      void * ws, long long ws_bytes, void * stream);
 
+/*
+ * ---- The operators of a server of many requests beside these products: adapters of their own, and experts in place of one projection.  The
+ * conventions are those of the section above (dtype, strides, units, streams, devices; the same call gives the same bits); ws is
+ * device memory aligned to 16 bytes, of at least what the _ws function gives, that no other call uses until this one has finished (one per
+ * captured graph that may run at once); nothing in it needs clearing.
+ *
+ * Low-rank adapters of many requests at once, next to a projection of k to n values whose result is base:
+ *   y[m] = base[m] + scales[a] B_a (A_a x[m]),  a = ids[m];   y[m] = base[m] where ids[m] is no adapter (below 0, n_adapters or more)
+ *   a, b     fp16 (ab_dtype 1) or bf16 (2): A [n_adapters][rank][k], B [n_adapters][n][rank]; rank 1..256
+ *   ranks    int [n_adapters] or NULL (rank): an adapter's first ranks[a] (clamped to 0 .. rank); what lies behind them is not used
+ *   scales   fp32 [n_adapters] or NULL (1); ids int [rows], in any order
+ *   base     fp32 [rows][base_stride] or NULL (0); may be y itself: added in place, behind mk_w4_units / mk_w4_rows
+ * x: plain rows (k a multiple of 32) or int8 units (of 64), k up to 2^20; n 1..2^24, rows 0..2^19, rows n up to 2^35.  Products are exact
+ * to 2^-23 and added in fp32; A x is rounded to fp32 (and taken to 2^-24).  An infinity or a NaN of x reaches its row alone, one of an
+ * adapter the rows of that adapter alone (where it may be a NaN in place of an infinity).
+ */
+long long mk_lora_ws(int rows, int k, int rank);
+int mk_lora_rows(int rows, int n, int k, int n_adapters, int rank, const void * a, const void * b, int ab_dtype, const int * ranks, const float * scales,
+                 const int * ids, const void * x, long long x_stride, int dtype, const float * base, long long base_stride, float * y, long long y_stride,
+                 void * ws, long long ws_bytes, void * stream);
+int mk_lora_units(int rows, int n, int k, int n_adapters, int rank, const void * a, const void * b, int ab_dtype, const int * ranks, const float * scales,
+                  const int * ids, const void * q32a, const void * q32b, const unsigned short * q32meta, const float * base, long long base_stride, float * y,
+                  long long y_stride, void * ws, long long ws_bytes, void * stream);
+
+/*
+ * The router of a mixture of experts: logits[m] = x[m] W^T (W [n_experts][dim] of w_dtype, summed in 64 bits and rounded to fp32 once, as the
+ * choice compares values that lie close), the top_k experts of each row and their weights.  rows 0..2^19, dim 1..2^17,
+ * n_experts 1..1024, top_k 1..16.
+ *   form     0: weights are softmax(logits) of the chosen ones, 1: softmax over the chosen ones, 2: sigmoid(logits), 3: sigmoid(logits) over
+ *            the chosen ones' sum; all times scale
+ *   bias     fp32 [n_experts] or NULL: forms 2 and 3 choose by sigmoid(logits) + bias; else by the logits
+ *   logits   fp32 [rows][n_experts]; ids int [rows][top_k], the largest first, of equal ones the lowest index; weights fp32 [rows][top_k]
+ * A NaN counts as below everything.  ids are always distinct experts; weights of a row with logits that are not finite may be NaN.
+ */
+long long mk_moe_route_ws(int rows, int dim, int n_experts);
+int mk_moe_route(int rows, int dim, int n_experts, int top_k, const void * x, long long x_stride, int dtype, const void * w, int w_dtype, const float * bias,
+                 int form, float scale, float * logits, int * ids, float * weights, void * ws, long long ws_bytes, void * stream);
+
+/*
+ * The experts of such a layer with 4-bit weights, for a few tokens (64 rows are one run; more, up to 4096, one run after another):
+ *   h_e = silu(G_e x[m]) * (U_e x[m]),   y[m] = sum over j of weights[m][j] D_e h_e, e = ids[m][j]   (in the order of j)
+ *   up, down    codes, fp16 scales and minimums (of both products or NULL for both) as mk_w4_units has them, of all experts one behind the
+ *               other: up [n_experts][2 inner][dim], of each expert the gate's rows G, then U; down [n_experts][dim][inner]
+ *   ids         int [rows][top_k], weights fp32 [rows][top_k] (of mk_moe_route, or a caller's own); ids that are no expert are left out
+ *   y           [rows][y_stride]: of x's type, for units fp32
+ * dim a multiple of 32 (units: 64), at most 16384; inner of 32, at most 32768; n_experts 1..1024, top_k 1..16.  x and h enter as integers
+ * of their block of 32 values: int8 units as they are, fp32 rows (and the h of both) to 2^-21 of the block's largest value, fp16 and bf16
+ * rows (and their h) to 2^-13; sums in fp32.  A row of x with an infinity or a NaN gives NaNs in that row of y alone.
+ * mk_moe_layer is mk_moe_route on the same rows and mk_moe_rows on its choice, in one call; mk_moe_ws covers all three calls.
+ */
+long long mk_moe_ws(int rows, int dim, int inner, int n_experts, int top_k);
+int mk_moe_rows(int rows, int dim, int inner, int n_experts, int top_k, int group, const void * up, const void * up_scales, const void * up_mins,
+                const void * down, const void * down_scales, const void * down_mins, const void * x, long long x_stride, int dtype, const int * ids,
+                const float * weights, void * y, long long y_stride, void * ws, long long ws_bytes, void * stream);
+int mk_moe_units(int rows, int dim, int inner, int n_experts, int top_k, int group, const void * up, const void * up_scales, const void * up_mins,
+                 const void * down, const void * down_scales, const void * down_mins, const void * q32a, const void * q32b, const unsigned short * q32meta,
+                 const int * ids, const float * weights, float * y, long long y_stride, void * ws, long long ws_bytes, void * stream);
+int mk_moe_layer(int rows, int dim, int inner, int n_experts, int top_k, int group, const void * up, const void * up_scales, const void * up_mins,
+                 const void * down, const void * down_scales, const void * down_mins, const void * x, long long x_stride, int dtype, const void * router,
+                 int router_dtype, const float * bias, int form, float scale, float * logits, int * ids, float * weights, void * y, long long y_stride, void * ws,
+                 long long ws_bytes, void * stream);
+
 /* Host-only geometry and grammar helpers (no GPU needed). */
 int mk_kv_window_start(int L, int win);  /* kv_ws, qwen38_mk.cu:2118-2126 */
 int mk_kv_ring_rows(int win);            /* kvrc, loader.cu:1479-1486 */

@@ -14,7 +14,7 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libqwen38_kv.so")
 SOURCES = ["kv_store.hip", "kv_attn.hip", "kv_attn_fused.hip", "kv_api.cpp", "step_norm.hip", "step_w4.hip", "step_verify.hip",
-           "step_api.cpp"]
+           "step_api.cpp", "step_lora.hip", "step_route.hip", "step_moe.hip", "step_mix_api.cpp"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

@@ -4,6 +4,8 @@
 #include "kv_dev.h"
 #include "step_launch.h"
 
+#include <atomic>
+
 namespace qkv {
 
 // 8 consecutive values as loads of 16 bytes that need no more than the type's own alignment (the rows of a strided or
@@ -120,6 +122,19 @@ template <class A> inline hipError_t launch(void (*k)(A), dim3 grid, dim3 block,
     return hipLaunchKernel(reinterpret_cast<const void *>(k), grid, block, args, lds, st);
 }
 
+// lets a kernel have more than 64 KiB of LDS: once per kernel and device (the flag is the kernel's own)
+template <class K> inline hipError_t allow_lds(K k, size_t lds, std::atomic<uint64_t> & done) {
+    if (lds <= 64 * 1024) return hipSuccess;
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return hipSuccess;
+    e = hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (e == hipSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
 // the first n (1..8) of 8 values, the rest zero
 template <int DT> __device__ __forceinline__ void load_n(const typename Elem<DT>::T * p, int n, float (&v)[8]) {
     if (n >= 8) return load8<DT>(p, v);
@@ -135,6 +150,20 @@ template <int DT> __device__ __forceinline__ void store_n(typename Elem<DT>::T *
 
 // a workgroup barrier for LDS data only: __syncthreads() also waits for the wave's loads and stores in flight
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// 16 bytes per lane from its own address to LDS at lds + 16 lane, without a register (waited for with vm_drain)
+__device__ __forceinline__ void dma16(const void * g, unsigned lds) {
+    lds = (unsigned) __builtin_amdgcn_readfirstlane(lds);
+    asm volatile(QKV_SET_M0 "global_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
+}
+__device__ __forceinline__ void vm_drain() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// the codes of one word as the four int8 pairs of dwords, 16 (code - 8): values 0..3, values 4..7
+__device__ __forceinline__ void w4_bytes(unsigned w, int & lo, int & hi) {
+    w ^= 0x88888888u;
+    lo = (int) ((w << 4) & 0xf0f0f0f0u);
+    hi = (int) (w & 0xf0f0f0f0u);
+}
 
 __device__ __forceinline__ double shfl_xor_d(double v, int m) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);

@@ -1,0 +1,80 @@
+// The operators of a server of many requests beside the 4-bit products (step_lora.hip, step_route.hip, step_moe.hip): their
+// arguments, checked by the C-ABI host code (step_mix_api.cpp), and their launchers.
+#pragma once
+#include "step_launch.h"
+
+namespace qkv {
+
+// y[m] = base[m] + scales[a] B_a (A_a x[m]), a = ids[m]; rows whose a is no adapter: y[m] = base[m]
+struct LoraArgs {
+    const void * a;      // [n_adapters][rank][k] fp16 or bf16
+    const void * b;      // [n_adapters][n][rank]
+    const int * ranks;   // optional [n_adapters]: the first ranks[a] of an adapter's (clamped to 0 .. rank)
+    const float * scales; // optional [n_adapters]
+    const int * ids;     // [rows]
+    const int8_t * xa;   // int8 units [rows][k / 32][16] (a / b), meta [rows][k / 32][4]; or
+    const int8_t * xb;
+    const uint16_t * xmeta;
+    const void * x;      // plain rows [rows][x_stride]
+    const float * base;  // optional [rows][base_stride] (may be y)
+    float * y;           // [rows][y_stride]
+    float * u;           // workspace [chunks][rows][rp]: A x by chunks of k
+    long long x_stride, base_stride, y_stride;
+    int rows, n, k, n_adapters, rank;
+    int rp, chunks, slots; // (set by lora_plan) rank padded to 16; chunks of k; adapters of a tile of 16 rows side by side
+};
+constexpr int LORA_MAX_ROWS = 1 << 19, LORA_MAX_N = 1 << 24, LORA_MAX_K = 1 << 20, LORA_MAX_RANK = 256, LORA_MAX_CHUNKS = 16;
+void lora_plan(LoraArgs & a);
+hipError_t launch_lora(const LoraArgs & a, int xform, int wtype, hipStream_t st); // xform: W4_UNITS or a Dtype
+
+// logits = x W^T (sums in 64 bits), the top_k experts of each row and their weights
+enum { ROUTE_SOFTMAX = 0, ROUTE_CHOSEN = 1, ROUTE_SIGMOID = 2, ROUTE_SIGMOID_NORM = 3 };
+struct RouteArgs {
+    const void * x;     // [rows][x_stride]
+    const void * w;     // [n_experts][dim]
+    const float * bias; // optional [n_experts]
+    float * logits;     // [rows][n_experts]
+    int * ids;          // [rows][top_k]
+    float * weights;    // [rows][top_k]
+    double * part;      // workspace [chunks][rows][n_experts] where chunks > 1
+    long long x_stride;
+    int rows, dim, n_experts, top_k, form;
+    float scale;
+    int chunks;         // (set by route_plan) parts of dim with partial sums of their own
+};
+constexpr int ROUTE_MAX_EXPERTS = 1024, ROUTE_MAX_TOP = 16, ROUTE_MAX_ROWS = 1 << 19, ROUTE_MAX_DIM = 1 << 17;
+void route_plan(RouteArgs & a);
+hipError_t launch_route(const RouteArgs & a, int dtype, int wtype, hipStream_t st);
+
+// 4-bit weights of every expert: codes [n_experts][n][k / 2], scales and minimums [n_experts][n][gs]
+struct MoeWeights {
+    const uint8_t * codes;
+    const uint16_t * scales;
+    const uint16_t * mins;
+};
+struct MoeArgs {
+    MoeWeights up;   // n = 2 inner (the gate's rows, then the up projection's), k = dim
+    MoeWeights down; // n = dim, k = inner
+    const int8_t * xa; // int8 units, or
+    const int8_t * xb;
+    const uint16_t * xmeta;
+    const void * x;  // plain rows [rows][x_stride]
+    const int * ids; // [rows][top_k]
+    const float * weights;
+    void * y;        // [rows][y_stride] of x's type (units: fp32)
+    long long x_stride, y_stride;
+    int rows, dim, inner, n_experts, top_k, gsh; // a scale serves 32 << gsh values
+    // workspace (set by moe_plan): of every pair (row, place among its experts) the inner values as int8 planes, per block of 32 a
+    // factor and (with minimums) a sum, and the expert's output
+    uint8_t * hq;    // [pairs][planes][inner padded to 256]
+    float * hd;      // [pairs][inner / 32]
+    float * hs;      // [pairs][inner / 32]
+    float * out;     // [pairs][dim]
+    int tp_up, tp_down; // (set by moe_plan) tokens of an expert that a pass holds in LDS
+};
+constexpr int MOE_ROWS = 64;   // rows of a launch; a call of more runs them one after another
+constexpr int MOE_MAX_ROWS = 4096, MOE_MAX_DIM = 16384, MOE_MAX_INNER = 32768;
+long long moe_plan(MoeArgs & a, int xform, uint8_t * ws); // -> bytes of workspace
+hipError_t launch_moe(const MoeArgs & a, int xform, hipStream_t st);
+
+} // namespace qkv

@@ -47,13 +47,6 @@ template <int MODE, int MR, bool MINS> __host__ __device__ __forceinline__ const
     return l;
 }
 
-// 16 bytes per lane from its own address to LDS at lds + 16 lane, without a register (waited for with vm_drain)
-__device__ __forceinline__ void dma16(const void * g, unsigned lds) {
-    lds = (unsigned) __builtin_amdgcn_readfirstlane(lds);
-    asm volatile(QKV_SET_M0 "global_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
-}
-__device__ __forceinline__ void vm_drain() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
 // a quarter of a block of plain x (8 values) on its way to LDS as fp16: piece i = 4 (MR block + row) + quarter of the blocks from
 // b0 and the rows from row0 on; zeros for rows past the last one and blocks past the row's end
 template <int DT> struct W4Eighth {
@@ -167,13 +160,7 @@ __device__ __forceinline__ void w4_stage(const W4Args & a, uint8_t * lds, int b0
     }
 }
 
-// the codes of one word as the four int8 pairs of dwords, 16 (code - 8): values 0..3, values 4..7
-__device__ __forceinline__ void w4_bytes(unsigned w, int & lo, int & hi) {
-    w ^= 0x88888888u;
-    lo = (int) ((w << 4) & 0xf0f0f0f0u);
-    hi = (int) (w & 0xf0f0f0f0u);
-}
-// ... as fp16 pairs (0, 2) (1, 3) (4, 6) (5, 7): 0x6400 | n is 1024 + n and 0x5400 | 16 n is 64 + n, both exact
+// the codes of one word as fp16 pairs (0, 2) (1, 3) (4, 6) (5, 7): 0x6400 | n is 1024 + n and 0x5400 | 16 n is 64 + n, both exact
 __device__ __forceinline__ half8 w4_halves(unsigned w) {
     const half2v b0 = {(_Float16) -1032.f, (_Float16) -1032.f}, b1 = {(_Float16) -72.f, (_Float16) -72.f};
     const unsigned v = w >> 8;
@@ -799,18 +786,6 @@ __global__ __launch_bounds__(WK * WN * 64, WK * WN / 4) void k_w4_wide(W4Args a)
 }
 
 constexpr int W4_LDS = 80 * 1024; // of k_w4: two workgroups per CU
-// lets a kernel have more than 64 KiB of LDS: once per kernel and device (the flag is the kernel's own)
-template <class K> static hipError_t allow_lds(K k, size_t lds, std::atomic<uint64_t> & done) {
-    if (lds <= 64 * 1024) return hipSuccess;
-    int dev = 0;
-    hipError_t e = hipGetDevice(&dev);
-    if (e != hipSuccess) return e;
-    const uint64_t bit = 1ull << (dev & 63);
-    if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return hipSuccess;
-    e = hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    if (e == hipSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
-    return e;
-}
 constexpr int W4_WAVES = 4096; // of k_w4: 16 for each of 256 CUs
 
 template <int MODE, int DT, int NR, int RG, int P, int W>

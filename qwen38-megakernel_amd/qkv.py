@@ -19,6 +19,12 @@ _P_ll = ctypes.POINTER(ctypes.c_longlong)
 _P_u64 = ctypes.POINTER(ctypes.c_ulonglong)
 _P_u16 = ctypes.POINTER(ctypes.c_ushort)
 
+# the arguments that calls of a kind share, in front of x and behind it
+_LORA = [_c_int] * 5 + [_c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp]
+_LORA_TAIL = [_c_vp, _c_ll, _c_vp, _c_ll, _c_vp, _c_ll, _c_vp]
+_MOE = [_c_int] * 6 + [_c_vp] * 6
+_MOE_TAIL = [_c_vp, _c_vp, _c_vp, _c_ll, _c_vp, _c_ll, _c_vp]
+
 # name -> (restype, argtypes): the exports of include/qwen38_kv.h
 SIGNATURES = {
     "mk_last_error": (_c_cp, []),
@@ -58,6 +64,15 @@ SIGNATURES = {
     "mk_verify_ws": (_c_ll, [_c_int, _c_int, _c_int]),
     "mk_verify_drafts": (_c_int, [_c_int, _c_int, _c_int, _c_vp, _c_ll, _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp,
                                   _c_ll, _c_vp]),
+    "mk_lora_ws": (_c_ll, [_c_int] * 3),
+    "mk_lora_rows": (_c_int, _LORA + [_c_vp, _c_ll, _c_int] + _LORA_TAIL),
+    "mk_lora_units": (_c_int, _LORA + [_c_vp] * 3 + _LORA_TAIL),
+    "mk_moe_route_ws": (_c_ll, [_c_int] * 3),
+    "mk_moe_route": (_c_int, [_c_int] * 4 + [_c_vp, _c_ll, _c_int, _c_vp, _c_int, _c_vp, _c_int, ctypes.c_float, _c_vp, _c_vp, _c_vp, _c_vp, _c_ll, _c_vp]),
+    "mk_moe_ws": (_c_ll, [_c_int] * 5),
+    "mk_moe_rows": (_c_int, _MOE + [_c_vp, _c_ll, _c_int] + _MOE_TAIL),
+    "mk_moe_units": (_c_int, _MOE + [_c_vp] * 3 + _MOE_TAIL),
+    "mk_moe_layer": (_c_int, _MOE + [_c_vp, _c_ll, _c_int, _c_vp, _c_int, _c_vp, _c_int, ctypes.c_float, _c_vp] + _MOE_TAIL),
     "mk_kv_window_start": (_c_int, [_c_int, _c_int]),
     "mk_kv_ring_rows": (_c_int, [_c_int]),
     "mk_kv_cap_T": (_c_int, [_c_int, _c_int]),
@@ -149,6 +164,60 @@ def verify_drafts(n_seq, n_draft, vocab, target, row_stride, dtype, probs, tempe
     """Accept drafts against the target's logits (probs 0) or probabilities (1) and draw the next token (mk_verify_drafts)."""
     _check(lib().mk_verify_drafts(n_seq, n_draft, vocab, target, row_stride, dtype, probs, temperature, draft_probs, drafts, n_drafts, u, accepted,
                                   tokens, draft_p, ws, ws_bytes, stream))
+
+
+# ---- adapters of many requests, a router and its experts
+def lora_ws(rows, k, rank):
+    """Bytes of workspace that lora_rows and lora_units need."""
+    return _check(lib().mk_lora_ws(rows, k, rank))
+
+
+def lora_rows(rows, n, k, n_adapters, rank, a, b, ab_dtype, ranks, scales, ids, x, x_stride, dtype, base, base_stride, y, y_stride, ws, ws_bytes, stream=0):
+    """y = base + scales[ids] B[ids] (A[ids] x) of plain rows x (mk_lora_rows)."""
+    _check(lib().mk_lora_rows(rows, n, k, n_adapters, rank, a, b, ab_dtype, ranks, scales, ids, x, x_stride, dtype, base, base_stride, y, y_stride, ws, ws_bytes,
+                              stream))
+
+
+def lora_units(rows, n, k, n_adapters, rank, a, b, ab_dtype, ranks, scales, ids, q32a, q32b, q32meta, base, base_stride, y, y_stride, ws, ws_bytes, stream=0):
+    """lora_rows on int8 units (mk_lora_units)."""
+    _check(lib().mk_lora_units(rows, n, k, n_adapters, rank, a, b, ab_dtype, ranks, scales, ids, q32a, q32b, q32meta, base, base_stride, y, y_stride, ws, ws_bytes,
+                               stream))
+
+
+def moe_route_ws(rows, dim, n_experts):
+    """Bytes of workspace that moe_route needs."""
+    return _check(lib().mk_moe_route_ws(rows, dim, n_experts))
+
+
+def moe_route(rows, dim, n_experts, top_k, x, x_stride, dtype, w, w_dtype, bias, form, scale, logits, ids, weights, ws, ws_bytes, stream=0):
+    """Logits of the experts, the top_k of each row and their weights (mk_moe_route)."""
+    _check(lib().mk_moe_route(rows, dim, n_experts, top_k, x, x_stride, dtype, w, w_dtype, bias, form, scale, logits, ids, weights, ws, ws_bytes, stream))
+
+
+def moe_ws(rows, dim, inner, n_experts, top_k):
+    """Bytes of workspace that moe_rows, moe_units and moe_layer need."""
+    return _check(lib().mk_moe_ws(rows, dim, inner, n_experts, top_k))
+
+
+def moe_rows(rows, dim, inner, n_experts, top_k, group, up, up_scales, up_mins, down, down_scales, down_mins, x, x_stride, dtype, ids, weights, y, y_stride, ws,
+             ws_bytes, stream=0):
+    """The chosen experts of each row, gated and summed by their weights, on plain rows x (mk_moe_rows)."""
+    _check(lib().mk_moe_rows(rows, dim, inner, n_experts, top_k, group, up, up_scales, up_mins, down, down_scales, down_mins, x, x_stride, dtype, ids, weights, y,
+                             y_stride, ws, ws_bytes, stream))
+
+
+def moe_units(rows, dim, inner, n_experts, top_k, group, up, up_scales, up_mins, down, down_scales, down_mins, q32a, q32b, q32meta, ids, weights, y, y_stride, ws,
+              ws_bytes, stream=0):
+    """moe_rows on int8 units (mk_moe_units)."""
+    _check(lib().mk_moe_units(rows, dim, inner, n_experts, top_k, group, up, up_scales, up_mins, down, down_scales, down_mins, q32a, q32b, q32meta, ids, weights, y,
+                              y_stride, ws, ws_bytes, stream))
+
+
+def moe_layer(rows, dim, inner, n_experts, top_k, group, up, up_scales, up_mins, down, down_scales, down_mins, x, x_stride, dtype, router, router_dtype, bias, form,
+              scale, logits, ids, weights, y, y_stride, ws, ws_bytes, stream=0):
+    """moe_route and moe_rows on its choice in one call (mk_moe_layer)."""
+    _check(lib().mk_moe_layer(rows, dim, inner, n_experts, top_k, group, up, up_scales, up_mins, down, down_scales, down_mins, x, x_stride, dtype, router,
+                              router_dtype, bias, form, scale, logits, ids, weights, y, y_stride, ws, ws_bytes, stream))
 
 
 class KVStore:
