@@ -70,7 +70,8 @@ struct MoeArgs {
     float * hd;      // [pairs][inner / 32]
     float * hs;      // [pairs][inner / 32]
     float * out;     // [pairs][dim]
-    int tp_up, tp_down; // (set by moe_plan) tokens of an expert that a pass holds in LDS
+    // (set by the launcher) tokens of an expert that a pass holds in LDS, and waves (1 << ..) that split k
+    int tp_up, tp_down, ks_up, ks_down;
 };
 constexpr int MOE_ROWS = 64;   // rows of a launch; a call of more runs them one after another
 constexpr int MOE_MAX_ROWS = 4096, MOE_MAX_DIM = 16384, MOE_MAX_INNER = 32768;

@@ -1,17 +1,19 @@
 // A mixture-of-experts layer with 4-bit weights for a few tokens: h = silu(G x) (U x) of every (token, expert) pair, then
 // y[m] = sum over the row's experts of w D h.  Three kernels: the gate's and the up projection's rows together, the down projection of every
-// pair, and the sum over a row's experts in their order (no atomics: the same bits every time).
+// pair, and the sum over a row's experts in their order (no atomics: the same bits every time); where the pairs are few the last two are
+// one.
 //
-// Workgroups stand for (a tile of weight rows, one of the experts that occur); each finds its expert and the pairs that chose it in
-// the row's choices itself.  An expert has few tokens, so what counts is the way of its codes: from HBM, and from 4 bits to an operand.  Codes
-// become int8 with four vector instructions for 8 of them (fp16 takes 13), so x is made integer too: per block of 32 values an exponent,
-// and two or three int8 planes (14 bits of the block's largest power of two for 16-bit x, 22 for fp32; int8 units are one plane as they are).  The
-// matrix instruction's sums are exact, a block's scales multiply its sum in fp32.
+// Workgroups stand for (columns, one of the experts that occur); each finds its expert and the pairs that chose it in the rows'
+// choices itself.  An expert has few tokens, so what counts is the way of its codes: from HBM, and from 4 bits to an operand.  Codes
+// become int8 with four vector instructions for 8 of them (fp16 takes 13), so x is made integer too: an exponent for every block, and two
+// or three int8 planes (14 bits of the block's largest power of two for 16-bit x, 22 for fp32; int8 units are one plane as
+// they are).  The matrix instruction's sums are exact, the scales multiply them in fp32.
 //
-// A wave has two tiles of 16 weight rows.  Lane (n = lane & 15, g = lane >> 4) loads the 16 bytes of block 8 R + 2 g + u of row n, u = 0, 1:
-// 32 bytes of its own, the 128 of a cache line for a row's four lanes, and both scales in 4 bytes.  The instruction contracts over all four
-// lane groups, but every block has scales of its own, so the planes go in on the diagonal: operand row 4 b + m holds plane m of block
-// b in lane group b and zeros in the others, and output row 4 b + m is that block's sum, in the lanes that hold its scale.
+// A wave has two tiles of 16 weight rows, lane (n = lane & 15, g = lane >> 4) 16 bytes, a block of 32 codes of row n, a step.  The instruction
+// contracts over all four lane groups, so blocks with scales of their own must not meet in it: the planes go in on a (block) diagonal,
+// operand rows for lane groups whose blocks share a weight scale, zeros in the other groups.  Blocks of 32 values with scales of their own:
+// four groups, 4 rows of planes each.  Weight groups of 64 or 128 values, and x with one exponent for as many: two lane groups or all
+// four share a sum, 8 or 16 rows of planes go in at a time, and every sum is scaled once for 64 or 128 values.
 #include "step_dev.h"
 #include "step_mix_launch.h"
 
@@ -24,34 +26,51 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32_u2 __attribute__((aligned(2)));
 
-constexpr int T_MAX = 16;     // tokens of an expert in a pass
 constexpr int MAX_PAIRS = MOE_ROWS * ROUTE_MAX_TOP;
 constexpr int WAVES = 8;
 
 constexpr int planes_of(int xform) { return xform == W4_UNITS ? 1 : xform == DT_F32 ? 3 : 2; }
 constexpr int inner_planes(int xform) { return xform == DT_F16 || xform == DT_BF16 ? 2 : 3; } // (y is fp32 else)
-constexpr int group_of(int P) { return P == 1 ? 4 : P == 2 ? 2 : 1; } // tokens of one matrix instruction
+// operand rows of a token (three planes: the fourth stays zero), tokens in a lane's sums of an instruction, tokens of an instruction; sg: lane
+// groups that share a sum are 1 << sg
+constexpr int op_rows(int P) { return P == 3 ? 4 : P; }
+constexpr int lane_tokens(int P) { return 4 / op_rows(P); }
+constexpr int group_of(int P, int sg) { return lane_tokens(P) << sg; }
 
-// LDS of a pass: rows of planes (token t's plane p is row t P + p), each [runs of 8 blocks][u][half][g][16 bytes], the rows 64 bytes
-// past a multiple of 256 so that an instruction's 16 pieces lie in different banks; 128 zeros; per block the tokens' factors, and
-// with minimums the tokens' sums
+// LDS of a pass: x as planes, token t's plane p is row t P + p: [runs of 8 blocks][u][half][rows][64 bytes: 16 of each lane group's block];
+// where more than four rows go in for a group, the groups' places are exchanged every four rows (their pieces lie in different banks); then zeros for the operand's
+// other lanes, per 32 << sg values the tokens' factors, and with minimums the tokens' sums
 struct Lds {
-    int row, zero, dx, ds, end;
+    int step, zero, dx, ds, end; // bytes of all rows' 64; offsets
 };
-__host__ __device__ __forceinline__ constexpr Lds lds_of(int P, int nbp, int tp, bool mins) {
+__host__ __device__ __forceinline__ constexpr Lds lds_of(int P, int sg, int nbp, int tp, bool mins) {
     Lds l{};
-    l.row = nbp * 32 + 64;
-    l.zero = tp * P * l.row;
-    l.dx = l.zero + 128;
-    l.ds = l.dx + nbp * tp * 4;
-    l.end = mins ? l.ds + nbp * tp * 4 : l.ds;
+    l.step = tp * P * 64;
+    l.zero = (nbp >> 1) * l.step;
+    l.dx = l.zero + l.step + 64; // (the operand's offsets within a step go for the zeros too)
+    l.ds = l.dx + (nbp >> sg) * tp * 4;
+    l.end = mins ? l.ds + (nbp >> sg) * tp * 4 : l.ds;
     return l;
 }
 __host__ __device__ __forceinline__ constexpr int padded(int blocks) { return (blocks + 7) & ~7; }
-// the place in a row of 16 bytes of a block
-__device__ __forceinline__ int piece(int block, int half) { return ((block >> 3) * 4 + (block & 1) * 2 + half) * 64 + (block >> 1 & 3) * 16; }
+// the block of lane group g in step u of a run of 8 blocks: groups that share a sum have blocks of one weight group, and a lane's two steps
+// have scales that lie next to each other
+template <int SG> __device__ __forceinline__ int block_of(int g, int u) {
+    return SG == 0 ? 2 * g + u : SG == 1 ? 4 * (g >> 1) + 2 * u + (g & 1) : 4 * u + g;
+}
+// 16 bytes of a block: its place among a row's 64-byte pieces, and its group in it
+template <int SG> __device__ __forceinline__ int piece_of(int block, int half) {
+    const int b = block & 7, u = SG == 0 ? b & 1 : SG == 1 ? b >> 1 & 1 : b >> 2;
+    return (block >> 3) * 4 + u * 2 + half;
+}
+template <int SG> __device__ __forceinline__ int group_in(int block) {
+    const int b = block & 7;
+    return SG == 0 ? b >> 1 : SG == 1 ? 2 * (b >> 2) + (b & 1) : b & 3;
+}
+template <int SG> __device__ __forceinline__ int turn(int row, int g) { return SG == 0 ? g : (g ^ (row >> 2)) & 3; }
+template <int SG> __device__ __forceinline__ int place(int row, int g) { return row * 64 + turn<SG>(row, g) * 16; }
 
-// a block's values as integers: times `up`, a power of two that brings the largest to [2^13, 2^14) (three planes: [2^21, 2^22)), and the
+// values as integers: times `up`, a power of two that brings the largest to [2^13, 2^14) (three planes: [2^21, 2^22)), and the
 // factor 1 / (16 up) of the products with codes 16 times as large
 struct Fixed {
     float up, dx;
@@ -71,98 +90,149 @@ template <int P> __device__ __forceinline__ void planes_split(int v, int (&q)[P]
     }
     q[0] = v;
 }
+template <int P> __device__ __forceinline__ int to_fixed(float v, float up) { return up == 0.f ? 0 : (int) __builtin_rintf(v * up); } // (0 inf is a NaN)
 
-// two tiles of 16 weight rows, the lane's row of each
-struct Rows {
-    const uint8_t * c[2];
-    const uint16_t * s[2], * m[2];
+// NT tiles of 16 weight rows: a tile's first row in scalars, the lane's in 32 bits behind it
+template <int NT> struct Rows {
+    const uint8_t * c[NT];
+    const uint16_t * s[NT], * m[NT];
+    unsigned vc[NT], vs[NT];
+    // tile t: rows from `first` on of an expert's, rows past its last one (of n) that one again
+    __device__ __forceinline__ void set(int t, const MoeWeights & w, int e, int n, int first, int nb, int gs) {
+        const int f = min(first, n - 1), r = min((int) (threadIdx.x & 15), n - 1 - f);
+        const size_t row = (size_t) e * n + f;
+        c[t] = w.codes + row * (nb * 16);
+        s[t] = w.scales + row * gs;
+        m[t] = w.mins + row * gs;
+        vc[t] = (unsigned) (r * nb * 16);
+        vs[t] = (unsigned) (r * gs);
+    }
 };
-// the sums of runs r0 .. r1 - 1 (of 8 blocks) for nt tokens in LDS
-template <int P, int GSH, bool MINS>
-__device__ __forceinline__ void products(const Rows & w, int nb, int r0, int r1, const uint8_t * lds, const Lds & L, int tp, int nt, float (&acc)[2][T_MAX]) {
-    constexpr int TG = group_of(P), VR = TG * P; // tokens and operand rows of an instruction
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, m = n & 3, gs = (nb + (1 << GSH) - 1) >> GSH;
-    const bool active = n >> 2 == g && m < VR;
-    const int aoff = active ? m * L.row + g * 16 : L.zero;
-    const unsigned amask = active ? ~0u : 0u;
+// a run's codes and scales in registers
+template <int NT, bool MINS> struct Run {
+    u32x4 c[NT][2];
+    unsigned s[NT], m[NT]; // of the two steps (groups of more than 32 without a shared sum: one)
+};
+template <int GSH, int SG> __device__ __forceinline__ unsigned run_scales(const uint16_t * p, unsigned v, int gs, int R, int g) {
+    const int i = ((8 * R) >> GSH) + (SG == GSH ? 2 * (g >> SG) : (2 * g) >> GSH);
+    if constexpr (SG != GSH) return p[v + (unsigned) min(i, gs - 1)];
+    if ((8 * R + 8) >> GSH <= gs) return *reinterpret_cast<const u32_u2 *>(p + (v + (unsigned) i));
+    return p[v + (unsigned) min(i, gs - 1)] | (unsigned) p[v + (unsigned) min(i + 1, gs - 1)] << 16;
+}
+template <int GSH, int SG, int NT, bool MINS> __device__ __forceinline__ Run<NT, MINS> load_run(const Rows<NT> & w, int nb, int R) {
+    const int g = threadIdx.x >> 4 & 3, gs = (nb + (1 << GSH) - 1) >> GSH;
+    Run<NT, MINS> r;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) r.c[t][u] = *reinterpret_cast<const u32x4 *>(w.c[t] + (w.vc[t] + (unsigned) min(8 * R + block_of<SG>(g, u), nb - 1) * 16)); // (past the last block zeros of x, or of its factors)
+        r.s[t] = run_scales<GSH, SG>(w.s[t], w.vs[t], gs, R, g);
+        if constexpr (MINS) r.m[t] = run_scales<GSH, SG>(w.m[t], w.vs[t], gs, R, g);
+    }
+    return r;
+}
+
+// the sums of runs r0 .. r1 - 1 (in: the first one's codes) for nt tokens in LDS, at most TM
+template <int P, int GSH, int SG, int NT, int TM, bool MINS>
+__device__ __forceinline__ void products(const Rows<NT> & w, Run<NT, MINS> in, int nb, int r0, int r1, const uint8_t * lds, const Lds & L, int tp, int nt, float (&acc)[NT][TM >> SG]) {
+    constexpr int PR = op_rows(P), TL = lane_tokens(P), TG = group_of(P, SG);
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, m = n & ((4 << SG) - 1), gs = (nb + (1 << GSH) - 1) >> GSH;
+    const bool active = n >> (2 + SG) == g >> SG && m % PR < P;
+    const int row = m / PR * P + m % PR;
+    const int first = (g & ((1 << SG) - 1)) * TL; // of a group's tokens, the first in the lane's sums
     const float * dx = reinterpret_cast<const float *>(lds + L.dx), * ds = reinterpret_cast<const float *>(lds + L.ds);
-    struct Run {
-        u32x4 c[2][2];
-        unsigned s[2], m[2]; // two scales
-    };
-    const auto scales = [&](const uint16_t * p, int R) -> unsigned {
-        if constexpr (GSH == 0) {
-            if (8 * R + 8 <= nb) return *reinterpret_cast<const u32_u2 *>(p + 8 * R + 2 * g);
-            return p[min(8 * R + 2 * g, nb - 1)] | (unsigned) p[min(8 * R + 2 * g + 1, nb - 1)] << 16;
-        } else return p[min((8 * R + 2 * g) >> GSH, gs - 1)];
-    };
-    const auto load = [&](int R) {
-        Run r;
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
+    for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int u = 0; u < 2; u++) r.c[t][u] = *reinterpret_cast<const u32x4 *>(w.c[t] + min(8 * R + 2 * g + u, nb - 1) * 16); // (past the last block factors of zero)
-            r.s[t] = scales(w.s[t], R);
-            if constexpr (MINS) r.m[t] = scales(w.m[t], R);
-        }
-        return r;
-    };
-    if (r0 >= r1) return;
-    Run nx = load(r0);
+        for (int i = 0; i < TM >> SG; i++) acc[t][i] = 0.f;
 #pragma unroll 1
     for (int R = r0; R < r1; R++) {
-        const Run cu = nx;
-        if (R + 1 < r1) nx = load(R + 1);
+        const int next = min(R + 1, r1 - 1); // (behind the last run that one again, unused)
+        float sc[NT][2], mn[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                sc[t][u] = h2f_bits((uint16_t) (in.s[t] >> (SG == GSH ? 16 * u : 0)));
+                if constexpr (MINS) mn[t][u] = h2f_bits((uint16_t) (in.m[t] >> (SG == GSH ? 16 * u : 0)));
+            }
+        }
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            i32x4 b[2][2];
-            float sc[2], mn[2];
+            i32x4 b[NT][2];
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
+            for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     int t0, t1;
-                    w4_bytes(cu.c[t][u][k], t0, t1);
+                    w4_bytes(in.c[t][u][k], t0, t1);
                     b[t][k >> 1][2 * (k & 1)] = t0;
                     b[t][k >> 1][2 * (k & 1) + 1] = t1;
                 }
-                sc[t] = h2f_bits((uint16_t) (cu.s[t] >> (GSH == 0 ? 16 * u : 0)));
-                if constexpr (MINS) mn[t] = h2f_bits((uint16_t) (cu.m[t] >> (GSH == 0 ? 16 * u : 0)));
+            __builtin_amdgcn_sched_barrier(0); // the codes leave their registers, then the next run's take them
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                in.c[t][u] = *reinterpret_cast<const u32x4 *>(w.c[t] + (w.vc[t] + (unsigned) min(8 * next + block_of<SG>(g, u), nb - 1) * 16));
+                if (u == 0) {
+                    in.s[t] = run_scales<GSH, SG>(w.s[t], w.vs[t], gs, next, g);
+                    if constexpr (MINS) in.m[t] = run_scales<GSH, SG>(w.m[t], w.vs[t], gs, next, g);
+                }
             }
-            const int block = 8 * R + 2 * g + u;
+            __builtin_amdgcn_sched_barrier(0);
+            const uint8_t * ap = lds + (active ? (R * 4 + u * 2) * L.step + row * 64 + (SG == 0 ? g * 16 : 0) : L.zero), * ah = ap + (active ? L.step : 0);
+            const int at = ((8 * R + block_of<SG>(g, u)) >> SG) * tp + first;
 #pragma unroll
-            for (int q = 0; q < T_MAX / TG; q++) {
+            for (int q = 0; q < TM / TG; q++) {
                 if (q * TG >= nt) continue;
-                const uint8_t * ap = lds + aoff + ((unsigned) (q * VR * L.row + (R * 4 + u * 2) * 64) & amask);
-                const i32x4 a0 = *reinterpret_cast<const i32x4 *>(ap), a1 = *reinterpret_cast<const i32x4 *>(ap + 64);
-                i32x4 c[2];
+                const int o = q * TG * P * 64 + (SG == 0 ? 0 : turn<SG>(TG * P % 16 ? row + q * TG * P : row, g) * 16);
+                const i32x4 a0 = *reinterpret_cast<const i32x4 *>(ap + o), a1 = *reinterpret_cast<const i32x4 *>(ah + o);
+                i32x4 c[NT];
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
+                for (int t = 0; t < NT; t++) {
                     c[t] = i32x4{0, 0, 0, 0};
                     c[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a0, b[t][0], c[t], 0, 0, 0);
                     c[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a1, b[t][1], c[t], 0, 0, 0);
                 }
 #pragma unroll
-                for (int i = 0; i < TG; i++) {
-                    const float d = dx[block * tp + q * TG + i];
+                for (int i = 0; i < TL; i++) {
+                    const float d = dx[at + q * TG + i];
 #pragma unroll
-                    for (int t = 0; t < 2; t++) {
+                    for (int t = 0; t < NT; t++) {
                         float v;
                         if constexpr (P == 1) v = (float) c[t][i];
                         else if constexpr (P == 2) v = (float) ((c[t][2 * i] << 8) + c[t][2 * i + 1]);
                         else v = __builtin_fmaf((float) ((c[t][0] << 8) + c[t][1]), 256.f, (float) c[t][2]);
-                        float & s = acc[t][q * TG + i];
-                        s = __builtin_fmaf(v, sc[t] * d, s);
-                        if constexpr (MINS) s = __builtin_fmaf(mn[t], ds[block * tp + q * TG + i], s);
+                        float & s = acc[t][q * TL + i];
+                        s = __builtin_fmaf(v, sc[t][u] * d, s);
+                        if constexpr (MINS) s = __builtin_fmaf(mn[t][u], ds[at + q * TG + i], s);
                     }
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
 }
+// the wave's sums of nt tokens to red[tile][tp][16]: added over the lane groups that have the same token
+template <int P, int SG, int NT, int TM> __device__ __forceinline__ void sums_out(float (&acc)[NT][TM >> SG], int tp, int nt, float * red) {
+    constexpr int TL = lane_tokens(P), TG = group_of(P, SG);
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, first = (g & ((1 << SG) - 1)) * TL;
+#pragma unroll
+    for (int q = 0; q < TM / TG; q++) {
+        if (q * TG >= nt) continue;
+#pragma unroll
+        for (int i = 0; i < TL; i++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                float v = acc[t][q * TL + i];
+                if constexpr (SG == 0) v = quad_sum(v);
+                if constexpr (SG == 1) v += shfl_xor(v, 32);
+                if (g >> SG == 0 && q * TG + first + i < tp) red[(t * tp + q * TG + first + i) * 16 + n] = v;
+            }
+    }
+}
 
-// The slot-th expert that occurs (ascending) and the pairs that chose it (in any order: a pair's results do not depend on its place);
-// -1 past the last one.  Choices that are no expert are left out.
+// The slot-th expert that occurs and the pairs that chose it (in any order: a pair's results do not depend on its place); -1 past the last
+// one.  Choices that are no expert are left out.
 struct Found {
     unsigned mark[ROUTE_MAX_EXPERTS / 32];
     int count;
@@ -170,8 +240,23 @@ struct Found {
 };
 constexpr int FOUND = (sizeof(Found) + 255) & ~255; // its place in LDS, in front of a pass's
 __device__ __forceinline__ int find(const int * ids, int pairs, int n_experts, int slot, Found & f) {
-    constexpr int NP = (MAX_PAIRS + WAVES * 64 - 1) / (WAVES * 64);
     const int lane = threadIdx.x & 63;
+    if (pairs <= 64) { // every wave by itself, in the order of their first pairs (the waves write the same list)
+        const int id = lane < pairs ? ids[lane] : -1;
+        uint64_t todo = __ballot((unsigned) id < (unsigned) n_experts), of = 0;
+        int e = -1;
+        for (; todo && slot >= 0; slot--) {
+            e = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
+            of = __ballot(id == e);
+            todo &= ~of;
+        }
+        if (slot >= 0) return -1;
+        if (id == e) f.pairs[__builtin_amdgcn_mbcnt_hi((unsigned) (of >> 32), __builtin_amdgcn_mbcnt_lo((unsigned) of, 0))] = (uint16_t) lane;
+        f.count = __builtin_popcountll(of);
+        __syncthreads();
+        return e;
+    }
+    constexpr int NP = (MAX_PAIRS + WAVES * 64 - 1) / (WAVES * 64);
     int id[NP];
     if (threadIdx.x < ROUTE_MAX_EXPERTS / 32) f.mark[threadIdx.x] = 0;
     if (threadIdx.x == 0) f.count = 0;
@@ -208,20 +293,22 @@ __device__ __forceinline__ unsigned lds_address(const uint8_t * lds) {
     return (unsigned) __builtin_amdgcn_readfirstlane((unsigned) (size_t) (const __attribute__((address_space(3))) uint8_t *) lds);
 }
 
-// x of tokens t0 .. t0 + nt - 1 of the expert into LDS
-template <int XF, bool MINS> __device__ __forceinline__ void stage_x(const MoeArgs & a, uint8_t * lds, const Lds & L, int tp, int nt, const uint16_t * pairs) {
+// x of nt tokens into LDS
+template <int XF, int SG, bool MINS> __device__ __forceinline__ void stage_x(const MoeArgs & a, uint8_t * lds, const Lds & L, int tp, int nt, const uint16_t * pairs) {
     constexpr int P = planes_of(XF);
     const int nb = a.dim >> 5, nbp = padded(nb), tid = threadIdx.x;
     float * dx = reinterpret_cast<float *>(lds + L.dx), * ds = reinterpret_cast<float *>(lds + L.ds);
     if constexpr (XF == W4_UNITS) {
+        static_assert(SG == 0, "a unit's blocks have scales of their own");
         const unsigned base = lds_address(lds);
-        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, per = (nbp * 2 + 63) >> 6;
-        for (int c = wave; c < nt * per; c += WAVES) { // 64 pieces a copy
-            const int t = c / per, i = (c - t * per) * 64 + lane, row = pairs[t] / a.top_k;
-            const int block = min((i >> 4) * 8 + (i & 3) * 2 + (i >> 3 & 1), nb - 1);
-            const int8_t * from = (block & 1 ? a.xb : a.xa) + ((size_t) row * nb + (block & ~1) + (i >> 2 & 1)) * 16;
-            if (i < nbp * 2) dma16(from, base + t * L.row + (c - t * per) * 1024);
-        }
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+        for (int c = wave; c < nbp >> 1; c += WAVES) // a piece of 16 rows a copy
+            for (int t0 = 0; t0 < nt; t0 += 16) {
+                const int t = t0 + (lane >> 2), g = lane & 3, row = pairs[min(t, nt - 1)] / a.top_k;
+                const int block = min((c >> 2) * 8 + block_of<0>(g, c >> 1 & 1), nb - 1);
+                const int8_t * from = (block & 1 ? a.xb : a.xa) + ((size_t) row * nb + (block & ~1) + (c & 1)) * 16;
+                if (t < nt) dma16(from, base + c * L.step + t0 * 64);
+            }
         for (int i = tid; i < nt * nbp; i += WAVES * 64) {
             const int t = i / nbp, block = i - t * nbp, row = pairs[t] / a.top_k;
             float d = 0.f, s = 0.f;
@@ -235,189 +322,170 @@ template <int XF, bool MINS> __device__ __forceinline__ void stage_x(const MoeAr
         }
         vm_drain();
     } else {
-        for (int i = tid; i < nt * nbp * 4; i += WAVES * 64) { // a quarter of a block
+        for (int i = tid; i < nt * nbp * 4; i += WAVES * 64) { // a quarter of a block (4 << SG lanes an exponent)
             const int t = i / (nbp * 4), j = i - t * nbp * 4, block = j >> 2, qt = j & 3;
-            const bool in = block < nb;
             float v[8], s = 0.f;
             typename Elem<XF>::Raw8 raw{};
-            if (in) raw = Elem<XF>::raw8(static_cast<const typename Elem<XF>::T *>(a.x) + (pairs[t] / a.top_k) * a.x_stride + 32 * block + 8 * qt);
+            if (block < nb) raw = Elem<XF>::raw8(static_cast<const typename Elem<XF>::T *>(a.x) + (pairs[t] / a.top_k) * a.x_stride + 32 * block + 8 * qt);
             unsigned top = Elem<XF>::top8(raw);
-            top = max(top, shfl_xor_u(top, 1));
-            top = max(top, shfl_xor_u(top, 2));
+#pragma unroll
+            for (int m = 1; m < 4 << SG; m <<= 1) top = max(top, shfl_xor_u(top, m));
             Elem<XF>::open8(raw, v);
             if (MINS) {
 #pragma unroll
                 for (int k = 0; k < 8; k++) s += v[k];
-                s += shfl_xor(s, 1);
-                s += shfl_xor(s, 2);
+#pragma unroll
+                for (int m = 1; m < 4 << SG; m <<= 1) s += shfl_xor(s, m);
             }
             const Fixed f = fixed_of<P>(top);
             unsigned out[P][2] = {};
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 int q[P];
-                planes_split<P>((int) __builtin_rintf(v[k] * f.up), q);
+                planes_split<P>(to_fixed<P>(v[k], f.up), q);
 #pragma unroll
                 for (int p = 0; p < P; p++) out[p][k >> 2] |= (unsigned) (q[p] & 255) << 8 * (k & 3);
             }
-            uint8_t * to = lds + t * P * L.row + piece(block, qt >> 1) + 8 * (qt & 1);
+            uint8_t * to = lds + piece_of<SG>(block, qt >> 1) * L.step + 8 * (qt & 1);
 #pragma unroll
-            for (int p = 0; p < P; p++) *reinterpret_cast<uint2 *>(to + p * L.row) = make_uint2(out[p][0], out[p][1]);
-            if (qt == 0) {
-                dx[block * tp + t] = in ? f.dx : 0.f;
-                if (MINS) ds[block * tp + t] = s;
+            for (int p = 0; p < P; p++) *reinterpret_cast<uint2 *>(to + place<SG>(t * P + p, group_in<SG>(block))) = make_uint2(out[p][0], out[p][1]);
+            if ((j & ((4 << SG) - 1)) == 0) {
+                dx[(block >> SG) * tp + t] = block < nb ? f.dx : 0.f;
+                if (MINS) ds[(block >> SG) * tp + t] = s;
             }
         }
     }
 }
 
-// the inner values' planes of an expert's tokens into LDS
-template <int P, bool MINS> __device__ __forceinline__ void stage_h(const MoeArgs & a, uint8_t * lds, const Lds & L, int tp, int nt, const uint16_t * pairs) {
-    const int nb = a.inner >> 5, nbp = padded(nb), tid = threadIdx.x, per = (nbp * 2 + 63) >> 6;
+// the inner values' planes of nt pairs into LDS
+template <int P, int SG, bool MINS> __device__ __forceinline__ void stage_h(const MoeArgs & a, uint8_t * lds, const Lds & L, int tp, int nt, const uint16_t * pairs) {
+    const int nb = a.inner >> 5, nbp = padded(nb), tid = threadIdx.x, ng = (nb + (1 << SG) - 1) >> SG;
     const unsigned base = lds_address(lds);
     float * dx = reinterpret_cast<float *>(lds + L.dx), * ds = reinterpret_cast<float *>(lds + L.ds);
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    for (int c = wave; c < nt * P * per; c += WAVES) {
-        const int r = c / per, t = r / P, i = (c - r * per) * 64 + lane;
-        if (i < nbp * 2) dma16(a.hq + ((size_t) pairs[t] * P + (r - t * P)) * nbp * 32 + i * 16, base + r * L.row + (c - r * per) * 1024);
-    }
-    for (int i = tid; i < nt * nbp; i += WAVES * 64) {
-        const int t = i / nbp, block = i - t * nbp;
-        dx[block * tp + t] = block < nb ? a.hd[(size_t) pairs[t] * nb + block] : 0.f;
-        if (MINS) ds[block * tp + t] = block < nb ? a.hs[(size_t) pairs[t] * nb + block] : 0.f;
+    for (int c = wave; c < nbp >> 1; c += WAVES) // a piece of 16 rows a copy
+        for (int r0 = 0; r0 < nt * P; r0 += 16) {
+            const int r = r0 + (lane >> 2), t = min(r / P, nt - 1), g = turn<SG>(r, lane & 3); // (its own inverse)
+            if (r < nt * P) dma16(a.hq + ((size_t) pairs[t] * P + (r - t * P)) * nbp * 32 + c * 64 + g * 16, base + c * L.step + r0 * 64);
+        }
+    for (int i = tid; i < nt * (nbp >> SG); i += WAVES * 64) {
+        const int t = i / (nbp >> SG), k = i - t * (nbp >> SG);
+        dx[k * tp + t] = k < ng ? a.hd[(size_t) pairs[t] * ng + k] : 0.f;
+        if (MINS) ds[k * tp + t] = k < ng ? a.hs[(size_t) pairs[t] * ng + k] : 0.f;
     }
     vm_drain();
 }
 __device__ __forceinline__ void zero_pieces(uint8_t * lds, const Lds & L) {
-    if (threadIdx.x < 32) reinterpret_cast<unsigned *>(lds + L.zero)[threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < (L.dx - L.zero) / 4; i += WAVES * 64) reinterpret_cast<unsigned *>(lds + L.zero)[i] = 0;
 }
 
-// h of 32 inner columns for the expert's tokens: waves (half of the columns, a quarter of dim)
-template <int XF, int GSH, bool MINS> __global__ __launch_bounds__(WAVES * 64, 2) void k_moe_up(MoeArgs a) {
-    constexpr int P = planes_of(XF), HP = inner_planes(XF), KS = WAVES / 2;
+// The gate and the up projection: a workgroup has 16 CG inner columns of an expert, its waves (16 columns of both, a KS-th of dim), CG KS = 8.
+// SG: lane groups that share a sum of x; SH: those of the down projection, whose x (h) this kernel leaves as planes.
+template <int XF, int GSH, int SH, int TM, bool MINS> __global__ __launch_bounds__(WAVES * 64, 4) void k_moe_up(MoeArgs a) {
+    constexpr int P = planes_of(XF), HP = inner_planes(XF), SG = P == 1 ? 0 : GSH;
     extern __shared__ __attribute__((aligned(16))) uint8_t all[];
     Found & found = *reinterpret_cast<Found *>(all);
     uint8_t * lds = all + FOUND;
     const int nb = a.dim >> 5, nbp = padded(nb), runs = nbp >> 3, tp = a.tp_up;
-    const Lds L = lds_of(P, nbp, tp, MINS);
-    float * red = reinterpret_cast<float *>(lds + ((L.end + 15) & ~15)); // [KS][2 halves][2][tp][16]
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, half = wave & 1, ks = wave >> 1;
+    const Lds L = lds_of(P, SG, nbp, tp, MINS);
+    float * red = reinterpret_cast<float *>(lds + ((L.end + 15) & ~15)); // [KS][CG][2][tp][16]
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int KS = 1 << a.ks_up, CG = WAVES >> a.ks_up, cg = wave & (CG - 1), ks = wave / CG;
     const int e = find(a.ids, a.rows * a.top_k, a.n_experts, blockIdx.y, found);
     if (e < 0) return;
-    const int cnt = found.count, gs = (nb + (1 << GSH) - 1) >> GSH;
-    Rows w;
-#pragma unroll
-    for (int t = 0; t < 2; t++) {
-        const size_t r = (size_t) e * 2 * a.inner + t * a.inner + blockIdx.x * 32 + half * 16 + n;
-        w.c[t] = a.up.codes + r * (a.dim >> 1);
-        w.s[t] = a.up.scales + r * gs;
-        w.m[t] = MINS ? a.up.mins + r * gs : nullptr;
-    }
+    const int cnt = found.count, gs = (nb + (1 << GSH) - 1) >> GSH, c0 = blockIdx.x * 16 * CG, r0 = (runs * ks) >> a.ks_up, r1 = (runs * (ks + 1)) >> a.ks_up;
+    Rows<2> w; // (columns past the last one: zeros below)
+    w.set(0, a.up, 2 * e, a.inner, c0 + cg * 16, nb, gs);
+    w.set(1, a.up, 2 * e + 1, a.inner, c0 + cg * 16, nb, gs);
     zero_pieces(lds, L);
     for (int t0 = 0; t0 < cnt; t0 += tp) {
         const int nt = min(tp, cnt - t0);
+        const Run<2, MINS> first = load_run<GSH, SG, 2, MINS>(w, nb, min(r0, runs - 1)); // (on its way while x is made ready)
         if (t0) __syncthreads();
-        stage_x<XF, MINS>(a, lds, L, tp, nt, found.pairs + t0);
+        stage_x<XF, SG, MINS>(a, lds, L, tp, nt, found.pairs + t0);
         __syncthreads();
-        float acc[2][T_MAX];
-#pragma unroll
-        for (int i = 0; i < T_MAX; i++) acc[0][i] = acc[1][i] = 0.f;
-        products<P, GSH, MINS>(w, nb, runs * ks / KS, runs * (ks + 1) / KS, lds, L, tp, nt, acc);
-#pragma unroll
-        for (int i = 0; i < T_MAX; i++) {
-            if (i >= nt) continue;
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const float v = quad_sum(acc[t][i]);
-                if (lane < 16) red[(((ks * 2 + half) * 2 + t) * tp + i) * 16 + n] = v;
-            }
-        }
+        float acc[2][TM >> SG];
+        products<P, GSH, SG, 2, TM, MINS>(w, first, nb, r0, r1, lds, L, tp, nt, acc);
+        sums_out<P, SG, 2, TM>(acc, tp, nt, red + (ks * CG + cg) * 2 * tp * 16);
         __syncthreads();
-        // 32 lanes per token: its 32 columns, one block of the down projection's x
-        const int i = threadIdx.x >> 5, col = threadIdx.x & 31;
-        if (i < nt) {
-            float gt = 0.f, up = 0.f;
-#pragma unroll
+        // four columns of a token a thread, 8 << SH threads for the values of an exponent of h
+        for (int j = threadIdx.x; j < nt * CG * 4; j += WAVES * 64) {
+            const int i = j / (CG * 4), col = (j - i * (CG * 4)) * 4, c = c0 + col;
+            f32x4 gt = {0.f, 0.f, 0.f, 0.f}, up = gt, h;
             for (int k = 0; k < KS; k++) {
-                const int at = (k * 2 + (col >> 4)) * 2;
-                gt += red[(at * tp + i) * 16 + (col & 15)];
-                up += red[((at + 1) * tp + i) * 16 + (col & 15)];
+                const float * p = red + (((k * CG + (col >> 4)) * 2 * tp + i) * 16 + (col & 15));
+                gt += *reinterpret_cast<const f32x4 *>(p);
+                up += *reinterpret_cast<const f32x4 *>(p + tp * 16);
             }
-            const float h = gt / (1.f + expf(-gt)) * up;
-            unsigned top = __builtin_bit_cast(unsigned, h) & 0x7fffffffu;
-            float s = h;
+            unsigned top = 0;
+            float s = 0.f;
 #pragma unroll
-            for (int m = 1; m < 32; m <<= 1) {
+            for (int k = 0; k < 4; k++) {
+                h[k] = c < a.inner ? gt[k] / (1.f + expf(-gt[k])) * up[k] : 0.f; // (inner is a multiple of 32)
+                const float hk = h[k]; // (a bit cast of a vector's element itself takes the first one)
+                top = max(top, __builtin_bit_cast(unsigned, hk) & 0x7fffffffu);
+                s += hk;
+            }
+#pragma unroll
+            for (int m = 1; m < 8 << SH; m <<= 1) {
                 top = max(top, shfl_xor_u(top, m));
                 if (MINS) s += shfl_xor(s, m);
             }
             const Fixed f = fixed_of<HP>(top);
-            int q[HP];
-            planes_split<HP>((int) __builtin_rintf(f.up == 0.f ? 0.f : h * f.up), q);
-            const int nbi = a.inner >> 5, block = blockIdx.x, pair = found.pairs[t0 + i];
-            uint8_t * to = a.hq + (size_t) pair * HP * padded(nbi) * 32 + piece(block, col >> 4) + (col & 15);
+            unsigned out[HP] = {};
 #pragma unroll
-            for (int p = 0; p < HP; p++) to[(size_t) p * padded(nbi) * 32] = (uint8_t) q[p];
-            if (col == 0) {
-                a.hd[(size_t) pair * nbi + block] = f.dx;
-                if (MINS) a.hs[(size_t) pair * nbi + block] = s;
+            for (int k = 0; k < 4; k++) {
+                int q[HP];
+                planes_split<HP>(to_fixed<HP>(h[k], f.up), q);
+#pragma unroll
+                for (int p = 0; p < HP; p++) out[p] |= (unsigned) (q[p] & 255) << 8 * k;
+            }
+            const int nbi = a.inner >> 5, ng = (nbi + (1 << SH) - 1) >> SH, block = c >> 5, pair = found.pairs[t0 + i];
+            if (block >= ng << SH) continue; // (what fills the last exponent's values up: zeros)
+            uint8_t * to = a.hq + (size_t) pair * HP * padded(nbi) * 32 + piece_of<SH>(block, c >> 4 & 1) * 64 + group_in<SH>(block) * 16 + (c & 15);
+#pragma unroll
+            for (int p = 0; p < HP; p++) *reinterpret_cast<unsigned *>(to + (size_t) p * padded(nbi) * 32) = out[p];
+            if ((c & ((32 << SH) - 1)) == 0) {
+                a.hd[(size_t) pair * ng + (block >> SH)] = f.dx;
+                if (MINS) a.hs[(size_t) pair * ng + (block >> SH)] = s;
             }
         }
     }
 }
 
-// the down projection of every pair: waves (32 columns, a part of inner), 1 << ks_log parts
-struct DownArgs {
-    MoeArgs a;
-    int ks_log;
-};
-template <int P, int GSH, bool MINS> __global__ __launch_bounds__(WAVES * 64, 2) void k_moe_down(DownArgs d) {
-    const MoeArgs & a = d.a;
+// the down projection of every pair: waves (32 columns, a KS-th of inner)
+template <int P, int GSH, int SG, int TM, bool MINS> __global__ __launch_bounds__(WAVES * 64, 4) void k_moe_down(MoeArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t all[];
     Found & found = *reinterpret_cast<Found *>(all);
     uint8_t * lds = all + FOUND;
     const int nb = a.inner >> 5, nbp = padded(nb), runs = nbp >> 3, tp = a.tp_down;
-    const Lds L = lds_of(P, nbp, tp, MINS);
-    float * red = reinterpret_cast<float *>(lds + ((L.end + 15) & ~15)); // [waves][2][tp][16]
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15;
-    const int KS = 1 << d.ks_log, ks = wave & (KS - 1), cg = wave >> d.ks_log, CG = WAVES >> d.ks_log;
+    const Lds L = lds_of(P, SG, nbp, tp, MINS);
+    float * red = reinterpret_cast<float *>(lds + ((L.end + 15) & ~15)); // [KS][CG][2][tp][16]
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int KS = 1 << a.ks_down, CG = WAVES >> a.ks_down, cg = wave & (CG - 1), ks = wave / CG;
     const int e = find(a.ids, a.rows * a.top_k, a.n_experts, blockIdx.y, found);
     if (e < 0) return;
-    const int cnt = found.count, gs = (nb + (1 << GSH) - 1) >> GSH, c0 = blockIdx.x * CG * 32;
-    Rows w;
-#pragma unroll
-    for (int t = 0; t < 2; t++) {
-        const size_t r = (size_t) e * a.dim + min(c0 + cg * 32 + t * 16 + n, a.dim - 1); // (columns past the last one: not stored)
-        w.c[t] = a.down.codes + r * (a.inner >> 1);
-        w.s[t] = a.down.scales + r * gs;
-        w.m[t] = MINS ? a.down.mins + r * gs : nullptr;
-    }
+    const int cnt = found.count, gs = (nb + (1 << GSH) - 1) >> GSH, c0 = blockIdx.x * CG * 32, r0 = (runs * ks) >> a.ks_down, r1 = (runs * (ks + 1)) >> a.ks_down;
+    Rows<2> w; // (columns past the last one: not stored)
+    w.set(0, a.down, e, a.dim, c0 + cg * 32, nb, gs);
+    w.set(1, a.down, e, a.dim, c0 + cg * 32 + 16, nb, gs);
     zero_pieces(lds, L);
     for (int t0 = 0; t0 < cnt; t0 += tp) {
         const int nt = min(tp, cnt - t0);
+        const Run<2, MINS> first = load_run<GSH, SG, 2, MINS>(w, nb, min(r0, runs - 1));
         if (t0) __syncthreads();
-        stage_h<P, MINS>(a, lds, L, tp, nt, found.pairs + t0);
+        stage_h<P, SG, MINS>(a, lds, L, tp, nt, found.pairs + t0);
         __syncthreads();
-        float acc[2][T_MAX];
-#pragma unroll
-        for (int i = 0; i < T_MAX; i++) acc[0][i] = acc[1][i] = 0.f;
-        products<P, GSH, MINS>(w, nb, (runs * ks) >> d.ks_log, (runs * (ks + 1)) >> d.ks_log, lds, L, tp, nt, acc);
-#pragma unroll
-        for (int i = 0; i < T_MAX; i++) {
-            if (i >= nt) continue;
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const float v = quad_sum(acc[t][i]);
-                if (lane < 16) red[((wave * 2 + t) * tp + i) * 16 + n] = v;
-            }
-        }
+        float acc[2][TM >> SG];
+        products<P, GSH, SG, 2, TM, MINS>(w, first, nb, r0, r1, lds, L, tp, nt, acc);
+        sums_out<P, SG, 2, TM>(acc, tp, nt, red + (ks * CG + cg) * 2 * tp * 16);
         __syncthreads();
-        for (int j = threadIdx.x; j < nt * CG * 32; j += WAVES * 64) {
-            const int i = j / (CG * 32), col = j - i * (CG * 32), c = c0 + col;
+        for (int j = threadIdx.x; j < nt * CG * 8; j += WAVES * 64) {
+            const int i = j / (CG * 8), col = (j - i * (CG * 8)) * 4, c = c0 + col;
             if (c >= a.dim) continue;
-            float v = 0.f;
-            for (int k = 0; k < KS; k++) v += red[((((col >> 5) * KS + k) * 2 + (col >> 4 & 1)) * tp + i) * 16 + (col & 15)];
-            a.out[(size_t) found.pairs[t0 + i] * a.dim + c] = v;
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < KS; k++) v += *reinterpret_cast<const f32x4 *>(red + (((k * CG + (col >> 5)) * 2 + (col >> 4 & 1)) * tp + i) * 16 + (col & 15));
+            *reinterpret_cast<f32x4 *>(a.out + (size_t) found.pairs[t0 + i] * a.dim + c) = v;
         }
     }
 }
@@ -440,38 +508,55 @@ template <int YT> __global__ __launch_bounds__(256) void k_moe_sum(MoeArgs a) {
     for (int i = 0; i < 4; i++) y[i] = Elem<YT>::down(v[i]);
 }
 
-template <int XF, int GSH, bool MINS> hipError_t run(const MoeArgs & a, hipStream_t st) {
-    constexpr int P = planes_of(XF), HP = inner_planes(XF);
-    static std::atomic<uint64_t> done_up, done_down;
+// (the gate's and) a projection's LDS
+template <class A> size_t lds_bytes(const A & a, int P, int sg, int blocks, int tp) {
+    return FOUND + ((lds_of(P, sg, padded(blocks), tp, a.up.mins).end + 15) & ~15) + (size_t) WAVES * 2 * tp * 16 * 4;
+}
+template <int XF, int GSH, int SH, int TM, bool MINS> hipError_t up(const MoeArgs & a, int slots, hipStream_t st) {
+    constexpr int P = planes_of(XF), SG = P == 1 ? 0 : GSH;
+    static std::atomic<uint64_t> done;
+    const size_t lds = lds_bytes(a, P, SG, a.dim / 32, a.tp_up);
+    const hipError_t e = allow_lds(k_moe_up<XF, GSH, SH, TM, MINS>, lds, done);
+    const int cols = 16 * (WAVES >> a.ks_up);
+    return e != hipSuccess ? e : launch(k_moe_up<XF, GSH, SH, TM, MINS>, dim3((a.inner + cols - 1) / cols, slots), dim3(WAVES * 64), lds, st, a);
+}
+template <int P, int GSH, int SG, int TM, bool MINS> hipError_t down(const MoeArgs & a, int slots, hipStream_t st) {
+    static std::atomic<uint64_t> done;
+    const size_t lds = lds_bytes(a, P, SG, a.inner / 32, a.tp_down);
+    const hipError_t e = allow_lds(k_moe_down<P, GSH, SG, TM, MINS>, lds, done);
+    const int cols = 32 * (WAVES >> a.ks_down);
+    return e != hipSuccess ? e : launch(k_moe_down<P, GSH, SG, TM, MINS>, dim3((a.dim + cols - 1) / cols, slots), dim3(WAVES * 64), lds, st, a);
+}
+template <int XF, int GSH, int SH, bool MINS> hipError_t run(const MoeArgs & a, hipStream_t st) {
+    constexpr int HP = inner_planes(XF), YT = XF == W4_UNITS ? DT_F32 : XF;
     const int slots = std::min(a.n_experts, a.rows * a.top_k);
-    size_t lds = FOUND + ((lds_of(P, padded(a.dim / 32), a.tp_up, MINS).end + 15) & ~15) + (size_t) WAVES * 2 * a.tp_up * 16 * 4;
-    hipError_t e = allow_lds(k_moe_up<XF, GSH, MINS>, lds, done_up);
+    hipError_t e = a.tp_up <= 8 ? up<XF, GSH, SH, 8, MINS>(a, slots, st) : up<XF, GSH, SH, 16, MINS>(a, slots, st);
     if (e != hipSuccess) return e;
-    e = launch(k_moe_up<XF, GSH, MINS>, dim3(a.inner / 32, slots), dim3(WAVES * 64), lds, st, a);
+    e = a.tp_down <= 8 ? down<HP, GSH, SH, 8, MINS>(a, slots, st) : down<HP, GSH, SH, 16, MINS>(a, slots, st);
     if (e != hipSuccess) return e;
-    const int runs = padded(a.inner / 32) / 8;
-    DownArgs d{a, runs >= 4 ? 2 : runs >= 2 ? 1 : 0};
-    lds = FOUND + ((lds_of(HP, padded(a.inner / 32), a.tp_down, MINS).end + 15) & ~15) + (size_t) WAVES * 2 * a.tp_down * 16 * 4;
-    e = allow_lds(k_moe_down<HP, GSH, MINS>, lds, done_down);
-    if (e != hipSuccess) return e;
-    const int cols = 32 * (WAVES >> d.ks_log);
-    e = launch(k_moe_down<HP, GSH, MINS>, dim3((a.dim + cols - 1) / cols, slots), dim3(WAVES * 64), lds, st, d);
-    if (e != hipSuccess) return e;
-    constexpr int YT = XF == W4_UNITS ? DT_F32 : XF;
     return launch(k_moe_sum<YT>, dim3((a.dim + 1023) / 1024, a.rows), dim3(256), 0, st, a);
+}
+template <int XF, int GSH, bool MINS> hipError_t run(const MoeArgs & a, hipStream_t st) {
+    if constexpr (GSH == 0) return run<XF, 0, 0, MINS>(a, st);
+    else return a.ks_up == 0 ? run<XF, GSH, GSH, MINS>(a, st) : run<XF, GSH, 0, MINS>(a, st);
 }
 template <int XF, bool MINS> hipError_t run(const MoeArgs & a, hipStream_t st) {
     return a.gsh == 0 ? run<XF, 0, MINS>(a, st) : a.gsh == 1 ? run<XF, 1, MINS>(a, st) : run<XF, 2, MINS>(a, st);
 }
 template <int XF> hipError_t run(const MoeArgs & a, hipStream_t st) { return a.up.mins ? run<XF, true>(a, st) : run<XF, false>(a, st); }
 
-// tokens of a pass: twice what an expert has on average, in at most `most` bytes of LDS, at least one instruction's
-int pass_tokens(const MoeArgs & a, int P, int blocks, int most) {
-    const int tg = group_of(P), avg = (a.rows * a.top_k + a.n_experts - 1) / a.n_experts;
-    int tp = (std::min(a.rows, std::max(2 * avg, 4)) + tg - 1) / tg * tg;
-    tp = std::min(tp, T_MAX);
-    while (tp > tg && lds_of(P, padded(blocks), tp, a.up.mins).end + WAVES * 2 * tp * 64 + FOUND > most) tp -= tg;
+// tokens of a pass: twice what an expert has on average (at most 16), in half of a CU's LDS where that holds an instruction's
+int pass_tokens(const MoeArgs & a, int P, int sg, int blocks) {
+    const int tg = group_of(P, sg), avg = (a.rows * a.top_k + a.n_experts - 1) / a.n_experts;
+    int tp = std::min((std::min(a.rows, std::max(2 * avg, 4)) + tg - 1) / tg * tg, 16);
+    while (tp > tg && lds_bytes(a, P, sg, blocks, tp) > 80 * 1024) tp -= tg;
     return tp;
+}
+// waves that split k: as few as leave `most` workgroups of `cols` columns each (times the waves that share them)
+int split(int experts, int n, int cols, int runs, int limit) {
+    int log = 0;
+    while (log < limit && experts * ((n + (cols * WAVES >> log) - 1) / (cols * WAVES >> log)) < 512 && runs >= 2 << log) log++;
+    return log;
 }
 
 } // namespace
@@ -489,12 +574,17 @@ long long moe_plan(MoeArgs & a, int xform, uint8_t * ws) {
     a.hd = reinterpret_cast<float *>(take(pairs * nbi * 4));
     a.hs = reinterpret_cast<float *>(take(a.up.mins ? pairs * nbi * 4 : 0));
     a.out = reinterpret_cast<float *>(take(pairs * a.dim * 4));
-    constexpr int HALF = 72 * 1024; // two workgroups per CU
-    MoeArgs b = a;
-    b.rows = std::min(a.rows, MOE_ROWS);
-    a.tp_up = pass_tokens(b, planes_of(xform), a.dim / 32, HALF);
-    a.tp_down = pass_tokens(b, HP, nbi, HALF);
     return at;
+}
+
+// (of one run of at most MOE_ROWS rows)
+static void split_work(MoeArgs & a, int xform) {
+    const int HP = inner_planes(xform), P = planes_of(xform), nbi = a.inner / 32;
+    const int experts = std::min(a.n_experts, a.rows * a.top_k);
+    a.ks_up = split(experts, a.inner, 16, padded(a.dim / 32) / 8, 2);
+    a.ks_down = split(experts, a.dim, 32, padded(nbi) / 8, 3);
+    a.tp_up = pass_tokens(a, P, P == 1 ? 0 : a.gsh, a.dim / 32);
+    a.tp_down = pass_tokens(a, HP, a.ks_up == 0 ? a.gsh : 0, nbi);
 }
 
 hipError_t launch_moe(const MoeArgs & all, int xform, hipStream_t st) {
@@ -510,6 +600,7 @@ hipError_t launch_moe(const MoeArgs & all, int xform, hipStream_t st) {
             a.xb += (size_t) row * nb * 16;
             a.xmeta += (size_t) row * nb * 4;
         } else a.x = static_cast<const char *>(a.x) + row * a.x_stride * xs;
+        split_work(a, xform);
         const hipError_t e = xform == W4_UNITS ? run<W4_UNITS>(a, st) : xform == DT_F32 ? run<DT_F32>(a, st) : xform == DT_F16 ? run<DT_F16>(a, st) : run<DT_BF16>(a, st);
         if (e != hipSuccess) return e;
     }
