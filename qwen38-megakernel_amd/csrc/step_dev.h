@@ -18,6 +18,8 @@ typedef _Float16 f16x8_u __attribute__((ext_vector_type(8), aligned(2)));
 typedef __bf16 bf16x8_u __attribute__((ext_vector_type(8), aligned(2)));
 
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4_u2 __attribute__((ext_vector_type(4), aligned(2)));
 
 // the largest of 8 16-bit floats by their bits without the sign
 __device__ __forceinline__ uint16_t top16(u16x8 v) {
@@ -163,6 +165,25 @@ __device__ __forceinline__ void w4_bytes(unsigned w, int & lo, int & hi) {
     w ^= 0x88888888u;
     lo = (int) ((w << 4) & 0xf0f0f0f0u);
     hi = (int) (w & 0xf0f0f0f0u);
+}
+
+// scales grp .. grp + 7 of a weight row of gs (p: its first), zeros past the row's end: the last eight of the row, moved down
+__device__ __forceinline__ u32x4 w4_scales(const uint16_t * p, int gs, int grp) {
+    if (__builtin_expect(gs < 8, 0)) {
+        unsigned v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = grp + k < gs ? p[grp + k] : 0;
+        return u32x4{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+    }
+    const int at = min(grp, gs - 8), off = grp - at;
+    u32x4 e = *reinterpret_cast<const u32x4_u2 *>(p + at);
+    if (__builtin_expect(off != 0, 0)) {
+        if (off & 4) e = u32x4{e[2], e[3], 0, 0};
+        if (off & 2) e = u32x4{e[1], e[2], e[3], 0};
+        if (off & 1) e = u32x4{e[0] >> 16 | e[1] << 16, e[1] >> 16 | e[2] << 16, e[2] >> 16 | e[3] << 16, e[3] >> 16};
+        if (off >= 8) e = u32x4{0, 0, 0, 0};
+    }
+    return e;
 }
 
 __device__ __forceinline__ double shfl_xor_d(double v, int m) {

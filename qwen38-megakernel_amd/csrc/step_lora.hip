@@ -16,7 +16,6 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // operands of a step: 8 values of a lane as `parts` 16-bit vectors
 constexpr bool f16_mfma(int xf, int wf) { return wf == DT_F16 && (xf == DT_F16 || xf == W4_UNITS); }

@@ -216,7 +216,7 @@ int moe(MoeArgs a, int xform, void * ws, long long ws_bytes, void * stream) {
     const Device d(stream);
     hold_moe(d, a);
     d.holds(ws, "ws");
-    ck(launch_moe(a, xform, static_cast<hipStream_t>(stream)), "moe");
+    ck(launch_moe(a, xform, nullptr, static_cast<hipStream_t>(stream)), "moe");
     return 0;
 }
 
@@ -287,7 +287,8 @@ int mk_moe_route(int rows, int dim, int n_experts, int top_k, const void * x, lo
         const Device d(stream);
         hold_route(d, a);
         if (want) d.holds(ws, "ws");
-        ck(launch_route(a, dtype, w_dtype, static_cast<hipStream_t>(stream)), "route");
+        ck(launch_logits(a, dtype, w_dtype, static_cast<hipStream_t>(stream)), "route");
+        ck(launch_pick(a, static_cast<hipStream_t>(stream)), "route");
         return 0;
     });
 }
@@ -358,8 +359,8 @@ int mk_moe_layer(int rows, int dim, int inner, int n_experts, int top_k, int gro
         hold_route(d, r);
         hold_moe(d, a);
         d.holds(ws, "ws");
-        ck(launch_route(r, dtype, router_dtype, static_cast<hipStream_t>(stream)), "route");
-        ck(launch_moe(a, dtype, static_cast<hipStream_t>(stream)), "moe");
+        ck(launch_logits(r, dtype, router_dtype, static_cast<hipStream_t>(stream)), "route");
+        ck(launch_moe(a, dtype, &r, static_cast<hipStream_t>(stream)), "moe");
         return 0;
     });
 }

@@ -42,9 +42,10 @@ struct RouteArgs {
     float scale;
     int chunks;         // (set by route_plan) parts of dim with partial sums of their own
 };
-constexpr int ROUTE_MAX_EXPERTS = 1024, ROUTE_MAX_TOP = 16, ROUTE_MAX_ROWS = 1 << 19, ROUTE_MAX_DIM = 1 << 17;
+constexpr int ROUTE_MAX_EXPERTS = 1024, ROUTE_MAX_TOP = 16, ROUTE_MAX_ROWS = 1 << 19, ROUTE_MAX_DIM = 1 << 17, ROUTE_MAX_CHUNKS = 8;
 void route_plan(RouteArgs & a);
-hipError_t launch_route(const RouteArgs & a, int dtype, int wtype, hipStream_t st);
+hipError_t launch_logits(const RouteArgs & a, int dtype, int wtype, hipStream_t st);
+hipError_t launch_pick(const RouteArgs & a, hipStream_t st);
 
 // 4-bit weights of every expert: codes [n_experts][n][k / 2], scales and minimums [n_experts][n][gs]
 struct MoeWeights {
@@ -64,18 +65,19 @@ struct MoeArgs {
     void * y;        // [rows][y_stride] of x's type (units: fp32)
     long long x_stride, y_stride;
     int rows, dim, inner, n_experts, top_k, gsh; // a scale serves 32 << gsh values
-    // workspace (set by moe_plan): of every pair (row, place among its experts) the inner values as int8 planes, per block of 32 a
-    // factor and (with minimums) a sum, and the expert's output
-    uint8_t * hq;    // [pairs][planes][inner padded to 256]
-    float * hd;      // [pairs][inner / 32]
-    float * hs;      // [pairs][inner / 32]
-    float * out;     // [pairs][dim]
+    // workspace (set by moe_plan).  x and h as int8 planes: of every row (h: of every pair of a row and a place among its experts) the
+    // planes' rows, as LDS holds them, a factor for every exponent, and a sum
+    uint8_t * lists; // the experts that occur and their pairs (step_moe.hip)
+    uint8_t * xq, * hq;
+    float * xd, * hd, * xs, * hs;
+    float * out;     // [pairs][dim]: the experts' outputs (where xq, xd and xs were)
     // (set by the launcher) tokens of an expert that a pass holds in LDS, and waves (1 << ..) that split k
     int tp_up, tp_down, ks_up, ks_down;
 };
 constexpr int MOE_ROWS = 64;   // rows of a launch; a call of more runs them one after another
 constexpr int MOE_MAX_ROWS = 4096, MOE_MAX_DIM = 16384, MOE_MAX_INNER = 32768;
 long long moe_plan(MoeArgs & a, int xform, uint8_t * ws); // -> bytes of workspace
-hipError_t launch_moe(const MoeArgs & a, int xform, hipStream_t st);
+// route: the router whose logits' partial sums are there, and whose choice is ids and weights (null: these are given)
+hipError_t launch_moe(const MoeArgs & a, int xform, const RouteArgs * route, hipStream_t st);
 
 } // namespace qkv

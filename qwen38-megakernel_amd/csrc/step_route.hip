@@ -1,8 +1,7 @@
 // The router of a mixture of experts: logits = x W^T, the top_k experts of every row and their weights.  The choice compares values that
 // can lie closer than fp32 sums are exact, so the logits are summed in 64 bits and rounded once; equal ones go to the lowest
 // index.
-#include "step_dev.h"
-#include "step_mix_launch.h"
+#include "step_route_dev.h"
 
 #include <algorithm>
 
@@ -51,89 +50,11 @@ template <int DT, int WT> __global__ __launch_bounds__(RW * 64) void k_route_log
     else a.logits[at] = (float) v;
 }
 
-// a double's order as an unsigned one; NaN below everything
-__device__ __forceinline__ uint64_t order(double v) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v == 0 ? 0.0 : v);
-    return v != v ? 0 : b >> 63 ? ~b : b | 0x8000000000000000ull;
-}
-__device__ __forceinline__ uint64_t shfl_xor_64(uint64_t v, int m) {
-    return (uint64_t) shfl_xor_u((unsigned) (v >> 32), m) << 32 | shfl_xor_u((unsigned) v, m);
-}
-
 constexpr int PW = 4; // rows (waves) of a workgroup of k_route_pick
 
-// A wave per row, lane l holds experts l, l + 64, ...: V a lane.
 template <int V> __global__ __launch_bounds__(PW * 64) void k_route_pick(RouteArgs a) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int row = blockIdx.x * PW + wave;
-    if (row >= a.rows) return;
-    float l[V];
-    double score[V];
-    uint64_t key[V];
-    float top = -__builtin_inff();
-#pragma unroll
-    for (int i = 0; i < V; i++) {
-        const int e = lane + 64 * i;
-        const size_t at = (size_t) row * a.n_experts + e;
-        l[i] = -__builtin_inff();
-        score[i] = 0;
-        key[i] = 0;
-        if (e >= a.n_experts) continue;
-        if (a.chunks > 1) {
-            double v = 0;
-            for (int c = 0; c < a.chunks; c++) v += a.part[(size_t) c * a.rows * a.n_experts + at];
-            a.logits[at] = l[i] = (float) v;
-        } else l[i] = a.logits[at];
-        score[i] = l[i];
-        if (a.form >= ROUTE_SIGMOID) score[i] = 1.0 / (1.0 + exp(-(double) l[i]));
-        key[i] = order(a.bias ? score[i] + (double) a.bias[e] : (double) l[i]);
-        top = fmaxf(top, l[i]);
-    }
-    // the largest key, the lowest index of equal ones, top_k times; lane j keeps the j-th
-    unsigned taken = 0;
-    int mine_id = 0;
-    double mine = 0;
-    for (int j = 0; j < a.top_k; j++) {
-        uint64_t best = 0;
-        int at = 0x7fffffff;
-        double s = 0;
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            const int e = lane + 64 * i;
-            if (e < a.n_experts && !(taken >> i & 1) && (at == 0x7fffffff || key[i] > best)) best = key[i], at = e, s = score[i];
-        }
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const uint64_t k = shfl_xor_64(best, m);
-            const int e = (int) shfl_xor_u((unsigned) at, m);
-            const double t = shfl_xor_d(s, m);
-            if (k > best || (k == best && e < at)) best = k, at = e, s = t;
-        }
-        if ((at & 63) == lane) taken |= 1u << (at >> 6);
-        if (lane == j) mine_id = at, mine = s;
-    }
-    const bool in = lane < a.top_k;
-    double w = mine;
-    if (a.form == ROUTE_SOFTMAX) {
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, shfl_xor(top, m));
-        double sum = 0;
-#pragma unroll
-        for (int i = 0; i < V; i++)
-            if (lane + 64 * i < a.n_experts) sum += exp((double) l[i] - (double) top);
-        w = exp(mine - (double) top) / wave_sum(sum);
-    } else if (a.form == ROUTE_CHOSEN) {
-        // (the first one is the largest)
-        const uint64_t b = __builtin_bit_cast(uint64_t, mine);
-        const double first = __builtin_bit_cast(double, (uint64_t) (unsigned) __builtin_amdgcn_readfirstlane((unsigned) (b >> 32)) << 32 |
-                                                            (unsigned) __builtin_amdgcn_readfirstlane((unsigned) b));
-        const double e = in ? exp(mine - first) : 0.0;
-        w = e / wave_sum(e);
-    } else if (a.form == ROUTE_SIGMOID_NORM) w = mine / wave_sum(in ? mine : 0.0);
-    if (in) {
-        a.ids[(size_t) row * a.top_k + lane] = mine_id;
-        a.weights[(size_t) row * a.top_k + lane] = (float) (w * (double) a.scale);
-    }
+    const int row = blockIdx.x * PW + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (row < a.rows) route_pick<V>(a, row);
 }
 
 template <int DT, int WT> hipError_t logits(const RouteArgs & a, hipStream_t st) {
@@ -145,11 +66,16 @@ template <int DT> hipError_t logits(const RouteArgs & a, int wtype, hipStream_t 
 
 } // namespace
 
-void route_plan(RouteArgs & a) { a.chunks = 1; }
+void route_plan(RouteArgs & a) {
+    // few tiles: dim in chunks of at least a step a wave, up to two workgroups a CU (and 16 KiB of partial sums an expert)
+    const int tiles = ((a.n_experts + 15) / 16) * ((a.rows + 15) / 16), steps = (a.dim + 31) / 32;
+    a.chunks = std::max(1, std::min({ROUTE_MAX_CHUNKS, 512 / std::max(tiles, 1), steps / RW, 2048 / std::max(a.rows, 1)}));
+}
 
-hipError_t launch_route(const RouteArgs & a, int dtype, int wtype, hipStream_t st) {
-    const hipError_t e = dtype == DT_F32 ? logits<DT_F32>(a, wtype, st) : dtype == DT_F16 ? logits<DT_F16>(a, wtype, st) : logits<DT_BF16>(a, wtype, st);
-    if (e != hipSuccess) return e;
+hipError_t launch_logits(const RouteArgs & a, int dtype, int wtype, hipStream_t st) {
+    return dtype == DT_F32 ? logits<DT_F32>(a, wtype, st) : dtype == DT_F16 ? logits<DT_F16>(a, wtype, st) : logits<DT_BF16>(a, wtype, st);
+}
+hipError_t launch_pick(const RouteArgs & a, hipStream_t st) {
     const dim3 grid((a.rows + PW - 1) / PW), block(PW * 64);
     const int v = (a.n_experts + 63) / 64;
     return v <= 1 ? launch(k_route_pick<1>, grid, block, 0, st, a) : v <= 2 ? launch(k_route_pick<2>, grid, block, 0, st, a)

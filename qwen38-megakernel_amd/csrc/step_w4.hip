@@ -18,9 +18,7 @@ namespace qkv {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4_u8 __attribute__((ext_vector_type(4), aligned(8)));
-typedef unsigned u32x4_u2 __attribute__((ext_vector_type(4), aligned(2)));
 
 enum { XM_UNITS = 0, XM_HALF = 1, XM_SPLIT = 2 }; // x as int8 units, as one fp16 part, as two
 
@@ -167,25 +165,6 @@ __device__ __forceinline__ half8 w4_halves(unsigned w) {
     const half2v p0 = as_h2((w & 0x000f000fu) | 0x64006400u) + b0, p1 = as_h2((v & 0x000f000fu) | 0x64006400u) + b0,
                  p2 = as_h2((w & 0x00f000f0u) | 0x54005400u) + b1, p3 = as_h2((v & 0x00f000f0u) | 0x54005400u) + b1;
     return half8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
-}
-
-// scales grp .. grp + 7 of a weight row of gs (p: its first), zeros past the row's end: the last eight of the row, moved down
-__device__ __forceinline__ u32x4 w4_scales(const uint16_t * p, int gs, int grp) {
-    if (__builtin_expect(gs < 8, 0)) {
-        unsigned v[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = grp + k < gs ? p[grp + k] : 0;
-        return u32x4{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
-    }
-    const int at = min(grp, gs - 8), off = grp - at;
-    u32x4 e = *reinterpret_cast<const u32x4_u2 *>(p + at);
-    if (__builtin_expect(off != 0, 0)) {
-        if (off & 4) e = u32x4{e[2], e[3], 0, 0};
-        if (off & 2) e = u32x4{e[1], e[2], e[3], 0};
-        if (off & 1) e = u32x4{e[0] >> 16 | e[1] << 16, e[1] >> 16 | e[2] << 16, e[2] >> 16 | e[3] << 16, e[3] >> 16};
-        if (off >= 8) e = u32x4{0, 0, 0, 0};
-    }
-    return e;
 }
 
 // Plain rows with minimums, results that are an infinity or a NaN: the folds add s (c - 8) x and m x apart, which of an infinite x
