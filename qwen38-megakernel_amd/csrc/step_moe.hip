@@ -358,23 +358,26 @@ template <int XF, int V> __global__ __launch_bounds__(PREP) void k_moe_prep(Prep
 __device__ __forceinline__ unsigned lds_address(const uint8_t * lds) {
     return (unsigned) __builtin_amdgcn_readfirstlane((unsigned) (size_t) (const __attribute__((address_space(3))) uint8_t *) lds);
 }
-// the planes, factors and sums of nt tokens, at the places that `at` gives, into LDS
+// the planes, factors and sums of nt tokens, lane t's `at` the place of the t-th, into LDS
 template <int P, bool MINS>
-__device__ __forceinline__ void stage(const uint8_t * q, const float * d, const float * s, int nd, int ng, uint8_t * lds, const Lds & L, int tp, int nt, const uint16_t * at) {
+__device__ __forceinline__ void stage(const uint8_t * q, const float * d, const float * s, int nd, int ng, uint8_t * lds, const Lds & L, int tp, int nt, int at) {
     const unsigned base = lds_address(lds);
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, bytes = P * L.row, per = (bytes + 1023) >> 10;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, bytes = L.row - 16, per = (bytes + 1023) >> 10;
     float * dx = reinterpret_cast<float *>(lds + L.dx), * ds = reinterpret_cast<float *>(lds + L.ds);
-    for (int t = 0, c = wave; t < nt; t++, c -= per) { // 1 KiB a copy, the waves in turn
-        const uint8_t * from = q + (size_t) (unsigned) __builtin_amdgcn_readfirstlane(at[t]) * bytes;
-        for (; c < per; c += WAVES)
-            if (c * 1024 + lane * 16 < bytes) dma16(from + (c * 1024 + lane * 16), base + t * bytes + c * 1024);
+    int c = wave;
+    for (int t = 0; t < nt; t++) { // 1 KiB a copy, the waves in turn
+        const uint8_t * from = q + (size_t) (unsigned) __builtin_amdgcn_readlane(at, t) * (P * L.row);
+#pragma unroll
+        for (int p = 0; p < P; p++, c -= per)
+            for (; c < per; c += WAVES)
+                if (c * 1024 + lane * 16 < bytes) dma16(from + (p * L.row + c * 1024 + lane * 16), base + (t * P + p) * L.row + c * 1024);
     }
     for (int k = tid; k < nd; k += WAVES * 64)
         for (int t0 = 0; t0 < nt; t0 += 4) { // (four loads, then their values)
             float v[4], w[4];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                const size_t i = (size_t) (unsigned) __builtin_amdgcn_readfirstlane(at[min(t0 + u, nt - 1)]) * nd + k;
+                const size_t i = (size_t) (unsigned) __builtin_amdgcn_readlane(at, min(t0 + u, nt - 1)) * nd + k;
                 v[u] = d[i];
                 if (MINS) w[u] = s[i];
             }
@@ -412,9 +415,10 @@ template <int XF, int GSH, int SH, int TM, bool MINS> __global__ __launch_bounds
     zero_pieces(lds, L);
     for (int t0 = 0; t0 < cnt; t0 += tp) {
         const int nt = min(tp, cnt - t0);
+        const int at = l->row[p0 + t0 + min((int) (threadIdx.x & 63), nt - 1)];
         const Run<2, MINS> first = load_run<GSH, SG, 2, MINS>(w, nb, min(r0, runs - 1)); // (on its way while x is made ready)
         if (t0) __syncthreads();
-        stage<P, MINS>(a.xq, a.xd, a.xs, nbp >> SG, (nb + (1 << SG) - 1) >> SG, lds, L, tp, nt, l->row + p0 + t0);
+        stage<P, MINS>(a.xq, a.xd, a.xs, nbp >> SG, (nb + (1 << SG) - 1) >> SG, lds, L, tp, nt, at);
         __syncthreads();
         float acc[2][TM >> SG];
         products<P, GSH, SG, 2, TM, MINS>(w, first, nb, r0, r1, lds, L, win, tp, nt, acc);
@@ -484,9 +488,10 @@ template <int P, int GSH, int SG, int TM, bool MINS> __global__ __launch_bounds_
     zero_pieces(lds, L);
     for (int t0 = 0; t0 < cnt; t0 += tp) {
         const int nt = min(tp, cnt - t0);
+        const int at = l->pair[p0 + t0 + min((int) (threadIdx.x & 63), nt - 1)];
         const Run<2, MINS> first = load_run<GSH, SG, 2, MINS>(w, nb, min(r0, runs - 1));
         if (t0) __syncthreads();
-        stage<P, MINS>(a.hq, a.hd, a.hs, nbp >> SG, (nb + (1 << SG) - 1) >> SG, lds, L, tp, nt, l->pair + p0 + t0);
+        stage<P, MINS>(a.hq, a.hd, a.hs, nbp >> SG, (nb + (1 << SG) - 1) >> SG, lds, L, tp, nt, at);
         __syncthreads();
         float acc[2][TM >> SG];
         products<P, GSH, SG, 2, TM, MINS>(w, first, nb, r0, r1, lds, L, win, tp, nt, acc);
