@@ -24,7 +24,7 @@ namespace {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int MAX_PAIRS = MOE_ROWS * ROUTE_MAX_TOP;
-constexpr int WAVES = 8;
+constexpr int WAVES_LOG = 2, WAVES = 1 << WAVES_LOG;
 
 constexpr int planes_of(int xform) { return xform == W4_UNITS ? 1 : xform == DT_F32 ? 3 : 2; }
 constexpr int inner_planes(int xform) { return xform == DT_F16 || xform == DT_BF16 ? 2 : 3; } // (y is fp32 else)
@@ -105,8 +105,9 @@ template <int NT> struct Rows {
 // fetch each cache line many times) and go through LDS of the wave's own.
 constexpr int WIN = 32, WROW = WIN + 8; // scales of a window, a row's place: 16 rows' 80 bytes begin in different banks
 constexpr int win_bytes(int nt, bool mins) { return nt * (mins ? 2 : 1) * 16 * WROW * 2; }
+// Two runs are on their way: one alone leaves a wave waiting for memory.
 template <int NT, bool MINS> struct Run {
-    u32x4 c[NT][2];
+    u32x4 c[2][NT][2];
     u32x4 s[NT], m[NT];
 };
 template <int GSH, int NT, bool MINS> __device__ __forceinline__ void load_window(const Rows<NT> & w, int nb, int R, Run<NT, MINS> & r) {
@@ -117,14 +118,22 @@ template <int GSH, int NT, bool MINS> __device__ __forceinline__ void load_windo
         if constexpr (MINS) r.m[t] = w4_scales(w.m[t] + w.vs[t], gs, at);
     }
 }
-template <int GSH, int SG, int NT, bool MINS> __device__ __forceinline__ Run<NT, MINS> load_run(const Rows<NT> & w, int nb, int R) {
-    const int g = threadIdx.x >> 4 & 3;
+template <int SG, int NT> __device__ __forceinline__ void load_codes(const Rows<NT> & w, int nb, int R, int t, int u, u32x4 & c) {
+    const int g = threadIdx.x >> 4 & 3; // (past the last block zeros of x, or of its factors)
+    c = *reinterpret_cast<const u32x4 *>(w.c[t] + (w.vc[t] + (unsigned) min(8 * R + block_of<SG>(g, u), nb - 1) * 16));
+}
+// the first two of runs R .. last
+template <int GSH, int SG, int NT, bool MINS> __device__ __forceinline__ Run<NT, MINS> load_runs(const Rows<NT> & w, int nb, int R, int last) {
     Run<NT, MINS> r;
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int u = 0; u < 2; u++) r.c[t][u] = *reinterpret_cast<const u32x4 *>(w.c[t] + (w.vc[t] + (unsigned) min(8 * R + block_of<SG>(g, u), nb - 1) * 16)); // (past the last block zeros of x, or of its factors)
+        for (int u = 0; u < 2; u++) load_codes<SG>(w, nb, R, t, u, r.c[0][t][u]);
     load_window<GSH>(w, nb, R, r);
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) load_codes<SG>(w, nb, min(R + 1, last), t, u, r.c[1][t][u]);
     return r;
 }
 
@@ -141,19 +150,9 @@ __device__ __forceinline__ void products(const Rows<NT> & w, Run<NT, MINS> in, i
     for (int t = 0; t < NT; t++)
 #pragma unroll
         for (int i = 0; i < TM >> SG; i++) acc[t][i] = 0.f;
-#pragma unroll 1
-    for (int R = r0; R < r1; R++) {
-        const int next = min(R + 1, r1 - 1); // (behind the last run that one again, unused)
+    const auto run = [&](int R, int buf) {
+        const int next = min(R + 2, r1 - 1); // (behind the last run that one again, unused)
         const int in_win = (R - r0) & ((4 << GSH) - 1);
-        if (in_win == 0) {
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                *reinterpret_cast<u32x4 *>(win + (t * 16 + n) * WROW + 8 * g) = in.s[t];
-                if constexpr (MINS) *reinterpret_cast<u32x4 *>(win + ((NT + t) * 16 + n) * WROW + 8 * g) = in.m[t];
-            }
-            asm volatile("" ::: "memory"); // (read below by other lanes and as another type)
-            if (R + (4 << GSH) < r1) load_window<GSH>(w, nb, R + (4 << GSH), in);
-        }
         float sc[NT][2], mn[NT][2];
         const auto scales = [&](const uint16_t * p, float (&v)[2]) {
             if constexpr (SG == GSH) {
@@ -175,13 +174,13 @@ __device__ __forceinline__ void products(const Rows<NT> & w, Run<NT, MINS> in, i
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     int t0, t1;
-                    w4_bytes(in.c[t][u][k], t0, t1);
+                    w4_bytes(in.c[buf][t][u][k], t0, t1);
                     b[t][k >> 1][2 * (k & 1)] = t0;
                     b[t][k >> 1][2 * (k & 1) + 1] = t1;
                 }
-            __builtin_amdgcn_sched_barrier(0); // the codes leave their registers, then the next run's take them
+            __builtin_amdgcn_sched_barrier(0); // the codes leave their registers, then those of a later run take them
 #pragma unroll
-            for (int t = 0; t < NT; t++) in.c[t][u] = *reinterpret_cast<const u32x4 *>(w.c[t] + (w.vc[t] + (unsigned) min(8 * next + block_of<SG>(g, u), nb - 1) * 16));
+            for (int t = 0; t < NT; t++) load_codes<SG>(w, nb, next, t, u, in.c[buf][t][u]);
             __builtin_amdgcn_sched_barrier(0);
             const uint8_t * ap = lds + (aoff + (R * 256 & amask)) + u * 128;
             const int at = ((8 * R + block_of<SG>(g, u)) >> SG) * tp + first;
@@ -214,6 +213,20 @@ __device__ __forceinline__ void products(const Rows<NT> & w, Run<NT, MINS> in, i
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+    };
+#pragma unroll 1
+    for (int R = r0; R < r1; R += 2) {
+        if (((R - r0) & ((4 << GSH) - 1)) == 0) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                *reinterpret_cast<u32x4 *>(win + (t * 16 + n) * WROW + 8 * g) = in.s[t];
+                if constexpr (MINS) *reinterpret_cast<u32x4 *>(win + ((NT + t) * 16 + n) * WROW + 8 * g) = in.m[t];
+            }
+            asm volatile("" ::: "memory"); // (read below by other lanes and as another type)
+            if (R + (4 << GSH) < r1) load_window<GSH>(w, nb, R + (4 << GSH), in);
+        }
+        run(R, 0);
+        if (R + 1 < r1) run(R + 1, 1);
     }
 }
 // the wave's sums of nt tokens to red[tile][tp][16]: added over the lane groups that have the same token
@@ -235,11 +248,12 @@ template <int P, int SG, int NT, int TM> __device__ __forceinline__ void sums_ou
     }
 }
 
-// The experts that occur, ascending, and the pairs that chose each (in any order: a pair's results do not depend on its place).  Choices
-// that are no expert are left out.
+// The experts that occur, those of more than LONG pairs first (their workgroups last longest), and the pairs that chose each (in any order: a
+// pair's results do not depend on its place).  Choices that are no expert are left out.
+constexpr int LONG = 8;
 struct Lists {
     int count;
-    uint16_t expert[ROUTE_MAX_EXPERTS], start[ROUTE_MAX_EXPERTS + 2], pair[MAX_PAIRS], row[MAX_PAIRS];
+    uint16_t expert[ROUTE_MAX_EXPERTS], start[ROUTE_MAX_EXPERTS], pairs[ROUTE_MAX_EXPERTS], pair[MAX_PAIRS], row[MAX_PAIRS];
 };
 
 struct PrepArgs {
@@ -255,7 +269,8 @@ template <int XF, int V> __global__ __launch_bounds__(PREP) void k_moe_prep(Prep
     constexpr int P = planes_of(XF);
     const int nb = a.dim >> 5, nbp = padded(nb), tid = threadIdx.x;
     if (blockIdx.x == 0) {
-        __shared__ int count[ROUTE_MAX_EXPERTS], sums[PREP / 64];
+        __shared__ int count[ROUTE_MAX_EXPERTS];
+        __shared__ unsigned sums[PREP / 64];
         __shared__ int16_t chosen[MAX_PAIRS];
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, pairs = a.rows * a.top_k;
         count[tid] = 0;
@@ -272,27 +287,29 @@ template <int XF, int V> __global__ __launch_bounds__(PREP) void k_moe_prep(Prep
         __syncthreads();
         if (e >= 0) atomicAdd(&count[e], 1);
         __syncthreads();
-        // pairs and experts in front of expert tid: pairs in the low half, experts in the high one
-        const int c = count[tid], v = c + (c ? 1 << 16 : 0);
-        int sum = v;
+        // in front of expert tid: pairs (11 bits), experts that occur (11), experts of many pairs (10)
+        const unsigned c = (unsigned) count[tid], v = c + (c ? 1u << 11 : 0) + (c > LONG ? 1u << 22 : 0);
+        unsigned sum = v;
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) {
-            const int o = __shfl_up(sum, m);
+            const unsigned o = __shfl_up(sum, m);
             if (lane >= m) sum += o;
         }
         if (lane == 63) sums[wave] = sum;
         __syncthreads();
-        for (int w = 0; w < wave; w++) sum += sums[w];
+        unsigned all = 0;
+        for (int w = 0; w < PREP / 64; w++) {
+            if (w == wave) sum += all;
+            all += sums[w];
+        }
         Lists * l = reinterpret_cast<Lists *>(a.lists);
-        const int at = (sum - v) >> 16, before = (sum - v) & 0xffff;
+        const int longs = (int) ((sum - v) >> 22), at = c > LONG ? longs : (int) (all >> 22) + (int) ((sum - v) >> 11 & 0x7ff) - longs, before = (int) ((sum - v) & 0x7ff);
         if (c) {
             l->expert[at] = (uint16_t) tid;
             l->start[at] = (uint16_t) before;
+            l->pairs[at] = (uint16_t) c;
         }
-        if (tid == PREP - 1) {
-            l->count = sum >> 16;
-            l->start[sum >> 16] = (uint16_t) (sum & 0xffff);
-        }
+        if (tid == 0) l->count = (int) (all >> 11 & 0x7ff);
         __syncthreads();
         count[tid] = before;
         __syncthreads();
@@ -396,12 +413,12 @@ __device__ __forceinline__ void zero_pieces(uint8_t * lds, const Lds & L) {
 
 // The gate and the up projection: a workgroup has 16 CG inner columns of an expert, its waves (16 columns of both, a KS-th of dim), CG KS = 8.
 // SG: lane groups that share a sum of x; SH: those of the down projection, whose x (h) this kernel leaves as planes.
-template <int XF, int GSH, int SH, int TM, bool MINS> __global__ __launch_bounds__(WAVES * 64, 4) void k_moe_up(MoeArgs a) {
+template <int XF, int GSH, int SH, int TM, bool MINS> __global__ __launch_bounds__(WAVES * 64, 3) void k_moe_up(MoeArgs a) {
     constexpr int P = planes_of(XF), HP = inner_planes(XF), SG = P == 1 ? 0 : GSH;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const Lists * l = reinterpret_cast<const Lists *>(a.lists);
     if ((int) blockIdx.y >= l->count) return;
-    const int e = l->expert[blockIdx.y], p0 = l->start[blockIdx.y], cnt = l->start[blockIdx.y + 1] - p0;
+    const int e = l->expert[blockIdx.y], p0 = l->start[blockIdx.y], cnt = l->pairs[blockIdx.y];
     const int nb = a.dim >> 5, nbp = padded(nb), runs = nbp >> 3, tp = a.tp_up;
     const Lds L = lds_of(P, SG, nb, tp, MINS);
     float * red = reinterpret_cast<float *>(lds + L.end); // [KS][CG][2][tp][16]
@@ -416,7 +433,7 @@ template <int XF, int GSH, int SH, int TM, bool MINS> __global__ __launch_bounds
     for (int t0 = 0; t0 < cnt; t0 += tp) {
         const int nt = min(tp, cnt - t0);
         const int at = l->row[p0 + t0 + min((int) (threadIdx.x & 63), nt - 1)];
-        const Run<2, MINS> first = load_run<GSH, SG, 2, MINS>(w, nb, min(r0, runs - 1)); // (on its way while x is made ready)
+        const Run<2, MINS> first = load_runs<GSH, SG, 2, MINS>(w, nb, min(r0, runs - 1), max(r0, r1 - 1)); // (on its way while x is made ready)
         if (t0) __syncthreads();
         stage<P, MINS>(a.xq, a.xd, a.xs, nbp >> SG, (nb + (1 << SG) - 1) >> SG, lds, L, tp, nt, at);
         __syncthreads();
@@ -426,7 +443,7 @@ template <int XF, int GSH, int SH, int TM, bool MINS> __global__ __launch_bounds
         __syncthreads();
         // four columns of a token a thread, 8 << SH threads for the values of an exponent of h
         for (int j = threadIdx.x; j < nt * CG * 4; j += WAVES * 64) {
-            const int i = j >> (5 - a.ks_up), col = (j & (CG * 4 - 1)) * 4, c = c0 + col;
+            const int i = j >> (WAVES_LOG + 2 - a.ks_up), col = (j & (CG * 4 - 1)) * 4, c = c0 + col;
             f32x4 gt = {0.f, 0.f, 0.f, 0.f}, up = gt, h;
             for (int k = 0; k < KS; k++) {
                 const float * p = red + (((k * CG + (col >> 4)) * 2 * tp + i) * 16 + (col & 15));
@@ -470,11 +487,11 @@ template <int XF, int GSH, int SH, int TM, bool MINS> __global__ __launch_bounds
 }
 
 // the down projection of every pair: waves (32 columns, a KS-th of inner)
-template <int P, int GSH, int SG, int TM, bool MINS> __global__ __launch_bounds__(WAVES * 64, 4) void k_moe_down(MoeArgs a) {
+template <int P, int GSH, int SG, int TM, bool MINS> __global__ __launch_bounds__(WAVES * 64, 3) void k_moe_down(MoeArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const Lists * l = reinterpret_cast<const Lists *>(a.lists);
     if ((int) blockIdx.y >= l->count) return;
-    const int e = l->expert[blockIdx.y], p0 = l->start[blockIdx.y], cnt = l->start[blockIdx.y + 1] - p0;
+    const int e = l->expert[blockIdx.y], p0 = l->start[blockIdx.y], cnt = l->pairs[blockIdx.y];
     const int nb = a.inner >> 5, nbp = padded(nb), runs = nbp >> 3, tp = a.tp_down;
     const Lds L = lds_of(P, SG, nb, tp, MINS);
     float * red = reinterpret_cast<float *>(lds + L.end); // [KS][CG][2][tp][16]
@@ -489,7 +506,7 @@ template <int P, int GSH, int SG, int TM, bool MINS> __global__ __launch_bounds_
     for (int t0 = 0; t0 < cnt; t0 += tp) {
         const int nt = min(tp, cnt - t0);
         const int at = l->pair[p0 + t0 + min((int) (threadIdx.x & 63), nt - 1)];
-        const Run<2, MINS> first = load_run<GSH, SG, 2, MINS>(w, nb, min(r0, runs - 1));
+        const Run<2, MINS> first = load_runs<GSH, SG, 2, MINS>(w, nb, min(r0, runs - 1), max(r0, r1 - 1));
         if (t0) __syncthreads();
         stage<P, MINS>(a.hq, a.hd, a.hs, nbp >> SG, (nb + (1 << SG) - 1) >> SG, lds, L, tp, nt, at);
         __syncthreads();
@@ -498,7 +515,7 @@ template <int P, int GSH, int SG, int TM, bool MINS> __global__ __launch_bounds_
         sums_out<P, SG, 2, TM>(acc, tp, nt, red + (ks * CG + cg) * 2 * tp * 16);
         __syncthreads();
         for (int j = threadIdx.x; j < nt * CG * 8; j += WAVES * 64) {
-            const int i = j >> (6 - a.ks_down), col = (j & (CG * 8 - 1)) * 4, c = c0 + col;
+            const int i = j >> (WAVES_LOG + 3 - a.ks_down), col = (j & (CG * 8 - 1)) * 4, c = c0 + col;
             if (c >= a.dim) continue;
             f32x4 v = {0.f, 0.f, 0.f, 0.f};
             for (int k = 0; k < KS; k++) v += *reinterpret_cast<const f32x4 *>(red + (((k * CG + (col >> 5)) * 2 + (col >> 4 & 1)) * tp + i) * 16 + (col & 15));
@@ -552,7 +569,7 @@ template <int XF, int GSH, int SH, bool MINS> hipError_t run(const MoeArgs & a, 
 }
 template <int XF, int GSH, bool MINS> hipError_t run(const MoeArgs & a, hipStream_t st) {
     if constexpr (GSH == 0) return run<XF, 0, 0, MINS>(a, st);
-    else return a.ks_up == 0 ? run<XF, GSH, GSH, MINS>(a, st) : run<XF, GSH, 0, MINS>(a, st);
+    else return a.ks_up == 0 ? run<XF, GSH, 1, MINS>(a, st) : run<XF, GSH, 0, MINS>(a, st);
 }
 template <int XF, bool MINS> hipError_t run(const MoeArgs & a, hipStream_t st) {
     return a.gsh == 0 ? run<XF, 0, MINS>(a, st) : a.gsh == 1 ? run<XF, 1, MINS>(a, st) : run<XF, 2, MINS>(a, st);
@@ -563,14 +580,14 @@ template <int XF> hipError_t run(const MoeArgs & a, hipStream_t st) { return a.u
 int pass_tokens(const MoeArgs & a, int P, int sg, int blocks) {
     const int tg = group_of(P, sg);
     int tp = std::min((std::min(a.rows, 16) + tg - 1) / tg * tg, 16);
-    while (tp > tg && lds_bytes(a, P, sg, blocks, tp) > 80 * 1024) tp -= tg;
+    while (tp > tg && lds_bytes(a, P, sg, blocks, tp) > 53 * 1024) tp -= tg;
     return tp;
 }
 // waves that split k (1 << ..): as many as leave the workgroups (of `cols` columns a wave) within one round of two a CU, as every round pays for its
 // start; `experts` are those that occur
 int split(double experts, int n, int cols, int runs, int limit) {
     int log = limit;
-    while (log > 0 && (experts * ((n + (cols * WAVES >> log) - 1) / (cols * WAVES >> log)) > 512 || runs < 1 << log)) log--;
+    while (log > 0 && (experts * ((n + (cols * WAVES >> log) - 1) / (cols * WAVES >> log)) > 768 || runs < 1 << log)) log--;
     return log;
 }
 
@@ -605,10 +622,10 @@ static void split_work(MoeArgs & a, int xform) {
     const int HP = inner_planes(xform), P = planes_of(xform), nbi = a.inner / 32;
     // the experts that occur where every choice is as likely as another
     const double experts = a.n_experts * (1 - std::pow(1 - 1.0 / a.n_experts, a.rows * a.top_k));
-    a.ks_up = split(experts, a.inner, 16, padded(a.dim / 32) / 8, 2);
-    a.ks_down = split(experts, a.dim, 32, padded(nbi) / 8, 3);
+    a.ks_up = split(experts, a.inner, 16, padded(a.dim / 32) / 8, WAVES_LOG - 1);
+    a.ks_down = split(experts, a.dim, 32, padded(nbi) / 8, WAVES_LOG);
     a.tp_up = pass_tokens(a, P, P == 1 ? 0 : a.gsh, a.dim / 32);
-    a.tp_down = pass_tokens(a, HP, a.ks_up == 0 ? a.gsh : 0, nbi);
+    a.tp_down = pass_tokens(a, HP, a.ks_up == 0 ? std::min(a.gsh, 1) : 0, nbi);
 }
 
 template <int XF> static hipError_t prep(const MoeArgs & a, const RouteArgs * route, hipStream_t st) {
