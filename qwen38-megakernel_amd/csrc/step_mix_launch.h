@@ -71,8 +71,8 @@ struct MoeArgs {
     uint8_t * xq, * hq;
     float * xd, * hd, * xs, * hs;
     float * out;     // [pairs][dim]: the experts' outputs (where xq, xd and xs were)
-    // (set by the launcher) tokens of an expert that a pass holds in LDS, and waves (1 << ..) that split k
-    int tp_up, tp_down, ks_up, ks_down;
+    // (set by the launcher) tokens of an expert that a pass holds in LDS, runs of k that it holds at a time, and waves (1 << ..) that split k
+    int tp_up, tp_down, cr_up, cr_down, ks_up, ks_down;
 };
 constexpr int MOE_ROWS = 64;   // rows of a launch; a call of more runs them one after another
 constexpr int MOE_MAX_ROWS = 4096, MOE_MAX_DIM = 16384, MOE_MAX_INNER = 32768;

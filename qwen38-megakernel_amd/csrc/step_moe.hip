@@ -37,18 +37,18 @@ constexpr int group_of(int P, int sg) { return lane_tokens(P) << sg; }
 __host__ __device__ __forceinline__ constexpr int padded(int blocks) { return (blocks + 7) & ~7; }
 // a row of a plane, in memory and in LDS: [runs of 8 blocks][u][half][g][16 bytes], then 16 bytes unused: 16 rows' pieces lie in different banks
 __host__ __device__ __forceinline__ constexpr int plane_bytes(int nb) { return padded(nb) * 32 + 16; }
-// LDS of a pass: token t's plane p is row t P + p; zeros for the operand's other lanes; per 32 << sg values the tokens' factors, and with
-// minimums the tokens' sums
+// LDS of a pass, for `cr` runs of k at a time: token t's plane p is row t P + p; zeros for the operand's other lanes; per 32 << sg values the
+// tokens' factors, and with minimums the tokens' sums
 struct Lds {
     int row, zero, dx, ds, end;
 };
-__host__ __device__ __forceinline__ constexpr Lds lds_of(int P, int sg, int nb, int tp, bool mins) {
+__host__ __device__ __forceinline__ constexpr Lds lds_of(int P, int sg, int cr, int tp, bool mins) {
     Lds l{};
-    l.row = plane_bytes(nb);
+    l.row = cr * 256 + 16;
     l.zero = tp * P * l.row;
     l.dx = l.zero + 256;
-    l.ds = l.dx + (padded(nb) >> sg) * tp * 4;
-    l.end = ((mins ? l.ds + (padded(nb) >> sg) * tp * 4 : l.ds) + 15) & ~15;
+    l.ds = l.dx + (cr * 8 >> sg) * tp * 4;
+    l.end = ((mins ? l.ds + (cr * 8 >> sg) * tp * 4 : l.ds) + 15) & ~15;
     return l;
 }
 // the block of lane group g in step u of a run of 8 blocks: groups that share a sum have blocks of one weight group, and a lane's two steps
@@ -137,21 +137,28 @@ template <int GSH, int SG, int NT, bool MINS> __device__ __forceinline__ Run<NT,
     return r;
 }
 
-// the sums of runs r0 .. r1 - 1 (in: the first one's codes) for nt tokens in LDS, at most TM
+// a wave's part of the runs of a chunk of k, and the chunk's first run
+struct Part {
+    int first, r0, r1;
+};
+// runs `chunk` .. of k, `cr` of them at a time, the ks-th of 1 << log parts (each has one at least)
+__device__ __forceinline__ Part part_of(int runs, int cr, int chunk, int ks, int log) {
+    const int c0 = chunk * cr, n = min(cr, runs - c0);
+    return Part{c0, c0 + ((n * ks) >> log), c0 + ((n * (ks + 1)) >> log)};
+}
+// adds the sums of the part p for nt tokens in LDS, at most TM, to acc.  in: the first two runs' codes and the first window of scales; those of the
+// part q behind
 template <int P, int GSH, int SG, int NT, int TM, bool MINS>
-__device__ __forceinline__ void products(const Rows<NT> & w, Run<NT, MINS> in, int nb, int r0, int r1, const uint8_t * lds, const Lds & L, uint16_t * win, int tp, int nt, float (&acc)[NT][TM >> SG]) {
+__device__ __forceinline__ void products(const Rows<NT> & w, Run<NT, MINS> & in, int nb, Part p, Part nx, const uint8_t * lds, const Lds & L, uint16_t * win, int tp, int nt, float (&acc)[NT][TM >> SG]) {
+    const int r0 = p.r0, r1 = p.r1;
     constexpr int PR = op_rows(P), TL = lane_tokens(P), TG = group_of(P, SG);
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, m = n & ((4 << SG) - 1);
     const bool active = n >> (2 + SG) == g >> SG && m % PR < P;
     const int amask = active ? ~0 : 0, aoff = active ? (m / PR * P + m % PR) * L.row + g * 16 : L.zero, astep = TG * P * L.row & amask;
     const int first = (g & ((1 << SG) - 1)) * TL; // of a group's tokens, the first in the lane's sums
     const float * dx = reinterpret_cast<const float *>(lds + L.dx), * ds = reinterpret_cast<const float *>(lds + L.ds);
-#pragma unroll
-    for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int i = 0; i < TM >> SG; i++) acc[t][i] = 0.f;
     const auto run = [&](int R, int buf) {
-        const int next = min(R + 2, r1 - 1); // (behind the last run that one again, unused)
+        const int next = R + 2 < r1 ? R + 2 : min(nx.r0 + buf, nx.r1 - 1);
         const int in_win = (R - r0) & ((4 << GSH) - 1);
         float sc[NT][2], mn[NT][2];
         const auto scales = [&](const uint16_t * p, float (&v)[2]) {
@@ -182,8 +189,8 @@ __device__ __forceinline__ void products(const Rows<NT> & w, Run<NT, MINS> in, i
 #pragma unroll
             for (int t = 0; t < NT; t++) load_codes<SG>(w, nb, next, t, u, in.c[buf][t][u]);
             __builtin_amdgcn_sched_barrier(0);
-            const uint8_t * ap = lds + (aoff + (R * 256 & amask)) + u * 128;
-            const int at = ((8 * R + block_of<SG>(g, u)) >> SG) * tp + first;
+            const uint8_t * ap = lds + (aoff + ((R - p.first) * 256 & amask)) + u * 128;
+            const int at = ((8 * (R - p.first) + block_of<SG>(g, u)) >> SG) * tp + first;
 #pragma unroll
             for (int q = 0; q < TM / TG; q++) {
                 if (q * TG >= nt) continue;
@@ -223,7 +230,7 @@ __device__ __forceinline__ void products(const Rows<NT> & w, Run<NT, MINS> in, i
                 if constexpr (MINS) *reinterpret_cast<u32x4 *>(win + ((NT + t) * 16 + n) * WROW + 8 * g) = in.m[t];
             }
             asm volatile("" ::: "memory"); // (read below by other lanes and as another type)
-            if (R + (4 << GSH) < r1) load_window<GSH>(w, nb, R + (4 << GSH), in);
+            load_window<GSH>(w, nb, R + (4 << GSH) < r1 ? R + (4 << GSH) : nx.r0, in);
         }
         run(R, 0);
         if (R + 1 < r1) run(R + 1, 1);
@@ -375,34 +382,35 @@ template <int XF, int V> __global__ __launch_bounds__(PREP) void k_moe_prep(Prep
 __device__ __forceinline__ unsigned lds_address(const uint8_t * lds) {
     return (unsigned) __builtin_amdgcn_readfirstlane((unsigned) (size_t) (const __attribute__((address_space(3))) uint8_t *) lds);
 }
-// the planes, factors and sums of nt tokens, lane t's `at` the place of the t-th, into LDS
+// the planes, factors and sums of nt tokens, lane t's `at` the place of the t-th, into LDS: of runs c0 .. c0 + n - 1 (rows of `row` bytes, nd factors, ng of
+// them in use)
 template <int P, bool MINS>
-__device__ __forceinline__ void stage(const uint8_t * q, const float * d, const float * s, int nd, int ng, uint8_t * lds, const Lds & L, int tp, int nt, int at) {
+__device__ __forceinline__ void stage(const uint8_t * q, const float * d, const float * s, int row, int nd, int ng, int c0, int n, int sg, uint8_t * lds, const Lds & L, int tp, int nt, int at) {
     const unsigned base = lds_address(lds);
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, bytes = L.row - 16, per = (bytes + 1023) >> 10;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, bytes = n * 256, per = (bytes + 1023) >> 10, d0 = c0 * 8 >> sg, dn = n * 8 >> sg;
     float * dx = reinterpret_cast<float *>(lds + L.dx), * ds = reinterpret_cast<float *>(lds + L.ds);
     int c = wave;
     for (int t = 0; t < nt; t++) { // 1 KiB a copy, the waves in turn
-        const uint8_t * from = q + (size_t) (unsigned) __builtin_amdgcn_readlane(at, t) * (P * L.row);
+        const uint8_t * from = q + (size_t) (unsigned) __builtin_amdgcn_readlane(at, t) * (P * row) + c0 * 256;
 #pragma unroll
         for (int p = 0; p < P; p++, c -= per)
             for (; c < per; c += WAVES)
-                if (c * 1024 + lane * 16 < bytes) dma16(from + (p * L.row + c * 1024 + lane * 16), base + (t * P + p) * L.row + c * 1024);
+                if (c * 1024 + lane * 16 < bytes) dma16(from + (p * row + c * 1024 + lane * 16), base + (t * P + p) * L.row + c * 1024);
     }
-    for (int k = tid; k < nd; k += WAVES * 64)
+    for (int k = tid; k < dn; k += WAVES * 64)
         for (int t0 = 0; t0 < nt; t0 += 4) { // (four loads, then their values)
             float v[4], w[4];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                const size_t i = (size_t) (unsigned) __builtin_amdgcn_readlane(at, min(t0 + u, nt - 1)) * nd + k;
+                const size_t i = (size_t) (unsigned) __builtin_amdgcn_readlane(at, min(t0 + u, nt - 1)) * nd + d0 + k;
                 v[u] = d[i];
                 if (MINS) w[u] = s[i];
             }
 #pragma unroll
             for (int u = 0; u < 4; u++)
                 if (t0 + u < nt) {
-                    dx[k * tp + t0 + u] = k < ng ? v[u] : 0.f; // (of blocks past the last one: nothing)
-                    if (MINS) ds[k * tp + t0 + u] = k < ng ? w[u] : 0.f;
+                    dx[k * tp + t0 + u] = d0 + k < ng ? v[u] : 0.f; // (of blocks past the last one: nothing)
+                    if (MINS) ds[k * tp + t0 + u] = d0 + k < ng ? w[u] : 0.f;
                 }
         }
     vm_drain();
@@ -420,12 +428,14 @@ template <int XF, int GSH, int SH, int TM, bool MINS> __global__ __launch_bounds
     if ((int) blockIdx.y >= l->count) return;
     const int e = l->expert[blockIdx.y], p0 = l->start[blockIdx.y], cnt = l->pairs[blockIdx.y];
     const int nb = a.dim >> 5, nbp = padded(nb), runs = nbp >> 3, tp = a.tp_up;
-    const Lds L = lds_of(P, SG, nb, tp, MINS);
-    float * red = reinterpret_cast<float *>(lds + L.end); // [KS][CG][2][tp][16]
+    const Lds L = lds_of(P, SG, a.cr_up, tp, MINS);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    uint16_t * win = reinterpret_cast<uint16_t *>(red + WAVES * 2 * tp * 16) + wave * (win_bytes(2, MINS) / 2);
+    // each wave's window of scales, then its sums: [KS][CG][2][tp][16]
+    constexpr int WB = win_bytes(2, MINS) / 4;
+    float * red = reinterpret_cast<float *>(lds + L.end);
+    uint16_t * win = reinterpret_cast<uint16_t *>(red + wave * WB);
     const int KS = 1 << a.ks_up, CG = WAVES >> a.ks_up, cg = wave & (CG - 1), ks = wave / CG;
-    const int gs = (nb + (1 << GSH) - 1) >> GSH, c0 = blockIdx.x * 16 * CG, r0 = (runs * ks) >> a.ks_up, r1 = (runs * (ks + 1)) >> a.ks_up;
+    const int gs = (nb + (1 << GSH) - 1) >> GSH, c0 = blockIdx.x * 16 * CG, chunks = (runs + a.cr_up - 1) / a.cr_up;
     Rows<2> w; // (columns past the last one: zeros below)
     w.set(0, a.up, 2 * e, a.inner, c0 + cg * 16, nb, gs);
     w.set(1, a.up, 2 * e + 1, a.inner, c0 + cg * 16, nb, gs);
@@ -433,20 +443,27 @@ template <int XF, int GSH, int SH, int TM, bool MINS> __global__ __launch_bounds
     for (int t0 = 0; t0 < cnt; t0 += tp) {
         const int nt = min(tp, cnt - t0);
         const int at = l->row[p0 + t0 + min((int) (threadIdx.x & 63), nt - 1)];
-        const Run<2, MINS> first = load_runs<GSH, SG, 2, MINS>(w, nb, min(r0, runs - 1), max(r0, r1 - 1)); // (on its way while x is made ready)
-        if (t0) __syncthreads();
-        stage<P, MINS>(a.xq, a.xd, a.xs, nbp >> SG, (nb + (1 << SG) - 1) >> SG, lds, L, tp, nt, at);
-        __syncthreads();
+        Part part = part_of(runs, a.cr_up, 0, ks, a.ks_up);
+        Run<2, MINS> in = load_runs<GSH, SG, 2, MINS>(w, nb, part.r0, part.r1 - 1); // (on its way while x is made ready)
         float acc[2][TM >> SG];
-        products<P, GSH, SG, 2, TM, MINS>(w, first, nb, r0, r1, lds, L, win, tp, nt, acc);
-        sums_out<P, SG, 2, TM>(acc, tp, nt, red + (ks * CG + cg) * 2 * tp * 16);
+#pragma unroll
+        for (int i = 0; i < TM >> SG; i++) acc[0][i] = acc[1][i] = 0.f;
+        for (int c = 0; c < chunks; c++) {
+            const Part next = part_of(runs, a.cr_up, min(c + 1, chunks - 1), ks, a.ks_up); // (behind the last chunk that one again, unused)
+            if (t0 + c) __syncthreads();
+            stage<P, MINS>(a.xq, a.xd, a.xs, plane_bytes(nb), nbp >> SG, (nb + (1 << SG) - 1) >> SG, part.first, min(a.cr_up, runs - part.first), SG, lds, L, tp, nt, at);
+            __syncthreads();
+            products<P, GSH, SG, 2, TM, MINS>(w, in, nb, part, next, lds, L, win, tp, nt, acc);
+            part = next;
+        }
+        sums_out<P, SG, 2, TM>(acc, tp, nt, red + (ks * CG + cg) * WB);
         __syncthreads();
         // four columns of a token a thread, 8 << SH threads for the values of an exponent of h
         for (int j = threadIdx.x; j < nt * CG * 4; j += WAVES * 64) {
             const int i = j >> (WAVES_LOG + 2 - a.ks_up), col = (j & (CG * 4 - 1)) * 4, c = c0 + col;
             f32x4 gt = {0.f, 0.f, 0.f, 0.f}, up = gt, h;
             for (int k = 0; k < KS; k++) {
-                const float * p = red + (((k * CG + (col >> 4)) * 2 * tp + i) * 16 + (col & 15));
+                const float * p = red + ((k * CG + (col >> 4)) * WB + i * 16 + (col & 15));
                 gt += *reinterpret_cast<const f32x4 *>(p);
                 up += *reinterpret_cast<const f32x4 *>(p + tp * 16);
             }
@@ -493,12 +510,14 @@ template <int P, int GSH, int SG, int TM, bool MINS> __global__ __launch_bounds_
     if ((int) blockIdx.y >= l->count) return;
     const int e = l->expert[blockIdx.y], p0 = l->start[blockIdx.y], cnt = l->pairs[blockIdx.y];
     const int nb = a.inner >> 5, nbp = padded(nb), runs = nbp >> 3, tp = a.tp_down;
-    const Lds L = lds_of(P, SG, nb, tp, MINS);
-    float * red = reinterpret_cast<float *>(lds + L.end); // [KS][CG][2][tp][16]
+    const Lds L = lds_of(P, SG, a.cr_down, tp, MINS);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    uint16_t * win = reinterpret_cast<uint16_t *>(red + WAVES * 2 * tp * 16) + wave * (win_bytes(2, MINS) / 2);
+    // each wave's window of scales, then its sums: [KS][CG][2][tp][16]
+    constexpr int WB = win_bytes(2, MINS) / 4;
+    float * red = reinterpret_cast<float *>(lds + L.end);
+    uint16_t * win = reinterpret_cast<uint16_t *>(red + wave * WB);
     const int KS = 1 << a.ks_down, CG = WAVES >> a.ks_down, cg = wave & (CG - 1), ks = wave / CG;
-    const int gs = (nb + (1 << GSH) - 1) >> GSH, c0 = blockIdx.x * CG * 32, r0 = (runs * ks) >> a.ks_down, r1 = (runs * (ks + 1)) >> a.ks_down;
+    const int gs = (nb + (1 << GSH) - 1) >> GSH, c0 = blockIdx.x * CG * 32, chunks = (runs + a.cr_down - 1) / a.cr_down;
     Rows<2> w; // (columns past the last one: not stored)
     w.set(0, a.down, e, a.dim, c0 + cg * 32, nb, gs);
     w.set(1, a.down, e, a.dim, c0 + cg * 32 + 16, nb, gs);
@@ -506,19 +525,26 @@ template <int P, int GSH, int SG, int TM, bool MINS> __global__ __launch_bounds_
     for (int t0 = 0; t0 < cnt; t0 += tp) {
         const int nt = min(tp, cnt - t0);
         const int at = l->pair[p0 + t0 + min((int) (threadIdx.x & 63), nt - 1)];
-        const Run<2, MINS> first = load_runs<GSH, SG, 2, MINS>(w, nb, min(r0, runs - 1), max(r0, r1 - 1));
-        if (t0) __syncthreads();
-        stage<P, MINS>(a.hq, a.hd, a.hs, nbp >> SG, (nb + (1 << SG) - 1) >> SG, lds, L, tp, nt, at);
-        __syncthreads();
+        Part part = part_of(runs, a.cr_down, 0, ks, a.ks_down);
+        Run<2, MINS> in = load_runs<GSH, SG, 2, MINS>(w, nb, part.r0, part.r1 - 1); // (on its way while x is made ready)
         float acc[2][TM >> SG];
-        products<P, GSH, SG, 2, TM, MINS>(w, first, nb, r0, r1, lds, L, win, tp, nt, acc);
-        sums_out<P, SG, 2, TM>(acc, tp, nt, red + (ks * CG + cg) * 2 * tp * 16);
+#pragma unroll
+        for (int i = 0; i < TM >> SG; i++) acc[0][i] = acc[1][i] = 0.f;
+        for (int c = 0; c < chunks; c++) {
+            const Part next = part_of(runs, a.cr_down, min(c + 1, chunks - 1), ks, a.ks_down); // (behind the last chunk that one again, unused)
+            if (t0 + c) __syncthreads();
+            stage<P, MINS>(a.hq, a.hd, a.hs, plane_bytes(nb), nbp >> SG, (nb + (1 << SG) - 1) >> SG, part.first, min(a.cr_down, runs - part.first), SG, lds, L, tp, nt, at);
+            __syncthreads();
+            products<P, GSH, SG, 2, TM, MINS>(w, in, nb, part, next, lds, L, win, tp, nt, acc);
+            part = next;
+        }
+        sums_out<P, SG, 2, TM>(acc, tp, nt, red + (ks * CG + cg) * WB);
         __syncthreads();
         for (int j = threadIdx.x; j < nt * CG * 8; j += WAVES * 64) {
             const int i = j >> (WAVES_LOG + 3 - a.ks_down), col = (j & (CG * 8 - 1)) * 4, c = c0 + col;
             if (c >= a.dim) continue;
             f32x4 v = {0.f, 0.f, 0.f, 0.f};
-            for (int k = 0; k < KS; k++) v += *reinterpret_cast<const f32x4 *>(red + (((k * CG + (col >> 5)) * 2 + (col >> 4 & 1)) * tp + i) * 16 + (col & 15));
+            for (int k = 0; k < KS; k++) v += *reinterpret_cast<const f32x4 *>(red + ((k * CG + (col >> 5)) * WB + ((col >> 4 & 1) * tp + i) * 16 + (col & 15)));
             *reinterpret_cast<f32x4 *>(a.out + (size_t) l->pair[p0 + t0 + i] * a.dim + c) = v;
         }
     }
@@ -542,18 +568,18 @@ template <int YT> __global__ __launch_bounds__(256) void k_moe_sum(MoeArgs a) {
     for (int i = 0; i < 4; i++) y[i] = Elem<YT>::down(v[i]);
 }
 
-size_t lds_bytes(const MoeArgs & a, int P, int sg, int blocks, int tp) { return lds_of(P, sg, blocks, tp, a.up.mins).end + (size_t) WAVES * (2 * tp * 16 * 4 + win_bytes(2, a.up.mins)); }
+size_t lds_bytes(const MoeArgs & a, int P, int sg, int cr, int tp) { return lds_of(P, sg, cr, tp, a.up.mins).end + (size_t) WAVES * win_bytes(2, a.up.mins); }
 template <int XF, int GSH, int SH, int TM, bool MINS> hipError_t up(const MoeArgs & a, int slots, hipStream_t st) {
     constexpr int P = planes_of(XF), SG = P == 1 ? 0 : GSH;
     static std::atomic<uint64_t> done;
-    const size_t lds = lds_bytes(a, P, SG, a.dim / 32, a.tp_up);
+    const size_t lds = lds_bytes(a, P, SG, a.cr_up, a.tp_up);
     const hipError_t e = allow_lds(k_moe_up<XF, GSH, SH, TM, MINS>, lds, done);
     const int cols = 16 * (WAVES >> a.ks_up);
     return e != hipSuccess ? e : launch(k_moe_up<XF, GSH, SH, TM, MINS>, dim3((a.inner + cols - 1) / cols, slots), dim3(WAVES * 64), lds, st, a);
 }
 template <int P, int GSH, int SG, int TM, bool MINS> hipError_t down(const MoeArgs & a, int slots, hipStream_t st) {
     static std::atomic<uint64_t> done;
-    const size_t lds = lds_bytes(a, P, SG, a.inner / 32, a.tp_down);
+    const size_t lds = lds_bytes(a, P, SG, a.cr_down, a.tp_down);
     const hipError_t e = allow_lds(k_moe_down<P, GSH, SG, TM, MINS>, lds, done);
     const int cols = 32 * (WAVES >> a.ks_down);
     return e != hipSuccess ? e : launch(k_moe_down<P, GSH, SG, TM, MINS>, dim3((a.dim + cols - 1) / cols, slots), dim3(WAVES * 64), lds, st, a);
@@ -576,12 +602,22 @@ template <int XF, bool MINS> hipError_t run(const MoeArgs & a, hipStream_t st) {
 }
 template <int XF> hipError_t run(const MoeArgs & a, hipStream_t st) { return a.up.mins ? run<XF, true>(a, st) : run<XF, false>(a, st); }
 
-// tokens of a pass: up to 16, in half of a CU's LDS where that holds an instruction's
-int pass_tokens(const MoeArgs & a, int P, int sg, int blocks) {
-    const int tg = group_of(P, sg);
-    int tp = std::min((std::min(a.rows, 16) + tg - 1) / tg * tg, 16);
-    while (tp > tg && lds_bytes(a, P, sg, blocks, tp) > 53 * 1024) tp -= tg;
-    return tp;
+// Tokens of a pass, up to 16, and runs of k that LDS holds at a time, three workgroups a CU: all of k where that leaves room for twice the tokens
+// that an expert has on average, else chunks of at least four runs a wave (47 rows of 8 experts, 16 tokens in chunks: 178 us, 8 at a time 205;
+// 3 rows, the other way round: 85 and 79).
+void pass(const MoeArgs & a, int P, int sg, int runs, int ks_log, int & tp, int & cr) {
+    constexpr size_t THIRD = 53 * 1024;
+    const int tg = group_of(P, sg), least = std::min(runs, 4 << ks_log), most = std::min((std::min(a.rows, 16) + tg - 1) / tg * tg, 16);
+    const int want = std::min(most, 2 * ((a.rows * a.top_k + a.n_experts - 1) / a.n_experts));
+    cr = runs;
+    for (tp = most; tp >= std::max(want, tg); tp -= tg)
+        if (lds_bytes(a, P, sg, cr, tp) <= THIRD) return;
+    for (tp = most;; tp -= tg) {
+        for (cr = runs; cr > least && lds_bytes(a, P, sg, cr, tp) > THIRD;) cr = std::max(least, (cr + 1) / 2);
+        if (tp <= tg || lds_bytes(a, P, sg, cr, tp) <= THIRD) break;
+    }
+    // (the last chunk has a run for every wave)
+    while (cr < runs && runs % cr && runs % cr < 1 << ks_log) cr++;
 }
 // waves that split k (1 << ..): as many as leave the workgroups (of `cols` columns a wave) within one round of two a CU, as every round pays for its
 // start; `experts` are those that occur
@@ -624,8 +660,8 @@ static void split_work(MoeArgs & a, int xform) {
     const double experts = a.n_experts * (1 - std::pow(1 - 1.0 / a.n_experts, a.rows * a.top_k));
     a.ks_up = split(experts, a.inner, 16, padded(a.dim / 32) / 8, WAVES_LOG - 1);
     a.ks_down = split(experts, a.dim, 32, padded(nbi) / 8, WAVES_LOG);
-    a.tp_up = pass_tokens(a, P, P == 1 ? 0 : a.gsh, a.dim / 32);
-    a.tp_down = pass_tokens(a, HP, a.ks_up == 0 ? std::min(a.gsh, 1) : 0, nbi);
+    pass(a, P, P == 1 ? 0 : a.gsh, padded(a.dim / 32) / 8, a.ks_up, a.tp_up, a.cr_up);
+    pass(a, HP, a.ks_up == 0 ? std::min(a.gsh, 1) : 0, padded(nbi) / 8, a.ks_down, a.tp_down, a.cr_down);
 }
 
 template <int XF> static hipError_t prep(const MoeArgs & a, const RouteArgs * route, hipStream_t st) {
