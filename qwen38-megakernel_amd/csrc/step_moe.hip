@@ -230,7 +230,8 @@ __device__ __forceinline__ void products(const Rows<NT> & w, Run<NT, MINS> & in,
                 if constexpr (MINS) *reinterpret_cast<u32x4 *>(win + ((NT + t) * 16 + n) * WROW + 8 * g) = in.m[t];
             }
             asm volatile("" ::: "memory"); // (read below by other lanes and as another type)
-            load_window<GSH>(w, nb, R + (4 << GSH) < r1 ? R + (4 << GSH) : nx.r0, in);
+            const bool more = R + (4 << GSH) < r1;
+            if (more || nx.first != p.first) load_window<GSH>(w, nb, more ? R + (4 << GSH) : nx.r0, in);
         }
         run(R, 0);
         if (R + 1 < r1) run(R + 1, 1);
@@ -449,7 +450,7 @@ template <int XF, int GSH, int SH, int TM, bool MINS> __global__ __launch_bounds
 #pragma unroll
         for (int i = 0; i < TM >> SG; i++) acc[0][i] = acc[1][i] = 0.f;
         for (int c = 0; c < chunks; c++) {
-            const Part next = part_of(runs, a.cr_up, min(c + 1, chunks - 1), ks, a.ks_up); // (behind the last chunk that one again, unused)
+            const Part next = c + 1 < chunks ? part_of(runs, a.cr_up, c + 1, ks, a.ks_up) : Part{part.first, part.r1 - 1, part.r1}; // (behind the last run that one again, unused)
             if (t0 + c) __syncthreads();
             stage<P, MINS>(a.xq, a.xd, a.xs, plane_bytes(nb), nbp >> SG, (nb + (1 << SG) - 1) >> SG, part.first, min(a.cr_up, runs - part.first), SG, lds, L, tp, nt, at);
             __syncthreads();
@@ -531,7 +532,7 @@ template <int P, int GSH, int SG, int TM, bool MINS> __global__ __launch_bounds_
 #pragma unroll
         for (int i = 0; i < TM >> SG; i++) acc[0][i] = acc[1][i] = 0.f;
         for (int c = 0; c < chunks; c++) {
-            const Part next = part_of(runs, a.cr_down, min(c + 1, chunks - 1), ks, a.ks_down); // (behind the last chunk that one again, unused)
+            const Part next = c + 1 < chunks ? part_of(runs, a.cr_down, c + 1, ks, a.ks_down) : Part{part.first, part.r1 - 1, part.r1}; // (behind the last run that one again, unused)
             if (t0 + c) __syncthreads();
             stage<P, MINS>(a.hq, a.hd, a.hs, plane_bytes(nb), nbp >> SG, (nb + (1 << SG) - 1) >> SG, part.first, min(a.cr_down, runs - part.first), SG, lds, L, tp, nt, at);
             __syncthreads();
