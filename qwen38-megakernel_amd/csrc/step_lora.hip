@@ -1,11 +1,13 @@
 // Low-rank adapters of many requests at once: y[m] = base[m] + s_a B_a (A_a x[m]) with a = ids[m], next to a projection whose
-// result base is.  Two kernels: u = A x of each row (a tile of 16 rows, the adapters in it one after another or side by
-// side in workgroups of their own), then y = base + B u.  A row belongs to one adapter, so a tile's rows are split among
-// its adapters; nothing is sorted, and an adapter's weights are read once per tile that has it.
+// result base is.  Two kernels: u = A x of each row, then y = base + B u.  Nothing is sorted: a workgroup has a tile of 16 rows (32 of
+// many) and takes the adapters in it one after another, or, where tiles are few, side by side in workgroups of their own; a row belongs
+// to one adapter, so a tile's rows are split among its adapters.
 //
-// Matrix instructions take 16-bit operands and add in fp32.  Where x or u has more bits it goes in as several bf16 parts
-// (truncated, 8 bits each: fp32 is three of them exactly, fp16 two), fp16 adapters as two; x of int8 units goes in as its codes,
-// whose block scale (the blocks have the length of a step) multiplies the step's result.
+// Matrix instructions take 16-bit operands and add in fp32.  The adapters' weights go in as they are.  Where x has more bits than their type it
+// goes in as several parts: bf16 adapters take fp16 x as two bf16 parts and fp32 x as three (truncated, 8 bits each: exact); fp16
+// adapters take bf16 x as one and fp32 x as two fp16 parts after a power of two per row and step of 32 values, which multiplies the step's
+// result (2^-39 and 2^-23 of the largest of the 32).  Int8 units go in as their codes, the block's scale multiplying the step's result.  u goes in
+// as three bf16 parts, or two fp16 parts after a power of two per row and 64 ranks.
 #include "step_dev.h"
 #include "step_mix_launch.h"
 
@@ -17,13 +19,13 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
-// operands of a step: 8 values of a lane as `parts` 16-bit vectors
-constexpr bool f16_mfma(int xf, int wf) { return wf == DT_F16 && (xf == DT_F16 || xf == W4_UNITS); }
-constexpr int x_parts(int xf, int wf) { return xf == DT_F32 ? 3 : xf == DT_F16 && wf != DT_F16 ? 2 : 1; }
-constexpr int w_parts(int xf, int wf) { return wf == DT_F16 && !f16_mfma(xf, wf) ? 2 : 1; }
+template <int WF> __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (WF == DT_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
 
 // v as P bf16 parts, each what is left of the ones before cut to 8 bits; an infinity or a NaN is the first part's alone
-template <int P> __device__ __forceinline__ void split(const float (&v)[8], u32x4 (&p)[P]) {
+template <int P> __device__ __forceinline__ void split_bf16(const float (&v)[8], u32x4 (&p)[P]) {
     float r[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) r[i] = v[i];
@@ -40,38 +42,54 @@ template <int P> __device__ __forceinline__ void split(const float (&v)[8], u32x
         for (int i = 0; i < 4; i++) p[q][i] = h[2 * i] >> 16 | h[2 * i + 1];
     }
 }
-
-template <bool F16> __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c) {
-    if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-// an adapter's 8 weights as they are in memory -> the operand's parts
-template <int WF, int P> __device__ __forceinline__ void open_w(u32x4 raw, u32x4 (&p)[P]) {
-    if constexpr (P == 1) p[0] = raw;
-    else {
-        float v[8];
-        Elem<DT_F16>::open8(__builtin_bit_cast(half8, raw), v);
-        split<P>(v, p);
+// The four lane groups' values of a row times 2^e, which brings the largest (its bits: top) to [2^14, 2^15), as P fp16 parts; returns 2^-e.
+// Beside an infinity or a NaN finite values are zeros (they cannot change the result).
+template <int P> __device__ __forceinline__ float split_f16(float (&v)[8], unsigned top, u32x4 (&p)[P]) {
+    const bool wild = top >= 0x7f800000u;
+    const int E = max((int) (top >> 23), 15);
+    const float up = __builtin_bit_cast(float, (unsigned) (268 - E) << 23);
+    half8 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float w = !wild ? v[i] * up : __builtin_fabsf(v[i]) < __builtin_inff() ? 0.f : v[i];
+        hi[i] = (_Float16) w;
+        lo[i] = (_Float16) (wild ? 0.f : w - (float) hi[i]);
     }
+    p[0] = __builtin_bit_cast(u32x4, hi);
+    if constexpr (P > 1) p[1] = __builtin_bit_cast(u32x4, lo);
+    return wild ? 1.f : __builtin_bit_cast(float, (unsigned) (E - 14) << 23);
+}
+__device__ __forceinline__ unsigned row_top(unsigned t) { // over the four lane groups
+    t = max(t, shfl_xor_u(t, 16));
+    return max(t, shfl_xor_u(t, 32));
 }
 
-// the adapters of a tile of 16 rows, one after another: a's rows in lanes (row n = lane & 15) of `mine`
-struct Adapters {
+// the adapters of a tile of RT x 16 rows, one after another: lane n = lane & 15 has rows n, 16 + n
+template <int RT> struct Adapters {
     unsigned todo; // rows whose adapter is still to come
-    int id;        // the lane's row's
-    bool has;
+    int id[RT];
+    bool has[RT];
     __device__ __forceinline__ Adapters(const LoraArgs & a, int row) {
-        id = row < a.rows ? a.ids[row] : -1;
-        has = (unsigned) id < (unsigned) a.n_adapters;
-        todo = (unsigned) __ballot(has) & 0xffffu;
+        todo = 0;
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            id[t] = row + 16 * t < a.rows ? a.ids[row + 16 * t] : -1;
+            has[t] = (unsigned) id[t] < (unsigned) a.n_adapters;
+            todo |= ((unsigned) __ballot(has[t]) & 0xffffu) << 16 * t;
+        }
     }
-    // the next one, or -1
-    __device__ __forceinline__ int next(bool & mine) {
+    // the next one and its rows, or -1
+    __device__ __forceinline__ int next(bool (&mine)[RT]) {
         if (!todo) return -1;
-        const int at = __builtin_amdgcn_readlane(id, __builtin_ctz(todo));
-        mine = has && id == at;
-        todo &= ~(unsigned) __ballot(mine);
+        const int b = __builtin_ctz(todo);
+        int at = __builtin_amdgcn_readlane(id[0], b & 15);
+        if constexpr (RT == 2)
+            if (b > 15) at = __builtin_amdgcn_readlane(id[1], b & 15);
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            mine[t] = has[t] && id[t] == at;
+            todo &= ~(((unsigned) __ballot(mine[t]) & 0xffffu) << 16 * t);
+        }
         return at;
     }
 };
@@ -79,227 +97,360 @@ __device__ __forceinline__ int rank_of(const LoraArgs & a, int id) { return a.ra
 
 constexpr int LW = 8; // waves of a workgroup of k_lora_down
 
+constexpr bool scaled(int xf, int wf) { return xf == W4_UNITS || (wf == DT_F16 && xf != DT_F16); } // a step's result has a factor of its own
+constexpr int x_parts(int xf, int wf) { return xf == DT_F32 ? (wf == DT_F16 ? 2 : 3) : xf == DT_F16 && wf != DT_F16 ? 2 : 1; }
+
 // u[chunk][m][i] = sum over the chunk's k of A[ids[m]][i][k] x[m][k].  A workgroup per (tile, adapter's place, chunk); its waves take every
-// LW-th step of 32 values each and add up in LDS; NT tiles of 16 ranks at a time.
-template <int XF, int WF, int NT> __global__ __launch_bounds__(LW * 64) void k_lora_down(LoraArgs a) {
-    constexpr bool F16 = f16_mfma(XF, WF), UNITS = XF == W4_UNITS;
-    constexpr int PX = x_parts(XF, WF), PW = w_parts(XF, WF), U = NT == 1 ? 4 : 2;
+// LW-th pair of steps of 32 values each (a cache line of every row), one or two pairs' loads at a time, and add up in LDS; NT tiles of 16 ranks
+// at a time.
+template <int XF, int WF, int NT, int RT> __global__ __launch_bounds__(LW * 64) void k_lora_down(LoraArgs a) {
+    constexpr bool UNITS = XF == W4_UNITS, SCALED = scaled(XF, WF);
+    constexpr int PX = x_parts(XF, WF), U = NT == 4 ? 2 : 4; // (registers for two workgroups a CU)
     constexpr int XT = UNITS ? DT_F16 : XF; // (units: not used)
-    __shared__ __attribute__((aligned(16))) float red[LW * NT * 256];
+    __shared__ __attribute__((aligned(16))) float red[LW * RT * NT * 256];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int row0 = blockIdx.x * 16, row = row0 + n, nb = a.k >> 5;
-    const int s0 = (int) ((long long) nb * blockIdx.z / a.chunks), s1 = (int) ((long long) nb * (blockIdx.z + 1) / a.chunks);
-    Adapters ad(a, row);
-    bool mine;
+    const int row0 = blockIdx.x * 16 * RT, row = row0 + n, nb = a.k >> 5, np = (nb + 1) >> 1;
+    const int p0 = (int) ((long long) np * blockIdx.z / a.chunks), p1 = (int) ((long long) np * (blockIdx.z + 1) / a.chunks);
+    Adapters<RT> ad(a, row);
+    bool mine[RT];
     int place = 0;
     for (int id = ad.next(mine); id >= 0; id = ad.next(mine), place++) {
-        if (place % a.slots != (int) blockIdx.y) continue;
+        if (a.slots > 1 && place != (int) blockIdx.y) continue; // (as many places as a tile has rows, or one workgroup for all)
         const int rk = rank_of(a, id);
         for (int t0 = 0; t0 < rk; t0 += 16 * NT) {
             const uint16_t * wp = static_cast<const uint16_t *>(a.a) + (size_t) id * a.rank * a.k;
-            f32x4 acc[NT];
+            f32x4 acc[RT][NT];
 #pragma unroll
-            for (int t = 0; t < NT; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-            for (int s = s0 + wave; s < s1; s += LW * U) {
+            for (int q = 0; q < RT; q++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) acc[q][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int p = p0 + wave; p < p1; p += LW * (U / 2)) {
                 u32x4 w[U][NT];
-                typename Elem<XT>::Raw8 xr[U];
-                u32x2 xq[U];
-                float xd[U];
+                typename Elem<XT>::Raw8 xr[U][RT];
+                u32x2 xq[U][RT];
+                float xd[U][RT];
+                const auto step = [&](int u) { return 2 * (p + LW * (u >> 1)) + (u & 1); };
+                const auto in = [&](int u) { return p + LW * (u >> 1) < p1 && step(u) < nb; };
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    const int st = s + LW * u;
-                    if (st >= s1) break;
+                    if (!in(u)) continue;
+                    const int st = step(u);
 #pragma unroll
                     for (int t = 0; t < NT; t++)
                         if (t0 + 16 * t < rk) // (ranks past the last one: its row again, not stored)
                             w[u][t] = __builtin_bit_cast(u32x4, *reinterpret_cast<const u16x8_u *>(wp + (size_t) min(t0 + 16 * t + n, rk - 1) * a.k + 32 * st + 8 * g));
-                    xr[u] = typename Elem<XT>::Raw8{};
-                    xq[u] = u32x2{0, 0};
-                    xd[u] = 0.f;
-                    if (mine) {
+#pragma unroll
+                    for (int q = 0; q < RT; q++) {
+                        xr[u][q] = typename Elem<XT>::Raw8{};
+                        xq[u][q] = u32x2{0, 0};
+                        xd[u][q] = 0.f;
+                        if (!mine[q]) continue;
+                        const int r = row + 16 * q;
                         if constexpr (UNITS) {
-                            const size_t unit = (size_t) row * nb + (st & ~1);
-                            xq[u] = *reinterpret_cast<const u32x2 *>((st & 1 ? a.xb : a.xa) + (unit + (g >> 1)) * 16 + 8 * (g & 1));
-                            xd[u] = h2f_bits(a.xmeta[unit * 4 + (st & 1)]);
-                        } else xr[u] = Elem<XT>::raw8(static_cast<const typename Elem<XT>::T *>(a.x) + row * a.x_stride + 32 * st + 8 * g);
+                            const size_t unit = (size_t) r * nb + (st & ~1);
+                            xq[u][q] = *reinterpret_cast<const u32x2 *>((st & 1 ? a.xb : a.xa) + (unit + (g >> 1)) * 16 + 8 * (g & 1));
+                            xd[u][q] = h2f_bits(a.xmeta[unit * 4 + (st & 1)]);
+                        } else xr[u][q] = Elem<XT>::raw8(static_cast<const typename Elem<XT>::T *>(a.x) + r * a.x_stride + 32 * st + 8 * g);
                     }
                 }
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    if (s + LW * u >= s1) break;
-                    u32x4 xp[PX];
-                    if constexpr (UNITS) {
-                        float v[8];
+                    if (!in(u)) continue;
 #pragma unroll
-                        for (int i = 0; i < 8; i++) v[i] = (float) (int8_t) (xq[u][i >> 2] >> 8 * (i & 3));
-                        if constexpr (F16) {
-                            half8 h;
-#pragma unroll
-                            for (int i = 0; i < 8; i++) h[i] = (_Float16) v[i];
-                            xp[0] = __builtin_bit_cast(u32x4, h);
-                        } else split<1>(v, xp); // (7 bits and a sign: exact)
-                    } else if constexpr (PX == 1) xp[0] = __builtin_bit_cast(u32x4, xr[u]);
-                    else {
-                        float v[8];
-                        Elem<XT>::open8(xr[u], v);
-                        split<PX>(v, xp);
-                    }
-#pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        if (t0 + 16 * t >= rk) break;
-                        u32x4 p[PW];
-                        open_w<WF>(w[u][t], p);
-                        f32x4 c = UNITS ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[t];
-                        // small parts first; the third of x times the second of A is below 2^-24 of the product
-#pragma unroll
-                        for (int q = PW - 1; q >= 0; q--)
-#pragma unroll
-                            for (int i = PX - 1; i >= 0; i--)
-                                if (i + q <= 2) c = mfma32<F16>(p[q], xp[i], c);
+                    for (int q = 0; q < RT; q++) {
+                        u32x4 xp[PX];
+                        float d = xd[u][q];
                         if constexpr (UNITS) {
+                            float v[8];
 #pragma unroll
-                            for (int r = 0; r < 4; r++) acc[t][r] = __builtin_fmaf(xd[u], c[r], acc[t][r]);
-                        } else acc[t] = c;
+                            for (int i = 0; i < 8; i++) v[i] = (float) (int8_t) (xq[u][q][i >> 2] >> 8 * (i & 3));
+                            if constexpr (WF == DT_F16) {
+                                half8 h;
+#pragma unroll
+                                for (int i = 0; i < 8; i++) h[i] = (_Float16) v[i];
+                                xp[0] = __builtin_bit_cast(u32x4, h);
+                            } else split_bf16<1>(v, xp); // (7 bits and a sign: exact)
+                        } else if constexpr (SCALED) {
+                            float v[8];
+                            Elem<XT>::open8(xr[u][q], v);
+                            d = split_f16<PX>(v, row_top(Elem<XT>::top8(xr[u][q])), xp);
+                        } else if constexpr (PX == 1) xp[0] = __builtin_bit_cast(u32x4, xr[u][q]);
+                        else {
+                            float v[8];
+                            Elem<XT>::open8(xr[u][q], v);
+                            split_bf16<PX>(v, xp);
+                        }
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            if (t0 + 16 * t >= rk) continue;
+                            f32x4 c = SCALED ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[q][t];
+#pragma unroll
+                            for (int i = PX - 1; i >= 0; i--) c = mfma32<WF>(w[u][t], xp[i], c); // (small parts first)
+                            if constexpr (SCALED) {
+#pragma unroll
+                                for (int r = 0; r < 4; r++) acc[q][t][r] = __builtin_fmaf(d, c[r], acc[q][t][r]);
+                            } else acc[q][t] = c;
+                        }
                     }
                 }
             }
             __syncthreads(); // (the sums before are read)
 #pragma unroll
-            for (int t = 0; t < NT; t++) *reinterpret_cast<f32x4 *>(red + ((wave * NT + t) * 16 + n) * 16 + 4 * g) = acc[t];
+            for (int q = 0; q < RT; q++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) *reinterpret_cast<f32x4 *>(red + (((wave * RT + q) * NT + t) * 16 + n) * 16 + 4 * g) = acc[q][t];
             __syncthreads();
             // rows of the adapter, one of its ranks a thread
-            const unsigned of = (unsigned) __ballot(mine) & 0xffffu;
-            for (int i = threadIdx.x; i < NT * 256; i += LW * 64) {
-                const int m = i >> 4 & 15, r = t0 + (i >> 8) * 16 + (i & 15);
-                if (!(of >> m & 1) || r >= rk) continue;
+            unsigned of[RT];
+#pragma unroll
+            for (int q = 0; q < RT; q++) of[q] = (unsigned) __ballot(mine[q]) & 0xffffu;
+            for (int i = threadIdx.x; i < RT * NT * 256; i += LW * 64) {
+                const int q = RT == 1 ? 0 : i / (NT * 256), m = i >> 4 & 15, r = t0 + (i >> 8) % NT * 16 + (i & 15);
+                if (!((q ? of[RT - 1] : of[0]) >> m & 1) || r >= rk) continue;
                 float v = 0.f;
 #pragma unroll
-                for (int w = 0; w < LW; w++) v += red[w * NT * 256 + i];
-                a.u[((size_t) blockIdx.z * a.rows + row0 + m) * a.rp + r] = v;
+                for (int w = 0; w < LW; w++) v += red[w * RT * NT * 256 + i];
+                a.u[((size_t) blockIdx.z * a.rows + row0 + 16 * q + m) * a.rp + r] = v;
             }
         }
     }
 }
 
-constexpr int UW = 4; // waves of a workgroup of k_lora_up
+constexpr int UW = 4, UP_WAVES = 3072; // waves of a workgroup of k_lora_up; of its grid, where the groups of columns are more
 
-// y = base + s B u: a wave takes CT tiles of 16 columns of a tile of 16 rows; the adapters of the tile split its rows.  u in three bf16
-// parts, whose products with B add up in fp32 (fp16 B: two parts).
-template <int WF, int CT> __global__ __launch_bounds__(UW * 64) void k_lora_up(LoraArgs a) {
-    constexpr int PW = WF == DT_F16 ? 2 : 1;
+// y = base + s B u: a wave has u of a tile's rows in registers (KH x 32 ranks of it; ranks past 64: 64 at a time, of every group anew) and takes
+// its share of the groups of CT x 16 columns, the next group's B and base on their way.
+template <int WF, int CT, int RT, int KH, bool BIG> __global__ __launch_bounds__(UW * 64) void k_lora_up(LoraArgs a) {
+    constexpr int PU = WF == DT_F16 ? 2 : 3;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int row = blockIdx.y * 16 + n, c0 = (blockIdx.x * UW + wave) * CT * 16;
-    if (c0 >= a.n) return;
-    Adapters ad(a, row);
-    // y of the lane's row, columns c0 + 16 t + 4 g on
-    const auto store = [&](const f32x4 (&acc)[CT]) {
+    const int row = blockIdx.y * 16 * RT + n, waves0 = gridDim.x * UW, wave0 = blockIdx.x * UW + wave, groups = (a.n + 16 * CT - 1) / (16 * CT);
+    Adapters<RT> ad(a, row);
+    // y of rows row + 16 q, four columns from c on
+    const auto load = [&](int q, int c) {
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (!a.base) return v;
+        const float * b = a.base + (row + 16 * q) * a.base_stride + c;
+        if (c + 4 <= a.n) return f32x4(*reinterpret_cast<const f32x4_u *>(b));
 #pragma unroll
-        for (int t = 0; t < CT; t++) {
-            const int c = c0 + 16 * t + 4 * g;
-            float * y = a.y + row * a.y_stride + c;
-            const float * b = a.base ? a.base + row * a.base_stride + c : nullptr;
-            if (c + 4 <= a.n) {
-                f32x4 v = acc[t];
-                if (b) v += *reinterpret_cast<const f32x4_u *>(b);
-                *reinterpret_cast<f32x4_u *>(y) = v;
-            } else {
+        for (int i = 0; i < 4; i++)
+            if (c + i < a.n) v[i] = b[i];
+        return v;
+    };
+    const auto store = [&](int q, int c, f32x4 v) {
+        float * y = a.y + (row + 16 * q) * a.y_stride + c;
+        if (c + 4 <= a.n) *reinterpret_cast<f32x4_u *>(y) = v;
+        else {
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (c + i < a.n) y[i] = b ? b[i] + acc[t][i] : acc[t][i];
-            }
+            for (int i = 0; i < 4; i++)
+                if (c + i < a.n) y[i] = v[i];
         }
     };
-    f32x4 acc[CT];
-    if (blockIdx.z == 0 && row < a.rows && !ad.has) {
+    // the tile's adapters share its waves: wave w has the (w mod D)-th of D, and those that have it share the columns
+    bool mine[RT];
+    int adapters = 0;
+    for (Adapters<RT> all = ad; all.next(mine) >= 0;) adapters++;
+    const int own = adapters ? wave0 % adapters : 0, first = adapters <= waves0 ? (adapters ? wave0 / adapters : wave0) : 0;
+    const int step = adapters <= waves0 ? (adapters ? (waves0 - own + adapters - 1) / adapters : waves0) : 1;
+    // rows without an adapter: base as it is
+    if (a.base != a.y) {
 #pragma unroll
-        for (int t = 0; t < CT; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        store(acc);
+        for (int q = 0; q < RT; q++) {
+            const bool none = row + 16 * q < a.rows && !ad.has[q];
+            if (!__ballot(none)) continue;
+            for (int cg = wave0; cg < groups; cg += waves0)
+#pragma unroll
+                for (int t = 0; t < CT; t++)
+                    if (none) store(q, cg * 16 * CT + 16 * t + 4 * g, load(q, cg * 16 * CT + 16 * t + 4 * g));
+        }
     }
-    bool mine;
     int place = 0;
     for (int id = ad.next(mine); id >= 0; id = ad.next(mine), place++) {
-        if (place % a.slots != (int) blockIdx.z) continue;
+        if (adapters <= waves0 ? place != own : place % waves0 != wave0) continue;
         const int rk = rank_of(a, id);
         const float sc = a.scales ? a.scales[id] : 1.f;
         const uint16_t * bp = static_cast<const uint16_t *>(a.b) + (size_t) id * a.n * a.rank;
+        u32x4 up[RT][KH][PU];
+        float back[RT];
+        const auto parts = [&](int r0) { // ranks r0 .. r0 + 32 KH - 1 of u
 #pragma unroll
-        for (int t = 0; t < CT; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int r0 = 0; r0 < rk; r0 += 32) {
-            const int r = r0 + 8 * g;
-            u32x4 raw[CT];
+            for (int q = 0; q < RT; q++) {
+                float v[KH][8];
+                unsigned top = 0;
 #pragma unroll
-            for (int t = 0; t < CT; t++) {
-                const uint16_t * p = bp + (size_t) min(c0 + 16 * t + n, a.n - 1) * a.rank + r;
-                raw[t] = u32x4{0, 0, 0, 0};
-                if (r + 8 <= rk) raw[t] = __builtin_bit_cast(u32x4, *reinterpret_cast<const u16x8_u *>(p));
-                else if (r < rk) {
-                    unsigned e[8];
+                for (int h = 0; h < KH; h++) {
+                    const int r = r0 + 32 * h + 8 * g;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) e[i] = r + i < rk ? p[i] : 0;
-                    raw[t] = u32x4{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
+                    for (int i = 0; i < 8; i++) v[h][i] = 0.f;
+                    if (mine[q] && r < a.rp) { // (rows of u are padded to 16 ranks; what lies past rk is left out below)
+                        const float * ur = a.u + (size_t) (row + 16 * q) * a.rp + r;
+                        const size_t chunk = (size_t) a.rows * a.rp;
+                        for (int c0 = 0; c0 < a.chunks; c0 += 4) { // (four loads, then their sums)
+                            f32x4 lo[4], hi[4];
+#pragma unroll
+                            for (int c = 0; c < 4; c++) {
+                                const float * p = ur + min(c0 + c, a.chunks - 1) * chunk;
+                                lo[c] = *reinterpret_cast<const f32x4 *>(p);
+                                hi[c] = *reinterpret_cast<const f32x4 *>(p + 4);
+                            }
+#pragma unroll
+                            for (int c = 0; c < 4; c++)
+                                if (c0 + c < a.chunks) {
+#pragma unroll
+                                    for (int i = 0; i < 4; i++) v[h][i] += lo[c][i], v[h][4 + i] += hi[c][i];
+                                }
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        v[h][i] = r + i < rk ? v[h][i] * sc : 0.f;
+                        top = max(top, __builtin_bit_cast(unsigned, v[h][i]) & 0x7fffffffu);
+                    }
+                }
+                back[q] = 1.f;
+                if constexpr (WF == DT_F16) {
+                    top = row_top(top);
+#pragma unroll
+                    for (int h = 0; h < KH; h++) back[q] = split_f16<PU>(v[h], top, up[q][h]);
+                } else {
+#pragma unroll
+                    for (int h = 0; h < KH; h++) split_bf16<PU>(v[h], up[q][h]);
                 }
             }
-            float v[8];
+        };
+        // 8 ranks of a row of B from r on, the elements past rk zeros; where the row ends before them its last 8 elements, moved down
+        const auto weights = [&](int cg, int r0, u32x4 (&raw)[CT][KH]) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = 0.f;
-            if (mine && r < rk) {
-                for (int c = 0; c < a.chunks; c++) { // (rows of u are padded to 16 ranks)
-                    const float * up = a.u + ((size_t) c * a.rows + row) * a.rp + r;
-                    const f32x4 lo = *reinterpret_cast<const f32x4 *>(up), hi = *reinterpret_cast<const f32x4 *>(up + 4);
+            for (int h = 0; h < KH; h++) {
+                const int r = r0 + 32 * h + 8 * g, over = max(r + 8 - a.rank, 0), left = rk - r;
+                u32x4 mask;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) v[i] += lo[i], v[4 + i] += hi[i];
+                for (int i = 0; i < 4; i++) mask[i] = left >= 2 * i + 2 ? ~0u : left == 2 * i + 1 ? 0xffffu : 0;
+#pragma unroll
+                for (int t = 0; t < CT; t++) {
+                    const uint16_t * p = bp + (size_t) min(cg * 16 * CT + 16 * t + n, a.n - 1) * a.rank + r;
+                    u32x4 v = {0, 0, 0, 0};
+                    if (a.rank < 8) {
+                        if (left > 0) {
+                            unsigned e[8];
+#pragma unroll
+                            for (int i = 0; i < 8; i++) e[i] = i < left ? p[i] : 0;
+                            v = u32x4{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
+                        }
+                    } else if (left > 0) {
+                        v = __builtin_bit_cast(u32x4, *reinterpret_cast<const u16x8_u *>(p - over));
+                        if (a.rank & 7) {
+                            if (over & 4) v = u32x4{v[2], v[3], 0, 0};
+                            if (over & 2) v = u32x4{v[1], v[2], v[3], 0};
+                            if (over & 1) v = u32x4{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+                        }
+                    }
+                    raw[t][h] = v & mask;
+                }
+            }
+        };
+        const auto bases = [&](int cg, f32x4 (&y)[RT][CT]) {
+#pragma unroll
+            for (int q = 0; q < RT; q++)
+#pragma unroll
+                for (int t = 0; t < CT; t++) y[q][t] = mine[q] ? load(q, cg * 16 * CT + 16 * t + 4 * g) : f32x4{0.f, 0.f, 0.f, 0.f};
+        };
+        const auto add = [&](int r0, const u32x4 (&raw)[CT][KH], f32x4 (&y)[RT][CT]) {
+#pragma unroll
+            for (int q = 0; q < RT; q++)
+#pragma unroll
+                for (int t = 0; t < CT; t++) {
+                    f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int h = KH - 1; h >= 0; h--) {
+                        if (r0 + 32 * h >= rk) continue;
+#pragma unroll
+                        for (int i = PU - 1; i >= 0; i--) c = mfma32<WF>(raw[t][h], up[q][h][i], c); // (small parts first)
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) y[q][t][i] = __builtin_fmaf(back[q], c[i], y[q][t][i]);
+                }
+        };
+        const auto stores = [&](int cg, const f32x4 (&y)[RT][CT]) {
+#pragma unroll
+            for (int q = 0; q < RT; q++)
+#pragma unroll
+                for (int t = 0; t < CT; t++)
+                    if (mine[q]) store(q, cg * 16 * CT + 16 * t + 4 * g, y[q][t]);
+        };
+        if (first >= groups) continue;
+        u32x4 raw[2][CT][KH];
+        f32x4 y[2][RT][CT];
+        if constexpr (BIG) {
+            for (int cg = first; cg < groups; cg += step) {
+                bases(cg, y[0]);
+                f32x4 sum[RT][CT] = {};
+                for (int r0 = 0; r0 < rk; r0 += 32 * KH) {
+                    weights(cg, r0, raw[0]);
+                    parts(r0);
+                    add(r0, raw[0], sum);
                 }
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = r + i < rk ? v[i] * sc : 0.f;
+                for (int q = 0; q < RT; q++)
+#pragma unroll
+                    for (int t = 0; t < CT; t++) y[0][q][t] += sum[q][t];
+                stores(cg, y[0]);
             }
-            u32x4 up[3];
-            split<3>(v, up);
-#pragma unroll
-            for (int t = 0; t < CT; t++) {
-                u32x4 p[PW];
-                open_w<WF>(raw[t], p);
-#pragma unroll
-                for (int q = PW - 1; q >= 0; q--)
-#pragma unroll
-                    for (int i = 2; i >= 0; i--)
-                        if (i + q <= 2) acc[t] = mfma32<false>(p[q], up[i], acc[t]);
+        } else {
+            weights(first, 0, raw[0]);
+            bases(first, y[0]);
+            parts(0);
+            const auto group = [&](int cg, int b) {
+                const int next = min(cg + step, groups - 1); // (behind the last group of all: that once more, unused)
+                weights(next, 0, raw[b ^ 1]);
+                bases(next, y[b ^ 1]);
+                add(0, raw[b], y[b]);
+                stores(cg, y[b]);
+            };
+            for (int cg = first; cg < groups; cg += 2 * step) {
+                group(cg, 0);
+                if (cg + step < groups) group(cg + step, 1);
             }
         }
-        if (mine) store(acc);
     }
 }
 
-template <int XF, int WF> hipError_t down(const LoraArgs & a, hipStream_t st) {
-    const dim3 grid((a.rows + 15) / 16, a.slots, a.chunks), block(LW * 64);
-    return a.rank <= 16 ? launch(k_lora_down<XF, WF, 1>, grid, block, 0, st, a) : launch(k_lora_down<XF, WF, 4>, grid, block, 0, st, a);
+template <int XF, int WF, int RT> hipError_t down(const LoraArgs & a, hipStream_t st) {
+    const dim3 grid((a.rows + 16 * RT - 1) / (16 * RT), a.slots, a.chunks), block(LW * 64);
+    return a.rank <= 16 ? launch(k_lora_down<XF, WF, 1, RT>, grid, block, 0, st, a) : a.rank <= 32 ? launch(k_lora_down<XF, WF, 2, RT>, grid, block, 0, st, a)
+                                                                                               : launch(k_lora_down<XF, WF, 4, RT>, grid, block, 0, st, a);
 }
-template <int WF, int CT> hipError_t up(const LoraArgs & a, hipStream_t st) {
-    return launch(k_lora_up<WF, CT>, dim3((a.n + 16 * CT * UW - 1) / (16 * CT * UW), (a.rows + 15) / 16, a.slots), dim3(UW * 64), 0, st, a);
+template <int WF, int CT, int RT> hipError_t up(const LoraArgs & a, hipStream_t st) {
+    const int tiles = (a.rows + 16 * RT - 1) / (16 * RT), groups = (a.n + 16 * CT - 1) / (16 * CT);
+    const int waves = std::max(1, (int) std::min<long long>((long long) groups * std::min(a.rows, 16 * RT), UP_WAVES / tiles));
+    const dim3 grid((waves + UW - 1) / UW, tiles), block(UW * 64);
+    return a.rank <= 32 ? launch(k_lora_up<WF, CT, RT, 1, false>, grid, block, 0, st, a) : a.rank <= 64 ? launch(k_lora_up<WF, CT, RT, 2, false>, grid, block, 0, st, a)
+                                                                                          : launch(k_lora_up<WF, CT, RT, 2, true>, grid, block, 0, st, a);
+}
+template <int WF, int RT> hipError_t run(const LoraArgs & a, int xform, hipStream_t st) {
+    const hipError_t e = xform == W4_UNITS ? down<W4_UNITS, WF, RT>(a, st) : xform == DT_F32 ? down<DT_F32, WF, RT>(a, st) : xform == DT_F16 ? down<DT_F16, WF, RT>(a, st) : down<DT_BF16, WF, RT>(a, st);
+    if (e != hipSuccess) return e;
+    if constexpr (RT == 2) return up<WF, 2, 2>(a, st);
+    else {
+        // 32 columns a wave, a cache line of a row, where that leaves a wave for every SIMD
+        const bool wide = (long long) ((a.n + 31) / 32) * ((a.rows + 15) / 16) >= 1024;
+        return wide ? up<WF, 2, 1>(a, st) : up<WF, 1, 1>(a, st);
+    }
 }
 
 } // namespace
 
 void lora_plan(LoraArgs & a) {
-    const int tiles = (a.rows + 15) / 16, steps = a.k / 32;
     a.rp = (a.rank + 15) / 16 * 16;
-    // few tiles: the adapters of a tile in workgroups of their own
+    // few rows: the adapters of a tile in workgroups of their own; many: tiles of 32 rows, which read A and B half as often
     a.slots = a.rows <= 256 ? std::min(16, std::max(a.rows, 1)) : 1;
-    // and k in chunks, of at least four steps a wave, until two workgroups a CU have work
-    const int busy = std::max(1, tiles * a.slots);
-    a.chunks = std::max(1, std::min({LORA_MAX_CHUNKS, 512 / busy, steps / (4 * LW)}));
+    const int rt = a.rows <= 256 ? 1 : 2, tiles = (a.rows + 16 * rt - 1) / (16 * rt), pairs = (a.k / 32 + 1) / 2;
+    // and k in chunks, of at least two pairs of steps a wave, until two workgroups a CU have work
+    a.chunks = std::max(1, std::min({LORA_MAX_CHUNKS, 512 / std::max(1, tiles * a.slots), pairs / (2 * LW)}));
 }
 
 hipError_t launch_lora(const LoraArgs & a, int xform, int wtype, hipStream_t st) {
-    hipError_t e;
-    if (wtype == DT_F16)
-        e = xform == W4_UNITS ? down<W4_UNITS, DT_F16>(a, st) : xform == DT_F32 ? down<DT_F32, DT_F16>(a, st) : xform == DT_F16 ? down<DT_F16, DT_F16>(a, st) : down<DT_BF16, DT_F16>(a, st);
-    else
-        e = xform == W4_UNITS ? down<W4_UNITS, DT_BF16>(a, st) : xform == DT_F32 ? down<DT_F32, DT_BF16>(a, st) : xform == DT_F16 ? down<DT_F16, DT_BF16>(a, st) : down<DT_BF16, DT_BF16>(a, st);
-    if (e != hipSuccess) return e;
-    // 64 columns a wave where that leaves a wave for every SIMD
-    const bool wide = (long long) ((a.n + 63) / 64) * ((a.rows + 15) / 16) >= 1024;
-    if (wtype == DT_F16) return wide ? up<DT_F16, 4>(a, st) : up<DT_F16, 1>(a, st);
-    return wide ? up<DT_BF16, 4>(a, st) : up<DT_BF16, 1>(a, st);
+    if (wtype == DT_F16) return a.rows <= 256 ? run<DT_F16, 1>(a, xform, st) : run<DT_F16, 2>(a, xform, st);
+    return a.rows <= 256 ? run<DT_BF16, 1>(a, xform, st) : run<DT_BF16, 2>(a, xform, st);
 }
 
 } // namespace qkv
