@@ -311,8 +311,9 @@ int mk_verify_drafts(int n_seq, int n_draft, int vocab, const void * target, lon
  *   scales   fp32 [n_adapters] or NULL (1); ids int [rows], in any order
  *   base     fp32 [rows][base_stride] or NULL (0); may be y itself: added in place, behind mk_w4_units / mk_w4_rows
  * x: plain rows (k a multiple of 32) or int8 units (of 64), k up to 2^20; n 1..2^24, rows 0..2^19, rows n up to 2^35.  Products are exact
- * to 2^-23 and added in fp32; A x is rounded to fp32 (and taken to 2^-24).  An infinity or a NaN of x reaches its row alone, one of an
- * adapter the rows of that adapter alone (where it may be a NaN in place of an infinity).
+ * to 2^-23 and added in fp32; A x is rounded to fp32 (with fp16 adapters values of x and A x are exact to 2^-39 of the largest of 32, and
+ * of 64, beside them).  An infinity or a NaN of x reaches its row alone, one of an adapter the rows of that adapter alone (where it may be a
+ * NaN in place of an infinity).
  */
 long long mk_lora_ws(int rows, int k, int rank);
 int mk_lora_rows(int rows, int n, int k, int n_adapters, int rank, const void * a, const void * b, int ab_dtype, const int * ranks, const float * scales,
@@ -324,8 +325,8 @@ int mk_lora_units(int rows, int n, int k, int n_adapters, int rank, const void *
 
 /*
  * The router of a mixture of experts: logits[m] = x[m] W^T (W [n_experts][dim] of w_dtype, summed in 64 bits and rounded to fp32 once, as the
- * choice compares values that lie close), the top_k experts of each row and their weights.  rows 0..2^19, dim 1..2^17,
- * n_experts 1..1024, top_k 1..16.
+ * choice compares values that lie close; of 1024 rows and more of 16-bit x and W those that cannot change the choice may be sums in fp32),
+ * the top_k experts of each row and their weights.  rows 0..2^19, dim 1..2^17, n_experts 1..1024, top_k 1..16.
  *   form     0: weights are softmax(logits) of the chosen ones, 1: softmax over the chosen ones, 2: sigmoid(logits), 3: sigmoid(logits) over
  *            the chosen ones' sum; all times scale
  *   bias     fp32 [n_experts] or NULL: forms 2 and 3 choose by sigmoid(logits) + bias; else by the logits
@@ -344,8 +345,8 @@ int mk_moe_route(int rows, int dim, int n_experts, int top_k, const void * x, lo
  *   ids         int [rows][top_k], weights fp32 [rows][top_k] (of mk_moe_route, or a caller's own); ids that are no expert are left out
  *   y           [rows][y_stride]: of x's type, for units fp32
  * dim a multiple of 32 (units: 64), at most 16384; inner of 32, at most 32768; n_experts 1..1024, top_k 1..16.  x and h enter as integers
- * of their block of 32 values: int8 units as they are, fp32 rows (and the h of both) to 2^-21 of the block's largest value, fp16 and bf16
- * rows (and their h) to 2^-13; sums in fp32.  A row of x with an infinity or a NaN gives NaNs in that row of y alone.
+ * of their block of 32 values (of plain rows and h as many as the group): int8 units as they are, fp32 rows (and the h of both) to 2^-21 of the
+ * block's largest value, fp16 and bf16 rows (and their h) to 2^-13; sums in fp32.  A row of x with an infinity or a NaN gives NaNs in that row of y alone.
  * mk_moe_layer is mk_moe_route on the same rows and mk_moe_rows on its choice, in one call; mk_moe_ws covers all three calls.
  */
 long long mk_moe_ws(int rows, int dim, int inner, int n_experts, int top_k);

@@ -287,8 +287,7 @@ int mk_moe_route(int rows, int dim, int n_experts, int top_k, const void * x, lo
         const Device d(stream);
         hold_route(d, a);
         if (want) d.holds(ws, "ws");
-        ck(launch_logits(a, dtype, w_dtype, static_cast<hipStream_t>(stream)), "route");
-        ck(launch_pick(a, static_cast<hipStream_t>(stream)), "route");
+        ck(launch_route(a, dtype, w_dtype, static_cast<hipStream_t>(stream)), "route");
         return 0;
     });
 }
@@ -359,8 +358,10 @@ int mk_moe_layer(int rows, int dim, int inner, int n_experts, int top_k, int gro
         hold_route(d, r);
         hold_moe(d, a);
         d.holds(ws, "ws");
-        ck(launch_logits(r, dtype, router_dtype, static_cast<hipStream_t>(stream)), "route");
-        ck(launch_moe(a, dtype, &r, static_cast<hipStream_t>(stream)), "moe");
+        // (of a few rows the choice is made where x is made ready)
+        const bool few = rows <= MOE_ROWS && n_experts <= MOE_PICK;
+        ck(few ? launch_logits(r, dtype, router_dtype, static_cast<hipStream_t>(stream)) : launch_route(r, dtype, router_dtype, static_cast<hipStream_t>(stream)), "route");
+        ck(launch_moe(a, dtype, few ? &r : nullptr, static_cast<hipStream_t>(stream)), "moe");
         return 0;
     });
 }

@@ -41,11 +41,13 @@ struct RouteArgs {
     int rows, dim, n_experts, top_k, form;
     float scale;
     int chunks;         // (set by route_plan) parts of dim with partial sums of their own
+    int buffers;        // (set by the launcher) of values in LDS
 };
 constexpr int ROUTE_MAX_EXPERTS = 1024, ROUTE_MAX_TOP = 16, ROUTE_MAX_ROWS = 1 << 19, ROUTE_MAX_DIM = 1 << 17, ROUTE_MAX_CHUNKS = 8;
 void route_plan(RouteArgs & a);
-hipError_t launch_logits(const RouteArgs & a, int dtype, int wtype, hipStream_t st);
-hipError_t launch_pick(const RouteArgs & a, hipStream_t st);
+hipError_t launch_route(const RouteArgs & a, int dtype, int wtype, hipStream_t st);
+hipError_t launch_logits(const RouteArgs & a, int dtype, int wtype, hipStream_t st); // its parts: logits, or their partial sums, ...
+hipError_t launch_pick(const RouteArgs & a, hipStream_t st);                         // ... and the choice
 
 // 4-bit weights of every expert: codes [n_experts][n][k / 2], scales and minimums [n_experts][n][gs]
 struct MoeWeights {
@@ -74,10 +76,11 @@ struct MoeArgs {
     // (set by the launcher) tokens of an expert that a pass holds in LDS, runs of k that it holds at a time, and waves (1 << ..) that split k
     int tp_up, tp_down, cr_up, cr_down, ks_up, ks_down;
 };
-constexpr int MOE_ROWS = 64;   // rows of a launch; a call of more runs them one after another
+constexpr int MOE_ROWS = 64, MOE_PICK = 256; // rows of a run; a call of more runs them one after another; experts that it can choose from itself
 constexpr int MOE_MAX_ROWS = 4096, MOE_MAX_DIM = 16384, MOE_MAX_INNER = 32768;
 long long moe_plan(MoeArgs & a, int xform, uint8_t * ws); // -> bytes of workspace
-// route: the router whose logits' partial sums are there, and whose choice is ids and weights (null: these are given)
+// route: the router whose logits, or their partial sums, are there and whose choice is ids and weights (null: these are given); at most MOE_ROWS
+// rows and MOE_PICK experts
 hipError_t launch_moe(const MoeArgs & a, int xform, const RouteArgs * route, hipStream_t st);
 
 } // namespace qkv

@@ -680,11 +680,6 @@ template <int XF> static hipError_t prep(const MoeArgs & a, const RouteArgs * ro
 
 hipError_t launch_moe(const MoeArgs & all, int xform, const RouteArgs * route, hipStream_t st) {
     const int xs = xform == DT_F32 ? 4 : 2, ys = xform == DT_F16 || xform == DT_BF16 ? 2 : 4, nb = all.dim / 32;
-    if (route && (all.rows > MOE_ROWS || all.n_experts > 256)) {
-        const hipError_t e = launch_pick(*route, st);
-        if (e != hipSuccess) return e;
-        route = nullptr;
-    }
     for (int row = 0; row < all.rows; row += MOE_ROWS) {
         MoeArgs a = all;
         a.rows = std::min(MOE_ROWS, all.rows - row);

@@ -26,30 +26,15 @@ __device__ __forceinline__ uint64_t order64(double v) {
 }
 __device__ __forceinline__ double sigmoid_d(double v) { return 1.0 / (1.0 + exp(-v)); }
 
-// Row `row`'s top_k experts and their weights; lane j returns the j-th expert (j < top_k).  Lane l holds experts V l .. V l + V - 1, so that of equal
-// keys the lowest index is the lowest lane's first.
-template <int V> __device__ __forceinline__ int route_pick(const RouteArgs & a, int row) {
+// the choice of one row from its logits in registers, lane l holding experts V l .. V l + V - 1 (of equal keys the lowest index is then the lowest
+// lane's first): lane j keeps the j-th, up to `most` of them
+template <int V> struct Chosen {
+    int expert;
+    float logit;
+};
+template <int V> __device__ __forceinline__ Chosen<V> route_choose(const RouteArgs & a, const float (&l)[V], int most) {
     const int lane = threadIdx.x & 63;
-    const size_t r0 = (size_t) row * a.n_experts;
-    float l[V];
     unsigned hi[V], lo[V]; // keys, 0 for no expert and for those taken; without a bias the logits' order alone
-    if (a.chunks > 1) {
-        double s[V];
-#pragma unroll
-        for (int i = 0; i < V; i++) s[i] = 0;
-#pragma unroll 4
-        for (int c = 0; c < a.chunks; c++)
-#pragma unroll
-            for (int i = 0; i < V; i++) s[i] += a.part[(size_t) c * a.rows * a.n_experts + r0 + min(lane * V + i, a.n_experts - 1)];
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            l[i] = (float) s[i];
-            if (lane * V + i < a.n_experts) a.logits[r0 + lane * V + i] = l[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; i++) l[i] = a.logits[r0 + min(lane * V + i, a.n_experts - 1)];
-    }
 #pragma unroll
     for (int i = 0; i < V; i++) {
         const int e = lane * V + i;
@@ -60,9 +45,8 @@ template <int V> __device__ __forceinline__ int route_pick(const RouteArgs & a, 
         } else hi[i] = order32(l[i]), lo[i] = 0;
         if (e >= a.n_experts) hi[i] = lo[i] = 0;
     }
-    int mine = 0;
-    float logit = 0.f;
-    for (int j = 0; j < a.top_k; j++) {
+    Chosen<V> c{0, 0.f};
+    for (int j = 0; j < most; j++) {
         unsigned h = hi[0], w = lo[0];
         int at = 0;
         float v = l[0];
@@ -80,8 +64,13 @@ template <int V> __device__ __forceinline__ int route_pick(const RouteArgs & a, 
 #pragma unroll
         for (int i = 0; i < V; i++)
             if (e == lane * V + i) hi[i] = lo[i] = 0;
-        if (lane == j) mine = e, logit = ve;
+        if (lane == j) c.expert = e, c.logit = ve;
     }
+    return c;
+}
+// its weights, and both to memory
+template <int V> __device__ __forceinline__ void route_weights(const RouteArgs & a, int row, const float (&l)[V], const Chosen<V> & c) {
+    const int lane = threadIdx.x & 63;
     const bool in = lane < a.top_k;
     double w;
     if (a.form == ROUTE_SOFTMAX) {
@@ -95,20 +84,46 @@ template <int V> __device__ __forceinline__ int route_pick(const RouteArgs & a, 
 #pragma unroll
         for (int i = 0; i < V; i++)
             if (lane * V + i < a.n_experts) sum += exp((double) l[i] - (double) top);
-        w = exp((double) logit - (double) top) / wave_sum(sum);
+        w = exp((double) c.logit - (double) top) / wave_sum(sum);
     } else if (a.form == ROUTE_CHOSEN) {
-        const float top = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, logit))); // (the first is the largest)
-        const double e = in ? exp((double) logit - (double) top) : 0.0;
+        const float top = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, c.logit))); // (the first is the largest)
+        const double e = in ? exp((double) c.logit - (double) top) : 0.0;
         w = e / wave_sum(e);
     } else {
-        w = in ? sigmoid_d(logit) : 0.0;
+        w = in ? sigmoid_d(c.logit) : 0.0;
         if (a.form == ROUTE_SIGMOID_NORM) w /= wave_sum(w);
     }
     if (in) {
-        a.ids[(size_t) row * a.top_k + lane] = mine;
+        a.ids[(size_t) row * a.top_k + lane] = c.expert;
         a.weights[(size_t) row * a.top_k + lane] = (float) (w * (double) a.scale);
     }
-    return mine;
+}
+
+// Row `row`'s top_k experts and their weights from the logits, or their partial sums; lane j returns the j-th expert (j < top_k).
+template <int V> __device__ __forceinline__ int route_pick(const RouteArgs & a, int row) {
+    const int lane = threadIdx.x & 63;
+    const size_t r0 = (size_t) row * a.n_experts;
+    float l[V];
+    if (a.chunks > 1) {
+        double s[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) s[i] = 0;
+#pragma unroll 4
+        for (int c = 0; c < a.chunks; c++)
+#pragma unroll
+            for (int i = 0; i < V; i++) s[i] += a.part[(size_t) c * a.rows * a.n_experts + r0 + min(lane * V + i, a.n_experts - 1)];
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            l[i] = (float) s[i];
+            if (lane * V + i < a.n_experts) a.logits[r0 + lane * V + i] = l[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) l[i] = a.logits[r0 + min(lane * V + i, a.n_experts - 1)];
+    }
+    const Chosen<V> c = route_choose<V>(a, l, a.top_k);
+    route_weights<V>(a, row, l, c);
+    return c.expert;
 }
 
 } // namespace qkv

@@ -34,7 +34,8 @@ def to_gpu(torch, v, name):
 # ------------------------------------------------------------------------------------------------ adapters
 def lora_ref(a, b, ranks, scales, ids, x, base, chunks):
     """a [na][r][k], b [na][n][r], x [rows][k] (float64) -> y and its bound.  A wave adds an eighth of a chunk's steps of 32 values, up to 5
-    products of parts each and 33 additions in each; then 8 waves and the chunks add up; what is left out of the products is below 2^-23 of them."""
+    products of parts each and 33 additions in each; then 8 waves and the chunks add up; what is left out of the products is below 2^-23 of them, and of the largest value of
+    x in a step (of u in 64 ranks) 2^-39 where those are made fp16."""
     rows, k = x.shape
     n, r = b.shape[1:]
     y, bound = np.zeros((rows, n)), np.zeros((rows, n))
@@ -46,9 +47,10 @@ def lora_ref(a, b, ranks, scales, ids, x, base, chunks):
             q = r if ranks is None else int(min(max(ranks[i], 0), r))
             s = 1.0 if scales is None else float(scales[i])
             A, B = a[i, :q], b[i, :, :q]
-            u, du = A @ x[m], down * STEP * (np.abs(A) @ np.abs(x[m]))
+            xs = np.abs(np.pad(x[m], (0, -k % 32))).reshape(-1, 32).max(1).repeat(32)[:k]
+            u, du = A @ x[m], np.abs(A) @ (down * STEP * np.abs(x[m]) + 2.0 ** -39 * xs)
             y[m] = s * (B @ u)
-            bound[m] = abs(s) * (np.abs(B) @ (du + up * STEP * (np.abs(u) + du)))
+            bound[m] = abs(s) * (np.abs(B) @ (du + up * STEP * (np.abs(u) + du) + 2.0 ** -39 * np.abs(u).max(initial=0)))
     if base is not None:
         y = y + base
     return y, bound + STEP * np.abs(y) + 1e-37
@@ -88,23 +90,24 @@ def w4_values(c, scales, mins, group):
     return w if mins is None else w + mins.astype(np.float64)[..., of]
 
 
-def _rounded(v, bits):
-    """How far an integer of v's block of 32 is off: half of the block's power of two times 2^-bits."""
-    b = np.abs(v).reshape(v.shape[0], -1, 32).max(-1)
+def _rounded(v, bits, block=32):
+    """How far an integer of v's block is off: half of the block's power of two times 2^-bits."""
+    k = v.shape[1]
+    b = np.abs(np.pad(v, ((0, 0), (0, -k % block)))).reshape(v.shape[0], -1, block).max(-1)
     with np.errstate(divide="ignore"):
         top = np.where(b > 0, 2.0 ** np.floor(np.log2(np.maximum(b, 1e-300))), 0)
-    return np.repeat(np.maximum(top, 2.0 ** -101), 32, 1) * 2.0 ** -(bits + 1)
+    return np.repeat(np.maximum(top, 2.0 ** -101), block, 1)[:, :k] * 2.0 ** -(bits + 1)
 
 
-def moe_ref(up, down, mags, x, xform, ids, weights, yname):
+def moe_ref(up, down, mags, x, xform, ids, weights, yname, group=32):
     """up [E][2 inner][dim], down [E][dim][inner] (float64), mags the sums of their terms' magnitudes (|scale (c - 8)| + |min|, of both),
-    x [rows][dim] -> y and its bound.  Rounding: x and h to 13 bits below their block's power of two (fp32: 21; h: 21 for
-    units too), every block's term to three steps, its addition and those of lanes and waves."""
+    x [rows][dim] -> y and its bound.  Rounding: x and h to 13 bits below the power of two of their block of `group` values, which
+    have one exponent (fp32: 21; h: 21 for units too), every block's term to three steps, its addition and those of lanes and waves."""
     rows, dim = x.shape
     inner = down.shape[2]
     xb, hb = {"units": (60, 21), "fp32": (21, 21)}.get(xform, (13, 13))
     ops = lambda k: (k // 32 + 24 + 4) * STEP
-    dxr = _rounded(x, xb)
+    dxr = _rounded(x, xb, group)
     y, bound = np.zeros((rows, dim)), np.zeros((rows, dim))
     for m in range(rows):
         for j, e in enumerate(ids[m]):
@@ -118,7 +121,7 @@ def moe_ref(up, down, mags, x, xform, ids, weights, yname):
             h = s * u
             ds = 1.1 * dg + 8 * STEP * np.abs(s)  # (the slope of silu is below 1.1; expf, a sum, a quotient)
             dh = ds * (np.abs(u) + du) + np.abs(s) * du + STEP * np.abs(h)
-            dh = dh + _rounded(((np.abs(h) + dh) * 1.0)[None], hb)[0]
+            dh = dh + _rounded(((np.abs(h) + dh) * 1.0)[None], hb, group)[0]
             o = down[e] @ h
             do = mags[1][e] @ (dh + ops(inner) * (np.abs(h) + dh))
             w = float(weights[m, j])

@@ -16,7 +16,7 @@ void route_plan(RouteArgs & a) { a.chunks = 2; }
 long long moe_plan(MoeArgs &, int, uint8_t *) { return 256; }
 hipError_t launch_lora(const LoraArgs &, int, int, hipStream_t st) { return launched(st); }
 hipError_t launch_logits(const RouteArgs &, int, int, hipStream_t st) { return launched(st); }
-hipError_t launch_pick(const RouteArgs &, hipStream_t st) { return launched(st); }
+hipError_t launch_route(const RouteArgs &, int, int, hipStream_t st) { return launched(st); }
 hipError_t launch_moe(const MoeArgs &, int, const RouteArgs *, hipStream_t st) { return launched(st); }
 } // namespace qkv
 

@@ -206,3 +206,19 @@ def test_far_offsets(qkv, torch_gpu):
     want = torch.zeros(1, n, device="cuda")
     want[0, n - 1] = 30
     assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("xform", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("wname", ["fp16", "bf16"])
+def test_wide_range(qkv, torch_gpu, xform, wname):
+    """Values whose size differs from step to step, and in one."""
+    rng = np.random.default_rng(9)
+    x = rng.standard_normal((33, 256)) * 2.0 ** rng.integers(-8, 5, (33, 8)).repeat(32, 1) * 2.0 ** rng.integers(-5, 3, (33, 256))
+    Case(torch_gpu, 33, 90, 256, 40, 3, xform, wname, x=x, seed=9).check(qkv)
+
+
+@pytest.mark.parametrize("wname", ["fp16", "bf16"])
+@pytest.mark.parametrize("rank", [64, 100, 256])
+def test_many_rows_long_ranks(qkv, torch_gpu, wname, rank):
+    """Tiles of 32 rows and more than one part of the ranks; runs of rows of one adapter, as of prompts."""
+    Case(torch_gpu, 530, 70, 64, rank, 4, "bf16", wname, ranks=True, ids=np.arange(530) // 130 - 1, seed=rank).check(qkv)

@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 
 
 class Case:
-    def __init__(self, torch, rows, dim, inner, e, top, group=32, mins=False, xform="bf16", ids=None, seed=0, pad=0, router=None):
+    def __init__(self, torch, rows, dim, inner, e, top, group=32, mins=False, xform="bf16", ids=None, seed=0, pad=0, router=None, x=None):
         rng = np.random.default_rng(seed)
         self.torch, self.rows, self.dim, self.inner, self.e, self.top, self.group, self.xform = torch, rows, dim, inner, e, top, group, xform
         self.w, self.dev, self.mags = [], [], []
@@ -23,7 +23,7 @@ class Case:
             self.mags.append(mag if m is None else mag + np.abs(m.astype(np.float64))[..., np.arange(k) // group])
             codes = pack_codes(c.reshape(e * n, k))
             self.dev.append([torch.from_numpy(codes).cuda(), torch.from_numpy(s).cuda(), None if m is None else torch.from_numpy(m).cuda()])
-        x = rng.standard_normal((rows, dim))
+        x = rng.standard_normal((rows, dim)) if x is None else x
         if xform == "units":
             u = units_of(x)
             q, sc, _ = unpack_units(*u)
@@ -66,7 +66,7 @@ class Case:
         return y
 
     def want(self):
-        return moe_ref(self.w[0], self.w[1], self.mags, self.xv, self.xform, self.ids, self.weights, self.yname)
+        return moe_ref(self.w[0], self.w[1], self.mags, self.xv, self.xform, self.ids, self.weights, self.yname, self.group)
 
     def check(self, qkv):
         y = self.run(qkv).double().cpu().numpy()
@@ -230,3 +230,32 @@ def test_far_offsets(qkv, torch_gpu):
     g = 12.0
     want = g / (1 + np.exp(-g)) * 6
     assert abs(float(y[0, dim - 1]) - want) <= 2.0 ** -20 * want and (y[0, :-1] == 0).all()
+
+
+@pytest.mark.parametrize("xform", FORMS[1:])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_wide_range(qkv, torch_gpu, xform, group):
+    """Values whose size differs from block to block, and in one: a block's small ones are off by its largest's steps."""
+    rng = np.random.default_rng(group)
+    size = 2.0 ** rng.integers(-9, 4, (6, 9)).repeat(32, 1) * 2.0 ** rng.integers(-3, 3, (6, 288))
+    Case(torch_gpu, 6, 288, 160, 4, 2, group, True, xform, x=rng.standard_normal((6, 288)) * size).check(qkv)
+
+
+@pytest.mark.parametrize("xform", FORMS)
+@pytest.mark.parametrize("group,mins", [(32, True), (128, False)])
+@pytest.mark.parametrize("dim,inner", [(8192, 32), (64, 6400)])
+def test_long_rows_of_many(qkv, torch_gpu, xform, group, mins, dim, inner):
+    """One expert's tokens past a workgroup's memory: k in parts."""
+    Case(torch_gpu, 40, dim, inner, 2, 1, group, mins, xform, ids=np.zeros((40, 1)), seed=dim).check(qkv)
+
+
+def test_layer_many_experts(qkv, torch_gpu):
+    """More experts than the choice beside the rows takes; runs of 64 rows."""
+    torch = torch_gpu
+    for rows in (3, 70):
+        c = Case(torch, rows, 96, 32, 300, 4, xform="bf16", seed=rows, router="bf16")
+        y = c.run(qkv, layer=True).clone()
+        c.ids, c.weights = c.chosen[0].cpu().numpy(), c.chosen[1].cpu().numpy()
+        ref, bound = c.want()
+        assert (np.abs(y.double().cpu().numpy() - ref) <= bound).all()
+        assert torch.equal(c.run(qkv), y)

@@ -82,6 +82,84 @@ def test_close(qkv, torch_gpu):
     assert np.array_equal(logits, rl) and np.array_equal(ids, ri)
 
 
+@pytest.mark.parametrize("name", ["fp16", "bf16"])
+@pytest.mark.parametrize("rows,dim,e,top,form", [(1024, 2048, 63, 6, 0), (1030, 64, 16, 16, 1), (2001, 96, 8, 1, 2), (1500, 512, 130, 8, 3), (1100, 1024, 256, 10, 1), (1025, 32, 1, 1, 0),
+                                                 (1040, 320, 72, 4, 2), (1024, 4096, 33, 16, 0)])
+@pytest.mark.parametrize("pad", [8, 3])  # (rows that do not start at 16 bytes are summed in 64 bits)
+def test_many(qkv, torch_gpu, name, rows, dim, e, top, form, pad):
+    """Many rows of 16-bit types: logits to the error of fp32 sums (a chain of dim / 32 instructions, of parts of dim fewer, each off by up to four half
+    steps of what it adds), the choice and its order as of 64-bit sums."""
+    rng = np.random.default_rng(rows + e)
+    x, xv = typed(rng.standard_normal((rows, dim)), name)
+    w, wv = typed(rng.standard_normal((e, dim)) / np.sqrt(dim), name)
+    x[5], xv[5] = 0, 0  # (a padded row)
+    logits, ids, wt = run(qkv, torch_gpu, x, name, w, name, None, form, 2.0, top, pad=pad)
+    exact = xv @ wv.T
+    bound = (dim // 32 + 40) * 2.0 ** -22 * np.linalg.norm(xv, axis=1)[:, None] * np.linalg.norm(wv, axis=1)
+    assert (np.abs(logits - exact) <= bound).all()
+    rl, ri, rw = route_ref(xv, wv, None, form, 2.0, top)
+    assert np.array_equal(ids, ri)
+    # the weights are those of the logits given: to their own rounding
+    _, _, gw = route_ref(logits.astype(np.float64), np.eye(e), None, form, 2.0, top)
+    assert (np.abs(wt - gw) <= 2.0 ** -23 * gw).all()
+
+
+@pytest.mark.parametrize("name", ["fp16", "bf16"])
+@pytest.mark.parametrize("e", [20, 100, 200])
+def test_many_close(qkv, torch_gpu, name, e):
+    """Experts whose logits differ past fp32's bits, equal ones among them: the choice is that of 64-bit sums, ties to the lowest index."""
+    rows, dim = 1200, 256
+    rng = np.random.default_rng(e)
+    xv = rng.integers(-64, 65, (rows, dim)).astype(np.float64)
+    xv[:, 1] = 2.0 ** -6
+    wv = np.tile(rng.integers(-64, 65, (1, dim)).astype(np.float64), (e, 1))
+    wv[:, 1] = rng.integers(-8, 9, e) * 2.0 ** -4  # logits of about 2^15 that differ by multiples of 2^-10
+    wv[::7, 0] += 3  # some apart from the others
+    x, xv = typed(xv, name)
+    w, wv = typed(wv, name)
+    logits, ids, _ = run(qkv, torch_gpu, x, name, w, name, None, 0, 1.0, 8)
+    rl, ri, _ = route_ref(xv, wv, None, 0, 1.0, 8)
+    assert np.array_equal(ids, ri)
+    assert np.array_equal(np.take_along_axis(logits, ids, 1), np.take_along_axis(rl, ids.astype(np.int64), 1))
+
+
+def test_many_small(qkv, torch_gpu):
+    """Rows and experts whose squares, and whose products, are below fp32's smallest."""
+    rows, dim, e = 1100, 256, 40
+    rng = np.random.default_rng(4)
+    xv = rng.integers(-64, 65, (rows, dim)).astype(np.float64)
+    xv[:, 1] = 2.0 ** -6
+    wv = np.tile(rng.integers(-64, 65, (1, dim)).astype(np.float64), (e, 1))
+    wv[:, 1] = rng.integers(-8, 9, e) * 2.0 ** -4
+    for by_x, by_w in ((-100, 0), (0, -100), (-70, -70), (60, 50)):
+        x, xt = typed(xv * 2.0 ** by_x, "bf16")
+        w, wt = typed(wv * 2.0 ** by_w, "bf16")
+        x[7] = xt[7] = 0
+        _, ids, _ = run(qkv, torch_gpu, x, "bf16", w, "bf16", None, 0, 1.0, 8)
+        assert np.array_equal(ids, route_ref(xt, wt, None, 0, 1.0, 8)[1])
+
+
+def test_many_not_finite(qkv, torch_gpu):
+    rng = np.random.default_rng(11)
+    x, xv = grid(rng, (1100, 96), "bf16")
+    w, wv = grid(rng, (33, 96), "bf16")
+    _, ri, _ = route_ref(xv, wv, None, 1, 1.0, 8)
+    bad = x.copy()
+    bad[3, 5], bad[4, 6], bad[5, :], bad[1099, 0] = 0x7f80, 0x7fc0, 0xff80, 0x7f80
+    _, ids, _ = run(qkv, torch_gpu, bad, "bf16", w, "bf16", None, 1, 1.0, 8)
+    for m in range(1100):
+        assert len(set(ids[m])) == 8 and (ids[m] >= 0).all() and (ids[m] < 33).all()
+        if m not in (3, 4, 5, 1099):
+            assert np.array_equal(ids[m], ri[m])
+    w2 = w.copy()
+    w2[7, 3] = 0x7fc0  # an expert of NaNs is below everything
+    _, ids, wt = run(qkv, torch_gpu, x, "bf16", w2, "bf16", None, 1, 1.0, 8)
+    assert not (ids == 7).any() and np.isfinite(wt).all()
+    w3, wv3 = w[[i for i in range(33) if i != 7]], wv[[i for i in range(33) if i != 7]]
+    _, r3, _ = route_ref(xv, wv3, None, 1, 1.0, 8)
+    assert np.array_equal(ids - (ids > 7), r3)
+
+
 def test_not_finite(qkv, torch_gpu):
     """Rows with infinities and NaNs: distinct experts all the same, other rows as without them."""
     rng = np.random.default_rng(9)

@@ -37,7 +37,7 @@ SIZE = 1 << 20
 CALLS = {
     "lora": (9, 1, lambda m, p, s: m.mk_lora_rows(1, 16, 64, 2, 8, p(0), p(1), 2, p(2), p(3), p(4), p(5), 64, 0, p(6), 16, p(7), 16, p(8), SIZE, s)),
     "lora_units": (11, 1, lambda m, p, s: m.mk_lora_units(1, 16, 64, 2, 8, p(0), p(1), 2, p(2), p(3), p(4), p(5), p(6), p(7), p(8), 16, p(9), 16, p(10), SIZE, s)),
-    "route": (7, 2, lambda m, p, s: m.mk_moe_route(1, 64, 8, 2, p(0), 64, 0, p(1), 0, p(2), 2, 1.0, p(3), p(4), p(5), p(6), SIZE, s)),
+    "route": (7, 1, lambda m, p, s: m.mk_moe_route(1, 64, 8, 2, p(0), 64, 0, p(1), 0, p(2), 2, 1.0, p(3), p(4), p(5), p(6), SIZE, s)),
     "rows": (11, 1, lambda m, p, s: m.mk_moe_rows(1, 64, 64, 8, 2, 32, p(0), p(1), p(2), p(3), p(4), p(5), p(6), 64, 0, p(7), p(8), p(9), 64, p(10), SIZE, s)),
     "units": (13, 1, lambda m, p, s: m.mk_moe_units(1, 64, 64, 8, 2, 32, p(0), p(1), p(2), p(3), p(4), p(5), p(6), p(7), p(8), p(9), p(10), p(11), 64, p(12), SIZE, s)),
     "layer": (14, 2, lambda m, p, s: m.mk_moe_layer(1, 64, 64, 8, 2, 32, p(0), p(1), p(2), p(3), p(4), p(5), p(6), 64, 0, p(7), 0, p(8), 3, 1.0, p(9), p(10), p(11), p(12), 64,
