@@ -12,6 +12,7 @@
 #include "step_mix_launch.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace qkv {
 namespace {
@@ -220,7 +221,7 @@ constexpr int UW = 4, UP_WAVES = 3072; // waves of a workgroup of k_lora_up; of 
 
 // y = base + s B u: a wave has u of a tile's rows in registers (KH x 32 ranks of it; ranks past 64: 64 at a time, of every group anew) and takes
 // its share of the groups of CT x 16 columns, the next group's B and base on their way.
-template <int WF, int CT, int RT, int KH, bool BIG> __global__ __launch_bounds__(UW * 64) void k_lora_up(LoraArgs a) {
+template <int WF, int CT, int RT, int KH, bool BIG> __global__ __launch_bounds__(UW * 64, 3) void k_lora_up(LoraArgs a) {
     constexpr int PU = WF == DT_F16 ? 2 : 3;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int row = blockIdx.y * 16 * RT + n, waves0 = gridDim.x * UW, wave0 = blockIdx.x * UW + wave, groups = (a.n + 16 * CT - 1) / (16 * CT);
@@ -269,6 +270,14 @@ template <int WF, int CT, int RT, int KH, bool BIG> __global__ __launch_bounds__
         const int rk = rank_of(a, id);
         const float sc = a.scales ? a.scales[id] : 1.f;
         const uint16_t * bp = static_cast<const uint16_t *>(a.b) + (size_t) id * a.n * a.rank;
+        // rows of others stand for the adapter's first one: loads, results and stores are the same, and no branch is in the loop, where the compiler
+        // would wait for the loads of the next group with this one's
+        unsigned rows = 0;
+#pragma unroll
+        for (int q = 0; q < RT; q++) rows |= ((unsigned) __ballot(mine[q]) & 0xffffu) << 16 * q;
+        long long at[RT];
+#pragma unroll
+        for (int q = 0; q < RT; q++) at[q] = mine[q] ? row + 16 * q : (int) blockIdx.y * 16 * RT + __builtin_ctz(rows);
         u32x4 up[RT][KH][PU];
         float back[RT];
         const auto parts = [&](int r0) { // ranks r0 .. r0 + 32 KH - 1 of u
@@ -281,8 +290,8 @@ template <int WF, int CT, int RT, int KH, bool BIG> __global__ __launch_bounds__
                     const int r = r0 + 32 * h + 8 * g;
 #pragma unroll
                     for (int i = 0; i < 8; i++) v[h][i] = 0.f;
-                    if (mine[q] && r < a.rp) { // (rows of u are padded to 16 ranks; what lies past rk is left out below)
-                        const float * ur = a.u + (size_t) (row + 16 * q) * a.rp + r;
+                    if (r < a.rp) { // (rows of u are padded to 16 ranks; what lies past rk is left out below)
+                        const float * ur = a.u + (size_t) at[q] * a.rp + r;
                         const size_t chunk = (size_t) a.rows * a.rp;
                         for (int c0 = 0; c0 < a.chunks; c0 += 4) { // (four loads, then their sums)
                             f32x4 lo[4], hi[4];
@@ -396,19 +405,67 @@ template <int WF, int CT, int RT, int KH, bool BIG> __global__ __launch_bounds__
                 stores(cg, y[0]);
             }
         } else {
-            weights(first, 0, raw[0]);
-            bases(first, y[0]);
-            parts(0);
-            const auto group = [&](int cg, int b) {
-                const int next = min(cg + step, groups - 1); // (behind the last group of all: that once more, unused)
-                weights(next, 0, raw[b ^ 1]);
-                bases(next, y[b ^ 1]);
-                add(0, raw[b], y[b]);
-                stores(cg, y[b]);
+            // groups of whole columns
+            const int whole = a.rank >= 8 ? a.n / (16 * CT) : 0;
+            const uint16_t * wq[KH];
+            u32x4 mask[KH];
+            int over[KH];
+#pragma unroll
+            for (int h = 0; h < KH; h++) {
+                const int r = 32 * h + 8 * g;
+                over[h] = max(r + 8 - a.rank, 0);
+                wq[h] = bp + (size_t) n * a.rank + r - over[h];
+#pragma unroll
+                for (int i = 0; i < 4; i++) mask[h][i] = rk - r >= 2 * i + 2 ? ~0u : rk - r == 2 * i + 1 ? 0xffffu : 0;
+            }
+            const auto fetch = [&](int cg, int b, auto with_base) {
+#pragma unroll
+                for (int h = 0; h < KH; h++)
+#pragma unroll
+                    for (int t = 0; t < CT; t++) raw[b][t][h] = __builtin_bit_cast(u32x4, *reinterpret_cast<const u16x8_u *>(wq[h] + (size_t) (cg * 16 * CT + 16 * t) * a.rank));
+#pragma unroll
+                for (int q = 0; q < RT; q++)
+#pragma unroll
+                    for (int t = 0; t < CT; t++) {
+                        y[b][q][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                        if constexpr (decltype(with_base)::value) y[b][q][t] = f32x4(*reinterpret_cast<const f32x4_u *>(a.base + at[q] * a.base_stride + (cg * 16 * CT + 16 * t + 4 * g)));
+                    }
             };
-            for (int cg = first; cg < groups; cg += 2 * step) {
-                group(cg, 0);
-                if (cg + step < groups) group(cg + step, 1);
+            const auto run = [&](auto with_base) {
+                const auto group = [&](int cg, int b) {
+                    fetch(cg + step < whole ? cg + step : cg, b ^ 1, with_base); // (behind the last group that one again, unused)
+#pragma unroll
+                    for (int h = 0; h < KH; h++)
+#pragma unroll
+                        for (int t = 0; t < CT; t++) {
+                            u32x4 & v = raw[b][t][h];
+                            if (a.rank & 7) {
+                                if (over[h] & 4) v = u32x4{v[2], v[3], 0, 0};
+                                if (over[h] & 2) v = u32x4{v[1], v[2], v[3], 0};
+                                if (over[h] & 1) v = u32x4{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+                            }
+                            v &= mask[h];
+                        }
+                    add(0, raw[b], y[b]);
+#pragma unroll
+                    for (int q = 0; q < RT; q++)
+#pragma unroll
+                        for (int t = 0; t < CT; t++) *reinterpret_cast<f32x4_u *>(a.y + at[q] * a.y_stride + (cg * 16 * CT + 16 * t + 4 * g)) = y[b][q][t];
+                };
+                for (int cg = first; cg < whole; cg += 2 * step) {
+                    group(cg, 0);
+                    if (cg + step < whole) group(cg + step, 1);
+                }
+            };
+            if (first < whole) a.base ? fetch(first, 0, std::true_type()) : fetch(first, 0, std::false_type());
+            parts(0);
+            if (first < whole) a.base ? run(std::true_type()) : run(std::false_type());
+            int cg = first < whole ? first + (whole - first + step - 1) / step * step : first;
+            for (; cg < groups; cg += step) {
+                weights(cg, 0, raw[0]);
+                bases(cg, y[0]);
+                add(0, raw[0], y[0]);
+                stores(cg, y[0]);
             }
         }
     }
@@ -423,13 +480,16 @@ template <int WF, int CT, int RT> hipError_t up(const LoraArgs & a, hipStream_t 
     const int tiles = (a.rows + 16 * RT - 1) / (16 * RT), groups = (a.n + 16 * CT - 1) / (16 * CT);
     const int waves = std::max(1, (int) std::min<long long>((long long) groups * std::min(a.rows, 16 * RT), UP_WAVES / tiles));
     const dim3 grid((waves + UW - 1) / UW, tiles), block(UW * 64);
-    return a.rank <= 32 ? launch(k_lora_up<WF, CT, RT, 1, false>, grid, block, 0, st, a) : a.rank <= 64 ? launch(k_lora_up<WF, CT, RT, 2, false>, grid, block, 0, st, a)
-                                                                                          : launch(k_lora_up<WF, CT, RT, 2, true>, grid, block, 0, st, a);
+    if constexpr (CT == 1 || RT == 1)
+        if (a.rank > 32 && a.rank <= 64) return launch(k_lora_up<WF, CT, RT, 2, false>, grid, block, 0, st, a);
+    if constexpr (CT == 2 || RT == 1) return a.rank <= 32 ? launch(k_lora_up<WF, CT, RT, 1, false>, grid, block, 0, st, a) : launch(k_lora_up<WF, CT, RT, 2, true>, grid, block, 0, st, a);
+    return hipErrorInvalidValue; // (not reached)
 }
 template <int WF, int RT> hipError_t run(const LoraArgs & a, int xform, hipStream_t st) {
     const hipError_t e = xform == W4_UNITS ? down<W4_UNITS, WF, RT>(a, st) : xform == DT_F32 ? down<DT_F32, WF, RT>(a, st) : xform == DT_F16 ? down<DT_F16, WF, RT>(a, st) : down<DT_BF16, WF, RT>(a, st);
     if (e != hipSuccess) return e;
-    if constexpr (RT == 2) return up<WF, 2, 2>(a, st);
+    // (of 33 to 64 ranks two parts of u lie in the registers)
+    if constexpr (RT == 2) return a.rank <= 32 || a.rank > 64 ? up<WF, 2, 2>(a, st) : up<WF, 1, 2>(a, st);
     else {
         // 32 columns a wave, a cache line of a row, where that leaves a wave for every SIMD
         const bool wide = (long long) ((a.n + 31) / 32) * ((a.rows + 15) / 16) >= 1024;
