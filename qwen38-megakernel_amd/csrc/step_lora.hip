@@ -8,6 +8,11 @@
 // adapters take bf16 x as one and fp32 x as two fp16 parts after a power of two per row and step of 32 values, which multiplies the step's
 // result (2^-39 and 2^-23 of the largest of the 32).  Int8 units go in as their codes, the block's scale multiplying the step's result.  u goes in
 // as three bf16 parts, or two fp16 parts after a power of two per row and 64 ranks.
+//
+// Memory bounds it at every size (4 rank operations for 2 bytes of an adapter, and 8 bytes of base and y a column).  1 fp32 row of 5,120 x 6,144 and
+// rank 16: 9.3 us, two launches and their chains of loads (in one launch, every workgroup computing u for itself, a bf16 row takes 10.4 where two take
+// 7.8).  61 rows of as many fp16 adapters of ranks up to 64, 17,408 x 5,120: 54 us, of them 36 for B, 2.9 TB/s.  4,001 rows of 6,144 x 5,120
+// and rank 32: 78 us, of them 56 for 197 MB of base and y.
 #include "step_dev.h"
 #include "step_mix_launch.h"
 
@@ -217,7 +222,7 @@ template <int XF, int WF, int NT, int RT> __global__ __launch_bounds__(LW * 64) 
     }
 }
 
-constexpr int UW = 4, UP_WAVES = 3072; // waves of a workgroup of k_lora_up; of its grid, where the groups of columns are more
+constexpr int UW = 4, UP_WAVES = 12 * 256; // waves of a workgroup of k_lora_up; of its grid, where the groups of columns are more
 
 // y = base + s B u: a wave has u of a tile's rows in registers (KH x 32 ranks of it; ranks past 64: 64 at a time, of every group anew) and takes
 // its share of the groups of CT x 16 columns, the next group's B and base on their way.

@@ -249,6 +249,19 @@ def test_long_rows_of_many(qkv, torch_gpu, xform, group, mins, dim, inner):
     Case(torch_gpu, 40, dim, inner, 2, 1, group, mins, xform, ids=np.zeros((40, 1)), seed=dim).check(qkv)
 
 
+def test_layer_of_many_rows(qkv, torch_gpu):
+    """Rows that the router takes in one kernel, 64 at a time through the experts."""
+    torch = torch_gpu
+    c = Case(torch, 1030, 64, 32, 6, 2, xform="fp16", seed=5, router="fp16")
+    y = c.run(qkv, layer=True).clone()
+    c.ids, c.weights = c.chosen[0].cpu().numpy(), c.chosen[1].cpu().numpy()
+    logits = c.xv @ c.rv.T
+    assert np.array_equal(c.ids, np.argsort(-logits, 1, kind="stable")[:, :2])
+    ref, bound = c.want()
+    assert (np.abs(y.double().cpu().numpy() - ref) <= bound).all()
+    assert torch.equal(c.run(qkv), y)
+
+
 def test_layer_many_experts(qkv, torch_gpu):
     """More experts than the choice beside the rows takes; runs of 64 rows."""
     torch = torch_gpu

@@ -189,3 +189,44 @@ def test_bias_masks(qkv, torch_gpu):
     b[[3, 9, 17]] = 0
     _, ids, _ = run(qkv, torch_gpu, x, "fp32", w, "fp32", b, 3, 1.0, 6)
     assert (np.sort(ids[:, :3], 1) == [3, 9, 17]).all() and (ids[:, 3:] == [0, 1, 2]).all()
+
+
+def test_same_bits_streams_graph(qkv, torch_gpu):
+    """The same bits on two streams at once, each with its workspace, and on replays of a graph between other work."""
+    torch = torch_gpu
+    rng = np.random.default_rng(21)
+    cs = []
+    for rows, dim, e, top in ((40, 512, 100, 8), (1100, 96, 72, 4)):
+        x, w = torch.from_numpy(rng.standard_normal((rows, dim))).to(torch.bfloat16).cuda(), torch.from_numpy(rng.standard_normal((e, dim))).to(torch.bfloat16).cuda()
+        need = qkv.moe_route_ws(rows, dim, e)
+        out = [torch.empty(rows, e, device="cuda"), torch.empty(rows, top, device="cuda", dtype=torch.int32), torch.empty(rows, top, device="cuda")]
+        cs.append((x, w, top, out, torch.empty(need + 16, device="cuda", dtype=torch.uint8), need))
+
+    def call(c, stream=0):
+        x, w, top, out, ws, need = c
+        qkv.moe_route(x.shape[0], x.shape[1], w.shape[0], top, x.data_ptr(), x.stride(0), 2, w.data_ptr(), 2, 0, 0, 1.5, *(t.data_ptr() for t in out), ws.data_ptr(), need, stream)
+        return out
+
+    want = [[t.clone() for t in call(c)] for c in cs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cs]
+    for _ in range(5):
+        for c, s in zip(cs, streams):
+            call(c, s.cuda_stream)
+    torch.cuda.synchronize()
+    for c, w in zip(cs, want):
+        assert all(torch.equal(a, b) for a, b in zip(c[3], w))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for c in cs:
+            call(c, torch.cuda.current_stream().cuda_stream)
+    for _ in range(4):
+        for c in cs:
+            c[0].mul_(-1.5)
+            c[3][0].zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        got = [[t.clone() for t in c[3]] for c in cs]
+        for c, o in zip(cs, got):
+            assert all(torch.equal(a, b) for a, b in zip(call(c), o))
+        torch.cuda.synchronize()
