@@ -74,7 +74,7 @@ struct MoeArgs {
     float * xd, * hd, * xs, * hs;
     float * out;     // [pairs][dim]: the experts' outputs (where xq, xd and xs were)
     // (set by the launcher) tokens of an expert that a pass holds in LDS, runs of k that it holds at a time, and waves (1 << ..) that split k
-    int tp_up, tp_down, cr_up, cr_down, ks_up, ks_down;
+    int tp_up, tp_down, cr_up, cr_down, ks_up, ks_down, ks_one;
 };
 constexpr int MOE_ROWS = 64, MOE_PICK = 256; // rows of a run; a call of more runs them one after another; experts that it can choose from itself
 constexpr int MOE_MAX_ROWS = 4096, MOE_MAX_DIM = 16384, MOE_MAX_INNER = 32768;

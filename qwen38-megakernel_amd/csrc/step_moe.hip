@@ -1,7 +1,7 @@
 // A mixture-of-experts layer with 4-bit weights for a few tokens: h = silu(G x) (U x) of every (token, expert) pair, then
 // y[m] = sum over the row's experts of w D h.  Four kernels: x made ready and the pairs sorted by their experts (with a router also the choice), the
 // gate's and the up projection's rows together, the down projection of every pair, and the sum over a row's experts in their order (no
-// atomics in sums: the same bits every time).
+// atomics in sums: the same bits every time); of a single row the last two in one.
 //
 // Workgroups stand for (columns, one of the experts that occur).  An expert has few tokens, so what counts is the way of its codes: from HBM,
 // and from 4 bits to an operand.  Codes become int8 with four vector instructions for 8 of them (fp16 takes 13), so x is made integer
@@ -385,7 +385,7 @@ __device__ __forceinline__ unsigned lds_address(const uint8_t * lds) {
 }
 // the planes, factors and sums of nt tokens, lane t's `at` the place of the t-th, into LDS: of runs c0 .. c0 + n - 1 (rows of `row` bytes, nd factors, ng of
 // them in use)
-template <int P, bool MINS>
+template <int P, bool MINS, int W = WAVES>
 __device__ __forceinline__ void stage(const uint8_t * q, const float * d, const float * s, int row, int nd, int ng, int c0, int n, int sg, uint8_t * lds, const Lds & L, int tp, int nt, int at) {
     const unsigned base = lds_address(lds);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, bytes = n * 256, per = (bytes + 1023) >> 10, d0 = c0 * 8 >> sg, dn = n * 8 >> sg;
@@ -395,10 +395,10 @@ __device__ __forceinline__ void stage(const uint8_t * q, const float * d, const 
         const uint8_t * from = q + (size_t) (unsigned) __builtin_amdgcn_readlane(at, t) * (P * row) + c0 * 256;
 #pragma unroll
         for (int p = 0; p < P; p++, c -= per)
-            for (; c < per; c += WAVES)
+            for (; c < per; c += W)
                 if (c * 1024 + lane * 16 < bytes) dma16(from + (p * row + c * 1024 + lane * 16), base + (t * P + p) * L.row + c * 1024);
     }
-    for (int k = tid; k < dn; k += WAVES * 64)
+    for (int k = tid; k < dn; k += W * 64)
         for (int t0 = 0; t0 < nt; t0 += 4) { // (four loads, then their values)
             float v[4], w[4];
 #pragma unroll
@@ -551,6 +551,59 @@ template <int P, int GSH, int SG, int TM, bool MINS> __global__ __launch_bounds_
     }
 }
 
+constexpr int OW = 16; // waves of a workgroup of k_moe_down_one
+
+// The down projection of a single row and the sum over its experts, in one launch: a workgroup has 16 NT columns of all of them, its waves (an expert,
+// a part of inner).  Tokens in LDS are the row's pairs; no list is needed.  A layer's row, 8 of 128 experts of 2,048 x 768: 26.3 us, 28.6 with k_moe_down and
+// k_moe_sum; 2 of 8 of 5,120 x 6,144 in fp32: 45 and 49.
+template <int P, int GSH, int SG, int NT, bool MINS, int YT> __global__ __launch_bounds__(OW * 64) void k_moe_down_one(MoeArgs a) {
+    constexpr int TG = group_of(P, SG), WB = win_bytes(NT, MINS);
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c0 = blockIdx.x * 16 * NT;
+    const int nb = a.inner >> 5, nbp = padded(nb), runs = nbp >> 3, gs = (nb + (1 << GSH) - 1) >> GSH, tp = a.top_k + TG;
+    const Lds L = lds_of(P, SG, runs, tp, MINS);
+    uint16_t * win = reinterpret_cast<uint16_t *>(lds + L.end + wave * WB);
+    float * red = reinterpret_cast<float *>(lds + L.end + OW * WB); // [OW][NT][16]
+    const int j = wave >> a.ks_one, ks = wave & ((1 << a.ks_one) - 1), e = j < a.top_k ? __builtin_amdgcn_readfirstlane(a.ids[min(j, a.top_k - 1)]) : -1;
+    const bool on = (unsigned) e < (unsigned) a.n_experts;
+    Rows<NT> w;
+    Run<NT, MINS> in;
+    const Part part = part_of(runs, runs, 0, ks, a.ks_one);
+    if (on) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) w.set(t, a.down, e, a.dim, c0 + 16 * t, nb, gs);
+        in = load_runs<GSH, SG, NT, MINS>(w, nb, part.r0, part.r1 - 1);
+    }
+    zero_pieces(lds, L);
+    stage<P, MINS, OW>(a.hq, a.hd, a.hs, plane_bytes(nb), nbp >> SG, (nb + (1 << SG) - 1) >> SG, 0, runs, SG, lds, L, tp, a.top_k, lane);
+    __syncthreads();
+    if (on) {
+        // its pair's planes come first; those behind them take part in the instruction, and their sums are not used
+        const int off = j * P * L.row;
+        Lds l = L;
+        l.zero -= off;
+        l.dx += 4 * j - off;
+        l.ds += 4 * j - off;
+        float acc[NT][TG >> SG];
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < TG >> SG; i++) acc[t][i] = 0.f;
+        products<P, GSH, SG, NT, TG, MINS>(w, in, nb, part, Part{part.first, part.r1 - 1, part.r1}, lds + off, l, win, tp, 1, acc);
+        sums_out<P, SG, NT, TG>(acc, 1, 1, red + wave * NT * 16);
+    }
+    __syncthreads();
+    if (threadIdx.x >= 16 * NT) return;
+    float v = 0.f;
+    for (int p = 0; p < a.top_k; p++) {
+        if ((unsigned) a.ids[p] >= (unsigned) a.n_experts) continue;
+        float o = 0.f;
+        for (int k = 0; k < 1 << a.ks_one; k++) o += red[((p << a.ks_one) + k) * NT * 16 + threadIdx.x];
+        v = __builtin_fmaf(a.weights[p], o, v);
+    }
+    static_cast<typename Elem<YT>::T *>(a.y)[c0 + threadIdx.x] = Elem<YT>::down(v);
+}
+
 // y[m] = sum over the row's places, in order, of w out
 template <int YT> __global__ __launch_bounds__(256) void k_moe_sum(MoeArgs a) {
     const int row = blockIdx.y, c = (blockIdx.x * 256 + threadIdx.x) * 4;
@@ -585,11 +638,22 @@ template <int P, int GSH, int SG, int TM, bool MINS> hipError_t down(const MoeAr
     const int cols = 32 * (WAVES >> a.ks_down);
     return e != hipSuccess ? e : launch(k_moe_down<P, GSH, SG, TM, MINS>, dim3((a.dim + cols - 1) / cols, slots), dim3(WAVES * 64), lds, st, a);
 }
+size_t one_lds(const MoeArgs & a, int P, int sg, int nt) {
+    return lds_of(P, sg, padded(a.inner >> 5) >> 3, a.top_k + group_of(P, sg), a.up.mins).end + (size_t) OW * (win_bytes(nt, a.up.mins) + nt * 64);
+}
+template <int P, int GSH, int SG, int NT, bool MINS, int YT> hipError_t down_one(const MoeArgs & a, hipStream_t st) {
+    static std::atomic<uint64_t> done;
+    const size_t lds = one_lds(a, P, SG, NT);
+    const hipError_t e = allow_lds(k_moe_down_one<P, GSH, SG, NT, MINS, YT>, lds, done);
+    return e != hipSuccess ? e : launch(k_moe_down_one<P, GSH, SG, NT, MINS, YT>, dim3(a.dim / (16 * NT)), dim3(OW * 64), lds, st, a);
+}
 template <int XF, int GSH, int SH, bool MINS> hipError_t run(const MoeArgs & a, hipStream_t st) {
     constexpr int HP = inner_planes(XF), YT = XF == W4_UNITS ? DT_F32 : XF;
     const int slots = std::min(a.n_experts, a.rows * a.top_k);
     hipError_t e = a.tp_up <= 8 ? up<XF, GSH, SH, 8, MINS>(a, slots, st) : up<XF, GSH, SH, 16, MINS>(a, slots, st);
     if (e != hipSuccess) return e;
+    // one row whose h LDS holds: its sum with the product (a workgroup a CU: 16 columns, or 32 where those would be more)
+    if (a.rows == 1 && one_lds(a, HP, SH, 2) <= 150 * 1024) return a.dim <= 256 * 16 ? down_one<HP, GSH, SH, 1, MINS, YT>(a, st) : down_one<HP, GSH, SH, 2, MINS, YT>(a, st);
     e = a.tp_down <= 8 ? down<HP, GSH, SH, 8, MINS>(a, slots, st) : down<HP, GSH, SH, 16, MINS>(a, slots, st);
     if (e != hipSuccess) return e;
     return launch(k_moe_sum<YT>, dim3((a.dim + 1023) / 1024, a.rows), dim3(256), 0, st, a);
@@ -661,6 +725,8 @@ static void split_work(MoeArgs & a, int xform) {
     const double experts = a.n_experts * (1 - std::pow(1 - 1.0 / a.n_experts, a.rows * a.top_k));
     a.ks_up = split(experts, a.inner, 16, padded(a.dim / 32) / 8, WAVES_LOG - 1);
     a.ks_down = split(experts, a.dim, 32, padded(nbi) / 8, WAVES_LOG);
+    a.ks_one = 0;
+    while (a.top_k << (a.ks_one + 1) <= OW && 1 << (a.ks_one + 1) <= padded(nbi) / 8) a.ks_one++;
     pass(a, P, P == 1 ? 0 : a.gsh, padded(a.dim / 32) / 8, a.ks_up, a.tp_up, a.cr_up);
     pass(a, HP, a.ks_up == 0 ? std::min(a.gsh, 1) : 0, padded(nbi) / 8, a.ks_down, a.tp_down, a.cr_down);
 }

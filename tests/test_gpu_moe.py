@@ -103,6 +103,17 @@ def test_larger(qkv, torch_gpu, xform, rows, dim, inner, e, top):
 
 
 @pytest.mark.parametrize("xform", FORMS)
+@pytest.mark.parametrize("group,mins,dim,inner,top", [(32, False, 64, 768, 2), (64, True, 4160, 288, 1), (128, True, 128, 2080, 3), (32, True, 192, 64, 16), (128, False, 4224, 544, 5)])
+def test_one_row(qkv, torch_gpu, xform, group, mins, dim, inner, top):
+    """A single row: parts of inner, two tiles of columns, the same expert twice, choices that are no expert, none at all."""
+    rng = np.random.default_rng(dim)
+    Case(torch_gpu, 1, dim, inner, max(5, top), top, group, mins, xform, ids=rng.integers(0, 5, (1, top)), seed=top).check(qkv)
+    Case(torch_gpu, 1, dim, inner, max(5, top), top, group, mins, xform, ids=rng.integers(-3, 8, (1, top)), seed=top).check(qkv)
+    y = Case(torch_gpu, 1, dim, inner, max(5, top), top, group, mins, xform, ids=np.full((1, top), 2 ** 31 - 1)).check(qkv)
+    assert (y == 0).all()
+
+
+@pytest.mark.parametrize("xform", FORMS)
 def test_skewed(qkv, torch_gpu, xform):
     """All rows on one expert (several passes), the same expert twice in a row, choices that are no expert."""
     for rows in (16, 33, 64):
