@@ -174,7 +174,7 @@ template <int DT, int V> __global__ __launch_bounds__(MW * 64) void k_route_many
         zero = !__any(some != 0);
     }
     const float lost = (float) a.dim * 0x1p-126f;
-    const float near = zero ? 0.f : 2.f * ((float) ((steps + KS - 1) / KS + 40) * 0x1p-22f * sqrtf(xs + lost) * sqrtf(wmax + lost) + lost); // (the bound on two errors)
+    const float near = zero ? 0.f : 2.f * ((float) (chunks * ((7 + KS) / KS) + 40) * 0x1p-22f * sqrtf(xs + lost) * sqrtf(wmax + lost) + lost); // (the bound on two errors; a wave's steps of a chunk are 8 / KS at most, rounded up)
     Chosen<V> c = route_choose<V>(a, l, most);
     const float v = c.logit, last = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), a.top_k - 1)) - near;
     const float up = __shfl_up(v, 1), down = __shfl_down(v, 1);
