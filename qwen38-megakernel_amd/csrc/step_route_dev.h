@@ -54,7 +54,7 @@ template <int V> __device__ __forceinline__ Chosen<V> route_choose(const RouteAr
         for (int i = 1; i < V; i++)
             if (hi[i] > h || (hi[i] == h && lo[i] > w)) h = hi[i], w = lo[i], at = i, v = l[i];
         uint64_t best = __ballot(h == wave_max_u(h));
-        if (a.bias) {
+        if (a.bias && (best & (best - 1))) { // (more lanes than one with the upper half)
             const bool in = best >> lane & 1;
             const unsigned m = wave_max_u(in ? w : 0);
             best = __ballot(in && w == m);
