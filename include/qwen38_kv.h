@@ -345,8 +345,8 @@ int mk_moe_route(int rows, int dim, int n_experts, int top_k, const void * x, lo
  *   ids         int [rows][top_k], weights fp32 [rows][top_k] (of mk_moe_route, or a caller's own); ids that are no expert are left out
  *   y           [rows][y_stride]: of x's type, for units fp32
  * dim a multiple of 32 (units: 64), at most 16384; inner of 32, at most 32768; n_experts 1..1024, top_k 1..16.  x and h enter as integers
- * of their block of 32 values (of plain rows and h as many as the group): int8 units as they are, fp32 rows (and the h of both) to 2^-21 of the
- * block's largest value, fp16 and bf16 rows (and their h) to 2^-13; sums in fp32.  A row of x with an infinity or a NaN gives NaNs in that row of y alone.
+ * of their block (of plain rows as many values as the group, of h 32 or 64): int8 units as they are, plain rows and h to 2^-21 of the power of
+ * two of the block's largest value, or of 2^-101 where that is larger (so an fp16 value within 2^-11 of it, and a bf16 value within 2^-14, are exact); sums in fp32.  A row of x with an infinity or a NaN gives NaNs in that row of y alone.
  * mk_moe_layer is mk_moe_route on the same rows and mk_moe_rows on its choice, in one call; mk_moe_ws covers all three calls.
  */
 long long mk_moe_ws(int rows, int dim, int inner, int n_experts, int top_k);

@@ -5,8 +5,10 @@
 //
 // Workgroups stand for (columns, one of the experts that occur).  An expert has few tokens, so what counts is the way of its codes: from HBM,
 // and from 4 bits to an operand.  Codes become int8 with four vector instructions for 8 of them (fp16 takes 13), so x is made integer
-// too: an exponent for every block, and two or three int8 planes (14 bits of the block's largest power of two for 16-bit x, 22 for fp32;
-// int8 units are one plane as they are).  The matrix instruction's sums are exact, the scales multiply them in fp32.
+// too: an exponent for every block, and three int8 planes (22 bits of the block's largest power of two; int8 units are one plane as they
+// are).  Two planes, 14 bits, are too few for 16-bit x as well: beside a value 256 times as large in its block they leave half of an fp16 layer's
+// results another than the nearest (47 rows, 2 of 8 experts 4,096 x 8,192: 176 us with two, 215 with three; 8 rows of 8 of 128 small ones 62 and 64).
+// The matrix instruction's sums are exact, the scales multiply them in fp32.
 //
 // A wave has two tiles of 16 weight rows, lane (n = lane & 15, g = lane >> 4) 16 bytes, a block of 32 codes of row n, a step.  The instruction
 // contracts over all four lane groups, so blocks with scales of their own must not meet in it: the planes go in on a (block) diagonal,
@@ -26,11 +28,11 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr int MAX_PAIRS = MOE_ROWS * ROUTE_MAX_TOP;
 constexpr int WAVES_LOG = 2, WAVES = 1 << WAVES_LOG;
 
-constexpr int planes_of(int xform) { return xform == W4_UNITS ? 1 : xform == DT_F32 ? 3 : 2; }
-constexpr int inner_planes(int xform) { return xform == DT_F16 || xform == DT_BF16 ? 2 : 3; } // (y is fp32 else)
+constexpr int planes_of(int xform) { return xform == W4_UNITS ? 1 : 3; }
+constexpr int HP = 3; // of h
 // operand rows of a token (three planes: the fourth stays zero), tokens in a lane's sums of an instruction, tokens of an instruction; sg: lane
 // groups that share a sum are 1 << sg
-constexpr int op_rows(int P) { return P == 3 ? 4 : P; }
+constexpr int op_rows(int P) { return P == 3 ? 4 : 1; }
 constexpr int lane_tokens(int P) { return 4 / op_rows(P); }
 constexpr int group_of(int P, int sg) { return lane_tokens(P) << sg; }
 
@@ -63,27 +65,27 @@ template <int SG> __device__ __forceinline__ int piece(int block, int half) {
 }
 __device__ __forceinline__ int piece(int sg, int block, int half) { return sg == 0 ? piece<0>(block, half) : sg == 1 ? piece<1>(block, half) : piece<2>(block, half); }
 
-// values as integers: times `up`, a power of two that brings the largest to [2^13, 2^14) (three planes: [2^21, 2^22)), and the
-// factor 1 / (16 up) of the products with codes 16 times as large
+// values as integers: times `up`, a power of two that brings the largest to [2^21, 2^22), and the factor 1 / (16 up) of the products with
+// codes 16 times as large
 struct Fixed {
     float up, dx;
 };
-template <int P> __device__ __forceinline__ Fixed fixed_of(unsigned top) {
-    constexpr int S = P == 3 ? 21 : 13;
+__device__ __forceinline__ Fixed fixed_of(unsigned top) {
+    constexpr int S = 21;
     const int E = max((int) (top >> 23), 26);
     if (top >= 0x7f800000u) return Fixed{0.f, __builtin_nanf("")}; // an infinity or a NaN: the row's results are NaN
     return Fixed{__builtin_bit_cast(float, (unsigned) (254 + S - E) << 23), __builtin_bit_cast(float, (unsigned) (E - S - 4) << 23)};
 }
-// plane p of P of the integer v: its bits from 8 (P - 1 - p) on as signed bytes
-template <int P> __device__ __forceinline__ void planes_split(int v, int (&q)[P]) {
+// plane p of the integer v: its bits from 8 (2 - p) on as signed bytes
+__device__ __forceinline__ void planes_split(int v, int (&q)[3]) {
 #pragma unroll
-    for (int p = P - 1; p > 0; p--) {
+    for (int p = 2; p > 0; p--) {
         q[p] = (int) (int8_t) v;
         v = (v - q[p]) >> 8;
     }
     q[0] = v;
 }
-template <int P> __device__ __forceinline__ int to_fixed(float v, float up) { return up == 0.f ? 0 : (int) __builtin_rintf(v * up); } // (0 inf is a NaN)
+__device__ __forceinline__ int to_fixed(float v, float up) { return up == 0.f ? 0 : (int) __builtin_rintf(v * up); } // (0 inf is a NaN)
 
 // NT tiles of 16 weight rows: a tile's first row in scalars, the lane's in 32 bits behind it
 template <int NT> struct Rows {
@@ -210,7 +212,6 @@ __device__ __forceinline__ void products(const Rows<NT> & w, Run<NT, MINS> & in,
                     for (int t = 0; t < NT; t++) {
                         float v;
                         if constexpr (P == 1) v = (float) c[t][i];
-                        else if constexpr (P == 2) v = (float) ((c[t][2 * i] << 8) + c[t][2 * i + 1]);
                         else v = __builtin_fmaf((float) ((c[t][0] << 8) + c[t][1]), 256.f, (float) c[t][2]);
                         float & s = acc[t][q * TL + i];
                         s = __builtin_fmaf(v, sc[t][u] * d, s);
@@ -362,12 +363,12 @@ template <int XF, int V> __global__ __launch_bounds__(PREP) void k_moe_prep(Prep
                 top = max(top, shfl_xor_u(top, m));
                 s += shfl_xor(s, m);
             }
-        const Fixed f = fixed_of<P>(top);
+        const Fixed f = fixed_of(top);
         unsigned out[P][2] = {};
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             int q[P];
-            planes_split<P>(to_fixed<P>(v[k], f.up), q);
+            planes_split(to_fixed(v[k], f.up), q);
 #pragma unroll
             for (int p = 0; p < P; p++) out[p][k >> 2] |= (unsigned) (q[p] & 255) << 8 * (k & 3);
         }
@@ -423,7 +424,7 @@ __device__ __forceinline__ void zero_pieces(uint8_t * lds, const Lds & L) {
 // The gate and the up projection: a workgroup has 16 CG inner columns of an expert, its waves (16 columns of both, a KS-th of dim), CG KS = 8.
 // SG: lane groups that share a sum of x; SH: those of the down projection, whose x (h) this kernel leaves as planes.
 template <int XF, int GSH, int SH, int TM, bool MINS> __global__ __launch_bounds__(WAVES * 64, 3) void k_moe_up(MoeArgs a) {
-    constexpr int P = planes_of(XF), HP = inner_planes(XF), SG = P == 1 ? 0 : GSH;
+    constexpr int P = planes_of(XF), SG = P == 1 ? 0 : GSH;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const Lists * l = reinterpret_cast<const Lists *>(a.lists);
     if ((int) blockIdx.y >= l->count) return;
@@ -482,12 +483,12 @@ template <int XF, int GSH, int SH, int TM, bool MINS> __global__ __launch_bounds
                 top = max(top, shfl_xor_u(top, m));
                 if (MINS) s += shfl_xor(s, m);
             }
-            const Fixed f = fixed_of<HP>(top);
+            const Fixed f = fixed_of(top);
             unsigned out[HP] = {};
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 int q[HP];
-                planes_split<HP>(to_fixed<HP>(h[k], f.up), q);
+                planes_split(to_fixed(h[k], f.up), q);
 #pragma unroll
                 for (int p = 0; p < HP; p++) out[p] |= (unsigned) (q[p] & 255) << 8 * k;
             }
@@ -648,7 +649,7 @@ template <int P, int GSH, int SG, int NT, bool MINS, int YT> hipError_t down_one
     return e != hipSuccess ? e : launch(k_moe_down_one<P, GSH, SG, NT, MINS, YT>, dim3(a.dim / (16 * NT)), dim3(OW * 64), lds, st, a);
 }
 template <int XF, int GSH, int SH, bool MINS> hipError_t run(const MoeArgs & a, hipStream_t st) {
-    constexpr int HP = inner_planes(XF), YT = XF == W4_UNITS ? DT_F32 : XF;
+    constexpr int YT = XF == W4_UNITS ? DT_F32 : XF;
     const int slots = std::min(a.n_experts, a.rows * a.top_k);
     hipError_t e = a.tp_up <= 8 ? up<XF, GSH, SH, 8, MINS>(a, slots, st) : up<XF, GSH, SH, 16, MINS>(a, slots, st);
     if (e != hipSuccess) return e;
@@ -695,7 +696,7 @@ int split(double experts, int n, int cols, int runs, int limit) {
 } // namespace
 
 long long moe_plan(MoeArgs & a, int xform, uint8_t * ws) {
-    const int HP = inner_planes(xform), P = planes_of(xform), nbx = a.dim / 32, nbi = a.inner / 32;
+    const int P = planes_of(xform), nbx = a.dim / 32, nbi = a.inner / 32;
     const long long rows = std::min(a.rows, MOE_ROWS), pairs = rows * a.top_k;
     long long at = 0;
     const auto take = [&](long long bytes) {
@@ -720,7 +721,7 @@ long long moe_plan(MoeArgs & a, int xform, uint8_t * ws) {
 
 // (of one run of at most MOE_ROWS rows)
 static void split_work(MoeArgs & a, int xform) {
-    const int HP = inner_planes(xform), P = planes_of(xform), nbi = a.inner / 32;
+    const int P = planes_of(xform), nbi = a.inner / 32;
     // the experts that occur where every choice is as likely as another
     const double experts = a.n_experts * (1 - std::pow(1 - 1.0 / a.n_experts, a.rows * a.top_k));
     a.ks_up = split(experts, a.inner, 16, padded(a.dim / 32) / 8, WAVES_LOG - 1);
