@@ -507,15 +507,15 @@ template <int WF, int RT> hipError_t run(const LoraArgs & a, int xform, hipStrea
 void lora_plan(LoraArgs & a) {
     a.rp = (a.rank + 15) / 16 * 16;
     // few rows: the adapters of a tile in workgroups of their own; many: tiles of 32 rows, which read A and B half as often
-    a.slots = a.rows <= 256 ? std::min(16, std::max(a.rows, 1)) : 1;
-    const int rt = a.rows <= 256 ? 1 : 2, tiles = (a.rows + 16 * rt - 1) / (16 * rt), pairs = (a.k / 32 + 1) / 2;
+    a.slots = a.rows <= LORA_FEW_ROWS ? std::min(16, std::max(a.rows, 1)) : 1;
+    const int rt = a.rows <= LORA_FEW_ROWS ? 1 : 2, tiles = (a.rows + 16 * rt - 1) / (16 * rt), pairs = (a.k / 32 + 1) / 2;
     // and k in chunks, of at least two pairs of steps a wave, until two workgroups a CU have work
     a.chunks = std::max(1, std::min({LORA_MAX_CHUNKS, 512 / std::max(1, tiles * a.slots), pairs / (2 * LW)}));
 }
 
 hipError_t launch_lora(const LoraArgs & a, int xform, int wtype, hipStream_t st) {
-    if (wtype == DT_F16) return a.rows <= 256 ? run<DT_F16, 1>(a, xform, st) : run<DT_F16, 2>(a, xform, st);
-    return a.rows <= 256 ? run<DT_BF16, 1>(a, xform, st) : run<DT_BF16, 2>(a, xform, st);
+    if (wtype == DT_F16) return a.rows <= LORA_FEW_ROWS ? run<DT_F16, 1>(a, xform, st) : run<DT_F16, 2>(a, xform, st);
+    return a.rows <= LORA_FEW_ROWS ? run<DT_BF16, 1>(a, xform, st) : run<DT_BF16, 2>(a, xform, st);
 }
 
 } // namespace qkv

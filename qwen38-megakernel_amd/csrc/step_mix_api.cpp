@@ -36,6 +36,23 @@ void check_ws(const void * ws, long long ws_bytes, long long want, const char * 
     aligned(ws, 16, "ws");
 }
 
+// The most bytes that calls of lo .. hi rows need, where plan(rows) gives a call of `max` parts at most and never more of more rows: of each number
+// of parts the most rows that still have it.
+template <class Plan, class Bytes> long long most_bytes(int lo, int hi, int max, Plan plan, Bytes bytes) {
+    long long most = 0;
+    for (int parts = 1; parts <= max && lo <= hi; parts++) {
+        if (plan(lo).chunks < parts) break;
+        int at = lo, end = hi; // plan(at) has as many
+        while (at < end) {
+            const int mid = at + (end - at + 1) / 2;
+            if (plan(mid).chunks >= parts) at = mid;
+            else end = mid - 1;
+        }
+        most = std::max(most, bytes(plan(at)));
+    }
+    return most;
+}
+
 // ------------------------------------------------------------------------------------------------ adapters
 void lora_shape(int rows, int k, int rank) {
     if (rows < 0 || rows > LORA_MAX_ROWS) bad("rows outside 0 .. 524288");
@@ -43,6 +60,18 @@ void lora_shape(int rows, int k, int rank) {
     if (rank < 1 || rank > LORA_MAX_RANK) bad("rank outside 1 .. 256");
 }
 long long lora_ws(const LoraArgs & a) { return (long long) a.chunks * a.rows * a.rp * 4; }
+// of up to `rows` rows: a workspace serves every smaller call too
+long long lora_ws_upto(int rows, int k, int rank) {
+    const auto plan = [&](int r) {
+        LoraArgs a{};
+        a.rows = r;
+        a.k = k;
+        a.rank = rank;
+        lora_plan(a);
+        return a;
+    };
+    return std::max(most_bytes(1, std::min(rows, LORA_FEW_ROWS), LORA_MAX_CHUNKS, plan, lora_ws), most_bytes(LORA_FEW_ROWS + 1, rows, LORA_MAX_CHUNKS, plan, lora_ws));
+}
 
 int lora(LoraArgs a, int ab_dtype, int xform, void * ws, long long ws_bytes, void * stream) {
     lora_shape(a.rows, a.k, a.rank);
@@ -111,6 +140,16 @@ void top_shape(int n_experts, int top_k) {
     if (top_k < 1 || top_k > ROUTE_MAX_TOP || top_k > n_experts) bad("top_k outside 1 .. 16 or above n_experts");
 }
 long long route_ws(const RouteArgs & a) { return a.chunks > 1 ? (long long) a.chunks * a.rows * a.n_experts * 8 : 0; }
+long long route_ws_upto(int rows, int dim, int n_experts) {
+    return most_bytes(1, rows, ROUTE_MAX_CHUNKS, [&](int r) {
+        RouteArgs a{};
+        a.rows = r;
+        a.dim = dim;
+        a.n_experts = n_experts;
+        route_plan(a);
+        return a;
+    }, route_ws);
+}
 
 void check_route(const RouteArgs & a, int dtype, int w_dtype) {
     (void) size_of(dtype);
@@ -227,12 +266,7 @@ extern "C" {
 long long mk_lora_ws(int rows, int k, int rank) {
     return guarded<long long>([&] {
         lora_shape(rows, k, rank);
-        LoraArgs a{};
-        a.rows = rows;
-        a.k = k;
-        a.rank = rank;
-        lora_plan(a);
-        return lora_ws(a);
+        return lora_ws_upto(rows, k, rank);
     });
 }
 
@@ -264,12 +298,7 @@ int mk_lora_units(int rows, int n, int k, int n_adapters, int rank, const void *
 long long mk_moe_route_ws(int rows, int dim, int n_experts) {
     return guarded<long long>([&] {
         route_shape(rows, dim, n_experts);
-        RouteArgs a{};
-        a.rows = rows;
-        a.dim = dim;
-        a.n_experts = n_experts;
-        route_plan(a);
-        return route_ws(a);
+        return route_ws_upto(rows, dim, n_experts);
     });
 }
 
@@ -302,12 +331,7 @@ long long mk_moe_ws(int rows, int dim, int inner, int n_experts, int top_k) {
         a.n_experts = n_experts;
         a.top_k = top_k;
         a.up.mins = reinterpret_cast<const uint16_t *>(8); // (the form that needs most)
-        RouteArgs r{};
-        r.rows = rows;
-        r.dim = dim;
-        r.n_experts = n_experts;
-        route_plan(r);
-        return up256(route_ws(r)) + moe_plan(a, DT_F32, nullptr);
+        return up256(route_ws_upto(rows, dim, n_experts)) + moe_plan(a, DT_F32, nullptr); // (which never falls with the rows)
     });
 }
 

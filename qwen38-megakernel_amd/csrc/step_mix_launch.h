@@ -23,6 +23,7 @@ struct LoraArgs {
     int rows, n, k, n_adapters, rank;
     int rp, chunks, slots; // (set by lora_plan) rank padded to 16; chunks of k; adapters of a tile of 16 rows side by side
 };
+constexpr int LORA_FEW_ROWS = 256; // up to them tiles of 16 rows, from there of 32
 constexpr int LORA_MAX_ROWS = 1 << 19, LORA_MAX_N = 1 << 24, LORA_MAX_K = 1 << 20, LORA_MAX_RANK = 256, LORA_MAX_CHUNKS = 16;
 void lora_plan(LoraArgs & a);
 hipError_t launch_lora(const LoraArgs & a, int xform, int wtype, hipStream_t st); // xform: W4_UNITS or a Dtype
