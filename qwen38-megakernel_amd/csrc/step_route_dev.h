@@ -90,7 +90,13 @@ template <int V> __device__ __forceinline__ void route_weights(const RouteArgs &
         const double e = in ? exp((double) c.logit - (double) top) : 0.0;
         w = e / wave_sum(e);
     } else {
-        w = in ? sigmoid_d(c.logit) : 0.0;
+        // (where all the chosen ones lie far below zero sigmoids are exponentials to 64 bits, and may leave their range: relative to the largest)
+        const bool far = a.form == ROUTE_SIGMOID_NORM && !__any(in && c.logit >= -600.f);
+        float top = in ? c.logit : -__builtin_inff();
+        if (far)
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, shfl_xor(top, m));
+        w = !in ? 0.0 : far ? exp((double) c.logit - (double) top) : sigmoid_d(c.logit);
         if (a.form == ROUTE_SIGMOID_NORM) w /= wave_sum(w);
     }
     if (in) {
