@@ -144,19 +144,17 @@ template <int DT, int V> __global__ __launch_bounds__(MW * 64) void k_route_many
         logit[i] = v;
         if (e < E && row0 + r < a.rows) a.logits[(size_t) (row0 + r) * E + e] = v;
     }
+    // (the square of a NaN's expert is a NaN, which fmaxf leaves out: its logits are NaNs, in 64 bits too, and the others' bound is the others')
     float wmax = 0.f;
 #pragma unroll
     for (int i = 0; i < V; i++) {
         float v = 0.f;
         if (lane * V + i < E)
             for (int k = 0; k < KS; k++) v += wsq[k][lane * V + i];
-        wmax = v != v ? v : fmaxf(wmax, v);
+        wmax = fmaxf(wmax, v);
     }
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const float o = shfl_xor(wmax, m);
-        wmax = o != o ? o : wmax != wmax ? wmax : fmaxf(wmax, o);
-    }
+    for (int m = 1; m < 64; m <<= 1) wmax = fmaxf(wmax, shfl_xor(wmax, m));
     __syncthreads();
     // a row a wave: the experts that lie too close to each other
     const int most = min(E, a.top_k + 4), r = wave;
