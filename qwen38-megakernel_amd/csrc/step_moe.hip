@@ -15,44 +15,14 @@
 // operand rows for lane groups whose blocks share a weight scale, zeros in the other groups.  Blocks of 32 values with scales of their own:
 // four groups, 4 rows of planes each.  Weight groups of 64 or 128 values, and x with one exponent for as many: two lane groups or all
 // four share a sum, 8 or 16 rows of planes go in at a time, and every sum is scaled once for 64 or 128 values.
+#include "step_moe_plan.h"
 #include "step_route_dev.h"
-
-#include <algorithm>
-#include <cmath>
 
 namespace qkv {
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int MAX_PAIRS = MOE_ROWS * ROUTE_MAX_TOP;
-constexpr int WAVES_LOG = 2, WAVES = 1 << WAVES_LOG;
-
-constexpr int planes_of(int xform) { return xform == W4_UNITS ? 1 : 3; }
-constexpr int HP = 3; // of h
-// operand rows of a token (three planes: the fourth stays zero), tokens in a lane's sums of an instruction, tokens of an instruction; sg: lane
-// groups that share a sum are 1 << sg
-constexpr int op_rows(int P) { return P == 3 ? 4 : 1; }
-constexpr int lane_tokens(int P) { return 4 / op_rows(P); }
-constexpr int group_of(int P, int sg) { return lane_tokens(P) << sg; }
-
-__host__ __device__ __forceinline__ constexpr int padded(int blocks) { return (blocks + 7) & ~7; }
-// a row of a plane, in memory and in LDS: [runs of 8 blocks][u][half][g][16 bytes], then 16 bytes unused: 16 rows' pieces lie in different banks
-__host__ __device__ __forceinline__ constexpr int plane_bytes(int nb) { return padded(nb) * 32 + 16; }
-// LDS of a pass, for `cr` runs of k at a time: token t's plane p is row t P + p; zeros for the operand's other lanes; per 32 << sg values the
-// tokens' factors, and with minimums the tokens' sums
-struct Lds {
-    int row, zero, dx, ds, end;
-};
-__host__ __device__ __forceinline__ constexpr Lds lds_of(int P, int sg, int cr, int tp, bool mins) {
-    Lds l{};
-    l.row = cr * 256 + 16;
-    l.zero = tp * P * l.row;
-    l.dx = l.zero + 256;
-    l.ds = l.dx + (cr * 8 >> sg) * tp * 4;
-    l.end = ((mins ? l.ds + (cr * 8 >> sg) * tp * 4 : l.ds) + 15) & ~15;
-    return l;
-}
 // the block of lane group g in step u of a run of 8 blocks: groups that share a sum have blocks of one weight group, and a lane's two steps
 // have scales that lie next to each other
 template <int SG> __device__ __forceinline__ int block_of(int g, int u) {
@@ -104,10 +74,7 @@ template <int NT> struct Rows {
     }
 };
 // A run's codes and a window's scales in registers.  Scales come 32 of a row at a time (64 contiguous bytes; a lane's own of every run would
-// fetch each cache line many times) and go through LDS of the wave's own.
-constexpr int WIN = 32, WROW = WIN + 8; // scales of a window, a row's place: 16 rows' 80 bytes begin in different banks
-constexpr int win_bytes(int nt, bool mins) { return nt * (mins ? 2 : 1) * 16 * WROW * 2; }
-// Two runs are on their way: one alone leaves a wave waiting for memory.
+// fetch each cache line many times) and go through LDS of the wave's own.  Two runs are on their way: one alone leaves a wave waiting for memory.
 template <int NT, bool MINS> struct Run {
     u32x4 c[2][NT][2];
     u32x4 s[NT], m[NT];
@@ -139,15 +106,6 @@ template <int GSH, int SG, int NT, bool MINS> __device__ __forceinline__ Run<NT,
     return r;
 }
 
-// a wave's part of the runs of a chunk of k, and the chunk's first run
-struct Part {
-    int first, r0, r1;
-};
-// runs `chunk` .. of k, `cr` of them at a time, the ks-th of 1 << log parts (each has one at least)
-__device__ __forceinline__ Part part_of(int runs, int cr, int chunk, int ks, int log) {
-    const int c0 = chunk * cr, n = min(cr, runs - c0);
-    return Part{c0, c0 + ((n * ks) >> log), c0 + ((n * (ks + 1)) >> log)};
-}
 // adds the sums of the part p for nt tokens in LDS, at most TM, to acc.  in: the first two runs' codes and the first window of scales; those of the
 // part q behind
 template <int P, int GSH, int SG, int NT, int TM, bool MINS>
@@ -421,7 +379,7 @@ __device__ __forceinline__ void zero_pieces(uint8_t * lds, const Lds & L) {
     if (threadIdx.x < 64) reinterpret_cast<unsigned *>(lds + L.zero)[threadIdx.x] = 0;
 }
 
-// The gate and the up projection: a workgroup has 16 CG inner columns of an expert, its waves (16 columns of both, a KS-th of dim), CG KS = 8.
+// The gate and the up projection: a workgroup has 16 CG inner columns of an expert, its waves (16 columns of both, a KS-th of dim), CG KS = WAVES.
 // SG: lane groups that share a sum of x; SH: those of the down projection, whose x (h) this kernel leaves as planes.
 template <int XF, int GSH, int SH, int TM, bool MINS> __global__ __launch_bounds__(WAVES * 64, 3) void k_moe_up(MoeArgs a) {
     constexpr int P = planes_of(XF), SG = P == 1 ? 0 : GSH;
@@ -552,8 +510,6 @@ template <int P, int GSH, int SG, int TM, bool MINS> __global__ __launch_bounds_
     }
 }
 
-constexpr int OW = 16; // waves of a workgroup of k_moe_down_one
-
 // The down projection of a single row and the sum over its experts, in one launch: a workgroup has 16 NT columns of all of them, its waves (an expert,
 // a part of inner).  Tokens in LDS are the row's pairs; no list is needed.  A layer's row, 8 of 128 experts of 2,048 x 768: 26.3 us, 28.6 with k_moe_down and
 // k_moe_sum; 2 of 8 of 5,120 x 6,144 in fp32: 45 and 49.
@@ -623,7 +579,6 @@ template <int YT> __global__ __launch_bounds__(256) void k_moe_sum(MoeArgs a) {
     for (int i = 0; i < 4; i++) y[i] = Elem<YT>::down(v[i]);
 }
 
-size_t lds_bytes(const MoeArgs & a, int P, int sg, int cr, int tp) { return lds_of(P, sg, cr, tp, a.up.mins).end + (size_t) WAVES * win_bytes(2, a.up.mins); }
 template <int XF, int GSH, int SH, int TM, bool MINS> hipError_t up(const MoeArgs & a, int slots, hipStream_t st) {
     constexpr int P = planes_of(XF), SG = P == 1 ? 0 : GSH;
     static std::atomic<uint64_t> done;
@@ -639,9 +594,6 @@ template <int P, int GSH, int SG, int TM, bool MINS> hipError_t down(const MoeAr
     const int cols = 32 * (WAVES >> a.ks_down);
     return e != hipSuccess ? e : launch(k_moe_down<P, GSH, SG, TM, MINS>, dim3((a.dim + cols - 1) / cols, slots), dim3(WAVES * 64), lds, st, a);
 }
-size_t one_lds(const MoeArgs & a, int P, int sg, int nt) {
-    return lds_of(P, sg, padded(a.inner >> 5) >> 3, a.top_k + group_of(P, sg), a.up.mins).end + (size_t) OW * (win_bytes(nt, a.up.mins) + nt * 64);
-}
 template <int P, int GSH, int SG, int NT, bool MINS, int YT> hipError_t down_one(const MoeArgs & a, hipStream_t st) {
     static std::atomic<uint64_t> done;
     const size_t lds = one_lds(a, P, SG, NT);
@@ -653,8 +605,8 @@ template <int XF, int GSH, int SH, bool MINS> hipError_t run(const MoeArgs & a, 
     const int slots = std::min(a.n_experts, a.rows * a.top_k);
     hipError_t e = a.tp_up <= 8 ? up<XF, GSH, SH, 8, MINS>(a, slots, st) : up<XF, GSH, SH, 16, MINS>(a, slots, st);
     if (e != hipSuccess) return e;
-    // one row whose h LDS holds: its sum with the product (a workgroup a CU: 16 columns, or 32 where those would be more)
-    if (a.rows == 1 && one_lds(a, HP, SH, 2) <= 150 * 1024) return a.dim <= 256 * 16 ? down_one<HP, GSH, SH, 1, MINS, YT>(a, st) : down_one<HP, GSH, SH, 2, MINS, YT>(a, st);
+    // (a workgroup a CU: 16 columns, or 32 where those would be more)
+    if (one_row(a)) return a.dim <= 256 * 16 ? down_one<HP, GSH, SH, 1, MINS, YT>(a, st) : down_one<HP, GSH, SH, 2, MINS, YT>(a, st);
     e = a.tp_down <= 8 ? down<HP, GSH, SH, 8, MINS>(a, slots, st) : down<HP, GSH, SH, 16, MINS>(a, slots, st);
     if (e != hipSuccess) return e;
     return launch(k_moe_sum<YT>, dim3((a.dim + 1023) / 1024, a.rows), dim3(256), 0, st, a);
@@ -667,31 +619,6 @@ template <int XF, bool MINS> hipError_t run(const MoeArgs & a, hipStream_t st) {
     return a.gsh == 0 ? run<XF, 0, MINS>(a, st) : a.gsh == 1 ? run<XF, 1, MINS>(a, st) : run<XF, 2, MINS>(a, st);
 }
 template <int XF> hipError_t run(const MoeArgs & a, hipStream_t st) { return a.up.mins ? run<XF, true>(a, st) : run<XF, false>(a, st); }
-
-// Tokens of a pass, up to 16, and runs of k that LDS holds at a time, three workgroups a CU: all of k where that leaves room for twice the tokens
-// that an expert has on average, else chunks of at least four runs a wave (47 rows of 8 experts, 16 tokens in chunks: 178 us, 8 at a time 205;
-// 3 rows, the other way round: 85 and 79).
-void pass(const MoeArgs & a, int P, int sg, int runs, int ks_log, int & tp, int & cr) {
-    constexpr size_t THIRD = 53 * 1024;
-    const int tg = group_of(P, sg), least = std::min(runs, 4 << ks_log), most = std::min((std::min(a.rows, 16) + tg - 1) / tg * tg, 16);
-    const int want = std::min(most, 2 * ((a.rows * a.top_k + a.n_experts - 1) / a.n_experts));
-    cr = runs;
-    for (tp = most; tp >= std::max(want, tg); tp -= tg)
-        if (lds_bytes(a, P, sg, cr, tp) <= THIRD) return;
-    for (tp = most;; tp -= tg) {
-        for (cr = runs; cr > least && lds_bytes(a, P, sg, cr, tp) > THIRD;) cr = std::max(least, (cr + 1) / 2);
-        if (tp <= tg || lds_bytes(a, P, sg, cr, tp) <= THIRD) break;
-    }
-    // (the last chunk has a run for every wave)
-    while (cr < runs && runs % cr && runs % cr < 1 << ks_log) cr++;
-}
-// waves that split k (1 << ..): as many as leave the workgroups (of `cols` columns a wave) within one round of two a CU, as every round pays for its
-// start; `experts` are those that occur
-int split(double experts, int n, int cols, int runs, int limit) {
-    int log = limit;
-    while (log > 0 && (experts * ((n + (cols * WAVES >> log) - 1) / (cols * WAVES >> log)) > 768 || runs < 1 << log)) log--;
-    return log;
-}
 
 } // namespace
 
@@ -717,19 +644,6 @@ long long moe_plan(MoeArgs & a, int xform, uint8_t * ws) {
     at = here;
     a.out = reinterpret_cast<float *>(take(pairs * a.dim * 4));
     return std::max(at, x_end);
-}
-
-// (of one run of at most MOE_ROWS rows)
-static void split_work(MoeArgs & a, int xform) {
-    const int P = planes_of(xform), nbi = a.inner / 32;
-    // the experts that occur where every choice is as likely as another
-    const double experts = a.n_experts * (1 - std::pow(1 - 1.0 / a.n_experts, a.rows * a.top_k));
-    a.ks_up = split(experts, a.inner, 16, padded(a.dim / 32) / 8, WAVES_LOG - 1);
-    a.ks_down = split(experts, a.dim, 32, padded(nbi) / 8, WAVES_LOG);
-    a.ks_one = 0;
-    while (a.top_k << (a.ks_one + 1) <= OW && 1 << (a.ks_one + 1) <= padded(nbi) / 8) a.ks_one++;
-    pass(a, P, P == 1 ? 0 : a.gsh, padded(a.dim / 32) / 8, a.ks_up, a.tp_up, a.cr_up);
-    pass(a, HP, a.ks_up == 0 ? std::min(a.gsh, 1) : 0, padded(nbi) / 8, a.ks_down, a.tp_down, a.cr_down);
 }
 
 template <int XF> static hipError_t prep(const MoeArgs & a, const RouteArgs * route, hipStream_t st) {
@@ -759,6 +673,7 @@ hipError_t launch_moe(const MoeArgs & all, int xform, const RouteArgs * route, h
             a.xmeta += (size_t) row * nb * 4;
         } else a.x = static_cast<const char *>(a.x) + row * a.x_stride * xs;
         split_work(a, xform);
+        if (!plan_holds(a, xform)) return hipErrorInvalidConfiguration; // (never: every shape that the entry points take has such a plan)
         hipError_t e = xform == W4_UNITS ? prep<W4_UNITS>(a, route, st) : xform == DT_F32 ? prep<DT_F32>(a, route, st) : xform == DT_F16 ? prep<DT_F16>(a, route, st) : prep<DT_BF16>(a, route, st);
         if (e != hipSuccess) return e;
         e = xform == W4_UNITS ? run<W4_UNITS>(a, st) : xform == DT_F32 ? run<DT_F32>(a, st) : xform == DT_F16 ? run<DT_F16>(a, st) : run<DT_BF16>(a, st);
