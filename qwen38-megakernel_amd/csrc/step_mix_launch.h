@@ -23,7 +23,10 @@ struct LoraArgs {
     int rows, n, k, n_adapters, rank;
     int rp, chunks, slots; // (set by lora_plan) rank padded to 16; chunks of k; adapters of a tile of 16 rows side by side
 };
-constexpr int LORA_FEW_ROWS = 256; // up to them tiles of 16 rows, from there of 32
+// Up to so many rows tiles of 16, whose adapters have workgroups of their own; from there tiles of 32, one workgroup for all of a tile's.  5,120 x 6,144,
+// rank 16, bf16, the first and the second: 257 rows of as many requests 34 and 103 us, 1,024 88 and 156; of 8 rows a request 19 and 25, 35 and 41; of 60
+// 20 and 21, 26 and 26; of one 20 and 19, 25 and 23 (320: 22 and 17).
+constexpr int LORA_FEW_ROWS = 1024;
 constexpr int LORA_MAX_ROWS = 1 << 19, LORA_MAX_N = 1 << 24, LORA_MAX_K = 1 << 20, LORA_MAX_RANK = 256, LORA_MAX_CHUNKS = 16;
 void lora_plan(LoraArgs & a);
 hipError_t launch_lora(const LoraArgs & a, int xform, int wtype, hipStream_t st); // xform: W4_UNITS or a Dtype

@@ -12,7 +12,7 @@ STEP = 2.0 ** -23
 
 @pytest.mark.parametrize("xform,terms", [("fp32", 1), ("fp16", 2), ("bf16", 3), ("units", 3)])
 @pytest.mark.parametrize("wname", ["fp16", "bf16"])
-@pytest.mark.parametrize("rows,rank", [(1, 16), (3, 40), (40, 8), (64, 100), (300, 33)])
+@pytest.mark.parametrize("rows,rank", [(1, 16), (3, 40), (40, 8), (64, 100), (300, 33), (1030, 20)])
 def test_exact(qkv, torch_gpu, xform, terms, wname, rows, rank):
     """Values of all the bits of their type; A takes one of them to each rank (of types of few bits several, one behind the other: up to 24 bits), B hands one on to
     each column.  bf16 adapters: exact.  fp16 adapters: values of up to 22 bits are exact, others (x, then A x) are off by 2^-23, or by 2^-39 of the largest beside them."""
@@ -58,7 +58,7 @@ def test_exact(qkv, torch_gpu, xform, terms, wname, rows, rank):
 
 @pytest.mark.parametrize("xform", ["fp32", "fp16", "bf16", "units"])
 @pytest.mark.parametrize("wname", ["fp16", "bf16"])
-@pytest.mark.parametrize("rows,rank", [(1, 16), (24, 64), (40, 24), (300, 32), (300, 100)])
+@pytest.mark.parametrize("rows,rank", [(1, 16), (24, 64), (40, 24), (300, 32), (300, 100), (1030, 64)])
 def test_errors(qkv, torch_gpu, xform, wname, rows, rank):
     """Errors as large as a step of fp32 for every instruction of a chain makes them (a sum's size: what its terms' squares add up to), to a factor of two."""
     k, n = 256, 200
