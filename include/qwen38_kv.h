@@ -325,8 +325,9 @@ int mk_lora_units(int rows, int n, int k, int n_adapters, int rank, const void *
 
 /*
  * The router of a mixture of experts: logits[m] = x[m] W^T (W [n_experts][dim] of w_dtype, summed in 64 bits and rounded to fp32 once, as the
- * choice compares values that lie close; of 1024 rows and more of 16-bit x and W those that cannot change the choice may be sums in fp32),
- * the top_k experts of each row and their weights.  rows 0..2^19, dim 1..2^17, n_experts 1..1024, top_k 1..16.
+ * choice compares values that lie close), the top_k experts of each row and their weights.  rows 0..2^19, dim 1..2^17, n_experts 1..1024, top_k 1..16.
+ * Of 1536 rows and more of x and W of one 16-bit type, without a bias, up to 256 experts, dim and x_stride multiples of 32 and 8, both aligned to 16
+ * bytes, logits that cannot change the choice or its order are sums in fp32, and weights are those of the logits given.
  *   form     0: weights are softmax(logits) of the chosen ones, 1: softmax over the chosen ones, 2: sigmoid(logits), 3: sigmoid(logits) over
  *            the chosen ones' sum; all times scale
  *   bias     fp32 [n_experts] or NULL: forms 2 and 3 choose by sigmoid(logits) + bias; else by the logits

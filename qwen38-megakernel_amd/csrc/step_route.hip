@@ -67,7 +67,11 @@ template <int V> __global__ __launch_bounds__(PW * 64) void k_route_pick(RouteAr
 // experts' norms.  An instruction rounds its products' sum, which |x| |w| bounds, and the sum so far: a chain of c of them is off by less than
 // (c + 40) 2^-22 |x| |w|.  Experts of a row that are among the first top_k, or within twice that of them, and lie that close to another of those,
 // are summed again in 64 bits by all waves together; the others' order is certain.
-constexpr int MW = 16, MANY_ROWS = 1024; // waves of a workgroup, one for a row's choice; rows from which it is taken
+constexpr int MW = 16; // waves of a workgroup, one for a row's choice
+// Rows from which it is taken.  A workgroup a CU up to 4,096 rows, its time hardly grows with them (bf16, us; behind it k_route_logits and k_route_pick):
+// 63 x 2,048: 1,024 rows 17.0, 13.5; 1,536 17.7, 19.0; 4,096 18.0, 29.  128 x 5,120: 41, 37; 44, 50; 44, 111.  256 x 7,168: 109, 84; 111, 118.  Small ones
+// gain later (8 x 2,048, 1,536 rows: 14.9, 12.2; 256 x 512 21.7, 19.0, and of 2,048 rows 21.7, 21.9).
+constexpr int MANY_ROWS = 1536;
 template <int DT> __device__ __forceinline__ f32x4 mfma16(const typename Elem<DT>::Raw8 & a, const typename Elem<DT>::Raw8 & b, f32x4 c) {
     if constexpr (DT == DT_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     else {

@@ -17,8 +17,8 @@ def far(logits, ids):
     return e / e.sum(1, keepdims=True)
 
 
-# (from 1024 rows on another kernel, which takes no bias)
-@pytest.mark.parametrize("rows,dim,e,top,bias", [(1, 64, 8, 3, False), (70, 64, 40, 8, True), (5, 2048, 200, 8, True), (9, 96, 300, 16, False), (1030, 64, 40, 4, False), (1030, 64, 40, 4, True)])
+# (from 1536 rows on another kernel, which takes no bias)
+@pytest.mark.parametrize("rows,dim,e,top,bias", [(1, 64, 8, 3, False), (70, 64, 40, 8, True), (5, 2048, 200, 8, True), (9, 96, 300, 16, False), (1030, 64, 40, 4, False), (1600, 64, 40, 4, False), (1600, 64, 40, 4, True)])
 def test_far_below_zero(qkv, torch_gpu, rows, dim, e, top, bias):
     """Logits about -600, -700, -800 and -2000, close to each other and far apart; a bias that leaves such experts alone."""
     rng = np.random.default_rng(rows + e)

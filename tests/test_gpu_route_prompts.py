@@ -14,7 +14,7 @@ pytestmark = pytest.mark.gpu
 def test_an_expert_of_nans(qkv, torch_gpu, name, e, nan):
     """Experts whose large terms cancel, so that fp32 sums lose what tells them apart; near each stand an expert of NaNs and small ones.  The choice among the
     others is that of 64-bit sums."""
-    rows, dim = 1030, 128
+    rows, dim = 1600, 128
     rng = np.random.default_rng(e + (nan or 0))
     xv = np.ones((rows, dim))
     xv[:, 32:96] = rng.integers(1, 9, (rows, 64)) / 8.0
@@ -39,7 +39,7 @@ def test_an_expert_of_nans(qkv, torch_gpu, name, e, nan):
 @pytest.mark.parametrize("name,least", [("fp16", -24), ("bf16", -133)])
 def test_below_the_smallest_normal(qkv, torch_gpu, name, least):
     """Rows, or experts, of subnormal values alone, and mixed with normal ones: they count in the choice and the logits."""
-    rows, dim, e = 1100, 256, 40
+    rows, dim, e = 1600, 256, 40
     rng = np.random.default_rng(3)
     small = rng.integers(-100, 101, (rows, dim)) * 2.0 ** least
     xs, xt = typed(small, name)
@@ -63,7 +63,7 @@ def test_below_the_smallest_normal(qkv, torch_gpu, name, least):
 
 @pytest.mark.parametrize("xname,wname,form,bias", [("bf16", "bf16", 3, True), ("fp16", "fp16", 2, True), ("bf16", "fp32", 3, True), ("fp32", "fp32", 0, False), ("bf16", "fp16", 1, False),
                                                    ("fp32", "bf16", 2, False)])
-@pytest.mark.parametrize("rows,dim,e,top", [(1023, 320, 40, 4), (1024, 320, 40, 4), (1500, 2048, 256, 8), (1100, 100, 300, 8)])
+@pytest.mark.parametrize("rows,dim,e,top", [(1023, 320, 40, 4), (1536, 320, 40, 4), (1600, 2048, 256, 8), (1700, 100, 300, 8)])
 def test_other_forms(qkv, torch_gpu, xname, wname, form, bias, rows, dim, e, top):
     """Prompts with a bias, fp32 weights, unequal types, more experts: the choice is that of 64-bit sums, the logits those sums rounded once."""
     rng = np.random.default_rng(rows + e)
@@ -72,7 +72,7 @@ def test_other_forms(qkv, torch_gpu, xname, wname, form, bias, rows, dim, e, top
     b = rng.standard_normal(e).astype(np.float32) if bias else None
     logits, ids, wt = run(qkv, torch_gpu, x, xname, w, wname, b, form, 2.0, top, pad=8)
     exact = xv @ wv.T
-    many = xname == wname != "fp32" and not bias and e <= 256 and dim % 32 == 0 and rows >= 1024
+    many = xname == wname != "fp32" and not bias and e <= 256 and dim % 32 == 0 and rows >= 1536
     assert not many  # (the kernel of many rows does not take these)
     assert (np.abs(logits - exact) <= 2.0 ** -24 * np.abs(exact) + dim * 2.0 ** -52 * (np.abs(xv) @ np.abs(wv).T)).all()
     _, ri, rw = route_ref(logits.astype(np.float64), np.eye(e), b, form, 2.0, top)
