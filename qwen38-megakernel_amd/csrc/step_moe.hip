@@ -381,8 +381,8 @@ __device__ __forceinline__ void zero_pieces(uint8_t * lds, const Lds & L) {
 
 // The gate and the up projection: a workgroup has 16 CG inner columns of an expert, its waves (16 columns of both, a KS-th of dim), CG KS = WAVES.
 // SG: lane groups that share a sum of x; SH: those of the down projection, whose x (h) this kernel leaves as planes.
-template <int XF, int GSH, int SH, int TM, bool MINS> __global__ __launch_bounds__(WAVES * 64, 3) void k_moe_up(MoeArgs a) {
-    constexpr int P = planes_of(XF), SG = P == 1 ? 0 : GSH;
+template <int P, int GSH, int SH, int TM, bool MINS> __global__ __launch_bounds__(WAVES * 64, PER_CU) void k_moe_up(MoeArgs a) {
+    constexpr int SG = P == 1 ? 0 : GSH;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const Lists * l = reinterpret_cast<const Lists *>(a.lists);
     if ((int) blockIdx.y >= l->count) return;
@@ -464,7 +464,8 @@ template <int XF, int GSH, int SH, int TM, bool MINS> __global__ __launch_bounds
 }
 
 // the down projection of every pair: waves (32 columns, a KS-th of inner)
-template <int P, int GSH, int SG, int TM, bool MINS> __global__ __launch_bounds__(WAVES * 64, 3) void k_moe_down(MoeArgs a) {
+template <int GSH, int SG, int TM, bool MINS> __global__ __launch_bounds__(WAVES * 64, PER_CU) void k_moe_down(MoeArgs a) {
+    constexpr int P = HP;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const Lists * l = reinterpret_cast<const Lists *>(a.lists);
     if ((int) blockIdx.y >= l->count) return;
@@ -513,8 +514,8 @@ template <int P, int GSH, int SG, int TM, bool MINS> __global__ __launch_bounds_
 // The down projection of a single row and the sum over its experts, in one launch: a workgroup has 16 NT columns of all of them, its waves (an expert,
 // a part of inner).  Tokens in LDS are the row's pairs; no list is needed.  A layer's row, 8 of 128 experts of 2,048 x 768: 26.3 us, 28.6 with k_moe_down and
 // k_moe_sum; 2 of 8 of 5,120 x 6,144 in fp32: 45 and 49.
-template <int P, int GSH, int SG, int NT, bool MINS, int YT> __global__ __launch_bounds__(OW * 64) void k_moe_down_one(MoeArgs a) {
-    constexpr int TG = group_of(P, SG), WB = win_bytes(NT, MINS);
+template <int GSH, int SG, int NT, bool MINS, int YT> __global__ __launch_bounds__(OW * 64) void k_moe_down_one(MoeArgs a) {
+    constexpr int P = HP, TG = group_of(P, SG), WB = win_bytes(NT, MINS);
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c0 = blockIdx.x * 16 * NT;
     const int nb = a.inner >> 5, nbp = padded(nb), runs = nbp >> 3, gs = (nb + (1 << GSH) - 1) >> GSH, tp = a.top_k + TG;
@@ -579,35 +580,35 @@ template <int YT> __global__ __launch_bounds__(256) void k_moe_sum(MoeArgs a) {
     for (int i = 0; i < 4; i++) y[i] = Elem<YT>::down(v[i]);
 }
 
-template <int XF, int GSH, int SH, int TM, bool MINS> hipError_t up(const MoeArgs & a, int slots, hipStream_t st) {
-    constexpr int P = planes_of(XF), SG = P == 1 ? 0 : GSH;
+template <int P, int GSH, int SH, int TM, bool MINS> hipError_t up(const MoeArgs & a, int slots, hipStream_t st) {
+    constexpr int SG = P == 1 ? 0 : GSH;
     static std::atomic<uint64_t> done;
     const size_t lds = lds_bytes(a, P, SG, a.cr_up, a.tp_up);
-    const hipError_t e = allow_lds(k_moe_up<XF, GSH, SH, TM, MINS>, lds, done);
+    const hipError_t e = allow_lds(k_moe_up<P, GSH, SH, TM, MINS>, lds, done);
     const int cols = 16 * (WAVES >> a.ks_up);
-    return e != hipSuccess ? e : launch(k_moe_up<XF, GSH, SH, TM, MINS>, dim3((a.inner + cols - 1) / cols, slots), dim3(WAVES * 64), lds, st, a);
+    return e != hipSuccess ? e : launch(k_moe_up<P, GSH, SH, TM, MINS>, dim3((a.inner + cols - 1) / cols, slots), dim3(WAVES * 64), lds, st, a);
 }
-template <int P, int GSH, int SG, int TM, bool MINS> hipError_t down(const MoeArgs & a, int slots, hipStream_t st) {
+template <int GSH, int SG, int TM, bool MINS> hipError_t down(const MoeArgs & a, int slots, hipStream_t st) {
     static std::atomic<uint64_t> done;
-    const size_t lds = lds_bytes(a, P, SG, a.cr_down, a.tp_down);
-    const hipError_t e = allow_lds(k_moe_down<P, GSH, SG, TM, MINS>, lds, done);
+    const size_t lds = lds_bytes(a, HP, SG, a.cr_down, a.tp_down);
+    const hipError_t e = allow_lds(k_moe_down<GSH, SG, TM, MINS>, lds, done);
     const int cols = 32 * (WAVES >> a.ks_down);
-    return e != hipSuccess ? e : launch(k_moe_down<P, GSH, SG, TM, MINS>, dim3((a.dim + cols - 1) / cols, slots), dim3(WAVES * 64), lds, st, a);
+    return e != hipSuccess ? e : launch(k_moe_down<GSH, SG, TM, MINS>, dim3((a.dim + cols - 1) / cols, slots), dim3(WAVES * 64), lds, st, a);
 }
-template <int P, int GSH, int SG, int NT, bool MINS, int YT> hipError_t down_one(const MoeArgs & a, hipStream_t st) {
+template <int GSH, int SG, int NT, bool MINS, int YT> hipError_t down_one(const MoeArgs & a, hipStream_t st) {
     static std::atomic<uint64_t> done;
-    const size_t lds = one_lds(a, P, SG, NT);
-    const hipError_t e = allow_lds(k_moe_down_one<P, GSH, SG, NT, MINS, YT>, lds, done);
-    return e != hipSuccess ? e : launch(k_moe_down_one<P, GSH, SG, NT, MINS, YT>, dim3(a.dim / (16 * NT)), dim3(OW * 64), lds, st, a);
+    const size_t lds = one_lds(a, HP, SG, NT);
+    const hipError_t e = allow_lds(k_moe_down_one<GSH, SG, NT, MINS, YT>, lds, done);
+    return e != hipSuccess ? e : launch(k_moe_down_one<GSH, SG, NT, MINS, YT>, dim3(a.dim / (16 * NT)), dim3(OW * 64), lds, st, a);
 }
 template <int XF, int GSH, int SH, bool MINS> hipError_t run(const MoeArgs & a, hipStream_t st) {
     constexpr int YT = XF == W4_UNITS ? DT_F32 : XF;
     const int slots = std::min(a.n_experts, a.rows * a.top_k);
-    hipError_t e = a.tp_up <= 8 ? up<XF, GSH, SH, 8, MINS>(a, slots, st) : up<XF, GSH, SH, 16, MINS>(a, slots, st);
+    hipError_t e = a.tp_up <= 8 ? up<planes_of(XF), GSH, SH, 8, MINS>(a, slots, st) : up<planes_of(XF), GSH, SH, 16, MINS>(a, slots, st);
     if (e != hipSuccess) return e;
     // (a workgroup a CU: 16 columns, or 32 where those would be more)
-    if (one_row(a)) return a.dim <= 256 * 16 ? down_one<HP, GSH, SH, 1, MINS, YT>(a, st) : down_one<HP, GSH, SH, 2, MINS, YT>(a, st);
-    e = a.tp_down <= 8 ? down<HP, GSH, SH, 8, MINS>(a, slots, st) : down<HP, GSH, SH, 16, MINS>(a, slots, st);
+    if (one_row(a)) return a.dim <= 256 * 16 ? down_one<GSH, SH, 1, MINS, YT>(a, st) : down_one<GSH, SH, 2, MINS, YT>(a, st);
+    e = a.tp_down <= 8 ? down<GSH, SH, 8, MINS>(a, slots, st) : down<GSH, SH, 16, MINS>(a, slots, st);
     if (e != hipSuccess) return e;
     return launch(k_moe_sum<YT>, dim3((a.dim + 1023) / 1024, a.rows), dim3(256), 0, st, a);
 }
