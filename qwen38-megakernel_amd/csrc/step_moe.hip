@@ -7,7 +7,7 @@
 // and from 4 bits to an operand.  Codes become int8 with four vector instructions for 8 of them (fp16 takes 13), so x is made integer
 // too: an exponent for every block, and three int8 planes (22 bits of the block's largest power of two; int8 units are one plane as they
 // are).  Two planes, 14 bits, are too few for 16-bit x as well: beside a value 256 times as large in its block they leave half of an fp16 layer's
-// results another than the nearest (47 rows, 2 of 8 experts 4,096 x 8,192: 176 us with two, 215 with three; 8 rows of 8 of 128 small ones 62 and 64).
+// results another than the nearest (47 rows, 2 of 8 experts 4,096 x 8,192: 176 us with two, 215 with three; 8 rows of 8 of 128 small ones 62 and 63).
 // The matrix instruction's sums are exact, the scales multiply them in fp32.
 //
 // A wave has two tiles of 16 weight rows, lane (n = lane & 15, g = lane >> 4) 16 bytes, a block of 32 codes of row n, a step.  The instruction
