@@ -510,7 +510,8 @@ void lora_plan(LoraArgs & a) {
     a.slots = a.rows <= LORA_FEW_ROWS ? std::min(16, std::max(a.rows, 1)) : 1;
     const int rt = a.rows <= LORA_FEW_ROWS ? 1 : 2, tiles = (a.rows + 16 * rt - 1) / (16 * rt), pairs = (a.k / 32 + 1) / 2;
     // and k in chunks, of at least two pairs of steps a wave, until two workgroups a CU have work
-    a.chunks = std::max(1, std::min({LORA_MAX_CHUNKS, 512 / std::max(1, tiles * a.slots), pairs / (2 * LW)}));
+    const int busy = a.rows <= LORA_SINGLE_ROWS ? a.slots : std::min(a.slots, LORA_TILE_ADAPTERS);
+    a.chunks = std::max(1, std::min({LORA_MAX_CHUNKS, 512 / std::max(1, tiles * busy), pairs / (2 * LW)}));
 }
 
 hipError_t launch_lora(const LoraArgs & a, int xform, int wtype, hipStream_t st) {

@@ -70,7 +70,9 @@ long long lora_ws_upto(int rows, int k, int rank) {
         lora_plan(a);
         return a;
     };
-    return std::max(most_bytes(1, std::min(rows, LORA_FEW_ROWS), LORA_MAX_CHUNKS, plan, lora_ws), most_bytes(LORA_FEW_ROWS + 1, rows, LORA_MAX_CHUNKS, plan, lora_ws));
+    return std::max({most_bytes(1, std::min(rows, LORA_SINGLE_ROWS), LORA_MAX_CHUNKS, plan, lora_ws),
+                     most_bytes(LORA_SINGLE_ROWS + 1, std::min(rows, LORA_FEW_ROWS), LORA_MAX_CHUNKS, plan, lora_ws),
+                     most_bytes(LORA_FEW_ROWS + 1, rows, LORA_MAX_CHUNKS, plan, lora_ws)});
 }
 
 int lora(LoraArgs a, int ab_dtype, int xform, void * ws, long long ws_bytes, void * stream) {

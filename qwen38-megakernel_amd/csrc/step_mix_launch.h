@@ -24,9 +24,12 @@ struct LoraArgs {
     int rp, chunks, slots; // (set by lora_plan) rank padded to 16; chunks of k; adapters of a tile of 16 rows side by side
 };
 // Up to so many rows tiles of 16, whose adapters have workgroups of their own; from there tiles of 32, one workgroup for all of a tile's.  5,120 x 6,144,
-// rank 16, bf16, the first and the second: 257 rows of as many requests 34 and 103 us, 1,024 88 and 156; of 8 rows a request 19 and 25, 35 and 41; of 60
-// 20 and 21, 26 and 26; of one 20 and 19, 25 and 23 (320: 22 and 17).
+// rank 16, bf16, the first and the second: 320 rows of as many requests 40 and 111 us, 1,024 87 and 156; of 8 rows a request 17 and 29, 34 and 41; of 60
+// 18 and 21, 27 and 26; of one 18 and 17, 22 and 23.
 constexpr int LORA_FEW_ROWS = 1024;
+// Up to so many rows k is cut as if a tile's rows had an adapter each, from there as if it had LORA_TILE_ADAPTERS (512 rows of one request 22 and 19 us, of 8
+// rows a request 22 and 19, of as many requests 47 and 52).
+constexpr int LORA_SINGLE_ROWS = 256, LORA_TILE_ADAPTERS = 4;
 constexpr int LORA_MAX_ROWS = 1 << 19, LORA_MAX_N = 1 << 24, LORA_MAX_K = 1 << 20, LORA_MAX_RANK = 256, LORA_MAX_CHUNKS = 16;
 void lora_plan(LoraArgs & a);
 hipError_t launch_lora(const LoraArgs & a, int xform, int wtype, hipStream_t st); // xform: W4_UNITS or a Dtype

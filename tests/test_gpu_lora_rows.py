@@ -32,6 +32,9 @@ def test_long_ranks(qkv, torch_gpu, wname, rank):
 def test_parts_of_k(qkv, torch_gpu):
     """Many rows and k in parts, prompts of ragged lengths."""
     Case(torch_gpu, 1500, 300, 2048, 32, 6, "fp32", "bf16", ids=np.sort(np.random.default_rng(2).integers(-1, 6, 1500)), seed=3).check(qkv)
+    # (and of rows whose tiles count as four adapters each, one or all of them there)
+    Case(torch_gpu, 600, 100, 2048, 20, 6, "bf16", "fp16", ids=np.arange(600) // 200, seed=4).check(qkv)
+    Case(torch_gpu, 300, 100, 5120, 20, 80, "units", "bf16", ids=np.arange(300) % 80, seed=5).check(qkv)
 
 
 def test_in_place_and_base_bits(qkv, torch_gpu):
