@@ -300,9 +300,10 @@ int mk_verify_drafts(int n_seq, int n_draft, int vocab, const void * target, lon
 
 /*
  * ---- The operators of a server of many requests beside these products: adapters of their own, and experts in place of one projection.  The
- * conventions are those of the section above (dtype, strides, units, streams, devices; the same call gives the same bits); ws is
- * device memory aligned to 16 bytes, of at least what the _ws function gives (for as many rows or more: it never falls with the rows), that
- * no other call uses until this one has finished (one per captured graph that may run at once); nothing in it needs clearing.
+ * conventions are those of the section above (dtype, strides, units, streams, devices; the same call gives the same bits, while a row's sums
+ * may be split otherwise in a call of another number of rows); ws is device memory aligned to 16 bytes, of at least what the _ws function gives
+ * (for as many rows or more: it never falls with the rows), that no other call uses until this one has finished (one per captured graph that may
+ * run at once); nothing in it needs clearing.
  *
  * Low-rank adapters of many requests at once, next to a projection of k to n values whose result is base:
  *   y[m] = base[m] + scales[a] B_a (A_a x[m]),  a = ids[m];   y[m] = base[m] where ids[m] is no adapter (below 0, n_adapters or more)
